@@ -661,6 +661,90 @@ int onnxl_amd_prepare_qqq(int64_t in_features, int64_t out_features, int64_t gro
                           const onnxl_amd_tensor *s_group, int32_t dtype, onnxl_amd_tensor *weight,
                           onnxl_amd_tensor *scale, void *stream);
 
+/* ---- Decoder-layer operators around the quantized products -----------------
+ *
+ * The pieces of a language model's decoder layer that feed the products above
+ * and read what they write.  No counterparts in the reference. */
+
+/* RMS norm with the residual's addition and 8-bit output.  x [.., D] FLOAT,
+ * FLOAT16 or BFLOAT16; weight [D] of x's type or FLOAT; residual (optional) of
+ * x's shape and type:
+ *   h = x + residual, rounded to x's type (written to `sum` if given, which
+ *       may be x's or the residual's own buffer),
+ *   v = h * (1 / sqrt(mean(h^2) + epsilon)) * weight, in fp32,
+ *   per block of block_size values (0: the row; 32, 64, 128 or 256):
+ *   y_scale = max|v| / qmax, y = the nearest code of v / y_scale,
+ * with y INT8 (qmax 127) or FLOAT8E4M3FN (qmax 448) and y_scale FLOAT
+ * [.., D / block_size] ([.., 1] for the row).  With y_scale FLOAT8E8M0 or UINT8
+ * (block_size 32, y FLOAT8E4M3FN) the output is MXFP8, as
+ * onnxl_amd_mx_quantize makes it, for onnxl_amd_mx_matmul.  A block with a
+ * value that is not finite gets a NaN scale and zero codes. */
+int onnxl_amd_rms_norm_quantize(const onnxl_amd_tensor *x, const onnxl_amd_tensor *weight,
+                                const onnxl_amd_tensor *residual, float epsilon, int64_t block_size,
+                                onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale, onnxl_amd_tensor *sum, void *stream);
+
+/* Microscaled quantization: x [.., K] FLOAT, FLOAT16 or BFLOAT16, K a multiple
+ * of 32; y FLOAT8E4M3FN (MXFP8) or FLOAT4E2M1 (MXFP4, two codes a byte) of the
+ * same shape; y_scale FLOAT8E8M0 or UINT8 [.., K / 32].  Per block of 32: the
+ * exponent is floor(log2(max|x|)) minus that of the type's largest value (8 /
+ * 2), at least -127, stored plus 127; the codes are the nearest to x / 2^e,
+ * ties to even, saturating.  A block with a value that is not finite gets the
+ * NaN scale 255 and zero codes. */
+int onnxl_amd_mx_quantize(const onnxl_amd_tensor *x, onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale, void *stream);
+
+/* Microscaled product: y[.., n] = sum over k of a[.., k] b[n, k], both in
+ * blocks of 32 with E8M0 scales, fp32 sums, rounded once to y (FLOAT16 or
+ * BFLOAT16 [.., N]).  b [N, K]: FLOAT4E2M1, or UINT8 [N, K / 2] as the
+ * "mxfp4" checkpoint encoding holds it; b_scale FLOAT8E8M0 or UINT8
+ * [N, K / 32].  a: FLOAT8E4M3FN or FLOAT4E2M1 (or packed UINT8) [.., K] with
+ * a_scale [.., K / 32] and a_type 0; or FLOAT16 / BFLOAT16 [.., K] of y's type
+ * without a_scale, quantized by the call to a_type (FLOAT8E4M3FN or
+ * FLOAT4E2M1) as onnxl_amd_mx_quantize does.  Codes must be 16-byte aligned. */
+int onnxl_amd_mx_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type,
+                        const onnxl_amd_tensor *b, const onnxl_amd_tensor *b_scale, onnxl_amd_tensor *y,
+                        void *stream);
+
+/* A paged key / value cache in 8 bits with one scale for each block of tokens
+ * and head:
+ *   k_cache INT8 or FLOAT8E4M3FN [blocks, kv_heads, block_tokens, head_dim],
+ *   v_cache the same type        [blocks, kv_heads, head_dim, block_tokens],
+ *   k_scale, v_scale FLOAT       [blocks, kv_heads],
+ * block_tokens 16, 32, 64, 128 or 256, head_dim a multiple of 16 up to 256, all
+ * in device memory, the codes 16-byte aligned.  A batch of sequences with new
+ * tokens is described by
+ *   block_table INT32 [batch, max_blocks]: the cache block of every
+ *               block_tokens tokens of a sequence,
+ *   query_start INT32 [batch + 1]: the first row of each sequence's new tokens,
+ *   lengths     INT32 [batch]: its tokens in the cache, the new ones included.
+ * No two sequences may append into one block.  Index tensors in host memory are
+ * checked by the call; with device-resident ones a sequence whose numbers do
+ * not fit (or that names a block outside the cache) is not appended, and its
+ * rows of the attention are NaN.
+ *
+ * Append: k, v FLOAT16 or BFLOAT16 [tokens, kv_heads, head_dim].  A block's
+ * scale becomes the larger of that of the tokens it keeps (none: 0) and
+ * max|new| / qmax (127 or 448); where it grew, the kept codes are rounded
+ * again to it; new codes are the nearest to value / scale.  New tokens that are
+ * not finite give the block a NaN scale. */
+int onnxl_amd_kv_cache_append(const onnxl_amd_tensor *k, const onnxl_amd_tensor *v, onnxl_amd_tensor *k_cache,
+                              onnxl_amd_tensor *v_cache, onnxl_amd_tensor *k_scale, onnxl_amd_tensor *v_scale,
+                              const onnxl_amd_tensor *block_table, const onnxl_amd_tensor *query_start,
+                              const onnxl_amd_tensor *lengths, void *stream);
+
+/* Attention of the new tokens over the cache (which holds them already):
+ * q and out FLOAT16 or BFLOAT16 [tokens, heads, head_dim], heads a multiple of
+ * kv_heads (consecutive heads share one).  The new token i of n of a sequence
+ * of length L sees the tokens 0 .. L - n + i:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,
+ * statistics and sums in fp32.  What the cache holds past a sequence's length
+ * is never used.  max_query: the most new tokens that a sequence has, where the
+ * caller knows it (0 otherwise); it only helps to choose the kernels. */
+int onnxl_amd_kv_cache_attention(const onnxl_amd_tensor *q, const onnxl_amd_tensor *k_cache,
+                                 const onnxl_amd_tensor *v_cache, const onnxl_amd_tensor *k_scale,
+                                 const onnxl_amd_tensor *v_scale, const onnxl_amd_tensor *block_table,
+                                 const onnxl_amd_tensor *query_start, const onnxl_amd_tensor *lengths, float scale,
+                                 int64_t max_query, onnxl_amd_tensor *out, void *stream);
+
 /* Waits for all work queued by this library on `stream`. */
 int onnxl_amd_synchronize(void *stream);
 

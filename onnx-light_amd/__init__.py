@@ -29,6 +29,7 @@ MAX_RANK = 8
 # ONNX TensorProto.DataType codes.
 FLOAT, UINT8, INT8, UINT16, INT16, INT32, INT64 = 1, 2, 3, 4, 5, 6, 7
 FLOAT16, DOUBLE, BFLOAT16, FLOAT8E4M3FN, UINT4, INT4 = 10, 11, 16, 17, 21, 22
+FLOAT4E2M1, FLOAT8E8M0 = 23, 24
 
 OK, INVALID_ARGUMENT, UNSUPPORTED, DEVICE_ERROR, NOT_INITIALIZED = 0, 1, 2, 3, 4
 DEVICE, HOST = 0, 1
@@ -145,6 +146,11 @@ def lib() -> ctypes.CDLL:
         L.onnxl_amd_qlinear_conv.argtypes = [TP] * 9 + [CA, TP, ctypes.c_void_p]
         L.onnxl_amd_prepare_weight_size.argtypes = [TP, ctypes.POINTER(ctypes.c_int64)]
         L.onnxl_amd_prepare_weight.argtypes = [TP, TP, ctypes.c_void_p]
+        L.onnxl_amd_rms_norm_quantize.argtypes = [TP, TP, TP, F32, I64, TP, TP, TP, ctypes.c_void_p]
+        L.onnxl_amd_mx_quantize.argtypes = [TP, TP, TP, ctypes.c_void_p]
+        L.onnxl_amd_mx_matmul.argtypes = [TP, TP, I32, TP, TP, TP, ctypes.c_void_p]
+        L.onnxl_amd_kv_cache_append.argtypes = [TP] * 9 + [ctypes.c_void_p]
+        L.onnxl_amd_kv_cache_attention.argtypes = [TP] * 8 + [F32, I64, TP, ctypes.c_void_p]
         L.onnxl_amd_synchronize.argtypes = [ctypes.c_void_p]
         _lib = L
     return _lib
@@ -930,6 +936,106 @@ def qlinear_conv(x, x_scale, x_zero_point, w, w_scale, w_zero_point, y_scale, y_
     return out
 
 
+# ---- decoder-layer operators (no reference kernels) --------------------------
+
+def rms_norm_quantize(x, weight, residual=None, epsilon: float = 1e-5, block_size: int = 0,
+                      output_dtype: int = FLOAT8E4M3FN, mx: bool = False, out=None):
+    """RMS norm with the residual's addition and 8-bit output: returns (y,
+    y_scale, sum), sum = x + residual in x's type (None without a residual).
+    y is INT8 or FLOAT8E4M3FN with one float32 scale per block_size values of a
+    row (0: one per row), or with ``mx`` MXFP8 (FLOAT8E4M3FN, blocks of 32,
+    uint8 E8M0 scales) for mx_matmul."""
+    torch = _torch()
+    shape, dev = _shape_of(x), _device_of(x)
+    if mx:
+        block_size = 32
+    if out is None:
+        blocks = shape[-1] // block_size if block_size else 1
+        out = (_empty(shape, torch.int8 if output_dtype == INT8 else torch.float8_e4m3fn, dev),
+               _empty((*shape[:-1], blocks), torch.uint8 if mx else torch.float32, dev),
+               torch.empty_like(x) if residual is not None else None)
+    y, y_scale, total = out
+    _check(lib().onnxl_amd_rms_norm_quantize(describe(x), describe(weight), describe(residual), epsilon, block_size,
+                                             describe(y), describe(y_scale), describe(total), _stream_of(x, y)))
+    return out
+
+
+def mx_quantize(x, output_dtype: int = FLOAT8E4M3FN, out=None):
+    """Microscaled quantization of x [.., K] in blocks of 32: (codes, scales),
+    the codes torch.float8_e4m3fn [.., K] or, for FLOAT4E2M1, packed uint8
+    [.., K / 2], the scales uint8 E8M0 [.., K / 32]."""
+    torch = _torch()
+    shape, dev = _shape_of(x), _device_of(x)
+    if out is None:
+        fp4 = output_dtype == FLOAT4E2M1
+        out = (_empty((*shape[:-1], shape[-1] // 2) if fp4 else shape, torch.uint8 if fp4 else torch.float8_e4m3fn, dev),
+               _empty((*shape[:-1], shape[-1] // 32), torch.uint8, dev))
+    y, y_scale = out
+    _check(lib().onnxl_amd_mx_quantize(describe(x), describe(y, output_dtype, shape), describe(y_scale),
+                                       _stream_of(x, y)))
+    return out
+
+
+def mx_matmul(a, b, b_scale, a_scale=None, a_type: int = FLOAT8E4M3FN, output_dtype=None, out=None):
+    """a @ b^T in microscaled types: b packed FLOAT4E2M1 uint8 [N, K / 2] with
+    b_scale uint8 E8M0 [N, K / 32] (the "mxfp4" checkpoint layout); a FLOAT16 /
+    BFLOAT16 [.., K], quantized by the call to a_type (FLOAT8E4M3FN or
+    FLOAT4E2M1), or codes with a_scale as mx_quantize returns them, then with
+    output_dtype a torch type (bfloat16 by default)."""
+    torch = _torch()
+    if a_scale is not None:
+        a_type = 0
+    if out is None:
+        dt = a.dtype if a_scale is None else output_dtype or torch.bfloat16
+        out = _empty((*_shape_of(a)[:-1], _shape_of(b)[0]), dt, _device_of(a, b))
+    _check(lib().onnxl_amd_mx_matmul(describe(a), describe(a_scale), a_type, describe(b), describe(b_scale),
+                                     describe(out), _stream_of(a, b, out)))
+    return out
+
+
+class KvCache:
+    """A paged 8-bit key / value cache on the device, one scale for each block
+    of tokens and head: k_cache [blocks, kv_heads, block_tokens, head_dim],
+    v_cache [blocks, kv_heads, head_dim, block_tokens] and float32 k_scale,
+    v_scale [blocks, kv_heads]."""
+
+    def __init__(self, blocks: int, kv_heads: int, block_tokens: int, head_dim: int, dtype: int = FLOAT8E4M3FN,
+                 device="cuda"):
+        torch = _torch()
+        dt = torch.int8 if dtype == INT8 else torch.float8_e4m3fn
+        self.k_cache = torch.empty((blocks, kv_heads, block_tokens, head_dim), dtype=dt, device=device)
+        self.v_cache = torch.empty((blocks, kv_heads, head_dim, block_tokens), dtype=dt, device=device)
+        self.k_scale = torch.empty((blocks, kv_heads), dtype=torch.float32, device=device)
+        self.v_scale = torch.empty((blocks, kv_heads), dtype=torch.float32, device=device)
+
+    def tensors(self) -> tuple:
+        return self.k_cache, self.v_cache, self.k_scale, self.v_scale
+
+
+def kv_cache_append(k, v, cache: KvCache, block_table, query_start, lengths) -> KvCache:
+    """Quantizes the new tokens' k and v [tokens, kv_heads, head_dim] into the
+    cache's blocks (int32 block_table [batch, max_blocks], query_start
+    [batch + 1], lengths [batch] with the new tokens); returns the cache."""
+    _check(lib().onnxl_amd_kv_cache_append(describe(k), describe(v), *(describe(t) for t in cache.tensors()),
+                                           describe(block_table), describe(query_start), describe(lengths),
+                                           _stream_of(k, v, cache.k_cache)))
+    return cache
+
+
+def kv_cache_attention(q, cache: KvCache, block_table, query_start, lengths, scale=None, max_query: int = 0, out=None):
+    """Causal attention of the new tokens q [tokens, heads, head_dim] over the
+    cache, which holds them already; scale defaults to head_dim ** -0.5,
+    max_query is the most new tokens of a sequence where known."""
+    if out is None:
+        out = _torch().empty_like(q)
+    if scale is None:
+        scale = float(_shape_of(q)[-1]) ** -0.5
+    _check(lib().onnxl_amd_kv_cache_attention(describe(q), *(describe(t) for t in cache.tensors()),
+                                              describe(block_table), describe(query_start), describe(lengths), scale,
+                                              max_query, describe(out), _stream_of(q, cache.k_cache, out)))
+    return out
+
+
 class MatMulInteger:
     """Kernel-class mirror of kernel::MatMulInteger."""
     name = "onnxl_amd:GPU:ai.onnx:MatMulInteger"
@@ -1059,6 +1165,50 @@ class DequantizeLinearGroupedMatMul:
                                                 transB, x_dtype, x_shape, out)
 
 
+class RmsNormQuantize:
+    """RMS norm with the residual's addition and 8-bit output (no reference
+    kernel); attributes epsilon, block_size, output_dtype and mx."""
+    name = "onnxl_amd:GPU:ai.rt.amd:RmsNormQuantize"
+
+    def __call__(self, x, weight, residual=None, epsilon=1e-5, block_size=0, output_dtype=FLOAT8E4M3FN, mx=False,
+                 out=None):
+        return rms_norm_quantize(x, weight, residual, epsilon, block_size, output_dtype, mx, out)
+
+
+class MxQuantize:
+    """Microscaled quantization (no reference kernel); attribute output_dtype."""
+    name = "onnxl_amd:GPU:ai.rt.amd:MxQuantize"
+
+    def __call__(self, x, output_dtype=FLOAT8E4M3FN, out=None):
+        return mx_quantize(x, output_dtype, out)
+
+
+class MxMatMul:
+    """Product with MXFP4 weights (no reference kernel); attributes a_type and
+    output_dtype."""
+    name = "onnxl_amd:GPU:ai.rt.amd:MxMatMul"
+
+    def __call__(self, a, b, b_scale, a_scale=None, a_type=FLOAT8E4M3FN, output_dtype=None, out=None):
+        return mx_matmul(a, b, b_scale, a_scale, a_type, output_dtype, out)
+
+
+class KvCacheAppend:
+    """New keys and values into a paged 8-bit cache (no reference kernel)."""
+    name = "onnxl_amd:GPU:ai.rt.amd:KvCacheAppend"
+
+    def __call__(self, k, v, cache, block_table, query_start, lengths):
+        return kv_cache_append(k, v, cache, block_table, query_start, lengths)
+
+
+class KvCacheAttention:
+    """Causal attention over a paged 8-bit cache (no reference kernel);
+    attributes scale and max_query."""
+    name = "onnxl_amd:GPU:ai.rt.amd:KvCacheAttention"
+
+    def __call__(self, q, cache, block_table, query_start, lengths, scale=None, max_query=0, out=None):
+        return kv_cache_attention(q, cache, block_table, query_start, lengths, scale, max_query, out)
+
+
 # Dispatch keys "<domain>:<op_type>" as the reference table uses them
 # (core/runtime/kernels/kernel_dispatch_table.h:148-164).
 KERNELS = {"ai.onnx:MatMulInteger": MatMulInteger, "ai.onnx:QLinearMatMul": QLinearMatMul,
@@ -1070,7 +1220,10 @@ KERNELS = {"ai.onnx:MatMulInteger": MatMulInteger, "ai.onnx:QLinearMatMul": QLin
            "ai.onnx:GroupedMatMul": GroupedMatMul,
            "ai.rt.amd:DequantizeLinearMatMul": DequantizeLinearMatMul,
            "ai.rt.amd:DequantizePackedMatMul": DequantizePackedMatMul,
-           "ai.rt.amd:DequantizeLinearGroupedMatMul": DequantizeLinearGroupedMatMul}
+           "ai.rt.amd:DequantizeLinearGroupedMatMul": DequantizeLinearGroupedMatMul,
+           "ai.rt.amd:RmsNormQuantize": RmsNormQuantize, "ai.rt.amd:MxQuantize": MxQuantize,
+           "ai.rt.amd:MxMatMul": MxMatMul, "ai.rt.amd:KvCacheAppend": KvCacheAppend,
+           "ai.rt.amd:KvCacheAttention": KvCacheAttention}
 
 
 class Prepared:

@@ -14,6 +14,7 @@
 
 #include "checkpoint_layout.hpp"
 #include "common.hpp"
+#include "decoder.hpp"
 #include "kernels.hpp"
 
 // Scratch of onnxl_amd_dequantize_linear_matmul_noalloc: a fixed array that
@@ -3187,6 +3188,341 @@ int PrepareQqq(int64_t k, int64_t n, int64_t group, int64_t bits, const onnxl_am
   return ONNXL_AMD_OK;
 }
 
+// ---------------------------------------------------------------------------
+// Decoder-layer operators around the quantized products (decoder.hpp).  No
+// reference kernels: argument errors follow this file's manner.
+
+constexpr const char *kRmsName = "RmsNormQuantize";
+constexpr const char *kMxqName = "MxQuantize";
+constexpr const char *kMxmName = "MxMatMul";
+constexpr const char *kKvaName = "KvCacheAppend";
+constexpr const char *kKvtName = "KvCacheAttention";
+
+bool Is16Bit(int32_t dt) { return dt == kFloat16 || dt == kBfloat16; }
+bool IsE8M0(int32_t dt) { return dt == kFloat8E8M0 || dt == kUint8; }
+
+void NeedShape(const onnxl_amd_tensor *t, const Shape &want, const char *op, const char *what) {
+  OLA_ENFORCE(ShapeOf(*t) == want, op, ": ", what, " has the wrong shape.");
+}
+
+int RmsNormQuantize(const onnxl_amd_tensor *x, const onnxl_amd_tensor *weight, const onnxl_amd_tensor *residual,
+                    float epsilon, int64_t block, onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale,
+                    onnxl_amd_tensor *sum, hipStream_t stream) {
+  OLA_ENFORCE(!Absent(x) && !Absent(weight) && !Absent(y) && !Absent(y_scale), kRmsName,
+              ": x, weight, y and y_scale are required.");
+  CheckDescriptor(x, "x");
+  CheckDescriptor(weight, "weight");
+  CheckDescriptor(residual, "residual");
+  CheckDescriptor(y, "y");
+  CheckDescriptor(y_scale, "y_scale");
+  CheckDescriptor(sum, "sum");
+  const bool has_r = !Absent(residual), has_sum = !Absent(sum);
+  const int32_t dt = x->data_type;
+  OLA_ENFORCE(dt == kFloat || Is16Bit(dt), kRmsName, ": x must be FLOAT, FLOAT16 or BFLOAT16.");
+  OLA_ENFORCE(x->rank >= 1, kRmsName, ": x must have a last dimension to normalise over.");
+  const Shape xs = ShapeOf(*x);
+  const int64_t D = xs.back();
+  OLA_ENFORCE(D > 0, kRmsName, ": the normalised dimension is empty.");
+  OLA_ENFORCE(weight->data_type == dt || weight->data_type == kFloat, kRmsName,
+              ": weight must have x's type or FLOAT.");
+  NeedShape(weight, {D}, kRmsName, "weight");
+  if (has_r) {
+    OLA_ENFORCE(residual->data_type == dt, kRmsName, ": residual must have x's type.");
+    NeedShape(residual, xs, kRmsName, "residual");
+  }
+  if (has_sum) {
+    OLA_ENFORCE(has_r, kRmsName, ": sum is an output of the residual's addition; there is no residual.");
+    OLA_ENFORCE(sum->data_type == dt, kRmsName, ": sum must have x's type.");
+    NeedShape(sum, xs, kRmsName, "sum");
+  }
+  OLA_ENFORCE(epsilon >= 0.f && epsilon < std::numeric_limits<float>::infinity(), kRmsName,
+              ": epsilon must be finite and not negative.");
+  OLA_ENFORCE(y->data_type == kInt8 || y->data_type == kFloat8E4M3FN, kRmsName, ": y must be INT8 or FLOAT8E4M3FN.");
+  NeedShape(y, xs, kRmsName, "y");
+  OLA_ENFORCE(block == 0 || block == 32 || block == 64 || block == 128 || block == 256, kRmsName,
+              ": block_size must be 0 (the row), 32, 64, 128 or 256.");
+  if (block == 0) block = D;
+  OLA_ENFORCE(D % block == 0, kRmsName, ": block_size must divide the normalised dimension.");
+  const bool mx = IsE8M0(y_scale->data_type);
+  OLA_ENFORCE(mx || y_scale->data_type == kFloat, kRmsName, ": y_scale must be FLOAT, or FLOAT8E8M0 / UINT8.");
+  OLA_ENFORCE(!mx || (block == 32 && y->data_type == kFloat8E4M3FN), kRmsName,
+              ": FLOAT8E8M0 scales go with FLOAT8E4M3FN codes in blocks of 32.");
+  Shape ss = xs;
+  ss.back() = D / block;
+  NeedShape(y_scale, ss, kRmsName, "y_scale");
+  const int64_t rows = NumElements(xs) / D;
+  OLA_ENFORCE(rows < (int64_t(1) << 31), kRmsName, ": more than 2^31 rows.");
+  if (rows == 0) return ONNXL_AMD_OK;
+  Ctx();
+  Staging st(stream, 0, {x, weight, has_r ? residual : nullptr}, {y, y_scale, has_sum ? sum : nullptr});
+  RmsNormParams p{};
+  p.x = st.In(x);
+  p.residual = has_r ? st.In(residual) : nullptr;
+  p.weight = st.In(weight);
+  p.y = st.Out(y);
+  p.scale = st.Out(y_scale);
+  p.sum = has_sum ? st.Out(sum) : nullptr;
+  p.rows = rows;
+  p.D = D;
+  p.block = block;
+  p.eps = epsilon;
+  p.x_dtype = dt;
+  p.weight_f32 = weight->data_type == kFloat;
+  p.y_fp8 = y->data_type == kFloat8E4M3FN;
+  p.scale_kind = mx ? kRnsE8M0 : kRnsFloat;
+  LaunchRmsNormQuantize(p, stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+int MxQuantize(const onnxl_amd_tensor *x, onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale, hipStream_t stream) {
+  OLA_ENFORCE(!Absent(x) && !Absent(y) && !Absent(y_scale), kMxqName, ": x, y and y_scale are required.");
+  CheckDescriptor(x, "x");
+  CheckDescriptor(y, "y");
+  CheckDescriptor(y_scale, "y_scale");
+  OLA_ENFORCE(x->data_type == kFloat || Is16Bit(x->data_type), kMxqName, ": x must be FLOAT, FLOAT16 or BFLOAT16.");
+  OLA_ENFORCE(x->rank >= 1 && x->dims[x->rank - 1] % 32 == 0, kMxqName,
+              ": the last dimension of x must be a multiple of the block size 32.");
+  OLA_ENFORCE(y->data_type == kFloat8E4M3FN || y->data_type == kFloat4E2M1, kMxqName,
+              ": y must be FLOAT8E4M3FN or FLOAT4E2M1.");
+  Shape s = ShapeOf(*x);
+  NeedShape(y, s, kMxqName, "y");
+  OLA_ENFORCE(IsE8M0(y_scale->data_type), kMxqName, ": y_scale must be FLOAT8E8M0 or UINT8.");
+  const int64_t K = s.back(), n = NumElements(s);
+  s.back() = K / 32;
+  NeedShape(y_scale, s, kMxqName, "y_scale");
+  if (n == 0) return ONNXL_AMD_OK;
+  Ctx();
+  Staging st(stream, 0, {x}, {y, y_scale});
+  MxQuantParams p{st.In(x), static_cast<uint8_t *>(st.Out(y)), static_cast<uint8_t *>(st.Out(y_scale)), n / K, K,
+                  x->data_type, y->data_type == kFloat4E2M1};
+  LaunchMxQuantize(p, stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+// Elements of the last dimension of MX codes: E2M1 codes are FLOAT4E2M1 [.., K]
+// or, as the "mxfp4" checkpoint encoding holds them, UINT8 [.., K / 2].
+int64_t MxLength(const onnxl_amd_tensor *t) {
+  return t->dims[t->rank - 1] * (t->data_type == kUint8 ? 2 : 1);
+}
+
+int MxMatMul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type, const onnxl_amd_tensor *b,
+             const onnxl_amd_tensor *b_scale, onnxl_amd_tensor *y, hipStream_t stream) {
+  OLA_ENFORCE(!Absent(a) && !Absent(b) && !Absent(b_scale) && !Absent(y), kMxmName,
+              ": a, b, b_scale and y are required.");
+  CheckDescriptor(a, "a");
+  CheckDescriptor(a_scale, "a_scale");
+  CheckDescriptor(b, "b");
+  CheckDescriptor(b_scale, "b_scale");
+  CheckDescriptor(y, "y");
+  OLA_ENFORCE(b->data_type == kFloat4E2M1 || b->data_type == kUint8, kMxmName,
+              ": b must be FLOAT4E2M1 [N, K] or its packed UINT8 [N, K / 2].");
+  OLA_ENFORCE(b->rank == 2 && a->rank >= 1, kMxmName, ": b must be 2-D and a at least 1-D.");
+  const bool quantise = Absent(a_scale);
+  Shape as = ShapeOf(*a);
+  if (quantise) {
+    OLA_ENFORCE(Is16Bit(a->data_type), kMxmName, ": a without a_scale must be FLOAT16 or BFLOAT16.");
+    OLA_ENFORCE(a_type == kFloat8E4M3FN || a_type == kFloat4E2M1, kMxmName,
+                ": a_type must be FLOAT8E4M3FN or FLOAT4E2M1, the type a is quantized to.");
+  } else {
+    OLA_ENFORCE(a->data_type == kFloat8E4M3FN || a->data_type == kFloat4E2M1 || a->data_type == kUint8, kMxmName,
+                ": a with a_scale must be FLOAT8E4M3FN, FLOAT4E2M1 or packed UINT8.");
+    OLA_ENFORCE(a_type == 0, kMxmName, ": a_type is for a 16-bit a; a is quantized already.");
+    OLA_ENFORCE(IsE8M0(a_scale->data_type), kMxmName, ": a_scale must be FLOAT8E8M0 or UINT8.");
+  }
+  OLA_ENFORCE(IsE8M0(b_scale->data_type), kMxmName, ": b_scale must be FLOAT8E8M0 or UINT8.");
+  const int64_t K = MxLength(b), N = b->dims[0];
+  OLA_ENFORCE(K % 32 == 0, kMxmName, ": K must be a multiple of the block size 32.");
+  OLA_ENFORCE((quantise ? as.back() : MxLength(a)) == K, kMxmName, ": a and b have different lengths of K.");
+  NeedShape(b_scale, {N, K / 32}, kMxmName, "b_scale");
+  Shape s = as;
+  s.back() = K / 32;
+  if (!quantise) NeedShape(a_scale, s, kMxmName, "a_scale");
+  int64_t M = 1;
+  for (size_t i = 0; i + 1 < as.size(); ++i) M *= as[i];
+  s.back() = N;
+  OLA_ENFORCE(Is16Bit(y->data_type) && (!quantise || y->data_type == a->data_type), kMxmName,
+              ": y must be FLOAT16 or BFLOAT16, and a's type where a has 16 bits.");
+  NeedShape(y, s, kMxmName, "y");
+  OLA_ENFORCE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31), kMxmName,
+              ": a dimension of 2^31 or more.");
+  if (M == 0 || N == 0) return ONNXL_AMD_OK;
+  Ctx();
+  const bool a4 = quantise ? a_type == kFloat4E2M1 : a->data_type != kFloat8E4M3FN;
+  const size_t codes = Scratch::Round((size_t)(a4 ? M * K / 2 : M * K)), scales = (size_t)(M * K / 32);
+  Staging st(stream, quantise ? codes + scales + 256 : 0, {a, quantise ? nullptr : a_scale, b, b_scale}, {y});
+  MxMatMulParams p{};
+  if (quantise) {
+    uint8_t *q = static_cast<uint8_t *>(st.Extra());
+    LaunchMxQuantize(MxQuantParams{st.In(a), q, q + codes, M, K, a->data_type, a4}, stream);
+    p.a = q;
+    p.a_scale = q + codes;
+  } else {
+    p.a = static_cast<const uint8_t *>(st.In(a));
+    p.a_scale = static_cast<const uint8_t *>(st.In(a_scale));
+  }
+  p.b = static_cast<const uint8_t *>(st.In(b));
+  p.b_scale = static_cast<const uint8_t *>(st.In(b_scale));
+  p.y = st.Out(y);
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.a_fp4 = a4;
+  p.y_bf16 = y->data_type == kBfloat16;
+  OLA_ENFORCE(reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0, kMxmName,
+              ": the codes must be 16-byte aligned.");
+  LaunchMxMatMul(p, stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+// The cache's tensors and the batch's index tensors.  The cache stays on the
+// device; index tensors in host memory are checked here, those on the device
+// by the kernels (decoder.hpp).
+KvCacheParams PlanKvCache(const char *op, const onnxl_amd_tensor *k_cache, const onnxl_amd_tensor *v_cache,
+                          const onnxl_amd_tensor *k_scale, const onnxl_amd_tensor *v_scale,
+                          const onnxl_amd_tensor *table, const onnxl_amd_tensor *start,
+                          const onnxl_amd_tensor *lengths, int64_t tokens) {
+  OLA_ENFORCE(!Absent(k_cache) && !Absent(v_cache) && !Absent(k_scale) && !Absent(v_scale) && !Absent(table) &&
+                  !Absent(start) && !Absent(lengths),
+              op, ": k_cache, v_cache, k_scale, v_scale, block_table, query_start and lengths are required.");
+  CheckDescriptor(k_cache, "k_cache");
+  CheckDescriptor(v_cache, "v_cache");
+  CheckDescriptor(k_scale, "k_scale");
+  CheckDescriptor(v_scale, "v_scale");
+  CheckDescriptor(table, "block_table");
+  CheckDescriptor(start, "query_start");
+  CheckDescriptor(lengths, "lengths");
+  OLA_ENFORCE(k_cache->data_type == kInt8 || k_cache->data_type == kFloat8E4M3FN, op,
+              ": the cache must be INT8 or FLOAT8E4M3FN.");
+  OLA_ENFORCE(v_cache->data_type == k_cache->data_type, op, ": k_cache and v_cache must have one type.");
+  OLA_ENFORCE(k_cache->rank == 4, op, ": k_cache must be [blocks, kv_heads, block_tokens, head_dim].");
+  const int64_t blocks = k_cache->dims[0], H = k_cache->dims[1], bt = k_cache->dims[2], D = k_cache->dims[3];
+  NeedShape(v_cache, {blocks, H, D, bt}, op, "v_cache ([blocks, kv_heads, head_dim, block_tokens])");
+  OLA_ENFORCE(bt == 16 || bt == 32 || bt == 64 || bt == 128 || bt == 256, op,
+              ": block_tokens must be 16, 32, 64, 128 or 256.");
+  OLA_ENFORCE(D > 0 && D <= 256 && D % 16 == 0, op, ": head_dim must be a multiple of 16 up to 256.");
+  OLA_ENFORCE(H > 0 && H < 65536, op, ": kv_heads must be from 1 to 65535.");
+  for (const onnxl_amd_tensor *t : {k_scale, v_scale}) {
+    OLA_ENFORCE(t->data_type == kFloat, op, ": k_scale and v_scale must be FLOAT.");
+    NeedShape(t, {blocks, H}, op, "k_scale or v_scale ([blocks, kv_heads])");
+  }
+  for (const onnxl_amd_tensor *t : {k_cache, v_cache, k_scale, v_scale})
+    OLA_ENFORCE(t->location == ONNXL_AMD_DEVICE, op, ": the cache and its scales must be device memory.");
+  OLA_ENFORCE(reinterpret_cast<uintptr_t>(k_cache->data) % 16 == 0 && reinterpret_cast<uintptr_t>(v_cache->data) % 16 == 0,
+              op, ": k_cache and v_cache must be 16-byte aligned.");
+  for (const onnxl_amd_tensor *t : {table, start, lengths})
+    OLA_ENFORCE(t->data_type == kInt32, op, ": block_table, query_start and lengths must be INT32.");
+  OLA_ENFORCE(table->rank == 2, op, ": block_table must be [batch, max_blocks].");
+  const int64_t B = table->dims[0], most = table->dims[1];
+  NeedShape(lengths, {B}, op, "lengths ([batch])");
+  NeedShape(start, {B + 1}, op, "query_start ([batch + 1])");
+  OLA_ENFORCE(B < 65536 && most * bt < (int64_t(1) << 31) && tokens < (int64_t(1) << 31), op,
+              ": more than 65535 sequences, or 2^31 tokens.");
+  const bool host = start->location == ONNXL_AMD_HOST && lengths->location == ONNXL_AMD_HOST;
+  if (host) {
+    const int32_t *s = static_cast<const int32_t *>(start->data), *l = static_cast<const int32_t *>(lengths->data);
+    for (int64_t b = 0; b < B; ++b) {
+      OLA_ENFORCE(s[b] >= 0 && s[b + 1] >= s[b] && s[b + 1] <= tokens, op,
+                  ": query_start must rise from 0 to the number of tokens.");
+      OLA_ENFORCE(l[b] >= s[b + 1] - s[b] && l[b] <= most * bt, op,
+                  ": lengths must cover the new tokens and fit the block table.");
+    }
+    if (table->location == ONNXL_AMD_HOST)
+      for (int64_t b = 0; b < B; ++b)
+        for (int64_t j = 0; s[b + 1] > s[b] && j < (l[b] + bt - 1) / bt; ++j) {
+          const int32_t blk = static_cast<const int32_t *>(table->data)[b * most + j];
+          OLA_ENFORCE(blk >= 0 && blk < blocks, op, ": a block of block_table is outside the cache.");
+        }
+  }
+  KvCacheParams c{};
+  c.k_cache = static_cast<uint8_t *>(k_cache->data);
+  c.v_cache = static_cast<uint8_t *>(v_cache->data);
+  c.k_scale = static_cast<float *>(k_scale->data);
+  c.v_scale = static_cast<float *>(v_scale->data);
+  c.num_blocks = blocks;
+  c.kv_heads = (int)H;
+  c.block_tokens = (int)bt;
+  c.block_shift = __builtin_ctz((unsigned)bt);
+  c.head_dim = (int)D;
+  c.batch = (int)B;
+  c.max_blocks = (int)most;
+  c.tokens = tokens;
+  c.fp8 = k_cache->data_type == kFloat8E4M3FN;
+  return c;
+}
+
+int KvCacheAppend(const onnxl_amd_tensor *k, const onnxl_amd_tensor *v, onnxl_amd_tensor *k_cache,
+                  onnxl_amd_tensor *v_cache, onnxl_amd_tensor *k_scale, onnxl_amd_tensor *v_scale,
+                  const onnxl_amd_tensor *table, const onnxl_amd_tensor *start, const onnxl_amd_tensor *lengths,
+                  hipStream_t stream) {
+  OLA_ENFORCE(!Absent(k) && !Absent(v), kKvaName, ": k and v are required.");
+  CheckDescriptor(k, "k");
+  CheckDescriptor(v, "v");
+  OLA_ENFORCE(k->rank == 3, kKvaName, ": k must be [tokens, kv_heads, head_dim].");
+  KvAppendParams p{};
+  p.c = PlanKvCache(kKvaName, k_cache, v_cache, k_scale, v_scale, table, start, lengths, k->dims[0]);
+  OLA_ENFORCE(Is16Bit(k->data_type) && v->data_type == k->data_type, kKvaName,
+              ": k and v must be FLOAT16 or BFLOAT16, both the same.");
+  const Shape want{k->dims[0], p.c.kv_heads, p.c.head_dim};
+  NeedShape(k, want, kKvaName, "k ([tokens, kv_heads, head_dim])");
+  NeedShape(v, want, kKvaName, "v ([tokens, kv_heads, head_dim])");
+  if (p.c.tokens == 0 || p.c.batch == 0) return ONNXL_AMD_OK;
+  Ctx();
+  Staging st(stream, 0, {k, v, table, start, lengths}, {});
+  p.c.table = static_cast<const int32_t *>(st.In(table));
+  p.c.start = static_cast<const int32_t *>(st.In(start));
+  p.c.lengths = static_cast<const int32_t *>(st.In(lengths));
+  p.k = st.In(k);
+  p.v = st.In(v);
+  p.bf16 = k->data_type == kBfloat16;
+  LaunchKvCacheAppend(p, stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+int KvCacheAttention(const onnxl_amd_tensor *q, const onnxl_amd_tensor *k_cache, const onnxl_amd_tensor *v_cache,
+                     const onnxl_amd_tensor *k_scale, const onnxl_amd_tensor *v_scale, const onnxl_amd_tensor *table,
+                     const onnxl_amd_tensor *start, const onnxl_amd_tensor *lengths, float scale, int64_t max_query,
+                     onnxl_amd_tensor *out, hipStream_t stream) {
+  OLA_ENFORCE(!Absent(q) && !Absent(out), kKvtName, ": q and out are required.");
+  CheckDescriptor(q, "q");
+  CheckDescriptor(out, "out");
+  OLA_ENFORCE(q->rank == 3, kKvtName, ": q must be [tokens, heads, head_dim].");
+  KvAttentionParams p{};
+  p.c = PlanKvCache(kKvtName, k_cache, v_cache, k_scale, v_scale, table, start, lengths, q->dims[0]);
+  OLA_ENFORCE(Is16Bit(q->data_type) && out->data_type == q->data_type, kKvtName,
+              ": q and out must be FLOAT16 or BFLOAT16, both the same.");
+  OLA_ENFORCE(q->dims[2] == p.c.head_dim, kKvtName, ": q and the cache have different head_dim.");
+  const int64_t heads = q->dims[1];
+  OLA_ENFORCE(heads > 0 && heads < 65536 && heads % p.c.kv_heads == 0, kKvtName,
+              ": heads must be a multiple of the cache's kv_heads, up to 65535.");
+  NeedShape(out, ShapeOf(*q), kKvtName, "out");
+  OLA_ENFORCE(std::isfinite(scale), kKvtName, ": scale must be finite.");
+  OLA_ENFORCE(max_query >= 0, kKvtName, ": max_query must not be negative.");
+  if (p.c.tokens == 0) return ONNXL_AMD_OK;
+  Ctx();
+  p.heads = (int)heads;
+  p.bf16 = q->data_type == kBfloat16;
+  p.scale = scale;
+  p.max_query = max_query;
+  Staging st(stream, KvAttentionScratchBytes(p), {q, table, start, lengths}, {out});
+  p.c.table = static_cast<const int32_t *>(st.In(table));
+  p.c.start = static_cast<const int32_t *>(st.In(start));
+  p.c.lengths = static_cast<const int32_t *>(st.In(lengths));
+  p.q = st.In(q);
+  p.out = st.Out(out);
+  LaunchKvCacheAttention(p, st.Extra(), stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
 // Validation runs before any device work, so argument errors are reported
 // even before onnxl_amd_init (the first device access then raises
 // NotInitialized).
@@ -3703,6 +4039,46 @@ int onnxl_amd_prepare_qqq(int64_t in_features, int64_t out_features, int64_t gro
   return Guard([&] {
     return PrepareQqq(in_features, out_features, group_size, bits, B, s_channel, s_group, dtype, weight, scale,
                       static_cast<hipStream_t>(stream));
+  });
+}
+
+int onnxl_amd_rms_norm_quantize(const onnxl_amd_tensor *x, const onnxl_amd_tensor *weight,
+                                const onnxl_amd_tensor *residual, float epsilon, int64_t block_size,
+                                onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale, onnxl_amd_tensor *sum, void *stream) {
+  return Guard([&] {
+    return RmsNormQuantize(x, weight, residual, epsilon, block_size, y, y_scale, sum,
+                           static_cast<hipStream_t>(stream));
+  });
+}
+
+int onnxl_amd_mx_quantize(const onnxl_amd_tensor *x, onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale, void *stream) {
+  return Guard([&] { return MxQuantize(x, y, y_scale, static_cast<hipStream_t>(stream)); });
+}
+
+int onnxl_amd_mx_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type,
+                        const onnxl_amd_tensor *b, const onnxl_amd_tensor *b_scale, onnxl_amd_tensor *y,
+                        void *stream) {
+  return Guard([&] { return MxMatMul(a, a_scale, a_type, b, b_scale, y, static_cast<hipStream_t>(stream)); });
+}
+
+int onnxl_amd_kv_cache_append(const onnxl_amd_tensor *k, const onnxl_amd_tensor *v, onnxl_amd_tensor *k_cache,
+                              onnxl_amd_tensor *v_cache, onnxl_amd_tensor *k_scale, onnxl_amd_tensor *v_scale,
+                              const onnxl_amd_tensor *block_table, const onnxl_amd_tensor *query_start,
+                              const onnxl_amd_tensor *lengths, void *stream) {
+  return Guard([&] {
+    return KvCacheAppend(k, v, k_cache, v_cache, k_scale, v_scale, block_table, query_start, lengths,
+                         static_cast<hipStream_t>(stream));
+  });
+}
+
+int onnxl_amd_kv_cache_attention(const onnxl_amd_tensor *q, const onnxl_amd_tensor *k_cache,
+                                 const onnxl_amd_tensor *v_cache, const onnxl_amd_tensor *k_scale,
+                                 const onnxl_amd_tensor *v_scale, const onnxl_amd_tensor *block_table,
+                                 const onnxl_amd_tensor *query_start, const onnxl_amd_tensor *lengths, float scale,
+                                 int64_t max_query, onnxl_amd_tensor *out, void *stream) {
+  return Guard([&] {
+    return KvCacheAttention(q, k_cache, v_cache, k_scale, v_scale, block_table, query_start, lengths, scale,
+                            max_query, out, static_cast<hipStream_t>(stream));
   });
 }
 
