@@ -718,8 +718,8 @@ int onnxl_amd_mx_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_sca
  *   lengths     INT32 [batch]: its tokens in the cache, the new ones included.
  * No two sequences may append into one block.  Index tensors in host memory are
  * checked by the call; with device-resident ones a sequence whose numbers do
- * not fit (or that names a block outside the cache) is not appended, and its
- * rows of the attention are NaN.
+ * not fit is not appended and its rows of the attention are NaN; new tokens of
+ * a block outside the cache are dropped, and rows that see one are NaN.
  *
  * Append: k, v FLOAT16 or BFLOAT16 [tokens, kv_heads, head_dim].  A block's
  * scale becomes the larger of that of the tokens it keeps (none: 0) and

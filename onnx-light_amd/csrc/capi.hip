@@ -3407,6 +3407,7 @@ KvCacheParams PlanKvCache(const char *op, const onnxl_amd_tensor *k_cache, const
               ": block_tokens must be 16, 32, 64, 128 or 256.");
   OLA_ENFORCE(D > 0 && D <= 256 && D % 16 == 0, op, ": head_dim must be a multiple of 16 up to 256.");
   OLA_ENFORCE(H > 0 && H < 65536, op, ": kv_heads must be from 1 to 65535.");
+  OLA_ENFORCE(blocks > 0 || tokens == 0, op, ": the cache has no blocks.");
   for (const onnxl_amd_tensor *t : {k_scale, v_scale}) {
     OLA_ENFORCE(t->data_type == kFloat, op, ": k_scale and v_scale must be FLOAT.");
     NeedShape(t, {blocks, H}, op, "k_scale or v_scale ([blocks, kv_heads])");

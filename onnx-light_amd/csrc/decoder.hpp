@@ -73,8 +73,9 @@ void LaunchMxMatMul(const MxMatMulParams &p, hipStream_t stream);
 //   new token of every sequence), lengths INT32 [batch] (tokens in the cache
 //   with the new ones).
 // A sequence whose numbers do not fit its tensors (new tokens < 0 or beyond
-// its length, a length beyond the table, rows past the last token), or that
-// names a block outside the cache, is not appended and its attention is NaN.
+// its length, a length beyond the table, rows past the last token) is not
+// appended and its attention is NaN; new tokens of a block outside the cache
+// are dropped, and rows that see one are NaN.
 
 struct KvCacheParams {
   uint8_t *k_cache, *v_cache;

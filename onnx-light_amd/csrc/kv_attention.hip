@@ -1,5 +1,30 @@
 // Causal attention of the newest tokens of every sequence over the paged 8-bit
 // cache.
+//
+// For one sequence and kv head the rows of a matrix product are the (new
+// token, head of the group) pairs, row = token * group + head, so that the
+// heads that share keys and values share every byte read.  A tile is 64 tokens
+// of the cache:
+//   S^T = K Q^T   (16 x 16 x 32 MFMA, A = 16 tokens of K, B = 16 rows of Q)
+//   P   = 2^(S - m)
+//   O^T += V^T P  (A = 16 dimensions of V^T, B = P)
+// Result lane 16 g + c of the first product holds 4 tokens of row c.  The token
+// in A's row r of the 16-token operand t is 16 (r / 4) + 4 t + r % 4, so over
+// the four operands lane group g gets the 16 consecutive tokens from 16 g, which
+// is what the second product's B operand wants of it (P never leaves the
+// registers) and, in the token-contiguous V cache, one 16-byte load per
+// dimension (no transposition).  Those 16 tokens lie in one cache block, so
+// both scales are one number per lane and tile.
+//
+// Codes become fp16 exactly (|int8| <= 128, E4M3 is a subset).  Q becomes fp16
+// after a power of two per row has brought its largest value to [1, 2): exact
+// but for what is below 2^-14 of that largest.  Sums, statistics and O are
+// fp32; P is rounded to fp16.  O is kept relative to its own running maximum of
+// S + log2(v scale), not of S, so that P times the block's v scale fills the
+// fp16 range whatever the scales are; the softmax sum is relative to m and takes
+// the unrounded P.
+#include <cfloat>
+
 #include "common.hpp"
 #include "decoder.hpp"
 #include "device_codecs.hpp"
@@ -7,64 +32,406 @@
 namespace onnxl_amd {
 namespace {
 
-__device__ __forceinline__ float CodeValue(uint8_t c, int fp8) { return fp8 ? Fp8E4M3ToF32(c) : (float)(int8_t)c; }
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
-// One wave per (token, head): lane l holds dimensions l, l + 64, ..; one pass
-// over the tokens with the running maximum m and sum s of the softmax.
-__global__ __launch_bounds__(64) void KvAttentionKernel(const KvAttentionParams p) {
+constexpr int kThreads = 256, kWaves = 4, kTile = 64;
+constexpr float kNone = -1e30f;  // below every score: the maximum of no token
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Eight codes (two dwords) as fp16, exact.
+template <bool FP8> __device__ __forceinline__ v8h Widen(int lo, int hi) {
+  v8h r;
+  v2h *h = reinterpret_cast<v2h *>(&r);
+  if constexpr (FP8) {
+    h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+    h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+    h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+    h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  } else {
+    // the byte c + 128 under the exponent of 1024 is 1024 + 128 + c
+    const v2h off = {(_Float16)-1152.f, (_Float16)-1152.f};
+    const unsigned a = (unsigned)lo ^ 0x80808080u, b = (unsigned)hi ^ 0x80808080u, e = 0x64646464u;
+    h[0] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(a, e, 0x00050004u)) + off;
+    h[1] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(a, e, 0x00070006u)) + off;
+    h[2] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(b, e, 0x00050004u)) + off;
+    h[3] = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(b, e, 0x00070006u)) + off;
+  }
+  return r;
+}
+
+__device__ __forceinline__ float QValue(const void *q, int64_t i, int bf16) {
+  const uint16_t u = static_cast<const uint16_t *>(q)[i];
+  return bf16 ? Bf16ToF32(u) : F16ToF32(u);
+}
+
+__device__ __forceinline__ uint2 Pack4(v4f v, int bf16) {
+  uint16_t h[4];
+  for (int i = 0; i < 4; ++i) h[i] = bf16 ? F32ToBf16(v[i]) : F32ToF16(v[i]);
+  return make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
+}
+
+// The larger over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float GroupMax(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float GroupSum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (decoding): the reading of the cache is the cost.  The tiles of all
+// (sequence, kv head, 16-row tile) jobs form one line of units, and every
+// workgroup takes an equal piece of it, whatever the lengths are; its waves
+// take the tiles of a job in turn and join in LDS.  A job inside the piece is
+// written out; the parts of a job that crosses pieces go to the workspace, at
+// most two per workgroup (the first and the last of its piece), and a second
+// kernel joins them in a fixed order.
+
+struct Line {        // units before every thread's share of the sequences
+  int64_t upto[kThreads];
+};
+
+struct Job {
+  int b, n, len, head, row0;  // sequence, its new tokens and length, kv head, first row
+  int tiles;                  // units of the job
+  int64_t first;              // its first unit on the line
+};
+
+struct Plan {
+  KvAttentionParams a;
+  int group;
+  int rows_max;     // sequences with more rows (new tokens * group) are not for this kernel
+  int fill;         // NaN for the rows of sequences that do not fit
+  float *part;      // parts: [workgroup][2][HD / 16][64] float4
+  float *stat;      // [workgroup][2][3][16]: m, the maximum of O, the sum
+};
+
+// New tokens of sequence b that this kernel has (0: none).
+__device__ __forceinline__ int RowsOf(const Plan &p, int b) {
+  const int n = KvNewTokens(p.a.c, b);
+  return n > 0 && (int64_t)n * p.group <= p.rows_max ? n : 0;
+}
+__device__ __forceinline__ int64_t UnitsOf(const Plan &p, int b) {
+  const int n = RowsOf(p, b);
+  if (n == 0) return 0;
+  return (int64_t)p.a.c.kv_heads * ((n * p.group + 15) / 16) * ((p.a.c.lengths[b] + kTile - 1) / kTile);
+}
+
+__device__ __forceinline__ int Uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t Uniform(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)Uniform((int)(v >> 32)) << 32 | (uint32_t)Uniform((int)v));
+}
+
+// Fills `line` and returns the number of units.
+__device__ __forceinline__ int64_t MakeLine(const Plan &p, Line &line) {
+  const int B = p.a.c.batch, share = (B + kThreads - 1) / kThreads, tid = threadIdx.x;
+  int64_t mine = 0;
+  for (int b = tid * share; b < min(B, (tid + 1) * share); ++b) mine += UnitsOf(p, b);
+  int64_t sum = mine;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t v = __shfl_up(sum, o);
+    if (tid % 64 >= o) sum += v;
+  }
+  line.upto[tid] = sum;
+  __syncthreads();
+  int64_t before = 0;
+  for (int w = 0; w < tid / 64; ++w) before += line.upto[64 * w + 63];
+  __syncthreads();
+  line.upto[tid] = sum + before;
+  __syncthreads();
+  return Uniform(line.upto[kThreads - 1]);
+}
+
+// The job of unit u, the same in every lane.
+__device__ __forceinline__ Job FindJob(const Plan &p, const Line &line, int64_t u) {
+  const int share = (p.a.c.batch + kThreads - 1) / kThreads;
+  int lo = 0, hi = kThreads - 1;
+  while (lo < hi) {  // the first thread whose share ends past u
+    const int mid = (lo + hi) / 2;
+    if (line.upto[mid] > u) hi = mid; else lo = mid + 1;
+  }
+  int64_t at = lo ? line.upto[lo - 1] : 0;
+  int b = lo * share;
+  for (;; ++b) {
+    const int64_t n = UnitsOf(p, b);
+    if (u < at + n) break;
+    at += n;
+  }
+  Job j;
+  j.b = b = Uniform(b);
+  j.n = Uniform(RowsOf(p, b));
+  j.len = Uniform(p.a.c.lengths[b]);
+  j.tiles = (j.len + kTile - 1) / kTile;
+  const int row_tiles = (j.n * p.group + 15) / 16;
+  const int64_t k = Uniform((u - at) / j.tiles);
+  j.head = (int)(k / row_tiles);
+  j.row0 = (int)(k % row_tiles) * 16;
+  j.first = Uniform(at) + k * j.tiles;
+  return j;
+}
+
+// Units of one workgroup: equal pieces, of at least one tile per wave.
+__device__ __forceinline__ int64_t PieceOf(int64_t units) {
+  const int64_t piece = (units + gridDim.x - 1) / gridDim.x;
+  return piece < kWaves ? kWaves : piece;
+}
+
+// Writes O * 2^(mo - m) / sum of the rows in lanes c < rows.
+__device__ __forceinline__ void StoreRows(const Plan &p, const Job &j, int t, v4f o, float m, float mo, float sum) {
+  const int c = threadIdx.x % 16, g = threadIdx.x % 64 / 16, row = j.row0 + c, d = 16 * t + 4 * g;
+  if (row >= j.n * p.group || d >= p.a.c.head_dim) return;
+  const float f = exp2f(mo - m) / sum;
+  const int64_t token = p.a.c.start[j.b] + row / p.group;
+  const int head = j.head * p.group + row % p.group;
+  uint16_t *out = static_cast<uint16_t *>(p.a.out) + (token * p.a.heads + head) * p.a.c.head_dim + d;
+  *reinterpret_cast<uint2 *>(out) = Pack4(o * f, p.a.bf16);
+}
+
+template <int HD, bool FP8, bool EXACT> __global__ __launch_bounds__(kThreads, 2) void KvDecodeKernel(const Plan p) {
+  constexpr int DT = HD / 16, CH = HD / 64;  // dimension tiles, 64-byte chunks of a key
+  __shared__ Line line;
+  __shared__ v4f so[kWaves][DT][64];
+  __shared__ float sm[kWaves][3][16];
+  const KvCacheParams &cp = p.a.c;
+  const int tid = threadIdx.x, lane = tid % 64, c = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int D = EXACT ? HD : cp.head_dim, H = cp.kv_heads, bt = cp.block_tokens;
+  if (p.fill) {
+    for (int b = blockIdx.x; b < cp.batch; b += gridDim.x) {
+      if (KvNewTokens(cp, b) >= 0) continue;
+      const int64_t lo = cp.start[b] < 0 ? 0 : cp.start[b], hi = cp.start[b + 1] < cp.tokens ? cp.start[b + 1] : cp.tokens;
+      const int64_t wide = (int64_t)p.a.heads * D;
+      for (int64_t i = lo * wide + tid; i < hi * wide; i += kThreads)
+        static_cast<uint16_t *>(p.a.out)[i] = p.a.bf16 ? 0x7fc0 : 0x7e00;
+    }
+  }
+  const int64_t units = MakeLine(p, line), piece = PieceOf(units);
+  int64_t u = (int64_t)blockIdx.x * piece;
+  const int64_t end = u + piece < units ? u + piece : units;
+  for (int part = 0; u < end; part = 1) {
+    const Job j = FindJob(p, line, u);
+    const int t0 = (int)(u - j.first), t1 = (int)(end - j.first < j.tiles ? end - j.first : j.tiles);
+    // Q of row c, 8 values per 32 dimensions: lane group g has the dimensions
+    // 64 q + 16 g + 8 s ..
+    const int row = j.row0 + c;
+    const bool live = row < j.n * p.group;
+    const int64_t token = cp.start[j.b] + (live ? row / p.group : 0);
+    const int64_t qat = (token * p.a.heads + j.head * p.group + (live ? row % p.group : 0)) * D;
+    const int last = j.len - j.n + (live ? row / p.group : 0);  // the last token the row sees
+    v8h q[CH][2];
+    float top = 0.f;
+    for (int i = 0; i < CH * 16; ++i) {
+      const int d = 64 * (i / 16) + 16 * g + i % 16;
+      if (live && (EXACT || d < D)) top = fmaxf(top, fabsf(QValue(p.a.q, qat + d, p.a.bf16)));
+    }
+    top = GroupMax(top);
+    const int e = top > 0.f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+    for (int i = 0; i < CH * 16; ++i) {
+      const int d = 64 * (i / 16) + 16 * g + i % 16;
+      const float v = live && (EXACT || d < D) ? QValue(p.a.q, qat + d, p.a.bf16) : 0.f;
+      q[i / 16][i % 16 / 8][i % 8] = (_Float16)__builtin_amdgcn_ldexpf(v, -e);
+    }
+    const float qf = __builtin_amdgcn_ldexpf(p.a.scale * kLog2e, e);
+
+    v4f o[DT];
+    for (int t = 0; t < DT; ++t) o[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    float m = kNone, mo = kNone, sum = 0.f;
+    const int32_t *table = cp.table + (int64_t)j.b * cp.max_blocks;
+    // Block of the 16 tokens from `at`, those past the end in the last block;
+    // -1 for one outside the cache, whose tokens get a NaN score.
+    auto block_of = [&](int at) {
+      const int blk = table[(at < j.len ? at : j.len - 1) >> cp.block_shift];
+      return blk >= 0 && blk < cp.num_blocks ? blk : -1;
+    };
+    for (int t = t0 + wave; t < t1; t += kWaves) {
+      const int base = t * kTile;
+      const int kt = base + 16 * (c / 4), vt = base + 16 * g;
+      const int kb = block_of(kt), vb = block_of(vt);
+      const uint8_t *kp = cp.k_cache + (((int64_t)(kb < 0 ? 0 : kb) * H + j.head) * bt + (kt & (bt - 1)) + c % 4) * D + 16 * g;
+      const uint8_t *vp = cp.v_cache + (((int64_t)(vb < 0 ? 0 : vb) * H + j.head) * D + c) * bt + (vt & (bt - 1));
+      v4i kr[4][CH], vr[DT];
+      for (int s = 0; s < 4; ++s)
+        for (int h = 0; h < CH; ++h) {
+          if (EXACT || 64 * h + 16 * g < D)
+            kr[s][h] = *reinterpret_cast<const v4i *>(kp + 4 * s * D + 64 * h);
+          else
+            kr[s][h] = v4i{0, 0, 0, 0};
+        }
+      for (int d = 0; d < DT; ++d) {
+        if (EXACT || 16 * d < D)
+          vr[d] = *reinterpret_cast<const v4i *>(vp + (int64_t)16 * d * bt);
+        else
+          vr[d] = v4i{0, 0, 0, 0};
+      }
+      const float ks = vb < 0 ? __builtin_nanf("") : cp.k_scale[(int64_t)vb * H + j.head];
+      const float vs = vb < 0 ? 0.f : cp.v_scale[(int64_t)vb * H + j.head];
+      v4f s[4];
+      for (int i = 0; i < 4; ++i) {
+        s[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < CH; ++h) {
+          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(kr[i][h][0], kr[i][h][1]), q[h][0], s[i], 0, 0, 0);
+          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(kr[i][h][2], kr[i][h][3]), q[h][1], s[i], 0, 0, 0);
+        }
+        s[i] *= ks * qf;
+      }
+      // tokens that the row does not see, in the tiles that have any
+      const bool edge = base + kTile > j.len - j.n + 1;
+      if (edge)
+        for (int i = 0; i < 16; ++i)
+          if (vt + i > last) s[i / 4][i % 4] = -__builtin_huge_valf();
+      float lm = s[0][0];
+      for (int i = 1; i < 16; ++i) lm = fmaxf(lm, s[i / 4][i % 4]);
+      const float lv = fmaxf(__builtin_amdgcn_logf(vs), -126.f);
+      const float mn = fmaxf(m, GroupMax(lm)), mon = fmaxf(mo, GroupMax(lm + lv));
+      const float keep = __builtin_amdgcn_exp2f(m - mn), keep_o = __builtin_amdgcn_exp2f(mo - mon);
+      // w * f <= 1, so f overflows only where every w is 0; a NaN scale stays
+      float f = vs * __builtin_amdgcn_exp2f(mn - mon);
+      f = f > FLT_MAX ? FLT_MAX : f;
+      m = mn;
+      mo = mon;
+      float ps = 0.f;
+      v8h pr[2];
+      for (int i = 0; i < 16; ++i) {
+        const float w = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - mn);
+        ps += w;
+        float wv = w * f;
+        if (edge && vt + i > last) wv = 0.f;
+        pr[i / 8][i % 8] = (_Float16)wv;
+      }
+      sum = sum * keep + ps;
+      if (edge) {
+        // what the cache holds past the end may be any code, NaN among them
+        const int left = j.len - vt;  // tokens of this lane that are there
+        for (int w = 0; w < 4; ++w) {
+          const int n = left - 4 * w;
+          const unsigned mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+          for (int d = 0; d < DT; ++d) vr[d][w] &= (int)mask;
+        }
+      }
+      for (int d = 0; d < DT; ++d) {
+        o[d] *= keep_o;
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(vr[d][0], vr[d][1]), pr[0], o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(vr[d][2], vr[d][3]), pr[1], o[d], 0, 0, 0);
+      }
+    }
+    sum = GroupSum(sum);
+
+    // the waves' parts become one
+    __syncthreads();
+    for (int d = 0; d < DT; ++d) so[wave][d][lane] = o[d];
+    if (g == 0) {
+      sm[wave][0][c] = m;
+      sm[wave][1][c] = mo;
+      sm[wave][2][c] = sum;
+    }
+    __syncthreads();
+    m = mo = kNone;
+    for (int w = 0; w < kWaves; ++w) {
+      m = fmaxf(m, sm[w][0][c]);
+      mo = fmaxf(mo, sm[w][1][c]);
+    }
+    sum = 0.f;
+    for (int w = 0; w < kWaves; ++w) sum += sm[w][2][c] * exp2f(sm[w][0][c] - m);
+    const bool whole = t0 == 0 && t1 == j.tiles;
+    const int64_t slot = (int64_t)blockIdx.x * 2 + part;
+    for (int d = wave; d < DT; d += kWaves) {
+      v4f a = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < kWaves; ++w) a += so[w][d][lane] * exp2f(sm[w][1][c] - mo);
+      if (whole)
+        StoreRows(p, j, d, a, m, mo, sum);
+      else if (live)
+        reinterpret_cast<v4f *>(p.part)[(slot * DT + d) * 64 + lane] = a;
+    }
+    if (!whole && wave == 0 && g == 0) {
+      p.stat[(slot * 3 + 0) * 16 + c] = m;
+      p.stat[(slot * 3 + 1) * 16 + c] = mo;
+      p.stat[(slot * 3 + 2) * 16 + c] = sum;
+    }
+    u = j.first + t1;
+  }
+}
+
+// Joins the parts of the job that starts in piece blockIdx.x and goes on in the
+// next ones: one wave per 16 dimensions.
+template <int HD> __global__ __launch_bounds__(kThreads) void KvJoinKernel(const Plan p) {
+  constexpr int DT = HD / 16;
+  __shared__ Line line;
+  const int lane = threadIdx.x % 64, c = lane % 16;
+  const int64_t units = MakeLine(p, line), piece = PieceOf(units);
+  const int64_t end = ((int64_t)blockIdx.x + 1) * piece;
+  if (end >= units) return;
+  const Job j = FindJob(p, line, end - 1);
+  if (j.first < end - piece || j.first + j.tiles <= end) return;
+  const int64_t w1 = (j.first + j.tiles - 1) / piece;
+  auto slot = [&](int64_t w) { return w * 2 + (w == (int64_t)blockIdx.x && j.first > end - piece ? 1 : 0); };
+  float m = kNone, mo = kNone, sum = 0.f;
+  for (int64_t w = blockIdx.x; w <= w1; ++w) {
+    m = fmaxf(m, p.stat[(slot(w) * 3 + 0) * 16 + c]);
+    mo = fmaxf(mo, p.stat[(slot(w) * 3 + 1) * 16 + c]);
+  }
+  const bool live = j.row0 + c < j.n * p.group;
+  const int d = blockIdx.y * kWaves + threadIdx.x / 64;
+  if (d >= DT) return;
+  v4f a = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int64_t w = blockIdx.x; w <= w1; ++w) {
+    sum += p.stat[(slot(w) * 3 + 2) * 16 + c] * exp2f(p.stat[(slot(w) * 3 + 0) * 16 + c] - m);
+    if (live)
+      a += reinterpret_cast<const v4f *>(p.part)[(slot(w) * DT + d) * 64 + lane] *
+           exp2f(p.stat[(slot(w) * 3 + 1) * 16 + c] - mo);
+  }
+  StoreRows(p, j, d, a, m, mo, sum);
+}
+
+int HeadTile(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+// Two workgroups per CU hold eight waves, enough loads in flight to fill the
+// memory; never more than there can be pieces of one tile per wave.
+int64_t DecodeGrid(const KvAttentionParams &p) {
   const KvCacheParams &c = p.c;
-  const int64_t row = blockIdx.x;
-  const int head = blockIdx.y, lane = threadIdx.x, D = c.head_dim, bt = c.block_tokens;
-  const int kvh = head / (p.heads / c.kv_heads);
-  int b = 0;
-  while (b < c.batch && !(c.start[b] <= row && row < c.start[b + 1])) ++b;
-  const int n = b < c.batch ? KvNewTokens(c, b) : -1;
-  const int64_t at = (row * p.heads + head) * D;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -__builtin_huge_valf(), s = 0.f;
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    const uint16_t u = d < D ? static_cast<const uint16_t *>(p.q)[at + d] : 0;
-    q[i] = p.bf16 ? Bf16ToF32(u) : F16ToF32(u);
-  }
-  bool good = n > 0;
-  const int64_t last = good ? (int64_t)c.lengths[b] - n + (row - c.start[b]) : -1;
-  for (int64_t t = 0; t <= last && good; ++t) {
-    const int64_t blk = c.table[(int64_t)b * c.max_blocks + t / bt];
-    if (blk < 0 || blk >= c.num_blocks) {
-      good = false;
-      break;
-    }
-    const int64_t base = (blk * c.kv_heads + kvh) * (int64_t)bt * D;
-    const int u = (int)(t % bt);
-    float dot = 0.f;
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < D) dot += q[i] * CodeValue(c.k_cache[base + (int64_t)u * D + d], c.fp8);
-    }
-    for (int w = 32; w > 0; w >>= 1) dot += __shfl_xor(dot, w);
-    const float z = dot * c.k_scale[blk * c.kv_heads + kvh] * p.scale, mn = fmaxf(m, z);
-    const float keep = __expf(m - mn), e = __expf(z - mn), ev = e * c.v_scale[blk * c.kv_heads + kvh];
-    s = s * keep + e;
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < D) o[i] = o[i] * keep + ev * CodeValue(c.v_cache[base + (int64_t)d * bt + u], c.fp8);
-    }
-    m = mn;
-  }
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    const float v = good ? o[i] / s : __builtin_nanf("");
-    if (d < D) static_cast<uint16_t *>(p.out)[at + d] = p.bf16 ? F32ToBf16(v) : F32ToF16(v);
-  }
+  const int64_t group = p.heads / c.kv_heads, jobs = (c.tokens * group / 16 + c.batch) * c.kv_heads;
+  const int64_t tiles = ((int64_t)c.max_blocks * c.block_tokens + kTile - 1) / kTile;
+  const int64_t pieces = (jobs * tiles + kWaves - 1) / kWaves;
+  return std::max<int64_t>(1, std::min<int64_t>(pieces, 2 * Ctx().num_cus));
+}
+
+template <int HD> void LaunchDecode(const Plan &p, int64_t grid, hipStream_t s) {
+  const dim3 g((unsigned)grid);
+  const bool exact = p.a.c.head_dim == HD;
+  if (p.a.c.fp8)
+    exact ? KvDecodeKernel<HD, true, true><<<g, kThreads, 0, s>>>(p) : KvDecodeKernel<HD, true, false><<<g, kThreads, 0, s>>>(p);
+  else
+    exact ? KvDecodeKernel<HD, false, true><<<g, kThreads, 0, s>>>(p) : KvDecodeKernel<HD, false, false><<<g, kThreads, 0, s>>>(p);
+  if (grid > 1) KvJoinKernel<HD><<<dim3((unsigned)grid, (HD / 16 + kWaves - 1) / kWaves), kThreads, 0, s>>>(p);
 }
 
 }  // namespace
 
-size_t KvAttentionScratchBytes(const KvAttentionParams &) { return 0; }
+size_t KvAttentionScratchBytes(const KvAttentionParams &p) {
+  const size_t slots = (size_t)DecodeGrid(p) * 2;
+  return Scratch::Round(slots * 16 * HeadTile(p.c.head_dim) * sizeof(float)) + slots * 48 * sizeof(float);
+}
 
-void LaunchKvCacheAttention(const KvAttentionParams &p, void *, hipStream_t stream) {
-  if (p.c.tokens == 0) return;
-  KvAttentionKernel<<<dim3((unsigned)p.c.tokens, (unsigned)p.heads), 64, 0, stream>>>(p);
+void LaunchKvCacheAttention(const KvAttentionParams &a, void *scratch, hipStream_t stream) {
+  const int64_t grid = DecodeGrid(a);
+  const int hd = HeadTile(a.c.head_dim);
+  Plan p{};
+  p.a = a;
+  p.group = a.heads / a.c.kv_heads;
+  p.rows_max = 0x7fffffff;
+  p.fill = 1;
+  p.part = static_cast<float *>(scratch);
+  p.stat = reinterpret_cast<float *>(static_cast<char *>(scratch) + Scratch::Round((size_t)grid * 2 * 16 * hd * sizeof(float)));
+  if (hd == 64)
+    LaunchDecode<64>(p, grid, stream);
+  else if (hd == 128)
+    LaunchDecode<128>(p, grid, stream);
+  else
+    LaunchDecode<256>(p, grid, stream);
 }
 
 }  // namespace onnxl_amd
