@@ -3422,8 +3422,8 @@ KvCacheParams PlanKvCache(const char *op, const onnxl_amd_tensor *k_cache, const
   const int64_t B = table->dims[0], most = table->dims[1];
   NeedShape(lengths, {B}, op, "lengths ([batch])");
   NeedShape(start, {B + 1}, op, "query_start ([batch + 1])");
-  OLA_ENFORCE(B < 65536 && most * bt < (int64_t(1) << 31) && tokens < (int64_t(1) << 31), op,
-              ": more than 65535 sequences, or 2^31 tokens.");
+  OLA_ENFORCE(B < 65536 && most * bt <= (int64_t(1) << 31) - 4096 && tokens < (int64_t(1) << 31), op,
+              ": more than 65535 sequences, or about 2^31 tokens.");
   const bool host = start->location == ONNXL_AMD_HOST && lengths->location == ONNXL_AMD_HOST;
   if (host) {
     const int32_t *s = static_cast<const int32_t *>(start->data), *l = static_cast<const int32_t *>(lengths->data);

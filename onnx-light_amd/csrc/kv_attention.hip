@@ -24,6 +24,7 @@
 // fp16 range whatever the scales are; the softmax sum is relative to m and takes
 // the unrounded P.
 #include <cfloat>
+#include <type_traits>
 
 #include "common.hpp"
 #include "decoder.hpp"
@@ -33,6 +34,7 @@ namespace onnxl_amd {
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -62,11 +64,6 @@ template <bool FP8> __device__ __forceinline__ v8h Widen(int lo, int hi) {
   return r;
 }
 
-__device__ __forceinline__ float QValue(const void *q, int64_t i, int bf16) {
-  const uint16_t u = static_cast<const uint16_t *>(q)[i];
-  return bf16 ? Bf16ToF32(u) : F16ToF32(u);
-}
-
 __device__ __forceinline__ uint2 Pack4(v4f v, int bf16) {
   uint16_t h[4];
   for (int i = 0; i < 4; ++i) h[i] = bf16 ? F32ToBf16(v[i]) : F32ToF16(v[i]);
@@ -89,8 +86,9 @@ __device__ __forceinline__ float GroupSum(float v) {
 // workgroup takes an equal piece of it, whatever the lengths are; its waves
 // take the tiles of a job in turn and join in LDS.  A job inside the piece is
 // written out; the parts of a job that crosses pieces go to the workspace, at
-// most two per workgroup (the first and the last of its piece), and a second
-// kernel joins them in a fixed order.
+// most two per workgroup (the first and the last of its piece), and the
+// workgroup that writes the last of them joins them, in the order of the pieces
+// whoever that is.
 
 struct Line {        // units before every thread's share of the sequences
   int64_t upto[kThreads];
@@ -109,6 +107,7 @@ struct Plan {
   int fill;         // NaN for the rows of sequences that do not fit
   float *part;      // parts: [workgroup][2][HD / 16][64] float4
   float *stat;      // [workgroup][2][3][16]: m, the maximum of O, the sum
+  unsigned *done;   // [workgroup] parts written of the job that starts last in its piece; zero between launches
 };
 
 // New tokens of sequence b that this kernel has (0: none).
@@ -189,23 +188,171 @@ __device__ __forceinline__ void StoreRows(const Plan &p, const Job &j, int t, v4
   const int64_t token = p.a.c.start[j.b] + row / p.group;
   const int head = j.head * p.group + row % p.group;
   uint16_t *out = static_cast<uint16_t *>(p.a.out) + (token * p.a.heads + head) * p.a.c.head_dim + d;
-  *reinterpret_cast<uint2 *>(out) = Pack4(o * f, p.a.bf16);
+  const uint2 h = Pack4(o * f, p.a.bf16);
+  __builtin_memcpy(out, &h, 8);
 }
 
-template <int HD, bool FP8, bool EXACT> __global__ __launch_bounds__(kThreads, 2) void KvDecodeKernel(const Plan p) {
+// 16 bytes from any address.
+__device__ __forceinline__ v4i Load16(const void *p) {
+  v4i v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// Q of one row as the first product's operand: lane group g holds the
+// dimensions 64 h + 16 g + 8 s + (0..7) at q[h][s], scaled by 2^-exponent.
+template <int CH, bool EXACT> struct QRow {
+  v4i raw[CH][2];
+  v8h q[CH][2];
+  int exponent;
+
+  __device__ __forceinline__ void Load(const KvAttentionParams &p, int64_t at, bool live, int g) {
+    for (int h = 0; h < CH; ++h)
+      for (int s = 0; s < 2; ++s) {
+        const int d = 64 * h + 16 * g + 8 * s;
+        raw[h][s] = live && (EXACT || d < p.c.head_dim) ? Load16(static_cast<const uint16_t *>(p.q) + at + d) : v4i{0, 0, 0, 0};
+      }
+  }
+  __device__ __forceinline__ void Scale(int bf16) {
+    float v[CH][2][8], top = 0.f;
+    for (int h = 0; h < CH; ++h)
+      for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < 8; ++i) {
+          const int w = raw[h][s][i / 2];
+          const uint16_t u = (uint16_t)((unsigned)w >> (16 * (i % 2)));
+          v[h][s][i] = bf16 ? Bf16ToF32(u) : F16ToF32(u);
+          top = fmaxf(top, fabsf(v[h][s][i]));
+        }
+    top = GroupMax(top);
+    exponent = top > 0.f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+    for (int h = 0; h < CH; ++h)
+      for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < 8; ++i) q[h][s][i] = (_Float16)__builtin_amdgcn_ldexpf(v[h][s][i], -exponent);
+  }
+};
+
+// One tile's codes and scales of a wave, loaded ahead of their use, and the
+// cache blocks of the tile after it.
+template <int HD, bool EXACT> struct TileLoad {
+  static constexpr int DT = HD / 16, CH = HD / 64;
+  int kb, vb;  // blocks of the tile to load next
+  const uint8_t *vp;
+  v4i k[4][CH], v[DT];
+  float ks, vs;
+
+  // Tokens past the end are looked up as the last there is.
+  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const Job &j, int t, int c, int g) {
+    const int32_t *table = p.table + (int64_t)j.b * p.max_blocks;
+    kb = table[min(t * kTile + 16 * (c / 4), j.len - 1) >> p.block_shift];
+    vb = table[min(t * kTile + 16 * g, j.len - 1) >> p.block_shift];
+  }
+  // Keys and scales of tile t.  A block outside the cache reads block 0 and gets
+  // a NaN score.
+  __device__ __forceinline__ void LoadK(const KvCacheParams &p, const Job &j, int t, int c, int g) {
+    const int kt = t * kTile + 16 * (c / 4), vt = t * kTile + 16 * g, D = EXACT ? HD : p.head_dim, bt = p.block_tokens;
+    const bool bad = vb < 0 || vb >= p.num_blocks;
+    const int64_t k_at = (int64_t)(kb >= 0 && kb < p.num_blocks ? kb : 0) * p.kv_heads + j.head;
+    const int64_t v_at = (int64_t)(bad ? 0 : vb) * p.kv_heads + j.head;
+    const uint8_t *kp = p.k_cache + (k_at * bt + (kt & (bt - 1)) + c % 4) * D + 16 * g;
+    vp = p.v_cache + (v_at * D + c) * bt + (vt & (bt - 1));
+    for (int s = 0; s < 4; ++s)
+      for (int h = 0; h < CH; ++h)
+        k[s][h] = EXACT || 64 * h + 16 * g < D ? *reinterpret_cast<const v4i *>(kp + 4 * s * D + 64 * h) : v4i{0, 0, 0, 0};
+    ks = p.k_scale[v_at];
+    ks = bad ? __builtin_nanf("") : ks;
+    vs = p.v_scale[v_at];
+  }
+  __device__ __forceinline__ void LoadV(const KvCacheParams &p) {
+    const int D = EXACT ? HD : p.head_dim;
+    for (int d = 0; d < DT; ++d)
+      v[d] = EXACT || 16 * d < D ? *reinterpret_cast<const v4i *>(vp + (int64_t)16 * d * p.block_tokens) : v4i{0, 0, 0, 0};
+  }
+};
+
+// Parts are written and read past the XCDs' own L2 caches (sc1), so that no
+// fence has to write those back or drop them.
+constexpr int kDeviceScope = 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t Rsrc(void *p) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, (short)0, 0x7fffffff, 0x00020000);
+}
+__device__ __forceinline__ void PutStat(const Plan &p, int slot, int i, int c, float v) {
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), Rsrc(p.stat), ((slot * 3 + i) * 16 + c) * 4, 0,
+                                        kDeviceScope);
+}
+__device__ __forceinline__ float GetStat(const Plan &p, int slot, int i, int c) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_raw_buffer_load_b32(Rsrc(p.stat), ((slot * 3 + i) * 16 + c) * 4, 0, kDeviceScope));
+}
+
+// Joins the parts of a job: slot `first` of piece w0, slots 2 w of the others.
+// The waves take the parts in turn, eight loads at a time in flight, and add up
+// in LDS.
+template <int HD, typename SO, typename SM>
+__device__ __forceinline__ void JoinParts(const Plan &p, const Job &j, int w0, int w1, int first, bool live,
+                                          SO &so, SM &sm) {
+  constexpr int DT = HD / 16;
+  const int lane = threadIdx.x % 64, c = lane % 16, wave = threadIdx.x / 64;
+  const int parts = w1 - w0 + 1;
+  auto slot = [&](int i) { return i == 0 ? first : (w0 + i) * 2; };
+  // statistics: 16 parts at a time, one per 16 lanes
+  float m = kNone, mo = kNone;
+  for (int i = threadIdx.x / 16; i < parts; i += kThreads / 16) {
+    m = fmaxf(m, GetStat(p, slot(i), 0, c));
+    mo = fmaxf(mo, GetStat(p, slot(i), 1, c));
+  }
+  m = GroupMax(m);
+  mo = GroupMax(mo);
+  __syncthreads();  // so and sm were read
+  if (lane < 16) {
+    sm[wave][0][c] = m;
+    sm[wave][1][c] = mo;
+  }
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) {
+    m = fmaxf(m, sm[w][0][c]);
+    mo = fmaxf(mo, sm[w][1][c]);
+  }
+  float sum = 0.f;
+  for (int i = threadIdx.x / 16; i < parts; i += kThreads / 16)
+    sum += GetStat(p, slot(i), 2, c) * exp2f(GetStat(p, slot(i), 0, c) - m);
+  sum = GroupSum(sum);
+  v4f a[DT];
+  for (int d = 0; d < DT; ++d) a[d] = v4f{0.f, 0.f, 0.f, 0.f};
+  if (live)
+    for (int i = wave; i < parts; i += kWaves) {
+      const float f = exp2f(GetStat(p, slot(i), 1, c) - mo);
+      for (int d = 0; d < DT; ++d)
+        a[d] += __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(
+                                            Rsrc(p.part), ((slot(i) * DT + d) * 64 + lane) * 16, 0, kDeviceScope)) * f;
+    }
+  __syncthreads();  // the maxima were read
+  for (int d = 0; d < DT; ++d) so[wave][d][lane] = a[d];
+  if (lane < 16) sm[wave][2][c] = sum;
+  __syncthreads();
+  sum = 0.f;
+  for (int w = 0; w < kWaves; ++w) sum += sm[w][2][c];
+  for (int d = wave; d < DT; d += kWaves) {
+    v4f t = so[0][d][lane];
+    for (int w = 1; w < kWaves; ++w) t += so[w][d][lane];
+    StoreRows(p, j, d, t, m, mo, sum);
+  }
+}
+
+template <int HD, bool FP8, bool EXACT>
+__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(const Plan p) {
   constexpr int DT = HD / 16, CH = HD / 64;  // dimension tiles, 64-byte chunks of a key
   __shared__ Line line;
   __shared__ v4f so[kWaves][DT][64];
   __shared__ float sm[kWaves][3][16];
+  __shared__ unsigned before;
   const KvCacheParams &cp = p.a.c;
   const int tid = threadIdx.x, lane = tid % 64, c = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
-  const int D = EXACT ? HD : cp.head_dim, H = cp.kv_heads, bt = cp.block_tokens;
   if (p.fill) {
     for (int b = blockIdx.x; b < cp.batch; b += gridDim.x) {
       if (KvNewTokens(cp, b) >= 0) continue;
       const int64_t lo = cp.start[b] < 0 ? 0 : cp.start[b], hi = cp.start[b + 1] < cp.tokens ? cp.start[b + 1] : cp.tokens;
-      const int64_t wide = (int64_t)p.a.heads * D;
+      const int64_t wide = (int64_t)p.a.heads * cp.head_dim;
       for (int64_t i = lo * wide + tid; i < hi * wide; i += kThreads)
         static_cast<uint16_t *>(p.a.out)[i] = p.a.bf16 ? 0x7fc0 : 0x7e00;
     }
@@ -216,69 +363,43 @@ template <int HD, bool FP8, bool EXACT> __global__ __launch_bounds__(kThreads, 2
   for (int part = 0; u < end; part = 1) {
     const Job j = FindJob(p, line, u);
     const int t0 = (int)(u - j.first), t1 = (int)(end - j.first < j.tiles ? end - j.first : j.tiles);
-    // Q of row c, 8 values per 32 dimensions: lane group g has the dimensions
-    // 64 q + 16 g + 8 s ..
     const int row = j.row0 + c;
     const bool live = row < j.n * p.group;
     const int64_t token = cp.start[j.b] + (live ? row / p.group : 0);
-    const int64_t qat = (token * p.a.heads + j.head * p.group + (live ? row % p.group : 0)) * D;
     const int last = j.len - j.n + (live ? row / p.group : 0);  // the last token the row sees
-    v8h q[CH][2];
-    float top = 0.f;
-    for (int i = 0; i < CH * 16; ++i) {
-      const int d = 64 * (i / 16) + 16 * g + i % 16;
-      if (live && (EXACT || d < D)) top = fmaxf(top, fabsf(QValue(p.a.q, qat + d, p.a.bf16)));
+    QRow<CH, EXACT> q;
+    TileLoad<HD, EXACT> ld;
+    q.Load(p.a, (token * p.a.heads + j.head * p.group + (live ? row % p.group : 0)) * cp.head_dim, live, g);
+    // the first tile's loads start before Q is looked at
+    int t = t0 + wave;
+    if (t < t1) {
+      ld.Lookup(cp, j, t, c, g);
+      ld.LoadK(cp, j, t, c, g);
+      ld.LoadV(cp);
+      ld.Lookup(cp, j, t + kWaves, c, g);
     }
-    top = GroupMax(top);
-    const int e = top > 0.f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
-    for (int i = 0; i < CH * 16; ++i) {
-      const int d = 64 * (i / 16) + 16 * g + i % 16;
-      const float v = live && (EXACT || d < D) ? QValue(p.a.q, qat + d, p.a.bf16) : 0.f;
-      q[i / 16][i % 16 / 8][i % 8] = (_Float16)__builtin_amdgcn_ldexpf(v, -e);
-    }
-    const float qf = __builtin_amdgcn_ldexpf(p.a.scale * kLog2e, e);
+    q.Scale(p.a.bf16);
+    const float qf = __builtin_amdgcn_ldexpf(p.a.scale * kLog2e, q.exponent);
 
     v4f o[DT];
-    for (int t = 0; t < DT; ++t) o[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
     float m = kNone, mo = kNone, sum = 0.f;
-    const int32_t *table = cp.table + (int64_t)j.b * cp.max_blocks;
-    // Block of the 16 tokens from `at`, those past the end in the last block;
-    // -1 for one outside the cache, whose tokens get a NaN score.
-    auto block_of = [&](int at) {
-      const int blk = table[(at < j.len ? at : j.len - 1) >> cp.block_shift];
-      return blk >= 0 && blk < cp.num_blocks ? blk : -1;
-    };
-    for (int t = t0 + wave; t < t1; t += kWaves) {
-      const int base = t * kTile;
-      const int kt = base + 16 * (c / 4), vt = base + 16 * g;
-      const int kb = block_of(kt), vb = block_of(vt);
-      const uint8_t *kp = cp.k_cache + (((int64_t)(kb < 0 ? 0 : kb) * H + j.head) * bt + (kt & (bt - 1)) + c % 4) * D + 16 * g;
-      const uint8_t *vp = cp.v_cache + (((int64_t)(vb < 0 ? 0 : vb) * H + j.head) * D + c) * bt + (vt & (bt - 1));
-      v4i kr[4][CH], vr[DT];
-      for (int s = 0; s < 4; ++s)
-        for (int h = 0; h < CH; ++h) {
-          if (EXACT || 64 * h + 16 * g < D)
-            kr[s][h] = *reinterpret_cast<const v4i *>(kp + 4 * s * D + 64 * h);
-          else
-            kr[s][h] = v4i{0, 0, 0, 0};
-        }
-      for (int d = 0; d < DT; ++d) {
-        if (EXACT || 16 * d < D)
-          vr[d] = *reinterpret_cast<const v4i *>(vp + (int64_t)16 * d * bt);
-        else
-          vr[d] = v4i{0, 0, 0, 0};
-      }
-      const float ks = vb < 0 ? __builtin_nanf("") : cp.k_scale[(int64_t)vb * H + j.head];
-      const float vs = vb < 0 ? 0.f : cp.v_scale[(int64_t)vb * H + j.head];
+    // One tile; with `more` the next one's keys load under its softmax and the
+    // values under the next scores.  The last tile is a copy of its own: behind
+    // a branch inside the loop every use would wait for all loads.
+    auto tile = [&](auto more) __attribute__((always_inline)) {
+      const int base = t * kTile, vt = base + 16 * g;
       v4f s[4];
       for (int i = 0; i < 4; ++i) {
         s[i] = v4f{0.f, 0.f, 0.f, 0.f};
         for (int h = 0; h < CH; ++h) {
-          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(kr[i][h][0], kr[i][h][1]), q[h][0], s[i], 0, 0, 0);
-          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(kr[i][h][2], kr[i][h][3]), q[h][1], s[i], 0, 0, 0);
+          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.k[i][h][0], ld.k[i][h][1]), q.q[h][0], s[i], 0, 0, 0);
+          s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.k[i][h][2], ld.k[i][h][3]), q.q[h][1], s[i], 0, 0, 0);
         }
-        s[i] *= ks * qf;
+        s[i] *= ld.ks * qf;
       }
+      const float vs = ld.vs;
+      if constexpr (more) ld.LoadK(cp, j, t + kWaves, c, g);
       // tokens that the row does not see, in the tiles that have any
       const bool edge = base + kTile > j.len - j.n + 1;
       if (edge)
@@ -310,15 +431,22 @@ template <int HD, bool FP8, bool EXACT> __global__ __launch_bounds__(kThreads, 2
         for (int w = 0; w < 4; ++w) {
           const int n = left - 4 * w;
           const unsigned mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
-          for (int d = 0; d < DT; ++d) vr[d][w] &= (int)mask;
+          for (int d = 0; d < DT; ++d) ld.v[d][w] &= (int)mask;
         }
       }
       for (int d = 0; d < DT; ++d) {
         o[d] *= keep_o;
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(vr[d][0], vr[d][1]), pr[0], o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(vr[d][2], vr[d][3]), pr[1], o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.v[d][0], ld.v[d][1]), pr[0], o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.v[d][2], ld.v[d][3]), pr[1], o[d], 0, 0, 0);
       }
-    }
+      if constexpr (more) {
+        ld.LoadV(cp);
+        ld.Lookup(cp, j, t + 2 * kWaves, c, g);
+      }
+      t += kWaves;
+    };
+    while (t + kWaves < t1) tile(std::true_type{});
+    if (t < t1) tile(std::false_type{});
     sum = GroupSum(sum);
 
     // the waves' parts become one
@@ -338,65 +466,49 @@ template <int HD, bool FP8, bool EXACT> __global__ __launch_bounds__(kThreads, 2
     sum = 0.f;
     for (int w = 0; w < kWaves; ++w) sum += sm[w][2][c] * exp2f(sm[w][0][c] - m);
     const bool whole = t0 == 0 && t1 == j.tiles;
-    const int64_t slot = (int64_t)blockIdx.x * 2 + part;
+    const int slot = (int)blockIdx.x * 2 + part;
     for (int d = wave; d < DT; d += kWaves) {
       v4f a = v4f{0.f, 0.f, 0.f, 0.f};
       for (int w = 0; w < kWaves; ++w) a += so[w][d][lane] * exp2f(sm[w][1][c] - mo);
       if (whole)
         StoreRows(p, j, d, a, m, mo, sum);
       else if (live)
-        reinterpret_cast<v4f *>(p.part)[(slot * DT + d) * 64 + lane] = a;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, a), Rsrc(p.part), ((slot * DT + d) * 64 + lane) * 16,
+                                               0, kDeviceScope);
     }
-    if (!whole && wave == 0 && g == 0) {
-      p.stat[(slot * 3 + 0) * 16 + c] = m;
-      p.stat[(slot * 3 + 1) * 16 + c] = mo;
-      p.stat[(slot * 3 + 2) * 16 + c] = sum;
+    if (!whole) {
+      if (wave == 0 && g == 0) {
+        PutStat(p, slot, 0, c, m);
+        PutStat(p, slot, 1, c, mo);
+        PutStat(p, slot, 2, c, sum);
+      }
+      const int w0 = Uniform((int)(j.first / piece)), w1 = Uniform((int)((j.first + j.tiles - 1) / piece));
+      // this part is in memory for every XCD before it is counted
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (tid == 0) before = atomicAdd(p.done + w0, 1u);
+      __syncthreads();
+      if (before == (unsigned)(w1 - w0)) {
+        if (tid == 0) p.done[w0] = 0;
+        // a job that starts inside a piece is the last in it
+        JoinParts<HD>(p, j, w0, w1, w0 * 2 + (j.first > w0 * piece ? 1 : 0), live, so, sm);
+      }
     }
     u = j.first + t1;
   }
 }
 
-// Joins the parts of the job that starts in piece blockIdx.x and goes on in the
-// next ones: one wave per 16 dimensions.
-template <int HD> __global__ __launch_bounds__(kThreads) void KvJoinKernel(const Plan p) {
-  constexpr int DT = HD / 16;
-  __shared__ Line line;
-  const int lane = threadIdx.x % 64, c = lane % 16;
-  const int64_t units = MakeLine(p, line), piece = PieceOf(units);
-  const int64_t end = ((int64_t)blockIdx.x + 1) * piece;
-  if (end >= units) return;
-  const Job j = FindJob(p, line, end - 1);
-  if (j.first < end - piece || j.first + j.tiles <= end) return;
-  const int64_t w1 = (j.first + j.tiles - 1) / piece;
-  auto slot = [&](int64_t w) { return w * 2 + (w == (int64_t)blockIdx.x && j.first > end - piece ? 1 : 0); };
-  float m = kNone, mo = kNone, sum = 0.f;
-  for (int64_t w = blockIdx.x; w <= w1; ++w) {
-    m = fmaxf(m, p.stat[(slot(w) * 3 + 0) * 16 + c]);
-    mo = fmaxf(mo, p.stat[(slot(w) * 3 + 1) * 16 + c]);
-  }
-  const bool live = j.row0 + c < j.n * p.group;
-  const int d = blockIdx.y * kWaves + threadIdx.x / 64;
-  if (d >= DT) return;
-  v4f a = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int64_t w = blockIdx.x; w <= w1; ++w) {
-    sum += p.stat[(slot(w) * 3 + 2) * 16 + c] * exp2f(p.stat[(slot(w) * 3 + 0) * 16 + c] - m);
-    if (live)
-      a += reinterpret_cast<const v4f *>(p.part)[(slot(w) * DT + d) * 64 + lane] *
-           exp2f(p.stat[(slot(w) * 3 + 1) * 16 + c] - mo);
-  }
-  StoreRows(p, j, d, a, m, mo, sum);
-}
-
 int HeadTile(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
 // Two workgroups per CU hold eight waves, enough loads in flight to fill the
-// memory; never more than there can be pieces of one tile per wave.
+// memory (head dimensions above 128 need the registers of both); never more
+// than there can be pieces of one tile per wave.
 int64_t DecodeGrid(const KvAttentionParams &p) {
   const KvCacheParams &c = p.c;
   const int64_t group = p.heads / c.kv_heads, jobs = (c.tokens * group / 16 + c.batch) * c.kv_heads;
   const int64_t tiles = ((int64_t)c.max_blocks * c.block_tokens + kTile - 1) / kTile;
   const int64_t pieces = (jobs * tiles + kWaves - 1) / kWaves;
-  return std::max<int64_t>(1, std::min<int64_t>(pieces, 2 * Ctx().num_cus));
+  return std::max<int64_t>(1, std::min<int64_t>(pieces, (c.head_dim > 128 ? 1 : 2) * Ctx().num_cus));
 }
 
 template <int HD> void LaunchDecode(const Plan &p, int64_t grid, hipStream_t s) {
@@ -406,7 +518,6 @@ template <int HD> void LaunchDecode(const Plan &p, int64_t grid, hipStream_t s) 
     exact ? KvDecodeKernel<HD, true, true><<<g, kThreads, 0, s>>>(p) : KvDecodeKernel<HD, true, false><<<g, kThreads, 0, s>>>(p);
   else
     exact ? KvDecodeKernel<HD, false, true><<<g, kThreads, 0, s>>>(p) : KvDecodeKernel<HD, false, false><<<g, kThreads, 0, s>>>(p);
-  if (grid > 1) KvJoinKernel<HD><<<dim3((unsigned)grid, (HD / 16 + kWaves - 1) / kWaves), kThreads, 0, s>>>(p);
 }
 
 }  // namespace
@@ -424,6 +535,7 @@ void LaunchKvCacheAttention(const KvAttentionParams &a, void *scratch, hipStream
   p.group = a.heads / a.c.kv_heads;
   p.rows_max = 0x7fffffff;
   p.fill = 1;
+  p.done = Ctx().ws.Counters((size_t)grid);
   p.part = static_cast<float *>(scratch);
   p.stat = reinterpret_cast<float *>(static_cast<char *>(scratch) + Scratch::Round((size_t)grid * 2 * 16 * hd * sizeof(float)));
   if (hd == 64)
