@@ -3503,6 +3503,7 @@ int KvCacheAttention(const onnxl_amd_tensor *q, const onnxl_amd_tensor *k_cache,
   const int64_t heads = q->dims[1];
   OLA_ENFORCE(heads > 0 && heads < 65536 && heads % p.c.kv_heads == 0, kKvtName,
               ": heads must be a multiple of the cache's kv_heads, up to 65535.");
+  OLA_ENFORCE(p.c.tokens * (heads / p.c.kv_heads) < (int64_t(1) << 31), kKvtName, ": 2^31 rows per kv head or more.");
   NeedShape(out, ShapeOf(*q), kKvtName, "out");
   OLA_ENFORCE(std::isfinite(scale), kKvtName, ": scale must be finite.");
   OLA_ENFORCE(max_query >= 0, kKvtName, ": max_query must not be negative.");

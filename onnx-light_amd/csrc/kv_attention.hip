@@ -19,11 +19,11 @@
 // Codes become fp16 exactly (|int8| <= 128, E4M3 is a subset).  Q becomes fp16
 // after a power of two per row has brought its largest value to [1, 2): exact
 // but for what is below 2^-14 of that largest.  Sums, statistics and O are
-// fp32; P is rounded to fp16.  O is kept relative to its own running maximum of
-// S + log2(v scale), not of S, so that P times the block's v scale fills the
-// fp16 range whatever the scales are; the softmax sum is relative to m and takes
-// the unrounded P.
-#include <cfloat>
+// fp32; P is rounded to fp16.  The weight of a token in O is its softmax weight
+// times its block's v scale, so P is taken relative to mo, the running maximum
+// of S + log2(v scale): P = 2^(S + log2 vs - mo) fills the fp16 range whatever
+// the scales are.  The softmax sum takes the unrounded P / vs (one
+// multiplication per 16 tokens), and O / sum needs no other reference.
 #include <type_traits>
 
 #include "common.hpp"
@@ -70,6 +70,19 @@ __device__ __forceinline__ uint2 Pack4(v4f v, int bf16) {
   return make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
 }
 
+// log2 of a token's weight in O: score (s * cs) plus log2 of its v scale, two
+// roundings, never fused, so that it is the same wherever it is computed.
+__device__ __forceinline__ float Weight(float s, float cs, float lv) {
+#pragma clang fp contract(off)
+  const float z = s * cs;
+  return z + lv;
+}
+
+// log2 of a v scale and its inverse.  A scale below 2^-100 (zero: a block of
+// zeros) counts as 2^-100; NaN stays.
+__device__ __forceinline__ float LogScale(float vs) { return vs > 0x1p-100f ? __builtin_amdgcn_logf(vs) : vs == vs ? -100.f : vs; }
+__device__ __forceinline__ float InvScale(float vs) { return vs > 0x1p-100f ? __builtin_amdgcn_rcpf(vs) : 0x1p100f; }
+
 // The larger over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float GroupMax(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -103,10 +116,10 @@ struct Job {
 struct Plan {
   KvAttentionParams a;
   int group;
-  int rows_max;     // sequences with more rows (new tokens * group) are not for this kernel
+  int rows_max;     // sequences with more rows (new tokens * group) are the prompt kernel's
   int fill;         // NaN for the rows of sequences that do not fit
   float *part;      // parts: [workgroup][2][HD / 16][64] float4
-  float *stat;      // [workgroup][2][3][16]: m, the maximum of O, the sum
+  float *stat;      // [workgroup][2][2][16]: mo, the sum
   unsigned *done;   // [workgroup] parts written of the job that starts last in its piece; zero between launches
 };
 
@@ -174,17 +187,29 @@ __device__ __forceinline__ Job FindJob(const Plan &p, const Line &line, int64_t 
   return j;
 }
 
+// NaN for the rows of sequences whose numbers do not fit.
+__device__ __forceinline__ void FillInvalid(const Plan &p) {
+  const KvCacheParams &c = p.a.c;
+  for (int b = blockIdx.x; b < c.batch; b += gridDim.x) {
+    if (KvNewTokens(c, b) >= 0) continue;
+    const int64_t lo = c.start[b] < 0 ? 0 : c.start[b], hi = c.start[b + 1] < c.tokens ? c.start[b + 1] : c.tokens;
+    const int64_t wide = (int64_t)p.a.heads * c.head_dim;
+    for (int64_t i = lo * wide + threadIdx.x; i < hi * wide; i += blockDim.x)
+      static_cast<uint16_t *>(p.a.out)[i] = p.a.bf16 ? 0x7fc0 : 0x7e00;
+  }
+}
+
 // Units of one workgroup: equal pieces, of at least one tile per wave.
 __device__ __forceinline__ int64_t PieceOf(int64_t units) {
   const int64_t piece = (units + gridDim.x - 1) / gridDim.x;
   return piece < kWaves ? kWaves : piece;
 }
 
-// Writes O * 2^(mo - m) / sum of the rows in lanes c < rows.
-__device__ __forceinline__ void StoreRows(const Plan &p, const Job &j, int t, v4f o, float m, float mo, float sum) {
+// Writes O / sum of the rows that there are.
+__device__ __forceinline__ void StoreRows(const Plan &p, const Job &j, int t, v4f o, float sum) {
   const int c = threadIdx.x % 16, g = threadIdx.x % 64 / 16, row = j.row0 + c, d = 16 * t + 4 * g;
   if (row >= j.n * p.group || d >= p.a.c.head_dim) return;
-  const float f = exp2f(mo - m) / sum;
+  const float f = 1.f / sum;
   const int64_t token = p.a.c.start[j.b] + row / p.group;
   const int head = j.head * p.group + row % p.group;
   uint16_t *out = static_cast<uint16_t *>(p.a.out) + (token * p.a.heads + head) * p.a.c.head_dim + d;
@@ -200,7 +225,8 @@ __device__ __forceinline__ v4i Load16(const void *p) {
 }
 
 // Q of one row as the first product's operand: lane group g holds the
-// dimensions 64 h + 16 g + 8 s + (0..7) at q[h][s], scaled by 2^-exponent.
+// dimensions 64 h + 16 g + 8 s + (0..7) at q[h][s], scaled by 2^-exponent and
+// with the sign of the softmax scale.
 template <int CH, bool EXACT> struct QRow {
   v4i raw[CH][2];
   v8h q[CH][2];
@@ -213,21 +239,24 @@ template <int CH, bool EXACT> struct QRow {
         raw[h][s] = live && (EXACT || d < p.c.head_dim) ? Load16(static_cast<const uint16_t *>(p.q) + at + d) : v4i{0, 0, 0, 0};
       }
   }
-  __device__ __forceinline__ void Scale(int bf16) {
+  __device__ __forceinline__ void Scale(const KvAttentionParams &p) {
     float v[CH][2][8], top = 0.f;
     for (int h = 0; h < CH; ++h)
       for (int s = 0; s < 2; ++s)
         for (int i = 0; i < 8; ++i) {
           const int w = raw[h][s][i / 2];
           const uint16_t u = (uint16_t)((unsigned)w >> (16 * (i % 2)));
-          v[h][s][i] = bf16 ? Bf16ToF32(u) : F16ToF32(u);
+          v[h][s][i] = p.bf16 ? Bf16ToF32(u) : F16ToF32(u);
           top = fmaxf(top, fabsf(v[h][s][i]));
         }
     top = GroupMax(top);
     exponent = top > 0.f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
     for (int h = 0; h < CH; ++h)
       for (int s = 0; s < 2; ++s)
-        for (int i = 0; i < 8; ++i) q[h][s][i] = (_Float16)__builtin_amdgcn_ldexpf(v[h][s][i], -exponent);
+        for (int i = 0; i < 8; ++i) {
+          const float x = __builtin_amdgcn_ldexpf(v[h][s][i], -exponent);
+          q[h][s][i] = (_Float16)(p.scale < 0.f ? -x : x);
+        }
   }
 };
 
@@ -276,12 +305,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t Rsrc(void *p) {
   return __builtin_amdgcn_make_buffer_rsrc(p, (short)0, 0x7fffffff, 0x00020000);
 }
 __device__ __forceinline__ void PutStat(const Plan &p, int slot, int i, int c, float v) {
-  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), Rsrc(p.stat), ((slot * 3 + i) * 16 + c) * 4, 0,
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), Rsrc(p.stat), ((slot * 2 + i) * 16 + c) * 4, 0,
                                         kDeviceScope);
 }
 __device__ __forceinline__ float GetStat(const Plan &p, int slot, int i, int c) {
   return __builtin_bit_cast(
-      float, __builtin_amdgcn_raw_buffer_load_b32(Rsrc(p.stat), ((slot * 3 + i) * 16 + c) * 4, 0, kDeviceScope));
+      float, __builtin_amdgcn_raw_buffer_load_b32(Rsrc(p.stat), ((slot * 2 + i) * 16 + c) * 4, 0, kDeviceScope));
 }
 
 // Joins the parts of a job: slot `first` of piece w0, slots 2 w of the others.
@@ -295,46 +324,35 @@ __device__ __forceinline__ void JoinParts(const Plan &p, const Job &j, int w0, i
   const int parts = w1 - w0 + 1;
   auto slot = [&](int i) { return i == 0 ? first : (w0 + i) * 2; };
   // statistics: 16 parts at a time, one per 16 lanes
-  float m = kNone, mo = kNone;
-  for (int i = threadIdx.x / 16; i < parts; i += kThreads / 16) {
-    m = fmaxf(m, GetStat(p, slot(i), 0, c));
-    mo = fmaxf(mo, GetStat(p, slot(i), 1, c));
-  }
-  m = GroupMax(m);
+  float mo = kNone;
+  for (int i = threadIdx.x / 16; i < parts; i += kThreads / 16) mo = fmaxf(mo, GetStat(p, slot(i), 0, c));
   mo = GroupMax(mo);
   __syncthreads();  // so and sm were read
-  if (lane < 16) {
-    sm[wave][0][c] = m;
-    sm[wave][1][c] = mo;
-  }
+  if (lane < 16) sm[wave][0][c] = mo;
   __syncthreads();
-  for (int w = 0; w < kWaves; ++w) {
-    m = fmaxf(m, sm[w][0][c]);
-    mo = fmaxf(mo, sm[w][1][c]);
-  }
+  for (int w = 0; w < kWaves; ++w) mo = fmaxf(mo, sm[w][0][c]);
   float sum = 0.f;
   for (int i = threadIdx.x / 16; i < parts; i += kThreads / 16)
-    sum += GetStat(p, slot(i), 2, c) * exp2f(GetStat(p, slot(i), 0, c) - m);
+    sum += GetStat(p, slot(i), 1, c) * __builtin_amdgcn_exp2f(GetStat(p, slot(i), 0, c) - mo);
   sum = GroupSum(sum);
   v4f a[DT];
   for (int d = 0; d < DT; ++d) a[d] = v4f{0.f, 0.f, 0.f, 0.f};
   if (live)
     for (int i = wave; i < parts; i += kWaves) {
-      const float f = exp2f(GetStat(p, slot(i), 1, c) - mo);
+      const float f = __builtin_amdgcn_exp2f(GetStat(p, slot(i), 0, c) - mo);
       for (int d = 0; d < DT; ++d)
         a[d] += __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(
                                             Rsrc(p.part), ((slot(i) * DT + d) * 64 + lane) * 16, 0, kDeviceScope)) * f;
     }
-  __syncthreads();  // the maxima were read
   for (int d = 0; d < DT; ++d) so[wave][d][lane] = a[d];
-  if (lane < 16) sm[wave][2][c] = sum;
+  if (lane < 16) sm[wave][1][c] = sum;
   __syncthreads();
   sum = 0.f;
-  for (int w = 0; w < kWaves; ++w) sum += sm[w][2][c];
+  for (int w = 0; w < kWaves; ++w) sum += sm[w][1][c];
   for (int d = wave; d < DT; d += kWaves) {
     v4f t = so[0][d][lane];
     for (int w = 1; w < kWaves; ++w) t += so[w][d][lane];
-    StoreRows(p, j, d, t, m, mo, sum);
+    StoreRows(p, j, d, t, sum);
   }
 }
 
@@ -343,20 +361,12 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
   constexpr int DT = HD / 16, CH = HD / 64;  // dimension tiles, 64-byte chunks of a key
   __shared__ Line line;
   __shared__ v4f so[kWaves][DT][64];
-  __shared__ float sm[kWaves][3][16];
+  __shared__ float sm[kWaves][2][16];
   __shared__ unsigned before;
   const KvCacheParams &cp = p.a.c;
   const int tid = threadIdx.x, lane = tid % 64, c = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
-  if (p.fill) {
-    for (int b = blockIdx.x; b < cp.batch; b += gridDim.x) {
-      if (KvNewTokens(cp, b) >= 0) continue;
-      const int64_t lo = cp.start[b] < 0 ? 0 : cp.start[b], hi = cp.start[b + 1] < cp.tokens ? cp.start[b + 1] : cp.tokens;
-      const int64_t wide = (int64_t)p.a.heads * cp.head_dim;
-      for (int64_t i = lo * wide + tid; i < hi * wide; i += kThreads)
-        static_cast<uint16_t *>(p.a.out)[i] = p.a.bf16 ? 0x7fc0 : 0x7e00;
-    }
-  }
+  if (p.fill) FillInvalid(p);
   const int64_t units = MakeLine(p, line), piece = PieceOf(units);
   int64_t u = (int64_t)blockIdx.x * piece;
   const int64_t end = u + piece < units ? u + piece : units;
@@ -378,64 +388,64 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
       ld.LoadV(cp);
       ld.Lookup(cp, j, t + kWaves, c, g);
     }
-    q.Scale(p.a.bf16);
-    const float qf = __builtin_amdgcn_ldexpf(p.a.scale * kLog2e, q.exponent);
+    q.Scale(p.a);
+    const float qf = __builtin_amdgcn_ldexpf(fabsf(p.a.scale) * kLog2e, q.exponent);
 
     v4f o[DT];
+#pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
-    float m = kNone, mo = kNone, sum = 0.f;
+    float mo = kNone, sum = 0.f;
     // One tile; with `more` the next one's keys load under its softmax and the
     // values under the next scores.  The last tile is a copy of its own: behind
     // a branch inside the loop every use would wait for all loads.
     auto tile = [&](auto more) __attribute__((always_inline)) {
       const int base = t * kTile, vt = base + 16 * g;
       v4f s[4];
+#pragma unroll
       for (int i = 0; i < 4; ++i) {
         s[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
         for (int h = 0; h < CH; ++h) {
           s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.k[i][h][0], ld.k[i][h][1]), q.q[h][0], s[i], 0, 0, 0);
           s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.k[i][h][2], ld.k[i][h][3]), q.q[h][1], s[i], 0, 0, 0);
         }
-        s[i] *= ld.ks * qf;
       }
-      const float vs = ld.vs;
+      const float cs = ld.ks * qf, lv = LogScale(ld.vs), inv = InvScale(ld.vs);
       if constexpr (more) ld.LoadK(cp, j, t + kWaves, c, g);
       // tokens that the row does not see, in the tiles that have any
       const bool edge = base + kTile > j.len - j.n + 1;
-      if (edge)
-        for (int i = 0; i < 16; ++i)
-          if (vt + i > last) s[i / 4][i % 4] = -__builtin_huge_valf();
-      float lm = s[0][0];
-      for (int i = 1; i < 16; ++i) lm = fmaxf(lm, s[i / 4][i % 4]);
-      const float lv = fmaxf(__builtin_amdgcn_logf(vs), -126.f);
-      const float mn = fmaxf(m, GroupMax(lm)), mon = fmaxf(mo, GroupMax(lm + lv));
-      const float keep = __builtin_amdgcn_exp2f(m - mn), keep_o = __builtin_amdgcn_exp2f(mo - mon);
-      // w * f <= 1, so f overflows only where every w is 0; a NaN scale stays
-      float f = vs * __builtin_amdgcn_exp2f(mn - mon);
-      f = f > FLT_MAX ? FLT_MAX : f;
-      m = mn;
-      mo = mon;
+      float top = -__builtin_huge_valf();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = edge && vt + i > last ? -__builtin_huge_valf() : Weight(s[i / 4][i % 4], cs, lv);
+        s[i / 4][i % 4] = x;
+        top = fmaxf(top, x);
+      }
+      const float now = fmaxf(mo, GroupMax(top)), keep = __builtin_amdgcn_exp2f(mo - now);
+      mo = now;
       float ps = 0.f;
       v8h pr[2];
+#pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float w = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - mn);
+        const float w = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - now);
         ps += w;
-        float wv = w * f;
-        if (edge && vt + i > last) wv = 0.f;
-        pr[i / 8][i % 8] = (_Float16)wv;
+        pr[i / 8][i % 8] = (_Float16)w;
       }
-      sum = sum * keep + ps;
+      sum = __builtin_fmaf(ps, inv, sum * keep);
       if (edge) {
         // what the cache holds past the end may be any code, NaN among them
         const int left = j.len - vt;  // tokens of this lane that are there
+#pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int n = left - 4 * w;
           const unsigned mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+#pragma unroll
           for (int d = 0; d < DT; ++d) ld.v[d][w] &= (int)mask;
         }
       }
+#pragma unroll
       for (int d = 0; d < DT; ++d) {
-        o[d] *= keep_o;
+        o[d] *= keep;
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.v[d][0], ld.v[d][1]), pr[0], o[d], 0, 0, 0);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.v[d][2], ld.v[d][3]), pr[1], o[d], 0, 0, 0);
       }
@@ -451,36 +461,39 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
 
     // the waves' parts become one
     __syncthreads();
+#pragma unroll
     for (int d = 0; d < DT; ++d) so[wave][d][lane] = o[d];
     if (g == 0) {
-      sm[wave][0][c] = m;
-      sm[wave][1][c] = mo;
-      sm[wave][2][c] = sum;
+      sm[wave][0][c] = mo;
+      sm[wave][1][c] = sum;
     }
     __syncthreads();
-    m = mo = kNone;
-    for (int w = 0; w < kWaves; ++w) {
-      m = fmaxf(m, sm[w][0][c]);
-      mo = fmaxf(mo, sm[w][1][c]);
-    }
+    mo = kNone;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mo = fmaxf(mo, sm[w][0][c]);
     sum = 0.f;
-    for (int w = 0; w < kWaves; ++w) sum += sm[w][2][c] * exp2f(sm[w][0][c] - m);
+    float f[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(sm[w][0][c] - mo);
+      sum += sm[w][1][c] * f[w];
+    }
     const bool whole = t0 == 0 && t1 == j.tiles;
     const int slot = (int)blockIdx.x * 2 + part;
     for (int d = wave; d < DT; d += kWaves) {
       v4f a = v4f{0.f, 0.f, 0.f, 0.f};
-      for (int w = 0; w < kWaves; ++w) a += so[w][d][lane] * exp2f(sm[w][1][c] - mo);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) a += so[w][d][lane] * f[w];
       if (whole)
-        StoreRows(p, j, d, a, m, mo, sum);
+        StoreRows(p, j, d, a, sum);
       else if (live)
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, a), Rsrc(p.part), ((slot * DT + d) * 64 + lane) * 16,
                                                0, kDeviceScope);
     }
     if (!whole) {
       if (wave == 0 && g == 0) {
-        PutStat(p, slot, 0, c, m);
-        PutStat(p, slot, 1, c, mo);
-        PutStat(p, slot, 2, c, sum);
+        PutStat(p, slot, 0, c, mo);
+        PutStat(p, slot, 1, c, sum);
       }
       const int w0 = Uniform((int)(j.first / piece)), w1 = Uniform((int)((j.first + j.tiles - 1) / piece));
       // this part is in memory for every XCD before it is counted
@@ -493,6 +506,392 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
         // a job that starts inside a piece is the last in it
         JoinParts<HD>(p, j, w0, w1, w0 * 2 + (j.first > w0 * piece ? 1 : 0), live, so, sm);
       }
+    }
+    u = j.first + t1;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows (prompts): the products are the cost.  A job is one kv head and a
+// tile of 8 waves * CT * 16 rows of a sequence, over the tokens that its last
+// row sees; each wave owns its rows, so nothing is joined between waves.  The
+// codes of a 64-token tile become fp16 once, in LDS (two buffers, one barrier
+// per tile), where every wave reads them: with CT 16-row tiles per wave an
+// operand read feeds CT MFMAs, CT = 2 keeping the LDS as busy as the matrix
+// cores and 3 at two thirds of them.  Rows of 16-byte chunks are XOR-swizzled
+// so that the 16 rows of an operand lie on 64 different banks.
+//
+// Jobs form a line of tiles as above, cut into equal pieces, so the causal
+// triangle, ragged lengths and few rows over long caches all keep every CU
+// busy; parts are joined the same way.
+//
+// The reference mo moves only when it is exceeded by 2^8 or more, which P has
+// room for in fp16.
+
+// Q of one row for the prompt kernel: lane group g holds the dimensions 32 k +
+// 8 g + (0..7) at q[k], scaled to [1, 2); qf gives the scores in powers of two,
+// and is not negative (the sign of the softmax scale goes to Q).
+template <int KS, bool EXACT>
+__device__ __forceinline__ void LoadQ(const KvAttentionParams &p, int64_t at, bool live, int g, v8h (&q)[KS], float &qf) {
+  float v[KS][8], top = 0.f;
+  for (int k = 0; k < KS; ++k) {
+    const int d = 32 * k + 8 * g;
+    const v4i raw = live && (EXACT || d < p.c.head_dim) ? Load16(static_cast<const uint16_t *>(p.q) + at + d) : v4i{0, 0, 0, 0};
+    for (int i = 0; i < 8; ++i) {
+      const int w = raw[i / 2];
+      const uint16_t u = (uint16_t)((unsigned)w >> (16 * (i % 2)));
+      v[k][i] = p.bf16 ? Bf16ToF32(u) : F16ToF32(u);
+      top = fmaxf(top, fabsf(v[k][i]));
+    }
+  }
+  top = GroupMax(top);
+  const int e = top > 0.f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+  for (int k = 0; k < KS; ++k)
+    for (int i = 0; i < 8; ++i) {
+      const float x = __builtin_amdgcn_ldexpf(v[k][i], -e);
+      q[k][i] = (_Float16)(p.scale < 0.f ? -x : x);
+    }
+  qf = __builtin_amdgcn_ldexpf(fabsf(p.scale) * kLog2e, e);
+}
+
+constexpr int kRowWaves = 8, kRowThreads = 64 * kRowWaves;
+constexpr float kLag = 8.f;
+
+struct RowLine {                // over the row tiles of all sequences
+  int64_t upto[kRowThreads];    // units before the end of every thread's share
+  int tiles_upto[kRowThreads];  // row tiles before the end of every thread's share of the sequences
+  int row_tiles;
+};
+
+__device__ __forceinline__ int64_t BlockScan(int64_t v, int64_t *s) {
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t w = __shfl_up(v, o);
+    if ((int)threadIdx.x % 64 >= o) v += w;
+  }
+  s[threadIdx.x] = v;
+  __syncthreads();
+  int64_t before = 0;
+  for (int w = 0; w < (int)threadIdx.x / 64; ++w) before += s[64 * w + 63];
+  __syncthreads();
+  return v + before;
+}
+
+struct RowTile {
+  int b, n, len, row0, tiles;
+};
+
+// Row tiles of sequence b (0 where its rows are the decoding kernel's).
+__device__ __forceinline__ int RowTilesOf(const Plan &p, int b, int rows) {
+  const int n = KvNewTokens(p.a.c, b);
+  return n > 0 && (int64_t)n * p.group > p.rows_max ? (n * p.group + rows - 1) / rows : 0;
+}
+
+// Row tile i of the batch; the longest of a sequence come first.
+__device__ __forceinline__ RowTile FindRowTile(const Plan &p, const RowLine &l, int i, int rows) {
+  const int share = (p.a.c.batch + kRowThreads - 1) / kRowThreads;
+  int lo = 0, hi = kRowThreads - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (l.tiles_upto[mid] > i) hi = mid; else lo = mid + 1;
+  }
+  int at = lo ? l.tiles_upto[lo - 1] : 0, b = lo * share, n = RowTilesOf(p, b, rows);
+  while (i >= at + n) {
+    at += n;
+    n = RowTilesOf(p, ++b, rows);
+  }
+  RowTile r;
+  r.b = b;
+  r.n = KvNewTokens(p.a.c, b);
+  r.len = p.a.c.lengths[b];
+  r.row0 = (n - 1 - (i - at)) * rows;
+  const int last_row = min(r.row0 + rows, r.n * p.group) - 1;
+  r.tiles = (r.len - r.n + last_row / p.group) / kTile + 1;
+  return r;
+}
+
+__device__ __forceinline__ int64_t MakeRowLine(const Plan &p, RowLine &l, int rows) {
+  const int B = p.a.c.batch, tid = threadIdx.x, share = (B + kRowThreads - 1) / kRowThreads;
+  int64_t mine = 0;
+  for (int b = tid * share; b < min(B, (tid + 1) * share); ++b) mine += RowTilesOf(p, b, rows);
+  l.tiles_upto[tid] = (int)BlockScan(mine, l.upto);
+  __syncthreads();
+  const int all = l.tiles_upto[kRowThreads - 1], per = (all + kRowThreads - 1) / kRowThreads;
+  mine = 0;
+  for (int i = tid * per; i < min(all, (tid + 1) * per); ++i)
+    mine += (int64_t)FindRowTile(p, l, i, rows).tiles * p.a.c.kv_heads;
+  const int64_t sum = BlockScan(mine, l.upto);
+  l.upto[tid] = sum;
+  if (tid == 0) l.row_tiles = all;
+  __syncthreads();
+  return Uniform(l.upto[kRowThreads - 1]);
+}
+
+__device__ __forceinline__ Job FindRowJob(const Plan &p, const RowLine &l, int64_t u, int rows) {
+  const int per = (l.row_tiles + kRowThreads - 1) / kRowThreads, H = p.a.c.kv_heads;
+  int lo = 0, hi = kRowThreads - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (l.upto[mid] > u) hi = mid; else lo = mid + 1;
+  }
+  int64_t at = lo ? l.upto[lo - 1] : 0;
+  int i = lo * per;
+  RowTile r = FindRowTile(p, l, i, rows);
+  while (u >= at + (int64_t)r.tiles * H) {
+    at += (int64_t)r.tiles * H;
+    r = FindRowTile(p, l, ++i, rows);
+  }
+  Job j;
+  j.b = Uniform(r.b);
+  j.n = Uniform(r.n);
+  j.len = Uniform(r.len);
+  j.row0 = Uniform(r.row0);
+  j.tiles = Uniform(r.tiles);
+  j.head = Uniform((int)((u - at) / r.tiles));
+  j.first = Uniform(at) + (int64_t)j.head * j.tiles;
+  return j;
+}
+
+// The 16-byte chunk of a row in LDS: keys have HD / 8 chunks per token, values
+// 8 per dimension.
+template <int HD> __device__ __forceinline__ int KeyChunk(int token, int chunk) {
+  const int key = HD == 64 ? (token >> 1 & 1) | (token >> 4) << 1 : (token & 3) | (token >> 4) << 2;
+  return token * (HD / 8) + (chunk ^ key);
+}
+__device__ __forceinline__ int ValueChunk(int dim, int chunk) { return dim * 8 + (chunk ^ (dim >> 1 & 7)); }
+
+// A workgroup's loads of one tile: every thread 16 bytes (HD 256: two times) of
+// the keys and of the values.
+template <int HD, bool FP8, bool EXACT> struct TileStage {
+  static constexpr int kEach = HD / 16 * kTile / kRowThreads > 0 ? HD / 16 * kTile / kRowThreads : 1;
+  static constexpr bool kAll = HD / 16 * kTile >= kRowThreads;  // every thread loads
+  int kb[kEach], vb[kEach];
+  v4i k[kEach], v[kEach];
+  float ks, vs;
+
+  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const Job &j, int t) {
+    const int32_t *table = p.table + (int64_t)j.b * p.max_blocks;
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kRowThreads;
+      kb[e] = table[min(t * kTile + i / (HD / 16) % kTile, j.len - 1) >> p.block_shift];
+      vb[e] = table[min(t * kTile + 16 * (i % 4), j.len - 1) >> p.block_shift];
+    }
+  }
+  __device__ __forceinline__ void Load(const KvCacheParams &p, const Job &j, int t) {
+    const int D = EXACT ? HD : p.head_dim, bt = p.block_tokens;
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kRowThreads;
+      const int token = i / (HD / 16) % kTile, kd = i % (HD / 16) * 16, dim = i / 4 % HD, vt = 16 * (i % 4);
+      const bool bad = vb[e] < 0 || vb[e] >= p.num_blocks;
+      const int64_t k_at = (int64_t)(kb[e] >= 0 && kb[e] < p.num_blocks ? kb[e] : 0) * p.kv_heads + j.head;
+      const int64_t v_at = (int64_t)(bad ? 0 : vb[e]) * p.kv_heads + j.head;
+      const int at = t * kTile & (bt - 1);
+      k[e] = EXACT || kd < D ? *reinterpret_cast<const v4i *>(p.k_cache + (k_at * bt + ((at + token) & (bt - 1))) * D + kd)
+                             : v4i{0, 0, 0, 0};
+      v[e] = EXACT || dim < D ? *reinterpret_cast<const v4i *>(p.v_cache + (v_at * D + dim) * bt + ((at + vt) & (bt - 1)))
+                              : v4i{0, 0, 0, 0};
+      if (e == 0) {
+        ks = p.k_scale[v_at];
+        ks = bad ? __builtin_nanf("") : ks;
+        vs = p.v_scale[v_at];
+      }
+    }
+  }
+  // Codes past the sequence's end may be any, NaN among them: those of v, which
+  // the second product multiplies by zero, become zero.
+  __device__ __forceinline__ void Store(v8h *sk, v8h *sv, float *ss, int left) {
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kRowThreads;
+      const int token = i / (HD / 16) % kTile, kc = i % (HD / 16) * 2, dim = i / 4 % HD, vt = 16 * (i % 4);
+      if (left < kTile)
+        for (int w = 0; w < 4; ++w) {
+          const int n = left - vt - 4 * w;
+          v[e][w] &= (int)(n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+        }
+      if (kAll || i < HD / 16 * kTile) {
+        sk[KeyChunk<HD>(token, kc)] = Widen<FP8>(k[e][0], k[e][1]);
+        sk[KeyChunk<HD>(token, kc + 1)] = Widen<FP8>(k[e][2], k[e][3]);
+        sv[ValueChunk(dim, i % 4 * 2)] = Widen<FP8>(v[e][0], v[e][1]);
+        sv[ValueChunk(dim, i % 4 * 2 + 1)] = Widen<FP8>(v[e][2], v[e][3]);
+      }
+    }
+    if (threadIdx.x < 4) {
+      ss[threadIdx.x] = ks;
+      ss[4 + threadIdx.x] = vs;
+    }
+  }
+};
+
+template <int HD, int CT, bool FP8, bool EXACT>
+__global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
+  constexpr int DT = HD / 16, KS = HD / 32, kRows = kRowWaves * CT * 16;
+  __shared__ v8h sk[2][kTile * HD / 8], sv[2][kTile * HD / 8];
+  __shared__ float ss[2][8];
+  __shared__ RowLine line;
+  __shared__ unsigned before;
+  const KvCacheParams &cp = p.a.c;
+  const int tid = threadIdx.x, lane = tid % 64, c = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  if (p.fill) FillInvalid(p);
+  const int64_t units = MakeRowLine(p, line, kRows);
+  const int64_t piece = (units + gridDim.x - 1) / gridDim.x;
+  int64_t u = (int64_t)blockIdx.x * piece;
+  const int64_t end = u + piece < units ? u + piece : units;
+  for (int part = 0; u < end; part = 1) {
+    const Job j = FindRowJob(p, line, u, kRows);
+    const int t0 = (int)(u - j.first), t1 = (int)(end - j.first < j.tiles ? end - j.first : j.tiles);
+    const int wrow = j.row0 + wave * CT * 16, rows = j.n * p.group, before_new = j.len - j.n;
+    TileStage<HD, FP8, EXACT> st;
+    st.Lookup(cp, j, t0);
+    st.Load(cp, j, t0);
+    st.Lookup(cp, j, min(t0 + 1, t1 - 1));
+    v8h q[CT][KS];
+    float qf[CT];
+    int last[CT];  // the last token that the row sees
+#pragma unroll
+    for (int r = 0; r < CT; ++r) {
+      const int row = wrow + 16 * r + c, token = row < rows ? row / p.group : 0;
+      const int64_t at = ((cp.start[j.b] + (int64_t)token) * p.a.heads + j.head * p.group + row % p.group) * cp.head_dim;
+      last[r] = before_new + token;
+      LoadQ<KS, EXACT>(p.a, at, row < rows, g, q[r], qf[r]);
+    }
+    __syncthreads();  // the buffers of the job before were read
+    st.Store(sk[0], sv[0], ss[0], j.len - t0 * kTile);
+    st.Load(cp, j, min(t0 + 1, t1 - 1));
+    st.Lookup(cp, j, min(t0 + 2, t1 - 1));
+    v4f o[CT][DT];
+    float mo[CT], sum[CT];
+#pragma unroll
+    for (int r = 0; r < CT; ++r) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[r][d] = v4f{0.f, 0.f, 0.f, 0.f};
+      mo[r] = kNone;
+      sum[r] = 0.f;
+    }
+    // the tokens that every row of the wave sees end here
+    const int all_see = before_new + min(wrow, rows - 1) / p.group + 1;
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1, base = t * kTile;
+      const v8h *ck = sk[buf], *cv = sv[buf];
+      v4f s[CT][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int r = 0; r < CT; ++r) s[r][i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const v8h a = ck[KeyChunk<HD>(16 * (c / 4) + 4 * i + c % 4, 4 * k + g)];
+#pragma unroll
+          for (int r = 0; r < CT; ++r) s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[r][k], s[r][i], 0, 0, 0);
+        }
+      }
+      const float ks = ss[buf][g], vs = ss[buf][4 + g];
+      const float lv = LogScale(vs), inv = InvScale(vs);
+      const bool edge = base + kTile > all_see;
+      v8h pr[CT][2];
+#pragma unroll
+      for (int r = 0; r < CT; ++r) {
+        const float cs = ks * qf[r];
+        const int seen = last[r] - base - 16 * g;  // the row sees the lane's tokens 0 .. seen
+        float top = s[r][0][0];
+        if (edge) {
+          top = -__builtin_huge_valf();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = i <= seen ? fmaxf(top, s[r][i / 4][i % 4]) : top;
+        } else {
+          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i / 4][i % 4]);
+        }
+        top = GroupMax(Weight(top, cs, lv));
+        if (__any(top > mo[r] + kLag)) {
+          const float now = fmaxf(mo[r], top), keep = __builtin_amdgcn_exp2f(mo[r] - now);
+          mo[r] = now;
+          sum[r] *= keep;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[r][d] *= keep;
+        }
+        const float off = lv - mo[r];
+        // one fused step rounds otherwise than mo was made, by an ulp of mo: from
+        // 2^12 on that is left to the exact difference
+        const bool slow = edge || __any(fabsf(mo[r]) > 4096.f && mo[r] > kNone);
+        float ps = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float x = __builtin_fmaf(s[r][i / 4][i % 4], cs, off);
+          if (slow) x = i > seen ? -__builtin_huge_valf() : Weight(s[r][i / 4][i % 4], cs, lv) - mo[r];
+          const float w = __builtin_amdgcn_exp2f(x);
+          ps += w;
+          pr[r][i / 8][i % 8] = (_Float16)w;
+        }
+        sum[r] = __builtin_fmaf(ps, inv, sum[r]);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const v8h a = cv[ValueChunk(16 * d + c, 2 * g + h)];
+#pragma unroll
+          for (int r = 0; r < CT; ++r) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pr[r][h], o[r][d], 0, 0, 0);
+        }
+      if (t + 1 < t1) {
+        st.Store(sk[buf ^ 1], sv[buf ^ 1], ss[buf ^ 1], j.len - (t + 1) * kTile);
+        st.Load(cp, j, min(t + 2, t1 - 1));
+        st.Lookup(cp, j, min(t + 3, t1 - 1));
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < CT; ++r) sum[r] = GroupSum(sum[r]);
+    const bool whole = t0 == 0 && t1 == j.tiles;
+    const int slot = (int)blockIdx.x * 2 + part;
+    if (!whole) {
+#pragma unroll
+      for (int r = 0; r < CT; ++r) {
+        const int at = (slot * kRowWaves + wave) * CT + r;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, o[r][d]), Rsrc(p.part), ((at * DT + d) * 64 + lane) * 16,
+                                                 0, kDeviceScope);
+        if (g == 0) {
+          PutStat(p, at, 0, c, mo[r]);
+          PutStat(p, at, 1, c, sum[r]);
+        }
+      }
+      const int w0 = Uniform((int)(j.first / piece)), w1 = Uniform((int)((j.first + j.tiles - 1) / piece));
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (tid == 0) before = atomicAdd(p.done + w0, 1u);
+      __syncthreads();
+      if (before != (unsigned)(w1 - w0)) {
+        u = j.first + t1;
+        continue;
+      }
+      if (tid == 0) p.done[w0] = 0;
+      const int first = w0 * 2 + (j.first > w0 * piece ? 1 : 0);
+#pragma unroll
+      for (int r = 0; r < CT; ++r) {
+        mo[r] = kNone;
+        sum[r] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int w = w0; w <= w1; ++w)
+          mo[r] = fmaxf(mo[r], GetStat(p, ((w == w0 ? first : w * 2) * kRowWaves + wave) * CT + r, 0, c));
+        for (int w = w0; w <= w1; ++w) {
+          const int at = ((w == w0 ? first : w * 2) * kRowWaves + wave) * CT + r;
+          const float f = __builtin_amdgcn_exp2f(GetStat(p, at, 0, c) - mo[r]);
+          sum[r] += GetStat(p, at, 1, c) * f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            o[r][d] += __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(
+                                                   Rsrc(p.part), ((at * DT + d) * 64 + lane) * 16, 0, kDeviceScope)) * f;
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < CT; ++r) {
+      Job rj = j;
+      rj.row0 = wrow + 16 * r;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) StoreRows(p, rj, d, o[r][d], sum[r]);
     }
     u = j.first + t1;
   }
@@ -520,30 +919,84 @@ template <int HD> void LaunchDecode(const Plan &p, int64_t grid, hipStream_t s) 
     exact ? KvDecodeKernel<HD, false, true><<<g, kThreads, 0, s>>>(p) : KvDecodeKernel<HD, false, false><<<g, kThreads, 0, s>>>(p);
 }
 
+template <int HD, int CT> void LaunchPrompt(const Plan &p, int64_t grid, hipStream_t s) {
+  const dim3 g((unsigned)grid);
+  const bool exact = p.a.c.head_dim == HD;
+  if (p.a.c.fp8)
+    exact ? KvPromptKernel<HD, CT, true, true><<<g, kRowThreads, 0, s>>>(p)
+          : KvPromptKernel<HD, CT, true, false><<<g, kRowThreads, 0, s>>>(p);
+  else
+    exact ? KvPromptKernel<HD, CT, false, true><<<g, kRowThreads, 0, s>>>(p)
+          : KvPromptKernel<HD, CT, false, false><<<g, kRowThreads, 0, s>>>(p);
+}
+
+// Sequences with at most this many rows (new tokens * heads of a group) take
+// the decoding kernel, the others the prompt kernel; a launch that no sequence
+// can need is left out.
+constexpr int kFewRows = 32;
+
+struct Split {
+  bool decode, prompt;
+  int64_t decode_grid, prompt_grid;
+};
+
+int64_t PromptRows(const KvAttentionParams &p) { return kRowWaves * 16 * (p.c.head_dim > 128 ? 1 : 2); }
+
+Split SplitOf(const KvAttentionParams &p) {
+  const KvCacheParams &c = p.c;
+  const int64_t group = p.heads / c.kv_heads;
+  // the most and the least rows that a sequence may have
+  const int64_t known = p.max_query > 0 && p.max_query < c.tokens ? p.max_query : c.tokens;
+  const int64_t most = known * group;
+  const int64_t least = c.tokens - (c.batch - 1) * known;
+  Split s;
+  s.prompt = c.batch > 0 && most > kFewRows;
+  s.decode = !s.prompt || least * group <= kFewRows;
+  s.decode_grid = DecodeGrid(p);
+  const int64_t jobs = (c.tokens * group / PromptRows(p) + c.batch) * c.kv_heads;
+  const int64_t tiles = ((int64_t)c.max_blocks * c.block_tokens + kTile - 1) / kTile;
+  s.prompt_grid = std::max<int64_t>(1, std::min<int64_t>(jobs * tiles, Ctx().num_cus));
+  return s;
+}
+
 }  // namespace
 
 size_t KvAttentionScratchBytes(const KvAttentionParams &p) {
-  const size_t slots = (size_t)DecodeGrid(p) * 2;
-  return Scratch::Round(slots * 16 * HeadTile(p.c.head_dim) * sizeof(float)) + slots * 48 * sizeof(float);
+  const Split s = SplitOf(p);
+  const size_t slots = 2 * std::max<size_t>(s.decode ? s.decode_grid * 16 : 0, s.prompt ? s.prompt_grid * PromptRows(p) : 0);
+  return Scratch::Round(slots * HeadTile(p.c.head_dim) * sizeof(float)) + slots * 2 * sizeof(float);
 }
 
 void LaunchKvCacheAttention(const KvAttentionParams &a, void *scratch, hipStream_t stream) {
-  const int64_t grid = DecodeGrid(a);
+  const Split sp = SplitOf(a);
   const int hd = HeadTile(a.c.head_dim);
+  const size_t slots = 2 * std::max<size_t>(sp.decode ? sp.decode_grid * 16 : 0, sp.prompt ? sp.prompt_grid * PromptRows(a) : 0);
   Plan p{};
   p.a = a;
   p.group = a.heads / a.c.kv_heads;
-  p.rows_max = 0x7fffffff;
+  // a launch that stands alone has every sequence, also where max_query was wrong
+  p.rows_max = !sp.prompt ? 0x7fffffff : !sp.decode ? 0 : kFewRows;
   p.fill = 1;
-  p.done = Ctx().ws.Counters((size_t)grid);
+  p.done = Ctx().ws.Counters((size_t)std::max(sp.decode_grid, sp.prompt_grid));
   p.part = static_cast<float *>(scratch);
-  p.stat = reinterpret_cast<float *>(static_cast<char *>(scratch) + Scratch::Round((size_t)grid * 2 * 16 * hd * sizeof(float)));
-  if (hd == 64)
-    LaunchDecode<64>(p, grid, stream);
-  else if (hd == 128)
-    LaunchDecode<128>(p, grid, stream);
-  else
-    LaunchDecode<256>(p, grid, stream);
+  p.stat = reinterpret_cast<float *>(static_cast<char *>(scratch) + Scratch::Round(slots * hd * sizeof(float)));
+  if (sp.prompt) {
+    if (hd == 64)
+      LaunchPrompt<64, 2>(p, sp.prompt_grid, stream);
+    else if (hd == 128)
+      LaunchPrompt<128, 2>(p, sp.prompt_grid, stream);
+    else
+      LaunchPrompt<256, 1>(p, sp.prompt_grid, stream);
+    p.fill = 0;
+  }
+  if (sp.decode) {
+    if (hd == 64)
+      LaunchDecode<64>(p, sp.decode_grid, stream);
+    else if (hd == 128)
+      LaunchDecode<128>(p, sp.decode_grid, stream);
+    else
+      LaunchDecode<256>(p, sp.decode_grid, stream);
+  }
 }
 
 }  // namespace onnxl_amd

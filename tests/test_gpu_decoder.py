@@ -470,6 +470,12 @@ def test_attention_of_what_does_not_fit_is_nan(gpu, n):
     assert torch.isnan(got[:3 * n]).all() and torch.equal(got[3 * n:], want[3 * n:])
 
 
+@pytest.mark.parametrize("hint", [1, 20, 50, 10 ** 6])
+def test_attention_with_a_wrong_hint(gpu, hint):
+    b = dc.Batch(3, [1, 50, 3, 20], [100, 90, 30, 300], 2, 64, 16, "fp8", torch.bfloat16, heads=4)
+    check_attention(gpu, b, max_query=hint)
+
+
 def test_nothing_to_do(gpu):
     b = dc.Batch(2, [0, 0], [5, 0], 2, 64, 16, "int8", torch.float16, heads=2)
     assert gpu.kv_cache_attention(b.q.cuda(), b.cache(gpu), *b.index()).shape == (0, 2, 64)
