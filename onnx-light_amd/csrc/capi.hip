@@ -3347,19 +3347,21 @@ int MxMatMul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t
   OLA_ENFORCE(Is16Bit(y->data_type) && (!quantise || y->data_type == a->data_type), kMxmName,
               ": y must be FLOAT16 or BFLOAT16, and a's type where a has 16 bits.");
   NeedShape(y, s, kMxmName, "y");
-  OLA_ENFORCE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31), kMxmName,
-              ": a dimension of 2^31 or more.");
+  OLA_ENFORCE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 22), kMxmName,
+              ": M or N of 2^31 or more, or K of 2^22 or more.");
   if (M == 0 || N == 0) return ONNXL_AMD_OK;
   Ctx();
-  const bool a4 = quantise ? a_type == kFloat4E2M1 : a->data_type != kFloat8E4M3FN;
-  const size_t codes = Scratch::Round((size_t)(a4 ? M * K / 2 : M * K)), scales = (size_t)(M * K / 32);
-  Staging st(stream, quantise ? codes + scales + 256 : 0, {a, quantise ? nullptr : a_scale, b, b_scale}, {y});
   MxMatMulParams p{};
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.x = quantise ? a->data : nullptr;
+  p.x_dtype = a->data_type;
+  p.a_fp4 = quantise ? a_type == kFloat4E2M1 : a->data_type != kFloat8E4M3FN;
+  p.y_bf16 = y->data_type == kBfloat16;
+  Staging st(stream, MxMatMulScratchBytes(p), {a, quantise ? nullptr : a_scale, b, b_scale}, {y});
   if (quantise) {
-    uint8_t *q = static_cast<uint8_t *>(st.Extra());
-    LaunchMxQuantize(MxQuantParams{st.In(a), q, q + codes, M, K, a->data_type, a4}, stream);
-    p.a = q;
-    p.a_scale = q + codes;
+    p.x = st.In(a);
   } else {
     p.a = static_cast<const uint8_t *>(st.In(a));
     p.a_scale = static_cast<const uint8_t *>(st.In(a_scale));
@@ -3367,14 +3369,9 @@ int MxMatMul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t
   p.b = static_cast<const uint8_t *>(st.In(b));
   p.b_scale = static_cast<const uint8_t *>(st.In(b_scale));
   p.y = st.Out(y);
-  p.M = M;
-  p.N = N;
-  p.K = K;
-  p.a_fp4 = a4;
-  p.y_bf16 = y->data_type == kBfloat16;
   OLA_ENFORCE(reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0, kMxmName,
               ": the codes must be 16-byte aligned.");
-  LaunchMxMatMul(p, stream);
+  LaunchMxMatMul(p, st.Extra(), stream);
   OLA_HIP(hipGetLastError());
   st.Finish();
   return ONNXL_AMD_OK;

@@ -50,18 +50,21 @@ struct MxQuantParams {
 };
 void LaunchMxQuantize(const MxQuantParams &p, hipStream_t stream);
 
-// y[m, n] = sum over blocks of 2^(sa + sb) * sum of a[m, k] b[n, k]
+// y[m, n] = sum over blocks of 2^(sa + sb) * sum of a[m, k] b[n, k]; M, N > 0
 struct MxMatMulParams {
-  const uint8_t *a;        // [M, K] E4M3 or E2M1 codes
+  const void *x;           // [M, K] FLOAT16 or BFLOAT16, quantized by the call; or nullptr and
+  const uint8_t *a;        // [M, K] E4M3 or E2M1 codes with
   const uint8_t *a_scale;  // [M, K / 32]
   const uint8_t *b;        // [N, K] E2M1 codes
   const uint8_t *b_scale;  // [N, K / 32]
   void *y;                 // [M, N] FLOAT16 or BFLOAT16
   int64_t M, N, K;
-  int a_fp4;
+  int x_dtype;             // of x
+  int a_fp4;               // a's codes are (or x's become) E2M1, else E4M3
   int y_bf16;
 };
-void LaunchMxMatMul(const MxMatMulParams &p, hipStream_t stream);
+size_t MxMatMulScratchBytes(const MxMatMulParams &p);
+void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream);
 
 // ---------------------------------------------------------------------------
 // Paged 8-bit cache.

@@ -3,85 +3,136 @@
 #include "common.hpp"
 #include "decoder.hpp"
 #include "device_codecs.hpp"
+#include "mx_gemm.hpp"
 #include "quant8.hpp"
 
 namespace onnxl_amd {
 namespace {
 
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-
-template <int DT> __device__ __forceinline__ float LoadX(const void *p, int64_t i) {
-  if constexpr (DT == kFloat) return static_cast<const float *>(p)[i];
-  if constexpr (DT == kFloat16) return F16ToF32(static_cast<const uint16_t *>(p)[i]);
-  return Bf16ToF32(static_cast<const uint16_t *>(p)[i]);
+// Eight values per thread, four neighbouring threads per block.  Where `tiles`
+// is given the output is the GEMM's (mx_gemm.hpp): scales there, rows padded to
+// whole steps with zero codes of scale 1.
+template <int DT, bool FP4> __device__ __forceinline__ void QuantizeRow8(const MxQuantParams &p, uint8_t *tiles, int64_t i) {
+  const int64_t steps = (p.K + 255) / 256, per_row = tiles ? steps * 32 : p.K / 8, row = i / per_row, k8 = i % per_row;
+  if (k8 * 8 >= p.K) {
+    if constexpr (FP4)
+      *reinterpret_cast<unsigned *>(p.y + i * 4) = 0;
+    else
+      *reinterpret_cast<uint2 *>(p.y + i * 8) = make_uint2(0, 0);
+    if (k8 % 4 == 0) tiles[mx::ScaleTileAt(row, k8 / 4, steps)] = 127;
+    return;
+  }
+  const int64_t at = row * p.K + k8 * 8;
+  float v[8];
+  if constexpr (DT == kFloat) {
+    const float *x = static_cast<const float *>(p.x) + at;
+    __builtin_memcpy(v, x, 32);
+  } else {
+    uint16_t u[8];
+    __builtin_memcpy(u, static_cast<const uint16_t *>(p.x) + at, 16);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = DT == kFloat16 ? F16ToF32(u[j]) : Bf16ToF32(u[j]);
+  }
+  // the largest magnitude as bits: a NaN is larger than any number, and stays
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, __builtin_bit_cast(unsigned, v[j]) & 0x7fffffffu);
+  top = max(top, (unsigned)__shfl_xor((int)top, 1));
+  top = max(top, (unsigned)__shfl_xor((int)top, 2));
+  const BlockScale s = MxScaleOf(__builtin_bit_cast(float, top), FP4 ? 2 : 8);
+  if (s.e8m0 == 255) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  }
+  if constexpr (FP4) {
+    unsigned c = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) c |= Fp4Codes2(v[j] * s.inv, v[j + 1] * s.inv) << (4 * j);
+    *reinterpret_cast<unsigned *>(p.y + i * 4) = c;
+  } else {
+    unsigned lo = Fp8Codes2(v[0] * s.inv, v[1] * s.inv) | Fp8Codes2(v[2] * s.inv, v[3] * s.inv) << 16;
+    unsigned hi = Fp8Codes2(v[4] * s.inv, v[5] * s.inv) | Fp8Codes2(v[6] * s.inv, v[7] * s.inv) << 16;
+    *reinterpret_cast<uint2 *>(p.y + i * 8) = make_uint2(lo, hi);
+  }
+  if (k8 % 4 == 0) {
+    if (tiles)
+      tiles[mx::ScaleTileAt(row, k8 / 4, steps)] = s.e8m0;
+    else
+      p.scale[i / 4] = s.e8m0;
+  }
 }
 
-// One block of 32 values per thread.
 template <int DT> __global__ __launch_bounds__(256) void MxQuantizeKernel(const MxQuantParams p) {
-  const int64_t blk = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (blk >= p.rows * (p.K / 32)) return;
-  float v[32], top = 0.f;
-  bool finite = true;
-  for (int i = 0; i < 32; ++i) {
-    v[i] = LoadX<DT>(p.x, blk * 32 + i);
-    finite = finite && fabsf(v[i]) < __builtin_huge_valf();
-    top = fmaxf(top, fabsf(v[i]));
-  }
-  const BlockScale s = MxScaleOf(finite ? top : __builtin_huge_valf(), p.fp4 ? 2 : 8);
-  p.scale[blk] = s.e8m0;
-  if (s.e8m0 == 255)
-    for (int i = 0; i < 32; ++i) v[i] = 0.f;
-  for (int i = 0; i < 32; i += 2) {
-    if (p.fp4) {
-      p.y[(blk * 32 + i) / 2] = (uint8_t)Fp4Codes2(v[i] * s.inv, v[i + 1] * s.inv);
-    } else {
-      p.y[blk * 32 + i] = Fp8Code(v[i] * s.inv);
-      p.y[blk * 32 + i + 1] = Fp8Code(v[i + 1] * s.inv);
-    }
-  }
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.rows * (p.K / 8)) return;
+  if (p.fp4)
+    QuantizeRow8<DT, true>(p, nullptr, i);
+  else
+    QuantizeRow8<DT, false>(p, nullptr, i);
 }
 
-// One wave per 16 x 16 outputs, operands straight from memory.  Lane l holds
-// row l % 16 of an operand: for E2M1 the 32 values from 32 (l / 16), for E4M3
-// the 16 from 16 (l / 16) and the 16 from 64 + 16 (l / 16), and the scale of
-// block l / 16 in both.
-template <bool A4> __global__ __launch_bounds__(64) void MxMatMulKernel(const MxMatMulParams p) {
-  const int lane = threadIdx.x, r = lane % 16, g = lane / 16;
-  const int64_t m = (int64_t)blockIdx.y * 16 + r, n = (int64_t)blockIdx.x * 16 + r;
-  const int64_t am = m < p.M ? m : p.M - 1, bn = n < p.N ? n : p.N - 1;
-  v4f acc = {0.f, 0.f, 0.f, 0.f};
-  auto load = [&](const uint8_t *row, int64_t at, int64_t bytes, v8i &dst, int first) {
-    for (int i = 0; i < 4; ++i)
-      dst[first + i] = at + 4 * i + 4 <= bytes ? *reinterpret_cast<const int *>(row + at + 4 * i) : 0;
-  };
-  for (int64_t k = 0; k < p.K; k += 128) {
-    v8i a = {0, 0, 0, 0, 0, 0, 0, 0}, b = {0, 0, 0, 0, 0, 0, 0, 0};
-    load(p.b + bn * (p.K / 2), k / 2 + 16 * g, p.K / 2, b, 0);
-    if constexpr (A4) {
-      load(p.a + am * (p.K / 2), k / 2 + 16 * g, p.K / 2, a, 0);
-    } else {
-      load(p.a + am * p.K, k + 16 * g, p.K, a, 0);
-      load(p.a + am * p.K, k + 64 + 16 * g, p.K, a, 4);
-    }
-    const int64_t blk = k / 32 + g, blocks = p.K / 32;
-    const int sa = blk < blocks ? p.a_scale[am * blocks + blk] : 127;
-    const int sb = blk < blocks ? p.b_scale[bn * blocks + blk] : 127;
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, A4 ? 4 : 0, 4, 0, sa, 0, sb);
+// ---------------------------------------------------------------------------
+// The GEMM's operands: b's scales (and a's, where a comes as codes) in tiles,
+// and a quantized where it has 16 bits, in one launch.
+
+// Eight blocks (a step) of one row per thread; blocks past the row's end get
+// the scale 1, for their codes read as zeros.
+__device__ __forceinline__ void TileScales(const uint8_t *scale, uint8_t *tiles, int64_t rows, int64_t K, int64_t i) {
+  const int64_t steps = (K + 255) / 256, blocks = K / 32, row = i % rows, t = i / rows;
+  const uint8_t *s = scale + row * blocks + t * 8;
+  uint8_t b[8];
+  if (t * 8 + 8 <= blocks) {
+    __builtin_memcpy(b, s, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = t * 8 + j < blocks ? s[j] : 127;
   }
-  for (int i = 0; i < 4; ++i) {
-    const int64_t mo = (int64_t)blockIdx.y * 16 + 4 * g + i;
-    if (mo < p.M && n < p.N)
-      static_cast<uint16_t *>(p.y)[mo * p.N + n] = p.y_bf16 ? F32ToBf16(acc[i]) : F32ToF16(acc[i]);
+  unsigned *d = reinterpret_cast<unsigned *>(tiles) + (row / 32 * steps + t) * 64 + row % 32;
+  d[0] = b[0] | b[2] << 8 | b[4] << 16 | (unsigned)b[6] << 24;
+  d[32] = b[1] | b[3] << 8 | b[5] << 16 | (unsigned)b[7] << 24;
+}
+
+struct MxOperands {
+  MxQuantParams q;            // a to be quantized: x set
+  const uint8_t *a, *a_scale, *b_scale;
+  uint8_t *codes;             // a's codes with padded rows, where K is not whole steps
+  uint8_t *a_tiles, *b_tiles;
+  int64_t M, N, K;
+  int64_t b_groups;           // workgroups of b's part
+};
+
+template <int DT> __global__ __launch_bounds__(256) void MxOperandsKernel(const MxOperands p) {
+  const int64_t steps = (p.K + 255) / 256;
+  if ((int64_t)blockIdx.x < p.b_groups) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < p.N * steps) TileScales(p.b_scale, p.b_tiles, p.N, p.K, i);
+    return;
   }
+  const int64_t i = ((int64_t)blockIdx.x - p.b_groups) * 256 + threadIdx.x;
+  if (!p.q.x) {
+    if (i < p.M * steps) TileScales(p.a_scale, p.a_tiles, p.M, p.K, i);
+    if (!p.codes) return;
+    const int64_t bytes = p.q.fp4 ? p.K / 2 : p.K, pitch = steps * (p.q.fp4 ? 128 : 256);
+    const int64_t row = i / (pitch / 16), c = i % (pitch / 16) * 16;
+    if (row >= p.M) return;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (c < bytes) v = *reinterpret_cast<const uint4 *>(p.a + row * bytes + c);
+    *reinterpret_cast<uint4 *>(p.codes + row * pitch + c) = v;
+    return;
+  }
+  if (i >= p.M * steps * 32) return;
+  if (p.q.fp4)
+    QuantizeRow8<DT, true>(p.q, p.a_tiles, i);
+  else
+    QuantizeRow8<DT, false>(p.q, p.a_tiles, i);
 }
 
 }  // namespace
 
 void LaunchMxQuantize(const MxQuantParams &p, hipStream_t stream) {
-  const int64_t blocks = p.rows * (p.K / 32);
-  if (blocks == 0) return;
-  const dim3 grid((unsigned)((blocks + 255) / 256));
+  const int64_t n = p.rows * (p.K / 8);
+  if (n == 0) return;
+  const dim3 grid((unsigned)((n + 255) / 256));
   if (p.x_dtype == kFloat)
     MxQuantizeKernel<kFloat><<<grid, 256, 0, stream>>>(p);
   else if (p.x_dtype == kFloat16)
@@ -90,12 +141,65 @@ void LaunchMxQuantize(const MxQuantParams &p, hipStream_t stream) {
     MxQuantizeKernel<kBfloat16><<<grid, 256, 0, stream>>>(p);
 }
 
-void LaunchMxMatMul(const MxMatMulParams &p, hipStream_t stream) {
-  const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)((p.M + 15) / 16));
+namespace {
+
+int64_t Ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Scratch: codes (where they are not a's own) and scale tiles of a, scale tiles
+// of b.
+struct MxScratch {
+  size_t codes, a_tiles, b_tiles;
+  explicit MxScratch(const MxMatMulParams &p)
+      : codes(p.x || p.K % 256 ? Scratch::Round((size_t)(p.M * Ceil(p.K, 256) * (p.a_fp4 ? 128 : 256))) : 0),
+        a_tiles(Scratch::Round((size_t)mx::ScaleTileBytes(p.M, p.K))),
+        b_tiles(Scratch::Round((size_t)mx::ScaleTileBytes(p.N, p.K))) {}
+};
+
+template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, hipStream_t s) {
+  using S = mx::Shape<A4, MB, NB>;
+  const int64_t tiles = Ceil(g.M, S::BM) * Ceil(g.N, S::BN);
+  mx::GemmKernel<A4, MB, NB><<<dim3((unsigned)tiles), 256, 0, s>>>(g);
+}
+
+}  // namespace
+
+size_t MxMatMulScratchBytes(const MxMatMulParams &p) {
+  const MxScratch s(p);
+  return s.codes + s.a_tiles + s.b_tiles;
+}
+
+void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) {
+  const MxScratch s(p);
+  uint8_t *codes = static_cast<uint8_t *>(scratch), *a_tiles = codes + s.codes, *b_tiles = a_tiles + s.a_tiles;
+  const int64_t steps = Ceil(p.K, 256);
+  MxOperands o{};
+  o.a_scale = p.a_scale;
+  o.b_scale = p.b_scale;
+  o.a_tiles = a_tiles;
+  o.b_tiles = b_tiles;
+  o.M = p.M;
+  o.N = p.N;
+  o.K = p.K;
+  o.b_groups = Ceil(p.N * steps, 256);
+  o.q = MxQuantParams{p.x, codes, nullptr, p.M, p.K, p.x_dtype, p.a_fp4};
+  o.a = p.a;
+  o.codes = s.codes ? codes : nullptr;
+  // a thread per 8 values to quantize, or 16 bytes of codes to copy, or a step's scales
+  const int64_t a_threads = p.M * steps * (p.x ? 32 : !s.codes ? 1 : p.a_fp4 ? 8 : 16);
+  const dim3 grid((unsigned)(o.b_groups + Ceil(a_threads, 256)));
+  if (grid.x == 0) {
+    // K = 0: no operands, sums of nothing
+  } else if (p.x_dtype == kFloat16) {
+    MxOperandsKernel<kFloat16><<<grid, 256, 0, stream>>>(o);
+  } else {
+    MxOperandsKernel<kBfloat16><<<grid, 256, 0, stream>>>(o);
+  }
+  const mx::GemmArgs g{s.codes ? codes : p.a, p.b, a_tiles, b_tiles, static_cast<uint16_t *>(p.y), p.M, p.N, p.K, p.y_bf16,
+                       p.N % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0};
   if (p.a_fp4)
-    MxMatMulKernel<true><<<grid, 64, 0, stream>>>(p);
+    LaunchGemm<true, 4, 4>(g, stream);
   else
-    MxMatMulKernel<false><<<grid, 64, 0, stream>>>(p);
+    LaunchGemm<false, 2, 4>(g, stream);
 }
 
 }  // namespace onnxl_amd
