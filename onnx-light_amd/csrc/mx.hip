@@ -4,6 +4,7 @@
 #include "decoder.hpp"
 #include "device_codecs.hpp"
 #include "mx_gemm.hpp"
+#include "mx_stream.hpp"
 #include "quant8.hpp"
 
 namespace onnxl_amd {
@@ -161,14 +162,58 @@ template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, hipStr
   mx::GemmKernel<A4, MB, NB><<<dim3((unsigned)tiles), 256, 0, s>>>(g);
 }
 
+// Few rows take the streaming kernel.
+constexpr int64_t kStreamRows = 64;
+bool Streams(const MxMatMulParams &p) { return p.M <= kStreamRows; }
+
+// Up to this many values every workgroup quantizes its activations itself
+// (eight at a time per thread); a launch for all costs about 4 us.
+constexpr int64_t kOwnQuant = 16384;
+bool OwnQuant(const MxMatMulParams &p) { return p.x && p.M <= 16 && p.M * Ceil(p.K, 512) * 512 <= kOwnQuant; }
+
+template <bool A4, int MT, bool QUANT> void LaunchStream(const mx::StreamArgs &a, hipStream_t s) {
+  const int64_t chunks = Ceil(a.K, 512);
+  const int waves = chunks > 8 ? mx::kStreamWaves<MT> : 8;
+  const size_t codes = QUANT ? (size_t)(a.M * chunks * ((A4 ? 256 : 512) + 16)) : 0;
+  const size_t lds = std::max(codes, (size_t)MT * waves * 1024);
+  mx::StreamKernel<A4, 1, MT, QUANT><<<dim3((unsigned)Ceil(a.N, 16)), 64 * waves, lds, s>>>(a);
+}
+
+template <bool A4> void LaunchStreamOf(const mx::StreamArgs &a, bool own, hipStream_t s) {
+  if (own)
+    LaunchStream<A4, 1, true>(a, s);
+  else if (a.M <= 16)
+    LaunchStream<A4, 1, false>(a, s);
+  else if (a.M <= 32)
+    LaunchStream<A4, 2, false>(a, s);
+  else if (a.M <= 48)
+    LaunchStream<A4, 3, false>(a, s);
+  else
+    LaunchStream<A4, 4, false>(a, s);
+}
+
 }  // namespace
 
 size_t MxMatMulScratchBytes(const MxMatMulParams &p) {
+  if (Streams(p)) return p.x && !OwnQuant(p) ? Scratch::Round((size_t)(p.M * p.K)) + (size_t)(p.M * p.K / 32) : 0;
   const MxScratch s(p);
   return s.codes + s.a_tiles + s.b_tiles;
 }
 
 void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) {
+  if (Streams(p)) {
+    mx::StreamArgs a{p.x, p.a, p.a_scale, p.b, p.b_scale, static_cast<uint16_t *>(p.y), (int)p.M, (int)p.N, (int)p.K,
+                     p.x_dtype == kBfloat16, p.y_bf16};
+    const bool own = OwnQuant(p);
+    if (p.x && !own) {
+      uint8_t *codes = static_cast<uint8_t *>(scratch), *scales = codes + Scratch::Round((size_t)(p.M * p.K));
+      LaunchMxQuantize(MxQuantParams{p.x, codes, scales, p.M, p.K, p.x_dtype, p.a_fp4}, stream);
+      a.a = codes;
+      a.as = scales;
+    }
+    p.a_fp4 ? LaunchStreamOf<true>(a, own, stream) : LaunchStreamOf<false>(a, own, stream);
+    return;
+  }
   const MxScratch s(p);
   uint8_t *codes = static_cast<uint8_t *>(scratch), *a_tiles = codes + s.codes, *b_tiles = a_tiles + s.a_tiles;
   const int64_t steps = Ceil(p.K, 256);

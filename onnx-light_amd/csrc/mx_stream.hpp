@@ -1,0 +1,218 @@
+// Block-scaled product for few rows (decoding): y[M, N] = a[M, K] b[N, K]^T with
+// the MXFP4 weight read once, straight into the operand registers of
+// v_mfma_scale_f32_16x16x128_f8f6f4.
+//
+// The weight's bytes are the cost, so the k of the instruction is dealt out for
+// their sake: of a chunk of 512 values (16 blocks of 32) lane group g = l / 16
+// takes the blocks 4 g .. 4 g + 3 of row l % 16, 64 consecutive bytes, and block
+// 4 g + j is its operand of the chunk's instruction j.  A chunk's 256 bytes of a
+// row are two whole lines, and its 16 scales one dword per lane, whose byte j is
+// selected by the instruction.  The activations follow the same order: E2M1
+// codes like the weight's; for E4M3 the instruction wants of lane group g the
+// half g % 2 of its blocks g / 2 and 2 + g / 2, which are the chunk's blocks
+// 4 (g / 2) + j and 4 (2 + g / 2) + j.
+//
+// A workgroup has 16 NT rows of the weight; its waves take the chunks in turn
+// and add up in LDS.  Activations of 16 bits that are few enough are quantized
+// by every workgroup for itself, into LDS, while its first weight bytes are on
+// their way: that costs less than a launch of its own.
+#pragma once
+
+#include <type_traits>
+
+#include "mx_gemm.hpp"
+#include "quant8.hpp"
+
+namespace onnxl_amd {
+namespace mx {
+
+struct StreamArgs {
+  const void *x;                // [M, K] 16 bits, quantized here (QUANT); else
+  const uint8_t *a, *as;        // codes [M, K] and scales [M, K / 32]
+  const uint8_t *b, *bs;        // weight codes [N, K / 2] and scales [N, K / 32]
+  uint16_t *y;
+  int M, N, K;
+  int x_bf16, bf16;
+};
+
+// Four block scales from `at` on of a row of `blocks`; those past the end are 1.
+__device__ __forceinline__ int Scales4(const uint8_t *row, int at, int blocks) {
+  int v;
+  if (at + 4 <= blocks) {
+    __builtin_memcpy(&v, row + at, 4);
+  } else {
+    v = 0x7f7f7f7f;
+    for (int i = 0; at + i < blocks; ++i) v = (v & ~(0xff << (8 * i))) | row[at + i] << (8 * i);
+  }
+  return v;
+}
+
+// Waves of a workgroup: more rows need the registers of half of them.
+template <int MT> constexpr int kStreamWaves = MT == 1 ? 16 : 8;
+
+template <bool A4, int NT, int MT, bool QUANT>
+__global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const StreamArgs p) {
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+  const int blocks = p.K / 32, chunks = (blocks + 15) / 16;
+  const int n0 = blockIdx.x * 16 * NT;
+  const int64_t pitch_b = p.K / 2, pitch_a = A4 ? p.K / 2 : p.K;
+
+  // the weight's rows of this lane (rows past the last repeat it)
+  const uint8_t *bp[NT], *sp[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int64_t row = min(n0 + 16 * n + c, p.N - 1);
+    bp[n] = p.b + row * pitch_b;
+    sp[n] = p.bs + row * blocks;
+  }
+  v4i w[NT][4];
+  int ws[NT];
+  // blocks past the end are read as block 0: the activations there are zeros
+  auto load = [&](int ch) __attribute__((always_inline)) {
+    const int blk = 16 * ch + 4 * g;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[n][j] = *reinterpret_cast<const v4i *>(bp[n] + 16 * (blk + j < blocks ? blk + j : 0));
+      ws[n] = Scales4(sp[n], blk, blocks);
+    }
+  };
+
+  // codes in LDS: rows of whole chunks, then their scales
+  const int lds_row = chunks * (A4 ? 256 : 512), lds_scale = chunks * 16;
+  char *lds_s = lds + (QUANT ? p.M * lds_row : 0);
+  if (wave < chunks) load(wave);
+  if constexpr (QUANT) {
+    // eight values a thread, four neighbours a block; past the row's end zero
+    // codes of scale 1
+    const int per_row = chunks * 64;
+    for (int i = tid; i < p.M * per_row; i += blockDim.x) {
+      const int row = i / per_row, k8 = i % per_row;
+      float v[8];
+      unsigned top = 0;
+      const bool in = k8 * 8 < p.K;
+      uint16_t u[8] = {};
+      if (in) __builtin_memcpy(u, static_cast<const uint16_t *>(p.x) + (int64_t)row * p.K + k8 * 8, 16);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = p.x_bf16 ? __builtin_bit_cast(float, (unsigned)u[j] << 16) : (float)__builtin_bit_cast(_Float16, u[j]);
+        top = max(top, __builtin_bit_cast(unsigned, v[j]) & 0x7fffffffu);
+      }
+      top = max(top, (unsigned)__shfl_xor((int)top, 1));
+      top = max(top, (unsigned)__shfl_xor((int)top, 2));
+      const BlockScale s = MxScaleOf(__builtin_bit_cast(float, top), A4 ? 2 : 8);
+      if (s.e8m0 == 255) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      }
+      if constexpr (A4) {
+        unsigned code = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) code |= Fp4Codes2(v[j] * s.inv, v[j + 1] * s.inv) << (4 * j);
+        *reinterpret_cast<unsigned *>(lds + row * lds_row + k8 * 4) = code;
+      } else {
+        const unsigned lo = Fp8Codes2(v[0] * s.inv, v[1] * s.inv) | Fp8Codes2(v[2] * s.inv, v[3] * s.inv) << 16;
+        const unsigned hi = Fp8Codes2(v[4] * s.inv, v[5] * s.inv) | Fp8Codes2(v[6] * s.inv, v[7] * s.inv) << 16;
+        *reinterpret_cast<uint2 *>(lds + row * lds_row + k8 * 8) = make_uint2(lo, hi);
+      }
+      if (k8 % 4 == 0) lds_s[row * lds_scale + k8 / 4] = in ? (char)s.e8m0 : 127;
+    }
+    __syncthreads();
+  }
+
+  v4f acc[NT][MT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[n][m] = v4f{0.f, 0.f, 0.f, 0.f};
+  typedef std::conditional_t<A4, v4i, v8i> Frag;
+  // one chunk; `more` loads the wave's next one as soon as the registers are free
+  auto chunk = [&](int ch, auto more) __attribute__((always_inline)) {
+    const bool tail = 16 * ch + 16 > blocks;
+    Frag x[MT][4];
+    int xs[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = min(16 * m + c, p.M - 1);  // rows past the last repeat it
+      if constexpr (QUANT) {
+        const char *xp = lds + row * lds_row;
+        xs[m] = *reinterpret_cast<const int *>(lds_s + row * lds_scale + 16 * ch + 4 * g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (A4) {
+            x[m][j] = *reinterpret_cast<const v4i *>(xp + (16 * ch + 4 * g + j) * 16);
+          } else {
+            const int at = (16 * ch + 4 * (g >> 1) + j) * 32 + 16 * (g & 1);
+            x[m][j] = __builtin_shufflevector(*reinterpret_cast<const v4i *>(xp + at),
+                                              *reinterpret_cast<const v4i *>(xp + at + 256), 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+        }
+      } else {
+        const uint8_t *xp = p.a + row * pitch_a;
+        xs[m] = Scales4(p.as + (int64_t)row * blocks, 16 * ch + 4 * g, blocks);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (A4) {
+            const int blk = 16 * ch + 4 * g + j;
+            x[m][j] = *reinterpret_cast<const v4i *>(xp + 16 * (blk < blocks ? blk : 0));
+            if (tail) x[m][j] = blk < blocks ? x[m][j] : v4i{0, 0, 0, 0};
+          } else {
+            const int lo = 16 * ch + 4 * (g >> 1) + j, hi = lo + 8;
+            v4i u = *reinterpret_cast<const v4i *>(xp + 32 * (lo < blocks ? lo : 0) + 16 * (g & 1));
+            v4i v = *reinterpret_cast<const v4i *>(xp + 32 * (hi < blocks ? hi : 0) + 16 * (g & 1));
+            if (tail) {
+              u = lo < blocks ? u : v4i{0, 0, 0, 0};
+              v = hi < blocks ? v : v4i{0, 0, 0, 0};
+            }
+            x[m][j] = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+        }
+      }
+    }
+    auto mma = [&](auto j) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(Operand(w[n][j]), Operand(x[m][j]), acc[n][m], 4,
+                                                                       A4 ? 4 : 0, j, ws[n], j, xs[m]);
+    };
+    mma(std::integral_constant<int, 0>{});
+    mma(std::integral_constant<int, 1>{});
+    mma(std::integral_constant<int, 2>{});
+    mma(std::integral_constant<int, 3>{});
+    if constexpr (more) load(ch + waves);
+  };
+  int ch = wave;
+  for (; ch + waves < chunks; ch += waves) chunk(ch, std::true_type{});
+  if (ch < chunks) chunk(ch, std::false_type{});
+
+  // lane (c, g) of a tile has the columns 4 g .. 4 g + 3 of row c of y
+  v4f *part = reinterpret_cast<v4f *>(lds);
+  __syncthreads();  // the codes were read
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) part[((n * MT + m) * waves + wave) * 64 + lane] = acc[n][m];
+  __syncthreads();
+  for (int i = wave; i < NT * MT; i += waves) {
+    v4f s = part[i * waves * 64 + lane];
+    for (int v = 1; v < waves; ++v) s += part[(i * waves + v) * 64 + lane];
+    const int row = i % MT * 16 + c, col = n0 + i / MT * 16 + 4 * g;
+    if (row >= p.M) continue;
+    uint16_t *y = p.y + (int64_t)row * p.N + col;
+    uint16_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = Half(s[e], p.bf16);
+    if (col + 4 <= p.N) {
+      __builtin_memcpy(y, v, 8);
+    } else {
+      for (int e = 0; col + e < p.N; ++e) y[e] = v[e];
+    }
+  }
+}
+
+}  // namespace mx
+}  // namespace onnxl_amd
