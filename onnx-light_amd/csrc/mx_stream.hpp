@@ -36,15 +36,20 @@ struct StreamArgs {
 };
 
 // Four block scales from `at` on of a row of `blocks`; those past the end are 1.
-__device__ __forceinline__ int Scales4(const uint8_t *row, int at, int blocks) {
+// Near the row's end the bytes are loaded one by one, none past it and all at
+// once (behind a branch per byte they came one after the other).
+__device__ __forceinline__ int Scales4(const uint8_t *row, int at, int blocks, bool tail) {
   int v;
-  if (at + 4 <= blocks) {
+  if (!tail) {
     __builtin_memcpy(&v, row + at, 4);
-  } else {
-    v = 0x7f7f7f7f;
-    for (int i = 0; at + i < blocks; ++i) v = (v & ~(0xff << (8 * i))) | row[at + i] << (8 * i);
+    return v;
   }
-  return v;
+  const int n = blocks - at;
+  unsigned b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = row[max(min(at + i, blocks - 1), 0)];
+  const unsigned mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << 8 * n) - 1u;
+  return (int)(((b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24) & mask) | (0x7f7f7f7fu & ~mask));
 }
 
 // Waves of a workgroup: more rows need the registers of half of them.
@@ -76,7 +81,7 @@ __global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const Stre
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[n][j] = *reinterpret_cast<const v4i *>(bp[n] + 16 * (blk + j < blocks ? blk + j : 0));
-      ws[n] = Scales4(sp[n], blk, blocks);
+      ws[n] = Scales4(sp[n], blk, blocks, 16 * ch + 16 > blocks);
     }
   };
 
@@ -151,7 +156,7 @@ __global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const Stre
         }
       } else {
         const uint8_t *xp = p.a + row * pitch_a;
-        xs[m] = Scales4(p.as + (int64_t)row * blocks, 16 * ch + 4 * g, blocks);
+        xs[m] = Scales4(p.as + (int64_t)row * blocks, 16 * ch + 4 * g, blocks, tail);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if constexpr (A4) {

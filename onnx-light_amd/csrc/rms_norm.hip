@@ -1,5 +1,14 @@
 // RMS norm with the residual's addition and 8-bit output with scales: what a
 // decoder layer runs in front of its quantized products.
+//
+// Bound by memory: x and the residual are read once, the sum and the codes
+// written once.  A workgroup has a row and keeps it in registers between the
+// sum of squares and the quantization; rows that do not fit are read again (from
+// the caches) in pieces.  Every thread has groups of 8 consecutive values, so a
+// scale block of 32, 64, 128 or 256 values is 4 .. 32 neighbouring threads of a
+// wave and its maximum a few lane exchanges; a scale for the whole row is one
+// more join in LDS.  The largest magnitude is found on the bit patterns, where a
+// NaN is above every number.
 #include "common.hpp"
 #include "decoder.hpp"
 #include "device_codecs.hpp"
@@ -8,92 +17,258 @@
 namespace onnxl_amd {
 namespace {
 
-constexpr int kThreads = 256;
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
-template <int DT> __device__ __forceinline__ float LoadX(const void *p, int64_t i) {
-  if constexpr (DT == kFloat) return static_cast<const float *>(p)[i];
-  if constexpr (DT == kFloat16) return F16ToF32(static_cast<const uint16_t *>(p)[i]);
-  return Bf16ToF32(static_cast<const uint16_t *>(p)[i]);
+// Eight values from i on as fp32; those from `end` on are 0.  Whole groups are
+// one or two 16-byte loads from any address.
+template <int DT> __device__ __forceinline__ void Load8(const void *p, int64_t i, int64_t end, float (&v)[8]) {
+  if constexpr (DT == kFloat) {
+    const float *x = static_cast<const float *>(p);
+    if (i + 8 <= end) {
+      __builtin_memcpy(v, x + i, 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + j < end ? x[i + j] : 0.f;
+    }
+  } else {
+    const uint16_t *x = static_cast<const uint16_t *>(p);
+    uint16_t u[8] = {};
+    if (i + 8 <= end) {
+      __builtin_memcpy(u, x + i, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j < end) u[j] = x[i + j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = DT == kFloat16 ? F16ToF32(u[j]) : Bf16ToF32(u[j]);
+  }
 }
 
-__device__ __forceinline__ float BlockReduce(float v, float *s, bool max) {
-  for (int o = 32; o > 0; o >>= 1) {
-    const float w = __shfl_xor(v, o);
-    v = max ? fmaxf(v, w) : v + w;
+// v rounded to DT, written to p (where given) and left in v.
+template <int DT> __device__ __forceinline__ void Round8(void *p, int64_t i, int64_t end, float (&v)[8]) {
+  if constexpr (DT == kFloat) {
+    if (!p) return;
+    float *y = static_cast<float *>(p);
+    if (i + 8 <= end) {
+      __builtin_memcpy(y + i, v, 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j < end) y[i + j] = v[j];
+    }
+  } else {
+    uint16_t u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u[j] = DT == kFloat16 ? F32ToF16(v[j]) : F32ToBf16(v[j]);
+      v[j] = DT == kFloat16 ? F16ToF32(u[j]) : Bf16ToF32(u[j]);
+    }
+    if (!p) return;
+    uint16_t *y = static_cast<uint16_t *>(p);
+    if (i + 8 <= end) {
+      __builtin_memcpy(y + i, u, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j < end) y[i + j] = u[j];
+    }
   }
-  __syncthreads();
+}
+
+__device__ __forceinline__ unsigned TopBits(const float (&v)[8]) {
+  unsigned t = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t = max(t, __builtin_bit_cast(unsigned, v[j]) & 0x7fffffffu);
+  return t;
+}
+
+// Codes of y = v * inv; codes of a scale that is not finite (inv 0) are 0.
+__device__ __forceinline__ void Store8(uint8_t *y, int64_t i, int64_t end, const float (&v)[8], float inv, bool fp8) {
+  uint8_t c[8];
+  if (fp8) {
+    unsigned w[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      w[j] = Fp8Codes2(v[4 * j] * inv, v[4 * j + 1] * inv) | Fp8Codes2(v[4 * j + 2] * inv, v[4 * j + 3] * inv) << 16;
+    __builtin_memcpy(c, w, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = Int8Code(v[j] * inv);
+  }
+  if (i + 8 <= end) {
+    __builtin_memcpy(y + i, c, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j < end) y[i + j] = c[j];
+  }
+}
+
+// Sum (max) over the workgroup; s holds one value per wave.
+template <int WAVES, bool MAX, typename T> __device__ __forceinline__ T Join(T v, T *s) {
+  for (int o = 32; o > 0; o >>= 1) {
+    const T w = __shfl_xor(v, o);
+    v = MAX ? (v > w ? v : w) : v + w;
+  }
+  if constexpr (WAVES == 1) return v;
   if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = v;
   __syncthreads();
-  return max ? fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) : (s[0] + s[1]) + (s[2] + s[3]);
+  v = s[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) v = MAX ? (v > s[w] ? v : s[w]) : v + s[w];
+  return v;
 }
 
-// One workgroup per row, three passes over it: the sum of squares, then for
-// each block its largest magnitude and its codes.
-template <int DT> __global__ __launch_bounds__(kThreads) void RmsNormKernel(const RmsNormParams p) {
-  __shared__ float red[4];
-  const int64_t row = blockIdx.x, at = row * p.D;
+// NG groups of 8 values per thread are kept; KEPT: they are the whole row.
+template <int DT, int THREADS, int NG, bool KEPT>
+__global__ __launch_bounds__(THREADS) void RmsNormKernel(const RmsNormParams p) {
+  constexpr int WAVES = THREADS / 64, kStep = THREADS * 8;
+  __shared__ float s_sum[WAVES];
+  __shared__ unsigned s_top[WAVES];
+  const int64_t row = blockIdx.x, at = row * p.D, end = at + p.D;
   const int tid = threadIdx.x;
-  auto h_of = [&](int64_t i) -> float {
-    const float x = LoadX<DT>(p.x, at + i);
-    if (!p.residual) return x;
-    const float h = x + LoadX<DT>(p.residual, at + i);
-    if constexpr (DT == kFloat) return h;
-    if constexpr (DT == kFloat16) return F16ToF32(F32ToF16(h));
-    return Bf16ToF32(F32ToBf16(h));
+  float v[NG][8];
+  // h of the group from i on (past the end: zeros)
+  auto load = [&](int64_t i, float (&h)[8], bool first) __attribute__((always_inline)) {
+    Load8<DT>(first || !p.sum ? p.x : p.sum, i, end, h);
+    if (p.residual && (first || !p.sum)) {
+      float r[8];
+      Load8<DT>(p.residual, i, end, r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] += r[j];
+      Round8<DT>(first ? p.sum : nullptr, i, end, h);
+    }
   };
   float ss = 0.f;
-  for (int64_t i = tid; i < p.D; i += kThreads) {
-    const float h = h_of(i);
-    ss += h * h;
-  }
-  const float rstd = 1.f / sqrtf(BlockReduce(ss, red, false) / (float)p.D + p.eps);
-  auto y_of = [&](int64_t i) {
-    const float w = p.weight_f32 ? static_cast<const float *>(p.weight)[i] : LoadX<DT>(p.weight, i);
-    return h_of(i) * rstd * w;
+  auto square = [&](const float (&h)[8]) __attribute__((always_inline)) {
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t = __builtin_fmaf(h[j], h[j], t);
+    ss += t;
   };
-  for (int64_t b = 0; b < p.D; b += p.block) {
-    float top = 0.f;
-    bool finite = true;
-    for (int64_t i = b + tid; i < b + p.block; i += kThreads) {
-      const float y = fabsf(y_of(i));
-      finite = finite && y < __builtin_huge_valf();
-      top = fmaxf(top, y);
+  if constexpr (KEPT) {
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      const int64_t i = at + k * kStep + tid * 8;
+      if (i < end) {
+        load(i, v[k], true);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+      }
     }
-    top = BlockReduce(finite ? top : __builtin_huge_valf(), red, true);
-    const BlockScale s = p.scale_kind == kRnsE8M0 ? MxScaleOf(top, 8) : ScaleOf(top, p.y_fp8 ? 448.f : 127.f);
-    if (tid == 0) {
-      const int64_t si = row * (p.D / p.block) + b / p.block;
-      if (p.scale_kind == kRnsE8M0)
-        static_cast<uint8_t *>(p.scale)[si] = s.e8m0;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) square(v[k]);
+  } else {
+    for (int64_t i = at + tid * 8; i < end; i += kStep) {
+      load(i, v[0], true);
+      square(v[0]);
+    }
+  }
+  const float rstd = 1.f / sqrtf(Join<WAVES, false>(ss, s_sum) / (float)p.D + p.eps);
+  auto scale_by_weight = [&](int64_t i, float (&h)[8]) __attribute__((always_inline)) {
+    float w[8];
+    if (p.weight_f32)
+      Load8<kFloat>(p.weight, i, p.D, w);
+    else
+      Load8<DT>(p.weight, i, p.D, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = h[j] * rstd * w[j];
+  };
+  const int64_t blocks = p.D / p.block;
+  auto put_scale = [&](int64_t b, const BlockScale &s) __attribute__((always_inline)) {
+    if (p.scale_kind == kRnsE8M0)
+      static_cast<uint8_t *>(p.scale)[row * blocks + b] = s.e8m0;
+    else
+      static_cast<float *>(p.scale)[row * blocks + b] = s.scale;
+  };
+  auto scale_of = [&](unsigned top) __attribute__((always_inline)) {
+    const float t = __builtin_bit_cast(float, top);
+    return p.scale_kind == kRnsE8M0 ? MxScaleOf(t, 8) : ScaleOf(t, p.y_fp8 ? kFp8Max : kInt8Max);
+  };
+  uint8_t *y = static_cast<uint8_t *>(p.y);
+  // one scale per block of neighbouring threads
+  auto quantize_blocks = [&](int64_t i, float (&h)[8]) __attribute__((always_inline)) {
+    unsigned top = TopBits(h);
+    for (int o = 1; o < (int)p.block / 8; o <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+    const BlockScale s = scale_of(top);
+    if (i >= p.D) return;
+    if (i % p.block == 0) put_scale(i / p.block, s);
+    Store8(y, at + i, end, h, s.inv, p.y_fp8);
+  };
+  const bool per_row = p.block == p.D && p.scale_kind == kRnsFloat;
+  if constexpr (KEPT) {
+#pragma unroll
+    for (int k = 0; k < NG; ++k)
+      if (k * kStep + tid * 8 < p.D) scale_by_weight(k * kStep + tid * 8, v[k]);
+    if (!per_row) {
+#pragma unroll
+      for (int k = 0; k < NG; ++k) quantize_blocks(k * kStep + tid * 8, v[k]);
+      return;
+    }
+    unsigned top = 0;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) top = max(top, TopBits(v[k]));
+    const BlockScale s = scale_of(Join<WAVES, true>(top, s_top));
+    if (tid == 0) put_scale(0, s);
+#pragma unroll
+    for (int k = 0; k < NG; ++k)
+      if (k * kStep + tid * 8 < p.D) Store8(y, at + k * kStep + tid * 8, end, v[k], s.inv, p.y_fp8);
+  } else {
+    unsigned top = 0;
+    // every thread takes every step: the block's maximum is a lane exchange
+    for (int64_t i = tid * 8; i < (p.D + kStep - 1) / kStep * kStep; i += kStep) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[0][j] = 0.f;
+      if (i < p.D) {
+        load(at + i, v[0], false);
+        scale_by_weight(i, v[0]);
+      }
+      if (per_row)
+        top = max(top, TopBits(v[0]));
       else
-        static_cast<float *>(p.scale)[si] = s.scale;
+        quantize_blocks(i, v[0]);
     }
-    for (int64_t i = b + tid; i < b + p.block; i += kThreads)
-      static_cast<uint8_t *>(p.y)[at + i] = p.y_fp8 ? Fp8Code(y_of(i) * s.inv) : Int8Code(y_of(i) * s.inv);
-  }
-  if (p.sum) {
-    // last: it may be x's or the residual's own memory
-    __syncthreads();
-    for (int64_t i = tid; i < p.D; i += kThreads) {
-      const float h = h_of(i);
-      if constexpr (DT == kFloat) static_cast<float *>(p.sum)[at + i] = h;
-      if constexpr (DT == kFloat16) static_cast<uint16_t *>(p.sum)[at + i] = F32ToF16(h);
-      if constexpr (DT == kBfloat16) static_cast<uint16_t *>(p.sum)[at + i] = F32ToBf16(h);
+    if (!per_row) return;
+    const BlockScale s = scale_of(Join<WAVES, true>(top, s_top));
+    if (tid == 0) put_scale(0, s);
+    for (int64_t i = tid * 8; i < p.D; i += kStep) {
+      load(at + i, v[0], false);
+      scale_by_weight(i, v[0]);
+      Store8(y, at + i, end, v[0], s.inv, p.y_fp8);
     }
   }
+}
+
+template <int DT> void Launch(const RmsNormParams &p, hipStream_t s) {
+  const dim3 grid((unsigned)p.rows);
+  // One group of 8 values per thread up to a full workgroup, then more of them:
+  // short rows are bound by latency, long ones by the bytes in flight.
+  if (p.D <= 512)
+    RmsNormKernel<DT, 64, 1, true><<<grid, 64, 0, s>>>(p);
+  else if (p.D <= 2048)
+    RmsNormKernel<DT, 256, 1, true><<<grid, 256, 0, s>>>(p);
+  else if (p.D <= 4096)
+    RmsNormKernel<DT, 512, 1, true><<<grid, 512, 0, s>>>(p);
+  else if (p.D <= 8192)
+    RmsNormKernel<DT, 512, 2, true><<<grid, 512, 0, s>>>(p);
+  else if (p.D <= 16384)
+    RmsNormKernel<DT, 512, 4, true><<<grid, 512, 0, s>>>(p);
+  else
+    RmsNormKernel<DT, 512, 1, false><<<grid, 512, 0, s>>>(p);
 }
 
 }  // namespace
 
 void LaunchRmsNormQuantize(const RmsNormParams &p, hipStream_t stream) {
   if (p.rows == 0) return;
-  const dim3 grid((unsigned)p.rows);
   if (p.x_dtype == kFloat)
-    RmsNormKernel<kFloat><<<grid, kThreads, 0, stream>>>(p);
+    Launch<kFloat>(p, stream);
   else if (p.x_dtype == kFloat16)
-    RmsNormKernel<kFloat16><<<grid, kThreads, 0, stream>>>(p);
+    Launch<kFloat16>(p, stream);
   else
-    RmsNormKernel<kBfloat16><<<grid, kThreads, 0, stream>>>(p);
+    Launch<kBfloat16>(p, stream);
 }
 
 }  // namespace onnxl_amd
