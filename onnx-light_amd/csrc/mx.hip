@@ -41,20 +41,10 @@ template <int DT, bool FP4> __device__ __forceinline__ void QuantizeRow8(const M
   top = max(top, (unsigned)__shfl_xor((int)top, 1));
   top = max(top, (unsigned)__shfl_xor((int)top, 2));
   const BlockScale s = MxScaleOf(__builtin_bit_cast(float, top), FP4 ? 2 : 8);
-  if (s.e8m0 == 255) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.f;
-  }
-  if constexpr (FP4) {
-    unsigned c = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) c |= Fp4Codes2(v[j] * s.inv, v[j + 1] * s.inv) << (4 * j);
-    *reinterpret_cast<unsigned *>(p.y + i * 4) = c;
-  } else {
-    unsigned lo = Fp8Codes2(v[0] * s.inv, v[1] * s.inv) | Fp8Codes2(v[2] * s.inv, v[3] * s.inv) << 16;
-    unsigned hi = Fp8Codes2(v[4] * s.inv, v[5] * s.inv) | Fp8Codes2(v[6] * s.inv, v[7] * s.inv) << 16;
-    *reinterpret_cast<uint2 *>(p.y + i * 8) = make_uint2(lo, hi);
-  }
+  if constexpr (FP4)
+    *reinterpret_cast<unsigned *>(p.y + i * 4) = MxFp4Codes8(v, s);
+  else
+    *reinterpret_cast<uint2 *>(p.y + i * 8) = MxFp8Codes8(v, s);
   if (k8 % 4 == 0) {
     if (tiles)
       tiles[mx::ScaleTileAt(row, k8 / 4, steps)] = s.e8m0;

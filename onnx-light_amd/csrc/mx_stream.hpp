@@ -108,20 +108,10 @@ __global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const Stre
       top = max(top, (unsigned)__shfl_xor((int)top, 1));
       top = max(top, (unsigned)__shfl_xor((int)top, 2));
       const BlockScale s = MxScaleOf(__builtin_bit_cast(float, top), A4 ? 2 : 8);
-      if (s.e8m0 == 255) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-      }
-      if constexpr (A4) {
-        unsigned code = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) code |= Fp4Codes2(v[j] * s.inv, v[j + 1] * s.inv) << (4 * j);
-        *reinterpret_cast<unsigned *>(lds + row * lds_row + k8 * 4) = code;
-      } else {
-        const unsigned lo = Fp8Codes2(v[0] * s.inv, v[1] * s.inv) | Fp8Codes2(v[2] * s.inv, v[3] * s.inv) << 16;
-        const unsigned hi = Fp8Codes2(v[4] * s.inv, v[5] * s.inv) | Fp8Codes2(v[6] * s.inv, v[7] * s.inv) << 16;
-        *reinterpret_cast<uint2 *>(lds + row * lds_row + k8 * 8) = make_uint2(lo, hi);
-      }
+      if constexpr (A4)
+        *reinterpret_cast<unsigned *>(lds + row * lds_row + k8 * 4) = MxFp4Codes8(v, s);
+      else
+        *reinterpret_cast<uint2 *>(lds + row * lds_row + k8 * 8) = MxFp8Codes8(v, s);
       if (k8 % 4 == 0) lds_s[row * lds_scale + k8 / 4] = in ? (char)s.e8m0 : 127;
     }
     __syncthreads();

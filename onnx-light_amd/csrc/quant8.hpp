@@ -45,27 +45,43 @@ __device__ __forceinline__ BlockScale MxScaleOf(float top, int emax) {
   return BlockScale{scale, inv, (uint8_t)e};
 }
 
-// Nearest code, ties to even; v is finite, or 0 * NaN in a block without a
-// finite scale, whose codes are 0.
-__device__ __forceinline__ uint8_t Int8Code(float v) {
-  const float c = __builtin_rintf(fminf(fmaxf(v, -kInt8Max), kInt8Max));
-  return v == v ? (uint8_t)(int8_t)(int)c : 0;
+// Nearest codes, ties to even, of v = y * inv of a block with a FLOAT scale.
+// |v| is at most the largest code (and an ulp), which no rounding leaves.  In a
+// block whose scale is NaN v may be NaN: its codes mean nothing.
+__device__ __forceinline__ uint8_t Int8Code(float v) { return (uint8_t)(int8_t)(int)__builtin_rintf(v); }
+__device__ __forceinline__ unsigned Int8Codes4(float a, float b, float c, float d) {
+  const unsigned lo = __builtin_amdgcn_perm((unsigned)(int)__builtin_rintf(b), (unsigned)(int)__builtin_rintf(a), 0x0c0c0400u);
+  const unsigned hi = __builtin_amdgcn_perm((unsigned)(int)__builtin_rintf(d), (unsigned)(int)__builtin_rintf(c), 0x04000c0cu);
+  return lo | hi;
 }
-
-// Two E4M3 codes in bits 0-15: the conversion gives NaN past 464, so values
-// are clamped to the largest first.
-__device__ __forceinline__ unsigned Fp8Codes2(float a, float b) {
-  a = a == a ? __builtin_amdgcn_fmed3f(a, -kFp8Max, kFp8Max) : 0.f;
-  b = b == b ? __builtin_amdgcn_fmed3f(b, -kFp8Max, kFp8Max) : 0.f;
-  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
+__device__ __forceinline__ unsigned Fp8Codes4(float a, float b, float c, float d) {
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
-__device__ __forceinline__ uint8_t Fp8Code(float v) { return (uint8_t)Fp8Codes2(v, 0.f); }
+__device__ __forceinline__ uint8_t Fp8Code(float v) { return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, 0.f, 0, false); }
 
-// Two E2M1 codes in bits 0-7, saturating, ties to even.
+// MX blocks: v = x * 2^-e may pass the largest code, and the conversion gives
+// NaN past 464, so it is clamped.
+__device__ __forceinline__ float ClampFp8(float v) { return __builtin_amdgcn_fmed3f(v, -kFp8Max, kFp8Max); }
+
+// Two E2M1 codes in bits 0-7, saturating.
 __device__ __forceinline__ unsigned Fp4Codes2(float a, float b) {
-  a = a == a ? a : 0.f;
-  b = b == b ? b : 0.f;
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, 1.f, 0) & 0xffu;
+}
+
+// Codes of eight values of an MX block; a block without a finite scale has zero
+// codes.
+__device__ __forceinline__ uint2 MxFp8Codes8(const float (&v)[8], const BlockScale &s) {
+  float c[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = ClampFp8(v[j] * s.inv);
+  const bool none = s.e8m0 == 255;
+  return make_uint2(none ? 0u : Fp8Codes4(c[0], c[1], c[2], c[3]), none ? 0u : Fp8Codes4(c[4], c[5], c[6], c[7]));
+}
+__device__ __forceinline__ unsigned MxFp4Codes8(const float (&v)[8], const BlockScale &s) {
+  unsigned c = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) c |= Fp4Codes2(v[j] * s.inv, v[j + 1] * s.inv) << (4 * j);
+  return s.e8m0 == 255 ? 0u : c;
 }
 
 }  // namespace onnxl_amd
