@@ -161,47 +161,89 @@ bool Streams(const MxMatMulParams &p) { return p.M <= kStreamRows; }
 constexpr int64_t kOwnQuant = 16384;
 bool OwnQuant(const MxMatMulParams &p) { return p.x && p.M <= 16 && p.M * Ceil(p.K, 512) * 512 <= kOwnQuant; }
 
-template <bool A4, int MT, bool QUANT> void LaunchStream(const mx::StreamArgs &a, hipStream_t s) {
-  const int64_t chunks = Ceil(a.K, 512);
-  const int waves = chunks > 8 ? mx::kStreamWaves<MT> : 8;
-  const size_t codes = QUANT ? (size_t)(a.M * chunks * ((A4 ? 256 : 512) + 16)) : 0;
-  const size_t lds = std::max(codes, (size_t)MT * waves * 1024);
-  mx::StreamKernel<A4, 1, MT, QUANT><<<dim3((unsigned)Ceil(a.N, 16)), 64 * waves, lds, s>>>(a);
+// How the streaming kernel covers a problem: row tiles of 16 nt rows of the
+// weight, `split` workgroups of `waves` waves for each.
+struct StreamPlan {
+  int nt, mt, waves, split;
+  int64_t tiles;
+};
+
+StreamPlan PlanStream(const MxMatMulParams &p) {
+  StreamPlan s;
+  const int64_t chunks = Ceil(p.K, 512);
+  s.mt = (int)Ceil(p.M, 16);
+  // Activations from memory are read by every wave for itself, all over the chip
+  // the same ones at about the same time, and cost as much per 16 rows as the
+  // weight: several row tiles share a read, while a wave for every CU's SIMD is
+  // left.
+  s.nt = OwnQuant(p) ? 1 : p.M <= 16 ? 2 : 4;
+  while (s.nt > 1 && Ceil(p.N, 16 * s.nt) * chunks < 4 * Ctx().num_cus) s.nt /= 2;
+  s.waves = s.nt == 4 ? 4 : s.nt == 1 && s.mt == 1 && chunks > 8 ? 16 : 8;
+  s.tiles = Ceil(p.N, 16 * s.nt);
+  // as many as give every wave one chunk, while there are not more than about
+  // two rounds of them
+  s.split = (int)std::max<int64_t>(1, std::min<int64_t>(Ceil(chunks, s.waves), 32 * Ctx().num_cus / (s.waves * s.tiles)));
+  return s;
 }
 
-template <bool A4> void LaunchStreamOf(const mx::StreamArgs &a, bool own, hipStream_t s) {
-  if (own)
-    LaunchStream<A4, 1, true>(a, s);
-  else if (a.M <= 16)
-    LaunchStream<A4, 1, false>(a, s);
-  else if (a.M <= 32)
-    LaunchStream<A4, 2, false>(a, s);
-  else if (a.M <= 48)
-    LaunchStream<A4, 3, false>(a, s);
+template <bool A4, int NT, int MT, bool QUANT> void LaunchStream(const mx::StreamArgs &a, const StreamPlan &s, hipStream_t st) {
+  const int64_t chunks = Ceil(a.K, 512);
+  const size_t codes = QUANT ? (size_t)(a.M * chunks * ((A4 ? 256 : 512) + 16)) : 0;
+  const size_t lds = std::max(codes, (size_t)NT * MT * s.waves * 1024);
+  mx::StreamKernel<A4, NT, MT, QUANT><<<dim3((unsigned)s.tiles, (unsigned)s.split), 64 * s.waves, lds, st>>>(a);
+}
+
+template <bool A4, int MT> void LaunchStreamRows(const mx::StreamArgs &a, const StreamPlan &s, hipStream_t st) {
+  if (s.nt == 4)
+    LaunchStream<A4, 4, MT, false>(a, s, st);
+  else if (s.nt == 2)
+    LaunchStream<A4, 2, MT, false>(a, s, st);
   else
-    LaunchStream<A4, 4, false>(a, s);
+    LaunchStream<A4, 1, MT, false>(a, s, st);
+}
+
+template <bool A4> void LaunchStreamOf(const mx::StreamArgs &a, bool own, const StreamPlan &s, hipStream_t st) {
+  if (own)
+    LaunchStream<A4, 1, 1, true>(a, s, st);
+  else if (s.mt == 1)
+    LaunchStreamRows<A4, 1>(a, s, st);
+  else if (s.mt == 2)
+    LaunchStreamRows<A4, 2>(a, s, st);
+  else if (s.mt == 3)
+    LaunchStreamRows<A4, 3>(a, s, st);
+  else
+    LaunchStreamRows<A4, 4>(a, s, st);
 }
 
 }  // namespace
 
 size_t MxMatMulScratchBytes(const MxMatMulParams &p) {
-  if (Streams(p)) return p.x && !OwnQuant(p) ? Scratch::Round((size_t)(p.M * p.K)) + (size_t)(p.M * p.K / 32) : 0;
+  if (Streams(p)) {
+    const size_t codes = p.x && !OwnQuant(p) ? Scratch::Round((size_t)(p.M * p.K)) + Scratch::Round((size_t)(p.M * p.K / 32)) : 0;
+    const StreamPlan s = PlanStream(p);
+    return codes + (s.split > 1 ? (size_t)s.tiles * s.split * s.nt * s.mt * 1024 : 0);
+  }
   const MxScratch s(p);
   return s.codes + s.a_tiles + s.b_tiles;
 }
 
 void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) {
   if (Streams(p)) {
+    const StreamPlan plan = PlanStream(p);
     mx::StreamArgs a{p.x, p.a, p.a_scale, p.b, p.b_scale, static_cast<uint16_t *>(p.y), (int)p.M, (int)p.N, (int)p.K,
-                     p.x_dtype == kBfloat16, p.y_bf16};
+                     p.x_dtype == kBfloat16, p.y_bf16, plan.split, nullptr, nullptr};
     const bool own = OwnQuant(p);
+    uint8_t *codes = static_cast<uint8_t *>(scratch), *scales = codes + Scratch::Round((size_t)(p.M * p.K));
+    if (a.split > 1) {
+      a.part = reinterpret_cast<float *>(p.x && !own ? scales + Scratch::Round((size_t)(p.M * p.K / 32)) : codes);
+      a.done = Ctx().ws.Counters((size_t)plan.tiles);
+    }
     if (p.x && !own) {
-      uint8_t *codes = static_cast<uint8_t *>(scratch), *scales = codes + Scratch::Round((size_t)(p.M * p.K));
       LaunchMxQuantize(MxQuantParams{p.x, codes, scales, p.M, p.K, p.x_dtype, p.a_fp4}, stream);
       a.a = codes;
       a.as = scales;
     }
-    p.a_fp4 ? LaunchStreamOf<true>(a, own, stream) : LaunchStreamOf<false>(a, own, stream);
+    p.a_fp4 ? LaunchStreamOf<true>(a, own, plan, stream) : LaunchStreamOf<false>(a, own, plan, stream);
     return;
   }
   const MxScratch s(p);

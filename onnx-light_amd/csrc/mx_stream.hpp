@@ -13,7 +13,9 @@
 // 4 (g / 2) + j and 4 (2 + g / 2) + j.
 //
 // A workgroup has 16 NT rows of the weight; its waves take the chunks in turn
-// and add up in LDS.  Activations of 16 bits that are few enough are quantized
+// and add up in LDS.  Where rows are few and K is long several workgroups share
+// the chunks, so that all of a wave's loads are in flight at once; the last of
+// them to finish adds up their sums, in the order of the chunks whoever that is.  Activations of 16 bits that are few enough are quantized
 // by every workgroup for itself, into LDS, while its first weight bytes are on
 // their way: that costs less than a launch of its own.
 #pragma once
@@ -33,6 +35,9 @@ struct StreamArgs {
   uint16_t *y;
   int M, N, K;
   int x_bf16, bf16;
+  int split;                    // workgroups (grid.y) that share the chunks
+  float *part;                  // their sums, [row tile][split][NT * MT][64] float4
+  unsigned *done;               // [row tile] workgroups that are done, zero between launches
 };
 
 // Four block scales from `at` on of a row of `blocks`; those past the end are 1.
@@ -52,11 +57,11 @@ __device__ __forceinline__ int Scales4(const uint8_t *row, int at, int blocks, b
   return (int)(((b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24) & mask) | (0x7f7f7f7fu & ~mask));
 }
 
-// Waves of a workgroup: more rows need the registers of half of them.
-template <int MT> constexpr int kStreamWaves = MT == 1 ? 16 : 8;
+// Most waves of a workgroup: what the registers of more rows and columns leave.
+template <int NT, int MT> constexpr int kStreamWaves = NT == 1 && MT == 1 ? 16 : NT == 4 ? 4 : 8;
 
 template <bool A4, int NT, int MT, bool QUANT>
-__global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const StreamArgs p) {
+__global__ __launch_bounds__((64 * kStreamWaves<NT, MT>)) void StreamKernel(const StreamArgs p) {
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
@@ -88,7 +93,8 @@ __global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const Stre
   // codes in LDS: rows of whole chunks, then their scales
   const int lds_row = chunks * (A4 ? 256 : 512), lds_scale = chunks * 16;
   char *lds_s = lds + (QUANT ? p.M * lds_row : 0);
-  if (wave < chunks) load(wave);
+  const int per = (chunks + p.split - 1) / p.split, ch0 = blockIdx.y * per, ch1 = min(chunks, ch0 + per);
+  if (ch0 + wave < ch1) load(ch0 + wave);
   if constexpr (QUANT) {
     // eight values a thread, four neighbours a block; past the row's end zero
     // codes of scale 1
@@ -180,9 +186,9 @@ __global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const Stre
     mma(std::integral_constant<int, 3>{});
     if constexpr (more) load(ch + waves);
   };
-  int ch = wave;
-  for (; ch + waves < chunks; ch += waves) chunk(ch, std::true_type{});
-  if (ch < chunks) chunk(ch, std::false_type{});
+  int ch = ch0 + wave;
+  for (; ch + waves < ch1; ch += waves) chunk(ch, std::true_type{});
+  if (ch < ch1) chunk(ch, std::false_type{});
 
   // lane (c, g) of a tile has the columns 4 g .. 4 g + 3 of row c of y
   v4f *part = reinterpret_cast<v4f *>(lds);
@@ -192,11 +198,12 @@ __global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const Stre
 #pragma unroll
     for (int m = 0; m < MT; ++m) part[((n * MT + m) * waves + wave) * 64 + lane] = acc[n][m];
   __syncthreads();
-  for (int i = wave; i < NT * MT; i += waves) {
-    v4f s = part[i * waves * 64 + lane];
-    for (int v = 1; v < waves; ++v) s += part[(i * waves + v) * 64 + lane];
+  constexpr int kScope = 16;  // sc1: past this XCD's L2, so that no fence is needed
+  const __amdgpu_buffer_rsrc_t rs = Rsrc(p.part, 0x7fffffff);
+  auto slot = [&](int s, int i) { return (int)(((blockIdx.x * p.split + s) * (NT * MT) + i) * 64 + lane) * 16; };
+  auto store = [&](int i, v4f s) {
     const int row = i % MT * 16 + c, col = n0 + i / MT * 16 + 4 * g;
-    if (row >= p.M) continue;
+    if (row >= p.M) return;
     uint16_t *y = p.y + (int64_t)row * p.N + col;
     uint16_t v[4];
 #pragma unroll
@@ -206,6 +213,28 @@ __global__ __launch_bounds__(64 * kStreamWaves<MT>) void StreamKernel(const Stre
     } else {
       for (int e = 0; col + e < p.N; ++e) y[e] = v[e];
     }
+  };
+  for (int i = wave; i < NT * MT; i += waves) {
+    v4f s = part[i * waves * 64 + lane];
+    for (int v = 1; v < waves; ++v) s += part[(i * waves + v) * 64 + lane];
+    if (p.split == 1)
+      store(i, s);
+    else
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, s), rs, slot(blockIdx.y, i), 0, kScope);
+  }
+  if (p.split == 1) return;
+  __shared__ unsigned before;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this part is where every XCD sees it before it is counted
+  __syncthreads();
+  if (tid == 0) before = atomicAdd(p.done + blockIdx.x, 1u);
+  __syncthreads();
+  if (before != (unsigned)p.split - 1) return;
+  if (tid == 0) p.done[blockIdx.x] = 0;
+  for (int i = wave; i < NT * MT; i += waves) {
+    v4f s = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int v = 0; v < p.split; ++v)
+      s += __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, slot(v, i), 0, kScope));
+    store(i, s);
   }
 }
 
