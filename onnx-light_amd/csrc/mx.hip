@@ -175,8 +175,8 @@ StreamPlan PlanStream(const MxMatMulParams &p) {
   // Activations from memory are read by every wave for itself, all over the chip
   // the same ones at about the same time, and cost as much per 16 rows as the
   // weight: several row tiles share a read, while a wave for every CU's SIMD is
-  // left.
-  s.nt = OwnQuant(p) ? 1 : p.M <= 16 ? 2 : 4;
+  // left.  More than these do not fit the registers of two waves per SIMD.
+  s.nt = OwnQuant(p) ? 1 : s.mt == 1 ? 2 : s.mt <= (p.a_fp4 ? 3 : 2) ? 4 : 2;
   while (s.nt > 1 && Ceil(p.N, 16 * s.nt) * chunks < 4 * Ctx().num_cus) s.nt /= 2;
   s.waves = s.nt == 4 ? 4 : s.nt == 1 && s.mt == 1 && chunks > 8 ? 16 : 8;
   s.tiles = Ceil(p.N, 16 * s.nt);
@@ -194,8 +194,9 @@ template <bool A4, int NT, int MT, bool QUANT> void LaunchStream(const mx::Strea
 }
 
 template <bool A4, int MT> void LaunchStreamRows(const mx::StreamArgs &a, const StreamPlan &s, hipStream_t st) {
-  if (s.nt == 4)
-    LaunchStream<A4, 4, MT, false>(a, s, st);
+  constexpr bool kFour = MT == 2 || (A4 && MT == 3);
+  if (kFour && s.nt == 4)
+    LaunchStream<A4, kFour ? 4 : 2, MT, false>(a, s, st);
   else if (s.nt == 2)
     LaunchStream<A4, 2, MT, false>(a, s, st);
   else

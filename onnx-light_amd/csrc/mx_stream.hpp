@@ -40,28 +40,29 @@ struct StreamArgs {
   unsigned *done;               // [row tile] workgroups that are done, zero between launches
 };
 
-// Four block scales from `at` on of a row of `blocks`; those past the end are 1.
-// Near the row's end the bytes are loaded one by one, none past it and all at
-// once (behind a branch per byte they came one after the other).
-__device__ __forceinline__ int Scales4(const uint8_t *row, int at, int blocks, bool tail) {
+// Four block scales from `at` (a multiple of 4) on of the row of `blocks` at
+// base + row.  Those
+// past the end are scales of other blocks of the row: their activations are
+// zeros, and a NaN among them makes the row NaN anyhow.  Nothing is done with
+// what is loaded, which would wait for it, but in the last chunk of rows that
+// are not whole dwords: there the bytes come one by one, all at once.
+__device__ __forceinline__ int Scales4(const uint8_t *base, unsigned row, int at, int blocks, bool tail) {
   int v;
-  if (!tail) {
-    __builtin_memcpy(&v, row + at, 4);
+  if (!tail || blocks % 4 == 0) {
+    __builtin_memcpy(&v, base + (row + (unsigned)(at < blocks ? at : 0)), 4);
     return v;
   }
-  const int n = blocks - at;
   unsigned b[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) b[i] = row[max(min(at + i, blocks - 1), 0)];
-  const unsigned mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << 8 * n) - 1u;
-  return (int)(((b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24) & mask) | (0x7f7f7f7fu & ~mask));
+  for (int i = 0; i < 4; ++i) b[i] = base[row + (unsigned)min(at + i, blocks - 1)];
+  return (int)(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24);
 }
 
 // Most waves of a workgroup: what the registers of more rows and columns leave.
 template <int NT, int MT> constexpr int kStreamWaves = NT == 1 && MT == 1 ? 16 : NT == 4 ? 4 : 8;
 
 template <bool A4, int NT, int MT, bool QUANT>
-__global__ __launch_bounds__((64 * kStreamWaves<NT, MT>)) void StreamKernel(const StreamArgs p) {
+__global__ __launch_bounds__((64 * kStreamWaves<NT, MT>), 2) void StreamKernel(const StreamArgs p) {
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
@@ -69,24 +70,29 @@ __global__ __launch_bounds__((64 * kStreamWaves<NT, MT>)) void StreamKernel(cons
   const int n0 = blockIdx.x * 16 * NT;
   const int64_t pitch_b = p.K / 2, pitch_a = A4 ? p.K / 2 : p.K;
 
-  // the weight's rows of this lane (rows past the last repeat it)
-  const uint8_t *bp[NT], *sp[NT];
+  // 32-bit offsets of this lane's rows (those past the last repeat it) from the
+  // tile's first
+  const uint8_t *tile_b = p.b + n0 * pitch_b, *tile_s = p.bs + (int64_t)n0 * blocks;
+  unsigned row_b[NT], row_s[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int64_t row = min(n0 + 16 * n + c, p.N - 1);
-    bp[n] = p.b + row * pitch_b;
-    sp[n] = p.bs + row * blocks;
+    const unsigned row = (unsigned)(min(n0 + 16 * n + c, p.N - 1) - n0);
+    row_b[n] = row * (unsigned)pitch_b;
+    row_s[n] = row * (unsigned)blocks;
   }
+  typedef std::conditional_t<A4, v4i, v8i> Frag;
   v4i w[NT][4];
   int ws[NT];
   // blocks past the end are read as block 0: the activations there are zeros
   auto load = [&](int ch) __attribute__((always_inline)) {
     const int blk = 16 * ch + 4 * g;
+    const bool tail = 16 * ch + 16 > blocks;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[n][j] = *reinterpret_cast<const v4i *>(bp[n] + 16 * (blk + j < blocks ? blk + j : 0));
-      ws[n] = Scales4(sp[n], blk, blocks, 16 * ch + 16 > blocks);
+      for (int j = 0; j < 4; ++j)
+        w[n][j] = *reinterpret_cast<const v4i *>(tile_b + (row_b[n] + 16u * (unsigned)(blk + j < blocks ? blk + j : 0)));
+      ws[n] = Scales4(tile_s, row_s[n], blk, blocks, tail);
     }
   };
 
@@ -128,60 +134,71 @@ __global__ __launch_bounds__((64 * kStreamWaves<NT, MT>)) void StreamKernel(cons
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[n][m] = v4f{0.f, 0.f, 0.f, 0.f};
-  typedef std::conditional_t<A4, v4i, v8i> Frag;
   // one chunk; `more` loads the wave's next one as soon as the registers are free
   auto chunk = [&](int ch, auto more) __attribute__((always_inline)) {
     const bool tail = 16 * ch + 16 > blocks;
-    Frag x[MT][4];
+    // activations of instruction j, a step ahead of their use
+    Frag x[2][MT];
     int xs[MT];
+    auto get = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = min(16 * m + c, p.M - 1);  // rows past the last repeat it
-      if constexpr (QUANT) {
-        const char *xp = lds + row * lds_row;
-        xs[m] = *reinterpret_cast<const int *>(lds_s + row * lds_scale + 16 * ch + 4 * g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (A4) {
-            x[m][j] = *reinterpret_cast<const v4i *>(xp + (16 * ch + 4 * g + j) * 16);
-          } else {
-            const int at = (16 * ch + 4 * (g >> 1) + j) * 32 + 16 * (g & 1);
-            x[m][j] = __builtin_shufflevector(*reinterpret_cast<const v4i *>(xp + at),
-                                              *reinterpret_cast<const v4i *>(xp + at + 256), 0, 1, 2, 3, 4, 5, 6, 7);
-          }
-        }
-      } else {
-        const uint8_t *xp = p.a + row * pitch_a;
-        xs[m] = Scales4(p.as + (int64_t)row * blocks, 16 * ch + 4 * g, blocks, tail);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (A4) {
-            const int blk = 16 * ch + 4 * g + j;
-            x[m][j] = *reinterpret_cast<const v4i *>(xp + 16 * (blk < blocks ? blk : 0));
-            if (tail) x[m][j] = blk < blocks ? x[m][j] : v4i{0, 0, 0, 0};
-          } else {
-            const int lo = 16 * ch + 4 * (g >> 1) + j, hi = lo + 8;
-            v4i u = *reinterpret_cast<const v4i *>(xp + 32 * (lo < blocks ? lo : 0) + 16 * (g & 1));
-            v4i v = *reinterpret_cast<const v4i *>(xp + 32 * (hi < blocks ? hi : 0) + 16 * (g & 1));
-            if (tail) {
-              u = lo < blocks ? u : v4i{0, 0, 0, 0};
-              v = hi < blocks ? v : v4i{0, 0, 0, 0};
-            }
-            x[m][j] = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-          }
+      for (int m = 0; m < MT; ++m) {
+        Frag &f = x[j % 2][m];
+        const int row = min(16 * m + c, p.M - 1);  // rows past the last repeat it
+        if constexpr (QUANT && A4) {
+          f = *reinterpret_cast<const v4i *>(lds + row * lds_row + (16 * ch + 4 * g + j) * 16);
+        } else if constexpr (QUANT) {
+          const char *xp = lds + row * lds_row + (16 * ch + 4 * (g >> 1) + j) * 32 + 16 * (g & 1);
+          f = __builtin_shufflevector(*reinterpret_cast<const v4i *>(xp), *reinterpret_cast<const v4i *>(xp + 256), 0, 1, 2, 3,
+                                      4, 5, 6, 7);
+        } else if constexpr (A4) {
+          const int blk = 16 * ch + 4 * g + j;
+          f = *reinterpret_cast<const v4i *>(p.a + ((unsigned)row * (unsigned)pitch_a + 16u * (unsigned)(blk < blocks ? blk : 0)));
+        } else {
+          const int lo = 16 * ch + 4 * (g >> 1) + j, hi = lo + 8;
+          const unsigned at = (unsigned)row * (unsigned)pitch_a + 16u * (g & 1);
+          f = __builtin_shufflevector(*reinterpret_cast<const v4i *>(p.a + (at + 32u * (unsigned)(lo < blocks ? lo : 0))),
+                                      *reinterpret_cast<const v4i *>(p.a + (at + 32u * (unsigned)(hi < blocks ? hi : 0))), 0, 1,
+                                      2, 3, 4, 5, 6, 7);
         }
       }
-    }
+    };
+    // codes of blocks past the end become zeros
+    auto cut = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if constexpr (A4) {
+          if (16 * ch + 4 * g + j >= blocks) x[j % 2][m] = v4i{0, 0, 0, 0};
+        } else {
+          const int lo = 16 * ch + 4 * (g >> 1) + j;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[j % 2][m][i] = lo + (i < 4 ? 0 : 8) < blocks ? x[j % 2][m][i] : 0;
+        }
+      }
+    };
     auto mma = [&](auto j) __attribute__((always_inline)) {
+      if (!QUANT && tail) cut(j);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(Operand(w[n][j]), Operand(x[m][j]), acc[n][m], 4,
+          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(Operand(w[n][j]), Operand(x[j % 2][m]), acc[n][m], 4,
                                                                        A4 ? 4 : 0, j, ws[n], j, xs[m]);
     };
+    get(0);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = min(16 * m + c, p.M - 1);
+      if constexpr (QUANT)
+        xs[m] = *reinterpret_cast<const int *>(lds_s + row * lds_scale + 16 * ch + 4 * g);
+      else
+        xs[m] = Scales4(p.as, (unsigned)row * (unsigned)blocks, 16 * ch + 4 * g, blocks, tail);
+    }
+    get(1);
     mma(std::integral_constant<int, 0>{});
+    get(2);
     mma(std::integral_constant<int, 1>{});
+    get(3);
     mma(std::integral_constant<int, 2>{});
     mma(std::integral_constant<int, 3>{});
     if constexpr (more) load(ch + waves);
