@@ -148,8 +148,19 @@ struct MxScratch {
 
 template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, hipStream_t s) {
   using S = mx::Shape<A4, MB, NB>;
-  const int64_t tiles = Ceil(g.M, S::BM) * Ceil(g.N, S::BN);
-  mx::GemmKernel<A4, MB, NB><<<dim3((unsigned)tiles), 256, 0, s>>>(g);
+  mx::GemmKernel<A4, MB, NB><<<dim3((unsigned)(Ceil(g.M, S::BM) * Ceil(g.N, S::BN))), 256, 0, s>>>(g);
+}
+
+// Large tiles (256 x 256, 128 x 256 for E4M3 activations) feed more MFMAs per
+// byte, small ones (128 x 128) leave fewer CUs idle; a round of large ones takes
+// about 1.45 times a round of small ones (of which two fit a CU for E2M1).
+// us, large / small: MXFP4 1000 x 4096 x 6144 40 / 27, 4096 x 8192 x 8192 174 /
+// 205; MXFP8 256 x 4096 x 4096 28 / 22, 1000 x 4096 x 6144 35 / 43.
+bool LargeTiles(const MxMatMulParams &p) {
+  const int64_t cus = Ctx().num_cus;
+  const int64_t large = Ceil(Ceil(p.M, p.a_fp4 ? 256 : 128) * Ceil(p.N, 256), cus);
+  const int64_t small = Ceil(Ceil(p.M, 128) * Ceil(p.N, 128), p.a_fp4 ? 2 * cus : cus);
+  return large * 29 <= small * 20;
 }
 
 // Few rows take the streaming kernel.
@@ -274,10 +285,10 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
   }
   const mx::GemmArgs g{s.codes ? codes : p.a, p.b, a_tiles, b_tiles, static_cast<uint16_t *>(p.y), p.M, p.N, p.K, p.y_bf16,
                        p.N % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0};
-  if (p.a_fp4)
-    LaunchGemm<true, 4, 4>(g, stream);
+  if (LargeTiles(p))
+    p.a_fp4 ? LaunchGemm<true, 4, 4>(g, stream) : LaunchGemm<false, 2, 4>(g, stream);
   else
-    LaunchGemm<false, 2, 4>(g, stream);
+    p.a_fp4 ? LaunchGemm<true, 2, 2>(g, stream) : LaunchGemm<false, 2, 2>(g, stream);
 }
 
 }  // namespace onnxl_amd

@@ -20,7 +20,11 @@
 // The fragments of a sub-step are read under the MFMAs of the one before; the
 // step's only barrier stands in the middle of its last sub-step, whose
 // fragments are in registers by then, so the stage just read is refilled and
-// the next one's reads begin under the remaining MFMAs.
+// the next one's reads begin under the remaining MFMAs.  The refill goes out in
+// thirds, in that sub-step and the next two: all at once it holds the MFMAs up in
+// the address unit, later it comes too late (4096 x 8192 x 8192, operands' launch
+// and all, MXFP4: at once 189 us, halves 176, thirds 174, quarters 176; MXFP8 281,
+// 261, 254, 264).
 #pragma once
 
 #include <type_traits>
@@ -218,15 +222,15 @@ __global__ __launch_bounds__(256, (Shape<A4, MB, NB>::kLds > 80 * 1024 ? 1 : 2))
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  constexpr int kEarly = L / 2;  // loads issued in the last sub-step of the step before
+  constexpr int kEarly = L / 3, kMid = 2 * L / 3;  // loads issued in the last sub-step of the step before
   // step t in stage s; its fragments of sub-step 0 and its scales are in
   // registers and the first kEarly loads of step t + 1 are out
   auto step = [&](int t, int s) __attribute__((always_inline)) {
     // the loads' and reads' addresses are made where they are used: all of them
     // kept across the loop do not fit beside 256 accumulators
     asm volatile("" : "+v"(a_g), "+v"(b_g0), "+v"(b_g1), "+v"(a_rd[0]), "+v"(a_rd[1]), "+v"(b_rd[0]), "+v"(b_rd[1]));
-    sub(std::integral_constant<int, 0>{}, t, s, 0, kEarly, L);
-    sub(std::integral_constant<int, 1>{}, t, s, 1, 0, 0);
+    sub(std::integral_constant<int, 0>{}, t, s, 0, kEarly, kMid);
+    sub(std::integral_constant<int, 1>{}, t, s, 1, kMid, L);
     sub(std::integral_constant<int, 2>{}, t, s, 0, 0, 0);
 #pragma unroll
     for (int x = 0; x < NM / 2; ++x) mma(std::integral_constant<int, 3>{}, 1, s, x);
