@@ -813,12 +813,21 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
         // one fused step rounds otherwise than mo was made, by an ulp of mo: from
         // 2^12 on that is left to the exact difference
         const bool slow = edge || __any(fabsf(mo[r]) > 4096.f && mo[r] > kNone);
+        float x[16];
+        if (slow) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float z = Weight(s[r][i / 4][i % 4], cs, lv) - mo[r];
+            x[i] = i > seen ? -__builtin_huge_valf() : z;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(s[r][i / 4][i % 4], cs, off);
+        }
         float ps = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float x = __builtin_fmaf(s[r][i / 4][i % 4], cs, off);
-          if (slow) x = i > seen ? -__builtin_huge_valf() : Weight(s[r][i / 4][i % 4], cs, lv) - mo[r];
-          const float w = __builtin_amdgcn_exp2f(x);
+          const float w = __builtin_amdgcn_exp2f(x[i]);
           ps += w;
           pr[r][i / 8][i % 8] = (_Float16)w;
         }
