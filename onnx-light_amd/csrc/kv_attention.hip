@@ -83,14 +83,21 @@ __device__ __forceinline__ float Weight(float s, float cs, float lv) {
 __device__ __forceinline__ float LogScale(float vs) { return vs > 0x1p-100f ? __builtin_amdgcn_logf(vs) : vs == vs ? -100.f : vs; }
 __device__ __forceinline__ float InvScale(float vs) { return vs > 0x1p-100f ? __builtin_amdgcn_rcpf(vs) : 0x1p100f; }
 
-// The larger over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
+// What the lanes l, l ^ 16, l ^ 32, l ^ 48 (the four lane groups) hold, joined:
+// two swaps of register halves, no trip through LDS.
+template <typename F> __device__ __forceinline__ float OverGroups(float v, F join) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const float w = join(__builtin_bit_cast(float, (unsigned)a[0]), __builtin_bit_cast(float, (unsigned)a[1]));
+  const unsigned x = __builtin_bit_cast(unsigned, w);
+  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return join(__builtin_bit_cast(float, (unsigned)b[0]), __builtin_bit_cast(float, (unsigned)b[1]));
+}
 __device__ __forceinline__ float GroupMax(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  return OverGroups(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float GroupSum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  return OverGroups(v, [](float a, float b) { return a + b; });
 }
 
 // ---------------------------------------------------------------------------
@@ -657,80 +664,103 @@ template <int HD> __device__ __forceinline__ int KeyChunk(int token, int chunk) 
   const int key = HD == 64 ? (token >> 1 & 1) | (token >> 4) << 1 : (token & 3) | (token >> 4) << 2;
   return token * (HD / 8) + (chunk ^ key);
 }
-__device__ __forceinline__ int ValueChunk(int dim, int chunk) { return dim * 8 + (chunk ^ (dim >> 1 & 7)); }
+__device__ __forceinline__ int ValueChunk(int dim, int chunk) {
+  const int key = (dim >> 1 & 1) | (dim >> 2 & 2) | ((dim >> 1 ^ dim) & 4);
+  return dim * 8 + (chunk ^ key);
+}
 
-// A workgroup's loads of one tile: every thread 16 bytes (HD 256: two times) of
-// the keys and of the values.
-template <int HD, bool FP8, bool EXACT> struct TileStage {
+// A workgroup's loads of a tile's codes, one kind (keys or values) at a time:
+// every thread 16 bytes (HD 256: two times).
+template <int HD, bool FP8, bool EXACT, bool VALUES> struct TileStage {
   static constexpr int kEach = HD / 16 * kTile / kRowThreads > 0 ? HD / 16 * kTile / kRowThreads : 1;
   static constexpr bool kAll = HD / 16 * kTile >= kRowThreads;  // every thread loads
-  int kb[kEach], vb[kEach];
-  v4i k[kEach], v[kEach];
-  float ks, vs;
+  int blk[kEach];
+  v4i r[kEach];
 
-  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const Job &j, int t) {
-    const int32_t *table = p.table + (int64_t)j.b * p.max_blocks;
-    for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kRowThreads;
-      kb[e] = table[min(t * kTile + i / (HD / 16) % kTile, j.len - 1) >> p.block_shift];
-      vb[e] = table[min(t * kTile + 16 * (i % 4), j.len - 1) >> p.block_shift];
-    }
+  // The 16 bytes' first token in the tile.
+  __device__ __forceinline__ static int Token(int i) { return VALUES ? 16 * (i % 4) : i / (HD / 16) % kTile; }
+
+  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const Job &j, int t, int tid) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      blk[e] = p.table[(int64_t)j.b * p.max_blocks +
+                       (min(t * kTile + Token(tid + e * kRowThreads), j.len - 1) >> p.block_shift)];
   }
-  __device__ __forceinline__ void Load(const KvCacheParams &p, const Job &j, int t) {
+  __device__ __forceinline__ void Load(const KvCacheParams &p, const Job &j, int t, int tid) {
     const int D = EXACT ? HD : p.head_dim, bt = p.block_tokens;
+#pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kRowThreads;
-      const int token = i / (HD / 16) % kTile, kd = i % (HD / 16) * 16, dim = i / 4 % HD, vt = 16 * (i % 4);
-      const bool bad = vb[e] < 0 || vb[e] >= p.num_blocks;
-      const int64_t k_at = (int64_t)(kb[e] >= 0 && kb[e] < p.num_blocks ? kb[e] : 0) * p.kv_heads + j.head;
-      const int64_t v_at = (int64_t)(bad ? 0 : vb[e]) * p.kv_heads + j.head;
-      const int at = t * kTile & (bt - 1);
-      k[e] = EXACT || kd < D ? *reinterpret_cast<const v4i *>(p.k_cache + (k_at * bt + ((at + token) & (bt - 1))) * D + kd)
-                             : v4i{0, 0, 0, 0};
-      v[e] = EXACT || dim < D ? *reinterpret_cast<const v4i *>(p.v_cache + (v_at * D + dim) * bt + ((at + vt) & (bt - 1)))
-                              : v4i{0, 0, 0, 0};
-      if (e == 0) {
-        ks = p.k_scale[v_at];
-        ks = bad ? __builtin_nanf("") : ks;
-        vs = p.v_scale[v_at];
-      }
+      const int i = tid + e * kRowThreads, at = (t * kTile + Token(i)) & (bt - 1);
+      const int64_t base = ((int64_t)(blk[e] >= 0 && blk[e] < p.num_blocks ? blk[e] : 0) * p.kv_heads + j.head) * bt * D;
+      const int dim = VALUES ? i / 4 % HD : i % (HD / 16) * 16;
+      if constexpr (VALUES)
+        r[e] = EXACT || dim < D ? *reinterpret_cast<const v4i *>(p.v_cache + base + dim * bt + at) : v4i{0, 0, 0, 0};
+      else
+        r[e] = EXACT || dim < D ? *reinterpret_cast<const v4i *>(p.k_cache + base + at * D + dim) : v4i{0, 0, 0, 0};
     }
   }
-  // Codes past the sequence's end may be any, NaN among them: those of v, which
-  // the second product multiplies by zero, become zero.
-  __device__ __forceinline__ void Store(v8h *sk, v8h *sv, float *ss, int left) {
+  // Codes past the sequence's end (`left` tokens of the tile are there) may be
+  // any, NaN among them: those of v, which the second product multiplies by
+  // zero, become zero.
+  __device__ __forceinline__ void Store(v8h *lds, int left, int tid) {
+#pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kRowThreads;
-      const int token = i / (HD / 16) % kTile, kc = i % (HD / 16) * 2, dim = i / 4 % HD, vt = 16 * (i % 4);
-      if (left < kTile)
+      const int i = tid + e * kRowThreads;
+      if (VALUES && left < kTile) {
+#pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const int n = left - vt - 4 * w;
-          v[e][w] &= (int)(n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+          const int n = left - Token(i) - 4 * w;
+          r[e][w] &= (int)(n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
         }
-      if (kAll || i < HD / 16 * kTile) {
-        sk[KeyChunk<HD>(token, kc)] = Widen<FP8>(k[e][0], k[e][1]);
-        sk[KeyChunk<HD>(token, kc + 1)] = Widen<FP8>(k[e][2], k[e][3]);
-        sv[ValueChunk(dim, i % 4 * 2)] = Widen<FP8>(v[e][0], v[e][1]);
-        sv[ValueChunk(dim, i % 4 * 2 + 1)] = Widen<FP8>(v[e][2], v[e][3]);
       }
-    }
-    if (threadIdx.x < 4) {
-      ss[threadIdx.x] = ks;
-      ss[4 + threadIdx.x] = vs;
+      if (!kAll && i >= HD / 16 * kTile) continue;
+      const int row = VALUES ? i / 4 % HD : Token(i), c = VALUES ? i % 4 * 2 : i % (HD / 16) * 2;
+      lds[VALUES ? ValueChunk(row, c) : KeyChunk<HD>(row, c)] = Widen<FP8>(r[e][0], r[e][1]);
+      lds[VALUES ? ValueChunk(row, c + 1) : KeyChunk<HD>(row, c + 1)] = Widen<FP8>(r[e][2], r[e][3]);
     }
   }
 };
+
+// Both scales of a lane group's 16 tokens, a tile ahead, and their block two
+// ahead.  A block outside the cache gives a NaN score.
+struct ScaleStage {
+  int blk;
+  float ks, vs;
+  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const Job &j, int t, int g) {
+    blk = p.table[(int64_t)j.b * p.max_blocks + (min(t * kTile + 16 * g, j.len - 1) >> p.block_shift)];
+  }
+  __device__ __forceinline__ void Load(const KvCacheParams &p, const Job &j) {
+    const bool bad = blk < 0 || blk >= p.num_blocks;
+    const int64_t at = (int64_t)(bad ? 0 : blk) * p.kv_heads + j.head;
+    ks = p.k_scale[at];
+    vs = p.v_scale[at];
+    if (bad) ks = __builtin_nanf("");
+  }
+};
+
+constexpr int kAhead = 6;
+
+// v, from which addresses are made anew at this place: kept over the loop they
+// would take more registers than there are.
+__device__ __forceinline__ int Here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// LDS writes and reads of this wave are done; so for all waves.  Loads stay in
+// flight.
+__device__ __forceinline__ void SlotBarrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int HD, int CT, bool FP8, bool EXACT>
 __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
   constexpr int DT = HD / 16, KS = HD / 32, kRows = kRowWaves * CT * 16;
   __shared__ v8h sk[2][kTile * HD / 8], sv[2][kTile * HD / 8];
-  __shared__ float ss[2][8];
   __shared__ RowLine line;
   __shared__ unsigned before;
   const KvCacheParams &cp = p.a.c;
   const int tid = threadIdx.x, lane = tid % 64, c = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const bool late = wave >= kRowWaves / 2;  // the half of the waves that runs a slot behind
   if (p.fill) FillInvalid(p);
   const int64_t units = MakeRowLine(p, line, kRows);
   const int64_t piece = (units + gridDim.x - 1) / gridDim.x;
@@ -740,10 +770,16 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     const Job j = FindRowJob(p, line, u, kRows);
     const int t0 = (int)(u - j.first), t1 = (int)(end - j.first < j.tiles ? end - j.first : j.tiles);
     const int wrow = j.row0 + wave * CT * 16, rows = j.n * p.group, before_new = j.len - j.n;
-    TileStage<HD, FP8, EXACT> st;
-    st.Lookup(cp, j, t0);
-    st.Load(cp, j, t0);
-    st.Lookup(cp, j, min(t0 + 1, t1 - 1));
+    TileStage<HD, FP8, EXACT, false> keys;
+    TileStage<HD, FP8, EXACT, true> values;
+    ScaleStage scales;
+    keys.Lookup(cp, j, t0, tid);
+    values.Lookup(cp, j, t0, tid);
+    scales.Lookup(cp, j, t0, g);
+    keys.Load(cp, j, t0, tid);
+    keys.Lookup(cp, j, t0 + 1, tid);
+    scales.Load(cp, j);
+    scales.Lookup(cp, j, t0 + 1, g);
     v8h q[CT][KS];
     float qf[CT];
     int last[CT];  // the last token that the row sees
@@ -755,10 +791,25 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
       LoadQ<KS, EXACT>(p.a, at, row < rows, g, q[r], qf[r]);
     }
     __syncthreads();  // the buffers of the job before were read
-    st.Store(sk[0], sv[0], ss[0], j.len - t0 * kTile);
-    st.Load(cp, j, min(t0 + 1, t1 - 1));
-    st.Lookup(cp, j, min(t0 + 2, t1 - 1));
-    v4f o[CT][DT];
+    keys.Store(sk[0], 0, tid);
+    keys.Load(cp, j, t0 + 1, tid);
+    keys.Lookup(cp, j, t0 + 2, tid);
+    values.Load(cp, j, t0, tid);
+    values.Lookup(cp, j, t0 + 1, tid);
+    // Stages the keys of tile a and the values of the one before, and loads one
+    // tile further.  Past the job's last tile that writes a buffer that nobody
+    // reads again.
+    auto stage = [&](int a) __attribute__((always_inline)) {
+      const int me = Here(tid);
+      keys.Store(sk[(a - t0) & 1], 0, me);
+      values.Store(sv[(a - 1 - t0) & 1], j.len - (a - 1) * kTile, me);
+      keys.Load(cp, j, a + 1, me);
+      values.Load(cp, j, a, me);
+      keys.Lookup(cp, j, a + 2, me);
+      values.Lookup(cp, j, a + 1, me);
+    };
+    v4f o[CT][DT], s[CT][4];
+    v8h pr[CT][2];
     float mo[CT], sum[CT];
 #pragma unroll
     for (int r = 0; r < CT; ++r) {
@@ -769,85 +820,142 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     }
     // the tokens that every row of the wave sees end here
     const int all_see = before_new + min(wrow, rows - 1) / p.group + 1;
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1, base = t * kTile;
-      const v8h *ck = sk[buf], *cv = sv[buf];
-      v4f s[CT][4];
+    // The products of a slot: values of tile tv (V), then keys of tile tk (K).  Each
+    // operand read from LDS serves CT MFMAs, which are shorter than the read takes:
+    // kAhead reads are in flight.
+    auto multiply = [&](auto V, auto K, int tv, int tk) __attribute__((always_inline)) {
+      constexpr int kV = decltype(V)::value ? 2 * DT : 0, kN = kV + (decltype(K)::value ? 4 * KS : 0);
+      const v8h *cv = sv[(tv - t0) & 1], *ck = sk[(tk - t0) & 1];
+      const int me = Here(lane), c = me % 16, g = me / 16;
+      // value operands in the order of pairs of d, key operands of pairs of i, so that
+      // an accumulator's next product is CT * 2 away
+      auto read = [&](int n) __attribute__((always_inline)) {
+        if (n < kV) return cv[ValueChunk(c, 2 * g + n / 2 % 2) + 16 * 8 * (n / 4 * 2 + n % 2)];
+        const int m = n - kV, i = m / (2 * KS) * 2 + m % 2;
+        return ck[KeyChunk<HD>(16 * (c / 4) + c % 4, 4 * (m / 2 % KS) + g) + 4 * HD / 8 * i];
+      };
+      v8h a[kN];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int n = 0; n < kAhead; ++n) a[n] = read(n);
 #pragma unroll
-        for (int r = 0; r < CT; ++r) s[r][i] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < kN; ++n) {
+        if (n + kAhead < kN) a[n + kAhead] = read(n + kAhead);
+        const int m = n - kV;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const v8h a = ck[KeyChunk<HD>(16 * (c / 4) + 4 * i + c % 4, 4 * k + g)];
-#pragma unroll
-          for (int r = 0; r < CT; ++r) s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[r][k], s[r][i], 0, 0, 0);
+        for (int r = 0; r < CT; ++r) {
+          if (n < kV) {
+            v4f &x = o[r][n / 4 * 2 + n % 2];
+            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[n], pr[r][n / 2 % 2], x, 0, 0, 0);
+          } else {
+            v4f &x = s[r][m / (2 * KS) * 2 + m % 2];
+            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[n], q[r][m / 2 % KS], m / 2 % KS ? x : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);  // or all reads go first, into registers that are not there
       }
-      const float ks = ss[buf][g], vs = ss[buf][4 + g];
-      const float lv = LogScale(vs), inv = InvScale(vs);
+    };
+    auto softmax = [&](int t) __attribute__((always_inline)) {
+      const int base = t * kTile;
+      const float lv = LogScale(scales.vs), inv = InvScale(scales.vs), ks = scales.ks;
+      scales.Load(cp, j);
+      scales.Lookup(cp, j, t + 2, g);
       const bool edge = base + kTile > all_see;
-      v8h pr[CT][2];
+      float top[CT], cs[CT], off[CT], ps[CT];
+      int seen[CT];  // the row sees the lane's tokens 0 .. seen
 #pragma unroll
       for (int r = 0; r < CT; ++r) {
-        const float cs = ks * qf[r];
-        const int seen = last[r] - base - 16 * g;  // the row sees the lane's tokens 0 .. seen
-        float top = s[r][0][0];
-        if (edge) {
-          top = -__builtin_huge_valf();
+        cs[r] = ks * qf[r];
+        seen[r] = last[r] - base - 16 * g;
+      }
+      if (edge) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top = i <= seen ? fmaxf(top, s[r][i / 4][i % 4]) : top;
-        } else {
-          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i / 4][i % 4]);
+        for (int r = 0; r < CT; ++r) {
+          top[r] = -__builtin_huge_valf();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top[r] = i <= seen[r] ? fmaxf(top[r], s[r][i / 4][i % 4]) : top[r];
         }
-        top = GroupMax(Weight(top, cs, lv));
-        if (__any(top > mo[r] + kLag)) {
-          const float now = fmaxf(mo[r], top), keep = __builtin_amdgcn_exp2f(mo[r] - now);
+      } else {
+#pragma unroll
+        for (int r = 0; r < CT; ++r) {
+          top[r] = s[r][0][0];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) top[r] = fmaxf(top[r], s[r][i / 4][i % 4]);
+        }
+      }
+      bool up = false, far = false;
+#pragma unroll
+      for (int r = 0; r < CT; ++r) {
+        top[r] = GroupMax(Weight(top[r], cs[r], lv));
+        up |= top[r] > mo[r] + kLag;
+      }
+      if (__any(up)) {
+#pragma unroll
+        for (int r = 0; r < CT; ++r) {
+          const float now = fmaxf(mo[r], top[r]), keep = __builtin_amdgcn_exp2f(mo[r] - now);
           mo[r] = now;
           sum[r] *= keep;
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[r][d] *= keep;
         }
-        const float off = lv - mo[r];
-        // one fused step rounds otherwise than mo was made, by an ulp of mo: from
-        // 2^12 on that is left to the exact difference
-        const bool slow = edge || __any(fabsf(mo[r]) > 4096.f && mo[r] > kNone);
-        float x[16];
-        if (slow) {
+      }
+#pragma unroll
+      for (int r = 0; r < CT; ++r) {
+        off[r] = lv - mo[r];
+        ps[r] = 0.f;
+        far |= fabsf(mo[r]) > 4096.f && mo[r] > kNone;
+      }
+      // one fused step rounds otherwise than mo was made, by an ulp of mo: from
+      // 2^12 on that is left to the exact difference
+      if (edge || __any(far)) {
+#pragma unroll
+        for (int r = 0; r < CT; ++r)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float z = Weight(s[r][i / 4][i % 4], cs, lv) - mo[r];
-            x[i] = i > seen ? -__builtin_huge_valf() : z;
+            const float z = Weight(s[r][i / 4][i % 4], cs[r], lv) - mo[r];
+            s[r][i / 4][i % 4] = i > seen[r] ? -__builtin_huge_valf() : z;
           }
-        } else {
+      } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(s[r][i / 4][i % 4], cs, off);
-        }
-        float ps = 0.f;
+        for (int r = 0; r < CT; ++r)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float w = __builtin_amdgcn_exp2f(x[i]);
-          ps += w;
+          for (int i = 0; i < 16; ++i) s[r][i / 4][i % 4] = __builtin_fmaf(s[r][i / 4][i % 4], cs[r], off[r]);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int r = 0; r < CT; ++r) {
+          const float w = __builtin_amdgcn_exp2f(s[r][i / 4][i % 4]);
+          ps[r] += w;
           pr[r][i / 8][i % 8] = (_Float16)w;
         }
-        sum[r] = __builtin_fmaf(ps, inv, sum[r]);
-      }
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const v8h a = cv[ValueChunk(16 * d + c, 2 * g + h)];
-#pragma unroll
-          for (int r = 0; r < CT; ++r) o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pr[r][h], o[r][d], 0, 0, 0);
-        }
-      if (t + 1 < t1) {
-        st.Store(sk[buf ^ 1], sv[buf ^ 1], ss[buf ^ 1], j.len - (t + 1) * kTile);
-        st.Load(cp, j, min(t + 2, t1 - 1));
-        st.Lookup(cp, j, min(t + 3, t1 - 1));
-      }
-      __syncthreads();
+      for (int r = 0; r < CT; ++r) sum[r] = __builtin_fmaf(ps[r], inv, sum[r]);
+    };
+    // Slots: in one half of the waves multiplies (values of tile t - 1, keys of
+    // tile t) while the other is at its softmax and staging; then they change
+    // places.  In slots 2 (t - t0) and the next, keys t and values t - 1 are read and
+    // keys t + 1 and values t are written, each into the other buffer.
+    const std::true_type yes;
+    const std::false_type no;
+    SlotBarrier();
+    if (late) {
+      stage(t0 + 1);
+      SlotBarrier();
     }
+    multiply(no, yes, t0, t0);
+    SlotBarrier();
+    for (int t = t0; t < t1 - 1; ++t) {
+      softmax(t);
+      stage(t + (late ? 2 : 1));
+      SlotBarrier();
+      multiply(yes, yes, t, t + 1);
+      SlotBarrier();
+    }
+    softmax(t1 - 1);
+    stage(t1 + (late ? 1 : 0));
+    SlotBarrier();
+    multiply(yes, no, t1 - 1, t1);
+    if (!late) SlotBarrier();
 #pragma unroll
     for (int r = 0; r < CT; ++r) sum[r] = GroupSum(sum[r]);
     const bool whole = t0 == 0 && t1 == j.tiles;
