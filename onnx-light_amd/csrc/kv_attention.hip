@@ -669,54 +669,98 @@ __device__ __forceinline__ int ValueChunk(int dim, int chunk) {
   return dim * 8 + (chunk ^ key);
 }
 
-// A workgroup's loads of a tile's codes, one kind (keys or values) at a time:
-// every thread 16 bytes (HD 256: two times).
-template <int HD, bool FP8, bool EXACT, bool VALUES> struct TileStage {
-  static constexpr int kEach = HD / 16 * kTile / kRowThreads > 0 ? HD / 16 * kTile / kRowThreads : 1;
-  static constexpr bool kAll = HD / 16 * kTile >= kRowThreads;  // every thread loads
+// The loads of a tile's codes by a workgroup, every thread 16 bytes (HD 256: two
+// times).  A block of the cache has fewer than 2^32 bytes.  With `at` the place
+// of the tile's first token in its block (zero for blocks of less than a tile),
+// a thread's place is that plus a constant.
+
+// Keys: the tokens of a wave's load lie in one block, so that its address is
+// scalar and the thread's part is 32 bits.
+template <int HD, bool FP8, bool EXACT> struct KeyStage {
+  static constexpr int kChunks = HD / 16, kEach = (kChunks * kTile + kRowThreads - 1) / kRowThreads;
   int blk[kEach];
   v4i r[kEach];
+  unsigned off;  // from the tile's first token to this thread's bytes, in the block
+  bool live;     // this thread's dimensions are there
 
-  // The 16 bytes' first token in the tile.
-  __device__ __forceinline__ static int Token(int i) { return VALUES ? 16 * (i % 4) : i / (HD / 16) % kTile; }
-
-  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const Job &j, int t, int tid) {
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      blk[e] = p.table[(int64_t)j.b * p.max_blocks +
-                       (min(t * kTile + Token(tid + e * kRowThreads), j.len - 1) >> p.block_shift)];
+  __device__ __forceinline__ static int Token(int e) { return (int)(threadIdx.x + e * kRowThreads) / kChunks % kTile; }
+  __device__ __forceinline__ void Start(const KvCacheParams &p) {
+    const int dim = (int)threadIdx.x % kChunks * 16;
+    live = EXACT || dim < p.head_dim;
+    off = (unsigned)((Token(0) & (p.block_tokens - 1)) * p.head_dim + (live ? dim : 0));
   }
-  __device__ __forceinline__ void Load(const KvCacheParams &p, const Job &j, int t, int tid) {
-    const int D = EXACT ? HD : p.head_dim, bt = p.block_tokens;
+  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const int32_t *table, int last, int t) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) blk[e] = table[min(t * kTile + Uniform(Token(e)), last) >> p.block_shift];
+  }
+  __device__ __forceinline__ void Load(const KvCacheParams &p, const uint8_t *head, unsigned stride, unsigned blocks, int t) {
+    const int bt = p.block_tokens;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = tid + e * kRowThreads, at = (t * kTile + Token(i)) & (bt - 1);
-      const int64_t base = ((int64_t)(blk[e] >= 0 && blk[e] < p.num_blocks ? blk[e] : 0) * p.kv_heads + j.head) * bt * D;
-      const int dim = VALUES ? i / 4 % HD : i % (HD / 16) * 16;
-      if constexpr (VALUES)
-        r[e] = EXACT || dim < D ? *reinterpret_cast<const v4i *>(p.v_cache + base + dim * bt + at) : v4i{0, 0, 0, 0};
-      else
-        r[e] = EXACT || dim < D ? *reinterpret_cast<const v4i *>(p.k_cache + base + at * D + dim) : v4i{0, 0, 0, 0};
+      const unsigned u = (unsigned)Uniform(blk[e]);
+      const int at = ((t * kTile) & (bt - 1)) + ((e * kRowThreads / kChunks) & (bt - 1));
+      const uint8_t *base = head + (uint64_t)(u < blocks ? u : 0) * stride + at * p.head_dim;
+      r[e] = *reinterpret_cast<const v4i *>(base + off);
+      if (!EXACT && !live) r[e] = v4i{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ void Store(char *lds) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (kChunks * kTile < kRowThreads && threadIdx.x >= kChunks * kTile) continue;
+      const unsigned at = KeyChunk<HD>(Token(e), (int)threadIdx.x % kChunks * 2) * 16;
+      *reinterpret_cast<v8h *>(lds + at) = Widen<FP8>(r[e][0], r[e][1]);
+      *reinterpret_cast<v8h *>(lds + (at ^ 16)) = Widen<FP8>(r[e][2], r[e][3]);
+    }
+  }
+};
+
+// Values: four lanes take the 64 tokens of a dimension.
+template <int HD, bool FP8, bool EXACT> struct ValueStage {
+  static constexpr int kEach = (HD * 4 + kRowThreads - 1) / kRowThreads;
+  int blk;
+  v4i r[kEach];
+  const uint8_t *base;  // this thread's bytes of the tile's first tokens in block 0
+  bool live[kEach];
+
+  __device__ __forceinline__ static int Token() { return 16 * (threadIdx.x % 4); }
+  __device__ __forceinline__ static int Dim(int e) { return (int)(threadIdx.x + e * kRowThreads) / 4 % HD; }
+  __device__ __forceinline__ void Start(const KvCacheParams &p, const uint8_t *head) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) live[e] = EXACT || Dim(e) < p.head_dim;
+    base = head + (live[0] ? Dim(0) * p.block_tokens : 0) + (Token() & (p.block_tokens - 1));
+  }
+  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const int32_t *table, int last, int t) {
+    blk = table[(unsigned)min(t * kTile + Token(), last) >> p.block_shift];
+  }
+  __device__ __forceinline__ void Load(const KvCacheParams &p, unsigned stride, unsigned blocks, int t) {
+    const unsigned u = (unsigned)blk < blocks ? (unsigned)blk : 0u;
+    const uint8_t *at = base + ((t * kTile) & (p.block_tokens - 1)) + (uint64_t)u * stride;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const bool here = EXACT || live[e];
+      r[e] = here ? *reinterpret_cast<const v4i *>(at + e * kRowThreads / 4 * p.block_tokens) : v4i{0, 0, 0, 0};
     }
   }
   // Codes past the sequence's end (`left` tokens of the tile are there) may be
-  // any, NaN among them: those of v, which the second product multiplies by
-  // zero, become zero.
-  __device__ __forceinline__ void Store(v8h *lds, int left, int tid) {
+  // any, NaN among them: as the second product multiplies them by zero, they
+  // become zero.
+  __device__ __forceinline__ void Store(char *lds, int left) {
+    if (left < kTile) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int n = left - Token() - 4 * w;
+        const int mask = (int)(n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) r[e][w] &= mask;
+      }
+    }
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = tid + e * kRowThreads;
-      if (VALUES && left < kTile) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int n = left - Token(i) - 4 * w;
-          r[e][w] &= (int)(n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
-        }
-      }
-      if (!kAll && i >= HD / 16 * kTile) continue;
-      const int row = VALUES ? i / 4 % HD : Token(i), c = VALUES ? i % 4 * 2 : i % (HD / 16) * 2;
-      lds[VALUES ? ValueChunk(row, c) : KeyChunk<HD>(row, c)] = Widen<FP8>(r[e][0], r[e][1]);
-      lds[VALUES ? ValueChunk(row, c + 1) : KeyChunk<HD>(row, c + 1)] = Widen<FP8>(r[e][2], r[e][3]);
+      if (HD * 4 < kRowThreads && threadIdx.x >= HD * 4) continue;
+      const unsigned at = ValueChunk(Dim(e), (int)threadIdx.x % 4 * 2) * 16;
+      *reinterpret_cast<v8h *>(lds + at) = Widen<FP8>(r[e][0], r[e][1]);
+      *reinterpret_cast<v8h *>(lds + (at ^ 16)) = Widen<FP8>(r[e][2], r[e][3]);
     }
   }
 };
@@ -726,12 +770,12 @@ template <int HD, bool FP8, bool EXACT, bool VALUES> struct TileStage {
 struct ScaleStage {
   int blk;
   float ks, vs;
-  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const Job &j, int t, int g) {
-    blk = p.table[(int64_t)j.b * p.max_blocks + (min(t * kTile + 16 * g, j.len - 1) >> p.block_shift)];
+  __device__ __forceinline__ void Lookup(const KvCacheParams &p, const int32_t *table, int last, int t, int g) {
+    blk = table[(unsigned)min(t * kTile + 16 * g, last) >> p.block_shift];
   }
-  __device__ __forceinline__ void Load(const KvCacheParams &p, const Job &j) {
-    const bool bad = blk < 0 || blk >= p.num_blocks;
-    const int64_t at = (int64_t)(bad ? 0 : blk) * p.kv_heads + j.head;
+  __device__ __forceinline__ void Load(const KvCacheParams &p, int head, unsigned blocks) {
+    const bool bad = (unsigned)blk >= blocks;
+    const uint64_t at = (uint64_t)(bad ? 0u : (unsigned)blk) * (unsigned)p.kv_heads + (unsigned)head;
     ks = p.k_scale[at];
     vs = p.v_scale[at];
     if (bad) ks = __builtin_nanf("");
@@ -740,13 +784,6 @@ struct ScaleStage {
 
 constexpr int kAhead = 6;
 
-// v, from which addresses are made anew at this place: kept over the loop they
-// would take more registers than there are.
-__device__ __forceinline__ int Here(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
 // LDS writes and reads of this wave are done; so for all waves.  Loads stay in
 // flight.
 __device__ __forceinline__ void SlotBarrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -754,7 +791,8 @@ __device__ __forceinline__ void SlotBarrier() { asm volatile("s_waitcnt lgkmcnt(
 template <int HD, int CT, bool FP8, bool EXACT>
 __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
   constexpr int DT = HD / 16, KS = HD / 32, kRows = kRowWaves * CT * 16;
-  __shared__ v8h sk[2][kTile * HD / 8], sv[2][kTile * HD / 8];
+  constexpr unsigned kBuffer = kTile * HD * 2, kValues = 2 * kBuffer;  // two buffers of keys, two of values
+  __shared__ __align__(16) char lds[4 * kBuffer];
   __shared__ RowLine line;
   __shared__ unsigned before;
   const KvCacheParams &cp = p.a.c;
@@ -770,16 +808,22 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     const Job j = FindRowJob(p, line, u, kRows);
     const int t0 = (int)(u - j.first), t1 = (int)(end - j.first < j.tiles ? end - j.first : j.tiles);
     const int wrow = j.row0 + wave * CT * 16, rows = j.n * p.group, before_new = j.len - j.n;
-    TileStage<HD, FP8, EXACT, false> keys;
-    TileStage<HD, FP8, EXACT, true> values;
+    const int32_t *table = cp.table + (int64_t)j.b * cp.max_blocks;
+    const unsigned stride = (unsigned)cp.kv_heads * (unsigned)(cp.block_tokens * cp.head_dim);
+    const unsigned blocks = (unsigned)(cp.num_blocks < INT64_C(0x80000000) ? cp.num_blocks : INT64_C(0x80000000));
+    const uint64_t head = (uint64_t)j.head * (unsigned)(cp.block_tokens * cp.head_dim);
+    KeyStage<HD, FP8, EXACT> keys;
+    ValueStage<HD, FP8, EXACT> values;
     ScaleStage scales;
-    keys.Lookup(cp, j, t0, tid);
-    values.Lookup(cp, j, t0, tid);
-    scales.Lookup(cp, j, t0, g);
-    keys.Load(cp, j, t0, tid);
-    keys.Lookup(cp, j, t0 + 1, tid);
-    scales.Load(cp, j);
-    scales.Lookup(cp, j, t0 + 1, g);
+    keys.Start(cp);
+    values.Start(cp, cp.v_cache + head);
+    keys.Lookup(cp, table, j.len - 1, t0);
+    values.Lookup(cp, table, j.len - 1, t0);
+    scales.Lookup(cp, table, j.len - 1, t0, g);
+    keys.Load(cp, cp.k_cache + head, stride, blocks, t0);
+    keys.Lookup(cp, table, j.len - 1, t0 + 1);
+    scales.Load(cp, j.head, blocks);
+    scales.Lookup(cp, table, j.len - 1, t0 + 1, g);
     v8h q[CT][KS];
     float qf[CT];
     int last[CT];  // the last token that the row sees
@@ -791,22 +835,21 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
       LoadQ<KS, EXACT>(p.a, at, row < rows, g, q[r], qf[r]);
     }
     __syncthreads();  // the buffers of the job before were read
-    keys.Store(sk[0], 0, tid);
-    keys.Load(cp, j, t0 + 1, tid);
-    keys.Lookup(cp, j, t0 + 2, tid);
-    values.Load(cp, j, t0, tid);
-    values.Lookup(cp, j, t0 + 1, tid);
+    keys.Store(lds);
+    keys.Load(cp, cp.k_cache + head, stride, blocks, t0 + 1);
+    keys.Lookup(cp, table, j.len - 1, t0 + 2);
+    values.Load(cp, stride, blocks, t0);
+    values.Lookup(cp, table, j.len - 1, t0 + 1);
     // Stages the keys of tile a and the values of the one before, and loads one
     // tile further.  Past the job's last tile that writes a buffer that nobody
     // reads again.
     auto stage = [&](int a) __attribute__((always_inline)) {
-      const int me = Here(tid);
-      keys.Store(sk[(a - t0) & 1], 0, me);
-      values.Store(sv[(a - 1 - t0) & 1], j.len - (a - 1) * kTile, me);
-      keys.Load(cp, j, a + 1, me);
-      values.Load(cp, j, a, me);
-      keys.Lookup(cp, j, a + 2, me);
-      values.Lookup(cp, j, a + 1, me);
+      keys.Store(lds + ((a - t0) & 1) * kBuffer);
+      values.Store(lds + kValues + ((a - 1 - t0) & 1) * kBuffer, j.len - (a - 1) * kTile);
+      keys.Load(cp, cp.k_cache + head, stride, blocks, a + 1);
+      values.Load(cp, stride, blocks, a);
+      keys.Lookup(cp, table, j.len - 1, a + 2);
+      values.Lookup(cp, table, j.len - 1, a + 1);
     };
     v4f o[CT][DT], s[CT][4];
     v8h pr[CT][2];
@@ -820,19 +863,20 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     }
     // the tokens that every row of the wave sees end here
     const int all_see = before_new + min(wrow, rows - 1) / p.group + 1;
+    // this lane's first operands; those of the other k are an exclusive or away
+    const unsigned my_keys = KeyChunk<HD>(16 * (c / 4) + c % 4, g) * 16, my_values = ValueChunk(c, 2 * g) * 16;
     // The products of a slot: values of tile tv (V), then keys of tile tk (K).  Each
     // operand read from LDS serves CT MFMAs, which are shorter than the read takes:
     // kAhead reads are in flight.
     auto multiply = [&](auto V, auto K, int tv, int tk) __attribute__((always_inline)) {
       constexpr int kV = decltype(V)::value ? 2 * DT : 0, kN = kV + (decltype(K)::value ? 4 * KS : 0);
-      const v8h *cv = sv[(tv - t0) & 1], *ck = sk[(tk - t0) & 1];
-      const int me = Here(lane), c = me % 16, g = me / 16;
       // value operands in the order of pairs of d, key operands of pairs of i, so that
       // an accumulator's next product is CT * 2 away
       auto read = [&](int n) __attribute__((always_inline)) {
-        if (n < kV) return cv[ValueChunk(c, 2 * g + n / 2 % 2) + 16 * 8 * (n / 4 * 2 + n % 2)];
         const int m = n - kV, i = m / (2 * KS) * 2 + m % 2;
-        return ck[KeyChunk<HD>(16 * (c / 4) + c % 4, 4 * (m / 2 % KS) + g) + 4 * HD / 8 * i];
+        const unsigned at = n < kV ? (my_values ^ (((tv - t0) & 1) * kBuffer | n / 2 % 2 * 16)) + kValues + 16 * 128 * (n / 4 * 2 + n % 2)
+                                   : (my_keys ^ (((tk - t0) & 1) * kBuffer | m / 2 % KS * 64)) + 8 * HD * i;
+        return *reinterpret_cast<const v8h *>(lds + at);
       };
       v8h a[kN];
 #pragma unroll
@@ -857,8 +901,8 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     auto softmax = [&](int t) __attribute__((always_inline)) {
       const int base = t * kTile;
       const float lv = LogScale(scales.vs), inv = InvScale(scales.vs), ks = scales.ks;
-      scales.Load(cp, j);
-      scales.Lookup(cp, j, t + 2, g);
+      scales.Load(cp, j.head, blocks);
+      scales.Lookup(cp, table, j.len - 1, t + 2, g);
       const bool edge = base + kTile > all_see;
       float top[CT], cs[CT], off[CT], ps[CT];
       int seen[CT];  // the row sees the lane's tokens 0 .. seen
