@@ -65,9 +65,11 @@ template <bool FP8> __device__ __forceinline__ v8h Widen(int lo, int hi) {
 }
 
 __device__ __forceinline__ uint2 Pack4(v4f v, int bf16) {
-  uint16_t h[4];
-  for (int i = 0; i < 4; ++i) h[i] = bf16 ? F32ToBf16(v[i]) : F32ToF16(v[i]);
-  return make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
+  typedef __bf16 v4b __attribute__((ext_vector_type(4)));
+  typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+  const uint2 b = __builtin_bit_cast(uint2, __builtin_convertvector(v, v4b));
+  const uint2 h = __builtin_bit_cast(uint2, __builtin_convertvector(v, v4h));
+  return make_uint2(bf16 ? b.x : h.x, bf16 ? b.y : h.y);
 }
 
 // log2 of a token's weight in O: score (s * cs) plus log2 of its v scale, two
@@ -83,21 +85,22 @@ __device__ __forceinline__ float Weight(float s, float cs, float lv) {
 __device__ __forceinline__ float LogScale(float vs) { return vs > 0x1p-100f ? __builtin_amdgcn_logf(vs) : vs == vs ? -100.f : vs; }
 __device__ __forceinline__ float InvScale(float vs) { return vs > 0x1p-100f ? __builtin_amdgcn_rcpf(vs) : 0x1p100f; }
 
-// What the lanes l, l ^ 16, l ^ 32, l ^ 48 (the four lane groups) hold, joined:
-// two swaps of register halves, no trip through LDS.
-template <typename F> __device__ __forceinline__ float OverGroups(float v, F join) {
+// What the G lane groups hold (lanes l, l ^ 32 and, of four, l ^ 16, l ^ 48),
+// joined: swaps of register halves, no trip through LDS.
+template <int G, typename F> __device__ __forceinline__ float OverGroups(float v, F join) {
   const unsigned u = __builtin_bit_cast(unsigned, v);
   const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   const float w = join(__builtin_bit_cast(float, (unsigned)a[0]), __builtin_bit_cast(float, (unsigned)a[1]));
+  if (G == 2) return w;
   const unsigned x = __builtin_bit_cast(unsigned, w);
   const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
   return join(__builtin_bit_cast(float, (unsigned)b[0]), __builtin_bit_cast(float, (unsigned)b[1]));
 }
-__device__ __forceinline__ float GroupMax(float v) {
-  return OverGroups(v, [](float a, float b) { return fmaxf(a, b); });
+template <int G = 4> __device__ __forceinline__ float GroupMax(float v) {
+  return OverGroups<G>(v, [](float a, float b) { return fmaxf(a, b); });
 }
-__device__ __forceinline__ float GroupSum(float v) {
-  return OverGroups(v, [](float a, float b) { return a + b; });
+template <int G = 4> __device__ __forceinline__ float GroupSum(float v) {
+  return OverGroups<G>(v, [](float a, float b) { return a + b; });
 }
 
 // ---------------------------------------------------------------------------
@@ -116,6 +119,7 @@ struct Line {        // units before every thread's share of the sequences
 
 struct Job {
   int b, n, len, head, row0;  // sequence, its new tokens and length, kv head, first row
+  int start;                  // its first new token
   int tiles;                  // units of the job
   int64_t first;              // its first unit on the line
 };
@@ -185,6 +189,7 @@ __device__ __forceinline__ Job FindJob(const Plan &p, const Line &line, int64_t 
   j.b = b = Uniform(b);
   j.n = Uniform(RowsOf(p, b));
   j.len = Uniform(p.a.c.lengths[b]);
+  j.start = Uniform(p.a.c.start[b]);
   j.tiles = (j.len + kTile - 1) / kTile;
   const int row_tiles = (j.n * p.group + 15) / 16;
   const int64_t k = Uniform((u - at) / j.tiles);
@@ -213,15 +218,19 @@ __device__ __forceinline__ int64_t PieceOf(int64_t units) {
 }
 
 // Writes O / sum of the rows that there are.
+// Where a row's output goes, and the dimensions from d on of it.
+__device__ __forceinline__ uint16_t *OutRow(const Plan &p, const Job &j, int row) {
+  const int64_t token = j.start + (int64_t)(row / p.group);
+  return static_cast<uint16_t *>(p.a.out) + (token * p.a.heads + j.head * p.group + row % p.group) * p.a.c.head_dim;
+}
+__device__ __forceinline__ void StoreDims(const Plan &p, uint16_t *out, int d, v4f o) {
+  if (d >= p.a.c.head_dim) return;
+  const uint2 h = Pack4(o, p.a.bf16);
+  __builtin_memcpy(out + d, &h, 8);
+}
 __device__ __forceinline__ void StoreRows(const Plan &p, const Job &j, int t, v4f o, float sum) {
-  const int c = threadIdx.x % 16, g = threadIdx.x % 64 / 16, row = j.row0 + c, d = 16 * t + 4 * g;
-  if (row >= j.n * p.group || d >= p.a.c.head_dim) return;
-  const float f = 1.f / sum;
-  const int64_t token = p.a.c.start[j.b] + row / p.group;
-  const int head = j.head * p.group + row % p.group;
-  uint16_t *out = static_cast<uint16_t *>(p.a.out) + (token * p.a.heads + head) * p.a.c.head_dim + d;
-  const uint2 h = Pack4(o * f, p.a.bf16);
-  __builtin_memcpy(out, &h, 8);
+  const int row = j.row0 + threadIdx.x % 16;
+  if (row < j.n * p.group) StoreDims(p, OutRow(p, j, row), 16 * t + threadIdx.x % 64 / 16 * 4, o * (1.f / sum));
 }
 
 // 16 bytes from any address.
@@ -538,22 +547,31 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
 // Q of one row for the prompt kernel: lane group g holds the dimensions 32 k +
 // 8 g + (0..7) at q[k], scaled to [1, 2); qf gives the scores in powers of two,
 // and is not negative (the sign of the softmax scale goes to Q).
-template <int KS, bool EXACT>
+template <int G, int KS, bool EXACT>
 __device__ __forceinline__ void LoadQ(const KvAttentionParams &p, int64_t at, bool live, int g, v8h (&q)[KS], float &qf) {
   float v[KS][8], top = 0.f;
+  v4i raw[KS];  // all loads first; `at` is a row that is there also where live is not set
+#pragma unroll
   for (int k = 0; k < KS; ++k) {
-    const int d = 32 * k + 8 * g;
-    const v4i raw = live && (EXACT || d < p.c.head_dim) ? Load16(static_cast<const uint16_t *>(p.q) + at + d) : v4i{0, 0, 0, 0};
+    const int d = 8 * (G * k + g);
+    raw[k] = Load16(static_cast<const uint16_t *>(p.q) + at + (EXACT || d < p.c.head_dim ? d : 0));
+  }
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    const bool here = live && (EXACT || 8 * (G * k + g) < p.c.head_dim);
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int w = raw[i / 2];
+      const int w = here ? raw[k][i / 2] : 0;
       const uint16_t u = (uint16_t)((unsigned)w >> (16 * (i % 2)));
       v[k][i] = p.bf16 ? Bf16ToF32(u) : F16ToF32(u);
       top = fmaxf(top, fabsf(v[k][i]));
     }
   }
-  top = GroupMax(top);
+  top = GroupMax<G>(top);
   const int e = top > 0.f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+#pragma unroll
   for (int k = 0; k < KS; ++k)
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = __builtin_amdgcn_ldexpf(v[k][i], -e);
       q[k][i] = (_Float16)(p.scale < 0.f ? -x : x);
@@ -584,7 +602,7 @@ __device__ __forceinline__ int64_t BlockScan(int64_t v, int64_t *s) {
 }
 
 struct RowTile {
-  int b, n, len, row0, tiles;
+  int b, n, len, row0, tiles, start;
 };
 
 // Row tiles of sequence b (0 where its rows are the decoding kernel's).
@@ -610,6 +628,7 @@ __device__ __forceinline__ RowTile FindRowTile(const Plan &p, const RowLine &l, 
   r.b = b;
   r.n = KvNewTokens(p.a.c, b);
   r.len = p.a.c.lengths[b];
+  r.start = p.a.c.start[b];
   r.row0 = (n - 1 - (i - at)) * rows;
   const int last_row = min(r.row0 + rows, r.n * p.group) - 1;
   r.tiles = (r.len - r.n + last_row / p.group) / kTile + 1;
@@ -633,7 +652,19 @@ __device__ __forceinline__ int64_t MakeRowLine(const Plan &p, RowLine &l, int ro
   return Uniform(l.upto[kRowThreads - 1]);
 }
 
-__device__ __forceinline__ Job FindRowJob(const Plan &p, const RowLine &l, int64_t u, int rows) {
+struct RowJob : Job {
+  int i;  // its row tile
+};
+__device__ __forceinline__ void Take(RowJob &j, const RowTile &r) {
+  j.b = Uniform(r.b);
+  j.n = Uniform(r.n);
+  j.len = Uniform(r.len);
+  j.row0 = Uniform(r.row0);
+  j.tiles = Uniform(r.tiles);
+  j.start = Uniform(r.start);
+}
+
+__device__ __forceinline__ RowJob FindRowJob(const Plan &p, const RowLine &l, int64_t u, int rows) {
   const int per = (l.row_tiles + kRowThreads - 1) / kRowThreads, H = p.a.c.kv_heads;
   int lo = 0, hi = kRowThreads - 1;
   while (lo < hi) {
@@ -647,25 +678,32 @@ __device__ __forceinline__ Job FindRowJob(const Plan &p, const RowLine &l, int64
     at += (int64_t)r.tiles * H;
     r = FindRowTile(p, l, ++i, rows);
   }
-  Job j;
-  j.b = Uniform(r.b);
-  j.n = Uniform(r.n);
-  j.len = Uniform(r.len);
-  j.row0 = Uniform(r.row0);
-  j.tiles = Uniform(r.tiles);
+  RowJob j;
+  Take(j, r);
+  j.i = Uniform(i);
   j.head = Uniform((int)((u - at) / r.tiles));
   j.first = Uniform(at) + (int64_t)j.head * j.tiles;
   return j;
 }
+// The job after j.
+__device__ __forceinline__ void NextRowJob(const Plan &p, const RowLine &l, RowJob &j, int rows) {
+  j.first += j.tiles;
+  if (++j.head < p.a.c.kv_heads) return;
+  j.head = 0;
+  Take(j, FindRowTile(p, l, ++j.i, rows));
+}
 
 // The 16-byte chunk of a row in LDS: keys have HD / 8 chunks per token, values
 // 8 per dimension.
-template <int HD> __device__ __forceinline__ int KeyChunk(int token, int chunk) {
-  const int key = HD == 64 ? (token >> 1 & 1) | (token >> 4) << 1 : (token & 3) | (token >> 4) << 2;
+// They are exchanged so that the lanes that read at one time, any 16 in a row or
+// the quads 0, 3, 5, 6 and 1, 2, 4, 7 of 32 (operands of W rows), take all banks.
+template <int HD, int W> __device__ __forceinline__ int KeyChunk(int token, int chunk) {
+  const int high = W == 32 ? (token >> 5 & 1) | (token >> 1 & 2) : token >> 4;
+  const int key = HD == 64 ? (token >> 1 & 1) | high << 1 : (token & 3) | high << 2;
   return token * (HD / 8) + (chunk ^ key);
 }
-__device__ __forceinline__ int ValueChunk(int dim, int chunk) {
-  const int key = (dim >> 1 & 1) | (dim >> 2 & 2) | ((dim >> 1 ^ dim) & 4);
+template <int W> __device__ __forceinline__ int ValueChunk(int dim, int chunk) {
+  const int key = W == 32 ? dim >> 1 & 7 : (dim >> 1 & 1) | (dim >> 2 & 2) | ((dim >> 1 ^ dim) & 4);
   return dim * 8 + (chunk ^ key);
 }
 
@@ -676,7 +714,7 @@ __device__ __forceinline__ int ValueChunk(int dim, int chunk) {
 
 // Keys: the tokens of a wave's load lie in one block, so that its address is
 // scalar and the thread's part is 32 bits.
-template <int HD, bool FP8, bool EXACT> struct KeyStage {
+template <int HD, int W, bool FP8, bool EXACT> struct KeyStage {
   static constexpr int kChunks = HD / 16, kEach = (kChunks * kTile + kRowThreads - 1) / kRowThreads;
   int blk[kEach];
   v4i r[kEach];
@@ -708,7 +746,7 @@ template <int HD, bool FP8, bool EXACT> struct KeyStage {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       if (kChunks * kTile < kRowThreads && threadIdx.x >= kChunks * kTile) continue;
-      const unsigned at = KeyChunk<HD>(Token(e), (int)threadIdx.x % kChunks * 2) * 16;
+      const unsigned at = KeyChunk<HD, W>(Token(e), (int)threadIdx.x % kChunks * 2) * 16;
       *reinterpret_cast<v8h *>(lds + at) = Widen<FP8>(r[e][0], r[e][1]);
       *reinterpret_cast<v8h *>(lds + (at ^ 16)) = Widen<FP8>(r[e][2], r[e][3]);
     }
@@ -716,7 +754,7 @@ template <int HD, bool FP8, bool EXACT> struct KeyStage {
 };
 
 // Values: four lanes take the 64 tokens of a dimension.
-template <int HD, bool FP8, bool EXACT> struct ValueStage {
+template <int HD, int W, bool FP8, bool EXACT> struct ValueStage {
   static constexpr int kEach = (HD * 4 + kRowThreads - 1) / kRowThreads;
   int blk;
   v4i r[kEach];
@@ -758,28 +796,47 @@ template <int HD, bool FP8, bool EXACT> struct ValueStage {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       if (HD * 4 < kRowThreads && threadIdx.x >= HD * 4) continue;
-      const unsigned at = ValueChunk(Dim(e), (int)threadIdx.x % 4 * 2) * 16;
+      const unsigned at = ValueChunk<W>(Dim(e), (int)threadIdx.x % 4 * 2) * 16;
       *reinterpret_cast<v8h *>(lds + at) = Widen<FP8>(r[e][0], r[e][1]);
       *reinterpret_cast<v8h *>(lds + (at ^ 16)) = Widen<FP8>(r[e][2], r[e][3]);
     }
   }
 };
 
-// Both scales of a lane group's 16 tokens, a tile ahead, and their block two
-// ahead.  A block outside the cache gives a NaN score.
-struct ScaleStage {
-  int blk;
-  float ks, vs;
+// Both scales of a lane group's tokens, 16 at a time, a tile ahead, and their
+// block two ahead.  A block outside the cache gives a NaN score.
+template <int G> struct ScaleStage {
+  static constexpr int kEach = 4 / G;
+  int blk[kEach];
+  bool bad[kEach];
+  float ks[kEach], vs[kEach];
   __device__ __forceinline__ void Lookup(const KvCacheParams &p, const int32_t *table, int last, int t, int g) {
-    blk = table[(unsigned)min(t * kTile + 16 * g, last) >> p.block_shift];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      blk[e] = table[(unsigned)min(t * kTile + 16 * (kEach * g + e), last) >> p.block_shift];
   }
   __device__ __forceinline__ void Load(const KvCacheParams &p, int head, unsigned blocks) {
-    const bool bad = (unsigned)blk >= blocks;
-    const uint64_t at = (uint64_t)(bad ? 0u : (unsigned)blk) * (unsigned)p.kv_heads + (unsigned)head;
-    ks = p.k_scale[at];
-    vs = p.v_scale[at];
-    if (bad) ks = __builtin_nanf("");
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      bad[e] = (unsigned)blk[e] >= blocks;
+      const uint64_t at = (uint64_t)(bad[e] ? 0u : (unsigned)blk[e]) * (unsigned)p.kv_heads + (unsigned)head;
+      ks[e] = p.k_scale[at];
+      vs[e] = p.v_scale[at];
+    }
   }
+};
+
+// The products of W x W results: lane W h + r of G = 64 / W groups has operand
+// row r at 8 h of the 8 G long sum, and of the results column r, rows
+// 4 G (e / 4) + 4 h + e % 4.
+template <int W> struct Mfma;
+template <> struct Mfma<16> {
+  typedef v4f Acc;
+  static __device__ __forceinline__ Acc Do(v8h a, v8h b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mfma<32> {
+  typedef float Acc __attribute__((ext_vector_type(16)));
+  static __device__ __forceinline__ Acc Do(v8h a, v8h b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
 constexpr int kAhead = 6;
@@ -788,15 +845,20 @@ constexpr int kAhead = 6;
 // flight.
 __device__ __forceinline__ void SlotBarrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int HD, int CT, bool FP8, bool EXACT>
+template <int HD, int W, bool FP8, bool EXACT>
 __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
-  constexpr int DT = HD / 16, KS = HD / 32, kRows = kRowWaves * CT * 16;
+  typedef Mfma<W> M;
+  typedef typename M::Acc Acc;
+  constexpr int G = 64 / W, E = W * W / 64, kRows = kRowWaves * W;
+  constexpr int DT = HD / W, KS = HD / (8 * G);       // results of O^T, steps of S^T
+  constexpr int NI = kTile / W, KK = kTile / (8 * G); // results of S^T, steps of O^T
+  constexpr int kOwn = kTile / G;                     // a lane's consecutive tokens of a tile
   constexpr unsigned kBuffer = kTile * HD * 2, kValues = 2 * kBuffer;  // two buffers of keys, two of values
   __shared__ __align__(16) char lds[4 * kBuffer];
   __shared__ RowLine line;
   __shared__ unsigned before;
   const KvCacheParams &cp = p.a.c;
-  const int tid = threadIdx.x, lane = tid % 64, c = lane % 16, g = lane / 16;
+  const int tid = threadIdx.x, lane = tid % 64, c = lane % W, g = lane / W;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const bool late = wave >= kRowWaves / 2;  // the half of the waves that runs a slot behind
   if (p.fill) FillInvalid(p);
@@ -804,17 +866,21 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
   const int64_t piece = (units + gridDim.x - 1) / gridDim.x;
   int64_t u = (int64_t)blockIdx.x * piece;
   const int64_t end = u + piece < units ? u + piece : units;
+  RowJob j;
   for (int part = 0; u < end; part = 1) {
-    const Job j = FindRowJob(p, line, u, kRows);
+    if (part == 0)
+      j = FindRowJob(p, line, u, kRows);
+    else
+      NextRowJob(p, line, j, kRows);
     const int t0 = (int)(u - j.first), t1 = (int)(end - j.first < j.tiles ? end - j.first : j.tiles);
-    const int wrow = j.row0 + wave * CT * 16, rows = j.n * p.group, before_new = j.len - j.n;
+    const int wrow = j.row0 + wave * W, rows = j.n * p.group, before_new = j.len - j.n;
     const int32_t *table = cp.table + (int64_t)j.b * cp.max_blocks;
     const unsigned stride = (unsigned)cp.kv_heads * (unsigned)(cp.block_tokens * cp.head_dim);
     const unsigned blocks = (unsigned)(cp.num_blocks < INT64_C(0x80000000) ? cp.num_blocks : INT64_C(0x80000000));
     const uint64_t head = (uint64_t)j.head * (unsigned)(cp.block_tokens * cp.head_dim);
-    KeyStage<HD, FP8, EXACT> keys;
-    ValueStage<HD, FP8, EXACT> values;
-    ScaleStage scales;
+    KeyStage<HD, W, FP8, EXACT> keys;
+    ValueStage<HD, W, FP8, EXACT> values;
+    ScaleStage<G> scales;
     keys.Start(cp);
     values.Start(cp, cp.v_cache + head);
     keys.Lookup(cp, table, j.len - 1, t0);
@@ -824,15 +890,14 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     keys.Lookup(cp, table, j.len - 1, t0 + 1);
     scales.Load(cp, j.head, blocks);
     scales.Lookup(cp, table, j.len - 1, t0 + 1, g);
-    v8h q[CT][KS];
-    float qf[CT];
-    int last[CT];  // the last token that the row sees
-#pragma unroll
-    for (int r = 0; r < CT; ++r) {
-      const int row = wrow + 16 * r + c, token = row < rows ? row / p.group : 0;
-      const int64_t at = ((cp.start[j.b] + (int64_t)token) * p.a.heads + j.head * p.group + row % p.group) * cp.head_dim;
-      last[r] = before_new + token;
-      LoadQ<KS, EXACT>(p.a, at, row < rows, g, q[r], qf[r]);
+    v8h q[KS];
+    float qf;
+    int last;  // the last token that the row sees
+    {
+      const int row = wrow + c, token = row < rows ? row / p.group : 0;
+      const int64_t at = ((j.start + (int64_t)token) * p.a.heads + j.head * p.group + row % p.group) * cp.head_dim;
+      last = before_new + token;
+      LoadQ<G, KS, EXACT>(p.a, at, row < rows, g, q, qf);
     }
     __syncthreads();  // the buffers of the job before were read
     keys.Store(lds);
@@ -840,42 +905,27 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     keys.Lookup(cp, table, j.len - 1, t0 + 2);
     values.Load(cp, stride, blocks, t0);
     values.Lookup(cp, table, j.len - 1, t0 + 1);
-    // Stages the keys of tile a and the values of the one before, and loads one
-    // tile further.  Past the job's last tile that writes a buffer that nobody
-    // reads again.
-    auto stage = [&](int a) __attribute__((always_inline)) {
-      keys.Store(lds + ((a - t0) & 1) * kBuffer);
-      values.Store(lds + kValues + ((a - 1 - t0) & 1) * kBuffer, j.len - (a - 1) * kTile);
-      keys.Load(cp, cp.k_cache + head, stride, blocks, a + 1);
-      values.Load(cp, stride, blocks, a);
-      keys.Lookup(cp, table, j.len - 1, a + 2);
-      values.Lookup(cp, table, j.len - 1, a + 1);
-    };
-    v4f o[CT][DT], s[CT][4];
-    v8h pr[CT][2];
-    float mo[CT], sum[CT];
+    Acc o[DT], s[NI];
+    v8h pr[KK];
+    float mo = kNone, sum = 0.f;
 #pragma unroll
-    for (int r = 0; r < CT; ++r) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[r][d] = v4f{0.f, 0.f, 0.f, 0.f};
-      mo[r] = kNone;
-      sum[r] = 0.f;
-    }
+    for (int d = 0; d < DT; ++d) o[d] = Acc(0.f);
     // the tokens that every row of the wave sees end here
     const int all_see = before_new + min(wrow, rows - 1) / p.group + 1;
-    // this lane's first operands; those of the other k are an exclusive or away
-    const unsigned my_keys = KeyChunk<HD>(16 * (c / 4) + c % 4, g) * 16, my_values = ValueChunk(c, 2 * g) * 16;
-    // The products of a slot: values of tile tv (V), then keys of tile tk (K).  Each
-    // operand read from LDS serves CT MFMAs, which are shorter than the read takes:
-    // kAhead reads are in flight.
-    auto multiply = [&](auto V, auto K, int tv, int tk) __attribute__((always_inline)) {
-      constexpr int kV = decltype(V)::value ? 2 * DT : 0, kN = kV + (decltype(K)::value ? 4 * KS : 0);
-      // value operands in the order of pairs of d, key operands of pairs of i, so that
-      // an accumulator's next product is CT * 2 away
+    // this lane's first operands; those of the other steps are an exclusive or away
+    const unsigned my_keys = KeyChunk<HD, W>(kOwn * (c / 4 % G) + c / (4 * G) * 4 + c % 4, g) * 16;
+    const unsigned my_values = ValueChunk<W>(c, 8 / G * g) * 16;
+    // The products of a slot: values of tile t - 1 (V), then keys of tile t (K).  A
+    // product is shorter than the read of its operand from LDS takes: kAhead
+    // reads are in flight.  With K also the staging of keys t + 1 and values t, and
+    // the loads of a tile further; past the job's last tile that writes a buffer
+    // that nobody reads again.
+    auto multiply = [&](auto V, auto K, int t) __attribute__((always_inline)) {
+      constexpr int kV = decltype(V)::value ? DT * KK : 0, kN = kV + (decltype(K)::value ? NI * KS : 0);
       auto read = [&](int n) __attribute__((always_inline)) {
-        const int m = n - kV, i = m / (2 * KS) * 2 + m % 2;
-        const unsigned at = n < kV ? (my_values ^ (((tv - t0) & 1) * kBuffer | n / 2 % 2 * 16)) + kValues + 16 * 128 * (n / 4 * 2 + n % 2)
-                                   : (my_keys ^ (((tk - t0) & 1) * kBuffer | m / 2 % KS * 64)) + 8 * HD * i;
+        const int m = n - kV;
+        const unsigned at = n < kV ? (my_values ^ (((t - 1 - t0) & 1) * kBuffer | n / DT * 16)) + kValues + W * 128 * (n % DT)
+                                   : (my_keys ^ (((t - t0) & 1) * kBuffer | m / NI * (16 * G))) + 2 * HD * E * (m % NI);
         return *reinterpret_cast<const v8h *>(lds + at);
       };
       v8h a[kN];
@@ -884,138 +934,127 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         if (n + kAhead < kN) a[n + kAhead] = read(n + kAhead);
-        const int m = n - kV;
-#pragma unroll
-        for (int r = 0; r < CT; ++r) {
-          if (n < kV) {
-            v4f &x = o[r][n / 4 * 2 + n % 2];
-            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[n], pr[r][n / 2 % 2], x, 0, 0, 0);
-          } else {
-            v4f &x = s[r][m / (2 * KS) * 2 + m % 2];
-            x = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[n], q[r][m / 2 % KS], m / 2 % KS ? x : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-          }
+        if (K && n == kN / 8) {
+          keys.Store(lds + ((t + 1 - t0) & 1) * kBuffer);
+          keys.Load(cp, cp.k_cache + head, stride, blocks, t + 2);
+          keys.Lookup(cp, table, j.len - 1, t + 3);
         }
+        if (K && n == kN / 2) {
+          values.Store(lds + kValues + ((t - t0) & 1) * kBuffer, j.len - t * kTile);
+          values.Load(cp, stride, blocks, t + 1);
+          values.Lookup(cp, table, j.len - 1, t + 2);
+        }
+        const int m = n - kV;
+        if (n < kV)
+          o[n % DT] = M::Do(a[n], pr[n / DT], o[n % DT]);
+        else
+          s[m % NI] = M::Do(a[n], q[m / NI], m / NI ? s[m % NI] : Acc(0.f));
         __builtin_amdgcn_sched_barrier(0);  // or all reads go first, into registers that are not there
       }
     };
+    // Value n of a lane is token kOwn * g + n of the tile.
     auto softmax = [&](int t) __attribute__((always_inline)) {
-      const int base = t * kTile;
-      const float lv = LogScale(scales.vs), inv = InvScale(scales.vs), ks = scales.ks;
+      constexpr int NS = kOwn / 16;  // scales
+      float lv[NS], inv[NS], cs[NS];
+#pragma unroll
+      for (int e = 0; e < NS; ++e) {
+        lv[e] = LogScale(scales.vs[e]);
+        inv[e] = InvScale(scales.vs[e]);
+        cs[e] = (scales.bad[e] ? __builtin_nanf("") : scales.ks[e]) * qf;
+      }
       scales.Load(cp, j.head, blocks);
       scales.Lookup(cp, table, j.len - 1, t + 2, g);
-      const bool edge = base + kTile > all_see;
-      float top[CT], cs[CT], off[CT], ps[CT];
-      int seen[CT];  // the row sees the lane's tokens 0 .. seen
-#pragma unroll
-      for (int r = 0; r < CT; ++r) {
-        cs[r] = ks * qf[r];
-        seen[r] = last[r] - base - 16 * g;
-      }
+      const bool edge = t * kTile + kTile > all_see;
+      const int seen = last - t * kTile - kOwn * g;  // the row sees the lane's tokens 0 .. seen
+      float top[NS], best = kNone;
       if (edge) {
 #pragma unroll
-        for (int r = 0; r < CT; ++r) {
-          top[r] = -__builtin_huge_valf();
+        for (int e = 0; e < NS; ++e) {
+          top[e] = -__builtin_huge_valf();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top[r] = i <= seen[r] ? fmaxf(top[r], s[r][i / 4][i % 4]) : top[r];
+          for (int n = 16 * e; n < 16 * e + 16; ++n) top[e] = n <= seen ? fmaxf(top[e], s[n / E][n % E]) : top[e];
         }
       } else {
 #pragma unroll
-        for (int r = 0; r < CT; ++r) {
-          top[r] = s[r][0][0];
+        for (int e = 0; e < NS; ++e) {
+          top[e] = s[16 * e / E][0];
 #pragma unroll
-          for (int i = 1; i < 16; ++i) top[r] = fmaxf(top[r], s[r][i / 4][i % 4]);
-        }
-      }
-      bool up = false, far = false;
-#pragma unroll
-      for (int r = 0; r < CT; ++r) {
-        top[r] = GroupMax(Weight(top[r], cs[r], lv));
-        up |= top[r] > mo[r] + kLag;
-      }
-      if (__any(up)) {
-#pragma unroll
-        for (int r = 0; r < CT; ++r) {
-          const float now = fmaxf(mo[r], top[r]), keep = __builtin_amdgcn_exp2f(mo[r] - now);
-          mo[r] = now;
-          sum[r] *= keep;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[r][d] *= keep;
+          for (int n = 16 * e + 1; n < 16 * e + 16; ++n) top[e] = fmaxf(top[e], s[n / E][n % E]);
         }
       }
 #pragma unroll
-      for (int r = 0; r < CT; ++r) {
-        off[r] = lv - mo[r];
-        ps[r] = 0.f;
-        far |= fabsf(mo[r]) > 4096.f && mo[r] > kNone;
+      for (int e = 0; e < NS; ++e) best = fmaxf(best, Weight(top[e], cs[e], lv[e]));
+      best = GroupMax<G>(best);
+      if (__any(best > mo + kLag)) {
+        const float now = fmaxf(mo, best), keep = __builtin_amdgcn_exp2f(mo - now);
+        mo = now;
+        sum *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= keep;
       }
       // one fused step rounds otherwise than mo was made, by an ulp of mo: from
       // 2^12 on that is left to the exact difference
-      if (edge || __any(far)) {
+      if (edge || __any(fabsf(mo) > 4096.f && mo > kNone)) {
 #pragma unroll
-        for (int r = 0; r < CT; ++r)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float z = Weight(s[r][i / 4][i % 4], cs[r], lv) - mo[r];
-            s[r][i / 4][i % 4] = i > seen[r] ? -__builtin_huge_valf() : z;
-          }
+        for (int n = 0; n < kOwn; ++n) {
+          const float z = Weight(s[n / E][n % E], cs[n / 16], lv[n / 16]) - mo;
+          s[n / E][n % E] = n > seen ? -__builtin_huge_valf() : z;
+        }
       } else {
 #pragma unroll
-        for (int r = 0; r < CT; ++r)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[r][i / 4][i % 4] = __builtin_fmaf(s[r][i / 4][i % 4], cs[r], off[r]);
+        for (int n = 0; n < kOwn; ++n) s[n / E][n % E] = __builtin_fmaf(s[n / E][n % E], cs[n / 16], lv[n / 16] - mo);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
+      for (int e = 0; e < NS; ++e) {
+        float ps = 0.f;
 #pragma unroll
-        for (int r = 0; r < CT; ++r) {
-          const float w = __builtin_amdgcn_exp2f(s[r][i / 4][i % 4]);
-          ps[r] += w;
-          pr[r][i / 8][i % 8] = (_Float16)w;
+        for (int n = 16 * e; n < 16 * e + 16; ++n) {
+          const float w = __builtin_amdgcn_exp2f(s[n / E][n % E]);
+          ps += w;
+          pr[n / 8][n % 8] = (_Float16)w;
         }
-#pragma unroll
-      for (int r = 0; r < CT; ++r) sum[r] = __builtin_fmaf(ps[r], inv, sum[r]);
+        sum = __builtin_fmaf(ps, inv[e], sum);
+      }
     };
-    // Slots: in one half of the waves multiplies (values of tile t - 1, keys of
-    // tile t) while the other is at its softmax and staging; then they change
-    // places.  In slots 2 (t - t0) and the next, keys t and values t - 1 are read and
-    // keys t + 1 and values t are written, each into the other buffer.
+    // Slots: one half of the waves multiplies and stages while the other is at its
+    // softmax; then they change places.  In the two slots that multiply values of
+    // tile t - 1 and keys of tile t, keys t + 1 and values t are written, each into
+    // the other buffer, which the slots before have read.
     const std::true_type yes;
     const std::false_type no;
     SlotBarrier();
-    if (late) {
-      stage(t0 + 1);
-      SlotBarrier();
-    }
-    multiply(no, yes, t0, t0);
+    if (late) SlotBarrier();
+    multiply(no, yes, t0);
     SlotBarrier();
     for (int t = t0; t < t1 - 1; ++t) {
       softmax(t);
-      stage(t + (late ? 2 : 1));
       SlotBarrier();
-      multiply(yes, yes, t, t + 1);
+      multiply(yes, yes, t + 1);
       SlotBarrier();
     }
     softmax(t1 - 1);
-    stage(t1 + (late ? 1 : 0));
     SlotBarrier();
-    multiply(yes, no, t1 - 1, t1);
+    multiply(yes, no, t1);
     if (!late) SlotBarrier();
-#pragma unroll
-    for (int r = 0; r < CT; ++r) sum[r] = GroupSum(sum[r]);
+    sum = GroupSum<G>(sum);
+    // The wave's results as parts: quads of dimensions, and both statistics of its
+    // rows by tiles of 16.
     const bool whole = t0 == 0 && t1 == j.tiles;
     const int slot = (int)blockIdx.x * 2 + part;
+    constexpr int kQuads = DT * E / 4;
     if (!whole) {
+      const int at = slot * kRowWaves + wave;
 #pragma unroll
-      for (int r = 0; r < CT; ++r) {
-        const int at = (slot * kRowWaves + wave) * CT + r;
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, o[r][d]), Rsrc(p.part), ((at * DT + d) * 64 + lane) * 16,
-                                                 0, kDeviceScope);
-        if (g == 0) {
-          PutStat(p, at, 0, c, mo[r]);
-          PutStat(p, at, 1, c, sum[r]);
+        for (int e = 0; e < E; e += 4) {
+          const v4f x{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), Rsrc(p.part),
+                                                 ((at * kQuads + (d * E + e) / 4) * 64 + lane) * 16, 0, kDeviceScope);
         }
+      if (g == 0) {
+        PutStat(p, at * (W / 16) + c / 16, 0, c % 16, mo);
+        PutStat(p, at * (W / 16) + c / 16, 1, c % 16, sum);
       }
       const int w0 = Uniform((int)(j.first / piece)), w1 = Uniform((int)((j.first + j.tiles - 1) / piece));
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1028,31 +1067,33 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
       }
       if (tid == 0) p.done[w0] = 0;
       const int first = w0 * 2 + (j.first > w0 * piece ? 1 : 0);
+      mo = kNone;
+      sum = 0.f;
 #pragma unroll
-      for (int r = 0; r < CT; ++r) {
-        mo[r] = kNone;
-        sum[r] = 0.f;
+      for (int d = 0; d < DT; ++d) o[d] = Acc(0.f);
+      auto part_of = [&](int w) { return (w == w0 ? first : w * 2) * kRowWaves + wave; };
+      for (int w = w0; w <= w1; ++w) mo = fmaxf(mo, GetStat(p, part_of(w) * (W / 16) + c / 16, 0, c % 16));
+      for (int w = w0; w <= w1; ++w) {
+        const int from = part_of(w);
+        const float f = __builtin_amdgcn_exp2f(GetStat(p, from * (W / 16) + c / 16, 0, c % 16) - mo);
+        sum += GetStat(p, from * (W / 16) + c / 16, 1, c % 16) * f;
+        v4u x[kQuads];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[r][d] = v4f{0.f, 0.f, 0.f, 0.f};
-        for (int w = w0; w <= w1; ++w)
-          mo[r] = fmaxf(mo[r], GetStat(p, ((w == w0 ? first : w * 2) * kRowWaves + wave) * CT + r, 0, c));
-        for (int w = w0; w <= w1; ++w) {
-          const int at = ((w == w0 ? first : w * 2) * kRowWaves + wave) * CT + r;
-          const float f = __builtin_amdgcn_exp2f(GetStat(p, at, 0, c) - mo[r]);
-          sum[r] += GetStat(p, at, 1, c) * f;
+        for (int i = 0; i < kQuads; ++i)
+          x[i] = __builtin_amdgcn_raw_buffer_load_b128(Rsrc(p.part), ((from * kQuads + i) * 64 + lane) * 16, 0, kDeviceScope);
+        __builtin_amdgcn_sched_barrier(0);  // all loads are on their way
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
-            o[r][d] += __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(
-                                                   Rsrc(p.part), ((at * DT + d) * 64 + lane) * 16, 0, kDeviceScope)) * f;
-        }
+        for (int i = 0; i < 4 * kQuads; ++i) o[i / E][i % E] += __builtin_bit_cast(v4f, x[i / 4])[i % 4] * f;
       }
     }
+    if (wrow + c < rows) {
+      uint16_t *out = OutRow(p, j, wrow + c);
+      const float f = 1.f / sum;
 #pragma unroll
-    for (int r = 0; r < CT; ++r) {
-      Job rj = j;
-      rj.row0 = wrow + 16 * r;
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) StoreRows(p, rj, d, o[r][d], sum[r]);
+        for (int e = 0; e < E; e += 4)
+          StoreDims(p, out, W * d + G * e + 4 * g, v4f{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]} * f);
     }
     u = j.first + t1;
   }
@@ -1080,15 +1121,15 @@ template <int HD> void LaunchDecode(const Plan &p, int64_t grid, hipStream_t s) 
     exact ? KvDecodeKernel<HD, false, true><<<g, kThreads, 0, s>>>(p) : KvDecodeKernel<HD, false, false><<<g, kThreads, 0, s>>>(p);
 }
 
-template <int HD, int CT> void LaunchPrompt(const Plan &p, int64_t grid, hipStream_t s) {
+template <int HD, int W> void LaunchPrompt(const Plan &p, int64_t grid, hipStream_t s) {
   const dim3 g((unsigned)grid);
   const bool exact = p.a.c.head_dim == HD;
   if (p.a.c.fp8)
-    exact ? KvPromptKernel<HD, CT, true, true><<<g, kRowThreads, 0, s>>>(p)
-          : KvPromptKernel<HD, CT, true, false><<<g, kRowThreads, 0, s>>>(p);
+    exact ? KvPromptKernel<HD, W, true, true><<<g, kRowThreads, 0, s>>>(p)
+          : KvPromptKernel<HD, W, true, false><<<g, kRowThreads, 0, s>>>(p);
   else
-    exact ? KvPromptKernel<HD, CT, false, true><<<g, kRowThreads, 0, s>>>(p)
-          : KvPromptKernel<HD, CT, false, false><<<g, kRowThreads, 0, s>>>(p);
+    exact ? KvPromptKernel<HD, W, false, true><<<g, kRowThreads, 0, s>>>(p)
+          : KvPromptKernel<HD, W, false, false><<<g, kRowThreads, 0, s>>>(p);
 }
 
 // Sequences with at most this many rows (new tokens * heads of a group) take
@@ -1101,7 +1142,7 @@ struct Split {
   int64_t decode_grid, prompt_grid;
 };
 
-int64_t PromptRows(const KvAttentionParams &p) { return kRowWaves * 16 * (p.c.head_dim > 128 ? 1 : 2); }
+int64_t PromptRows(const KvAttentionParams &p) { return kRowWaves * (p.c.head_dim > 128 ? 16 : 32); }
 
 Split SplitOf(const KvAttentionParams &p) {
   const KvCacheParams &c = p.c;
@@ -1143,11 +1184,11 @@ void LaunchKvCacheAttention(const KvAttentionParams &a, void *scratch, hipStream
   p.stat = reinterpret_cast<float *>(static_cast<char *>(scratch) + Scratch::Round(slots * hd * sizeof(float)));
   if (sp.prompt) {
     if (hd == 64)
-      LaunchPrompt<64, 2>(p, sp.prompt_grid, stream);
+      LaunchPrompt<64, 32>(p, sp.prompt_grid, stream);
     else if (hd == 128)
-      LaunchPrompt<128, 2>(p, sp.prompt_grid, stream);
+      LaunchPrompt<128, 32>(p, sp.prompt_grid, stream);
     else
-      LaunchPrompt<256, 1>(p, sp.prompt_grid, stream);
+      LaunchPrompt<256, 16>(p, sp.prompt_grid, stream);
     p.fill = 0;
   }
   if (sp.decode) {
