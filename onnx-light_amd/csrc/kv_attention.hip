@@ -611,6 +611,12 @@ __device__ __forceinline__ int RowTilesOf(const Plan &p, int b, int rows) {
   return n > 0 && (int64_t)n * p.group > p.rows_max ? (n * p.group + rows - 1) / rows : 0;
 }
 
+// Tiles of the cache that some row from row0 on sees.
+__device__ __forceinline__ int TilesOf(const Plan &p, int len, int n, int row0, int rows) {
+  const int last_row = min(row0 + rows, n * p.group) - 1;
+  return (len - n + last_row / p.group) / kTile + 1;
+}
+
 // Row tile i of the batch; the longest of a sequence come first.
 __device__ __forceinline__ RowTile FindRowTile(const Plan &p, const RowLine &l, int i, int rows) {
   const int share = (p.a.c.batch + kRowThreads - 1) / kRowThreads;
@@ -630,8 +636,7 @@ __device__ __forceinline__ RowTile FindRowTile(const Plan &p, const RowLine &l, 
   r.len = p.a.c.lengths[b];
   r.start = p.a.c.start[b];
   r.row0 = (n - 1 - (i - at)) * rows;
-  const int last_row = min(r.row0 + rows, r.n * p.group) - 1;
-  r.tiles = (r.len - r.n + last_row / p.group) / kTile + 1;
+  r.tiles = TilesOf(p, r.len, r.n, r.row0, rows);
   return r;
 }
 
@@ -644,7 +649,7 @@ __device__ __forceinline__ int64_t MakeRowLine(const Plan &p, RowLine &l, int ro
   const int all = l.tiles_upto[kRowThreads - 1], per = (all + kRowThreads - 1) / kRowThreads;
   mine = 0;
   for (int i = tid * per; i < min(all, (tid + 1) * per); ++i)
-    mine += (int64_t)FindRowTile(p, l, i, rows).tiles * p.a.c.kv_heads;
+    mine += FindRowTile(p, l, i, rows).tiles;
   const int64_t sum = BlockScan(mine, l.upto);
   l.upto[tid] = sum;
   if (tid == 0) l.row_tiles = all;
@@ -664,33 +669,43 @@ __device__ __forceinline__ void Take(RowJob &j, const RowTile &r) {
   j.start = Uniform(r.start);
 }
 
-__device__ __forceinline__ RowJob FindRowJob(const Plan &p, const RowLine &l, int64_t u, int rows) {
-  const int per = (l.row_tiles + kRowThreads - 1) / kRowThreads, H = p.a.c.kv_heads;
+// The job of unit u; `head` units are the row tiles of one kv head.
+__device__ __forceinline__ RowJob FindRowJob(const Plan &p, const RowLine &l, int64_t u, int64_t head, int rows) {
+  const int per = (l.row_tiles + kRowThreads - 1) / kRowThreads;
+  RowJob j;
+  j.head = Uniform((int)(u / head));
+  const int64_t in_head = u - j.head * head;
   int lo = 0, hi = kRowThreads - 1;
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
-    if (l.upto[mid] > u) hi = mid; else lo = mid + 1;
+    if (l.upto[mid] > in_head) hi = mid; else lo = mid + 1;
   }
   int64_t at = lo ? l.upto[lo - 1] : 0;
   int i = lo * per;
   RowTile r = FindRowTile(p, l, i, rows);
-  while (u >= at + (int64_t)r.tiles * H) {
-    at += (int64_t)r.tiles * H;
+  while (in_head >= at + r.tiles) {
+    at += r.tiles;
     r = FindRowTile(p, l, ++i, rows);
   }
-  RowJob j;
   Take(j, r);
   j.i = Uniform(i);
-  j.head = Uniform((int)((u - at) / r.tiles));
-  j.first = Uniform(at) + (int64_t)j.head * j.tiles;
+  j.first = j.head * head + Uniform(at);
   return j;
 }
 // The job after j.
 __device__ __forceinline__ void NextRowJob(const Plan &p, const RowLine &l, RowJob &j, int rows) {
   j.first += j.tiles;
-  if (++j.head < p.a.c.kv_heads) return;
-  j.head = 0;
-  Take(j, FindRowTile(p, l, ++j.i, rows));
+  ++j.i;
+  if (j.row0 > 0) {
+    j.row0 -= rows;
+    j.tiles = TilesOf(p, j.len, j.n, j.row0, rows);
+    return;
+  }
+  if (j.i == l.row_tiles) {
+    j.i = 0;
+    ++j.head;
+  }
+  Take(j, FindRowTile(p, l, j.i, rows));
 }
 
 // The 16-byte chunk of a row in LDS: keys have HD / 8 chunks per token, values
@@ -862,14 +877,17 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const bool late = wave >= kRowWaves / 2;  // the half of the waves that runs a slot behind
   if (p.fill) FillInvalid(p);
-  const int64_t units = MakeRowLine(p, line, kRows);
+  const int64_t head_units = MakeRowLine(p, line, kRows), units = head_units * cp.kv_heads;
   const int64_t piece = (units + gridDim.x - 1) / gridDim.x;
-  int64_t u = (int64_t)blockIdx.x * piece;
+  // the workgroups of one XCD (every eighth) take pieces in a row, so that they
+  // share few heads' keys and values in its L2
+  const int me = gridDim.x % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+  int64_t u = (int64_t)me * piece;
   const int64_t end = u + piece < units ? u + piece : units;
   RowJob j;
   for (int part = 0; u < end; part = 1) {
     if (part == 0)
-      j = FindRowJob(p, line, u, kRows);
+      j = FindRowJob(p, line, u, head_units, kRows);
     else
       NextRowJob(p, line, j, kRows);
     const int t0 = (int)(u - j.first), t1 = (int)(end - j.first < j.tiles ? end - j.first : j.tiles);
@@ -1029,7 +1047,9 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     for (int t = t0; t < t1 - 1; ++t) {
       softmax(t);
       SlotBarrier();
+      __builtin_amdgcn_s_setprio(1);  // or the older half's softmax holds up the younger's products
       multiply(yes, yes, t + 1);
+      __builtin_amdgcn_s_setprio(0);
       SlotBarrier();
     }
     softmax(t1 - 1);
@@ -1040,7 +1060,7 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     // The wave's results as parts: quads of dimensions, and both statistics of its
     // rows by tiles of 16.
     const bool whole = t0 == 0 && t1 == j.tiles;
-    const int slot = (int)blockIdx.x * 2 + part;
+    const int slot = me * 2 + part;
     constexpr int kQuads = DT * E / 4;
     if (!whole) {
       const int at = slot * kRowWaves + wave;
