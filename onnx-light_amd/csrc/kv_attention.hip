@@ -529,23 +529,34 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
 
 // ---------------------------------------------------------------------------
 // Many rows (prompts): the products are the cost.  A job is one kv head and a
-// tile of 8 waves * CT * 16 rows of a sequence, over the tokens that its last
-// row sees; each wave owns its rows, so nothing is joined between waves.  The
-// codes of a 64-token tile become fp16 once, in LDS (two buffers, one barrier
-// per tile), where every wave reads them: with CT 16-row tiles per wave an
-// operand read feeds CT MFMAs, CT = 2 keeping the LDS as busy as the matrix
-// cores and 3 at two thirds of them.  Rows of 16-byte chunks are XOR-swizzled
-// so that the 16 rows of an operand lie on 64 different banks.
+// tile of 8 waves * W rows of a sequence, over the tokens that its last row sees;
+// each wave owns its W rows, so nothing is joined between waves.  The products
+// are W x W (Mfma below), W = 32; 16 for head dimensions above 128, whose O would
+// not fit the registers otherwise.  A lane then holds a quarter or half of the
+// tile's tokens of one row, in a row: 16 or 32 of them, one or two scales.
 //
-// Jobs form a line of tiles as above, cut into equal pieces, so the causal
-// triangle, ragged lengths and few rows over long caches all keep every CU
-// busy; parts are joined the same way.
+// The codes of a 64-token tile become fp16 once, in LDS (two buffers), where
+// every wave reads them.  A SIMD has two waves; what a wave does for a tile takes
+// about as long on the vector unit (softmax, widening, addresses) as on the
+// matrix unit, and a wave alone cannot overlap the two, so one half of the waves
+// multiplies while the other is at its softmax (the slots below).  The waves that
+// multiply go first (s_setprio): without it the older half's softmax delays the
+// younger half's products, and 32 heads of 128 over two prompts of 4096 new
+// tokens, 8192 in all, take 649 us, not 617.
+//
+// Jobs form a line of tiles as above (kv heads outermost), cut into equal pieces,
+// so the causal triangle, ragged lengths and few rows over long caches all keep
+// every CU busy; parts are joined the same way.  Workgroups of one XCD take
+// neighbouring pieces: the keys and values that they share stay in its L2, 617 ->
+// 586 us (930 TFLOP/s; a wave's part of a tile 5400 -> 4300 clocks, and the clock
+// gave way to power from 2.4 to 2.05 GHz).  With the 16 x 16 products for 128
+// dimensions the issue slots that MFMAs take from the vector unit double.
 //
 // The reference mo moves only when it is exceeded by 2^8 or more, which P has
 // room for in fp16.
 
-// Q of one row for the prompt kernel: lane group g holds the dimensions 32 k +
-// 8 g + (0..7) at q[k], scaled to [1, 2); qf gives the scores in powers of two,
+// Q of one row for the prompt kernel: lane group g of G holds the dimensions
+// 8 (G k + g) + (0..7) at q[k], scaled to [1, 2); qf gives the scores in powers of two,
 // and is not negative (the sign of the softmax scale goes to Q).
 template <int G, int KS, bool EXACT>
 __device__ __forceinline__ void LoadQ(const KvAttentionParams &p, int64_t at, bool live, int g, v8h (&q)[KS], float &qf) {
@@ -854,7 +865,12 @@ template <> struct Mfma<32> {
   static __device__ __forceinline__ Acc Do(v8h a, v8h b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
-constexpr int kAhead = 6;
+constexpr int kAhead = 4;  // 6 and 8 want registers that are not there
+
+// Tiles that a workgroup takes at least.  One sequence of 256 rows, 8192 tokens:
+// pieces of 4, 8, 16 tiles 68, 56, 63 us; the parts of a job, 128 KB each, are
+// joined by one CU, at about 75 GB/s.
+constexpr int kLeastPiece = 8;
 
 // LDS writes and reads of this wave are done; so for all waves.  Loads stay in
 // flight.
@@ -878,7 +894,7 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
   const bool late = wave >= kRowWaves / 2;  // the half of the waves that runs a slot behind
   if (p.fill) FillInvalid(p);
   const int64_t head_units = MakeRowLine(p, line, kRows), units = head_units * cp.kv_heads;
-  const int64_t piece = (units + gridDim.x - 1) / gridDim.x;
+  const int64_t piece = max((units + gridDim.x - 1) / gridDim.x, (int64_t)kLeastPiece);
   // the workgroups of one XCD (every eighth) take pieces in a row, so that they
   // share few heads' keys and values in its L2
   const int me = gridDim.x % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
@@ -949,26 +965,35 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
       v8h a[kN];
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) a[n] = read(n);
+      auto products = [&](auto from, auto to) __attribute__((always_inline)) {
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        if (n + kAhead < kN) a[n + kAhead] = read(n + kAhead);
-        if (K && n == kN / 8) {
-          keys.Store(lds + ((t + 1 - t0) & 1) * kBuffer);
-          keys.Load(cp, cp.k_cache + head, stride, blocks, t + 2);
-          keys.Lookup(cp, table, j.len - 1, t + 3);
+        for (int n = decltype(from)::value; n < decltype(to)::value; ++n) {
+          if (n + kAhead < kN) a[n + kAhead] = read(n + kAhead);
+          const int m = n - kV;
+          if (n < kV)
+            o[n % DT] = M::Do(a[n], pr[n / DT], o[n % DT]);
+          else
+            s[m % NI] = M::Do(a[n], q[m / NI], m / NI ? s[m % NI] : Acc(0.f));
+          __builtin_amdgcn_sched_barrier(0);  // or all reads go first, into registers that are not there
         }
-        if (K && n == kN / 2) {
-          values.Store(lds + kValues + ((t - t0) & 1) * kBuffer, j.len - t * kTile);
-          values.Load(cp, stride, blocks, t + 1);
-          values.Lookup(cp, table, j.len - 1, t + 2);
-        }
-        const int m = n - kV;
-        if (n < kV)
-          o[n % DT] = M::Do(a[n], pr[n / DT], o[n % DT]);
-        else
-          s[m % NI] = M::Do(a[n], q[m / NI], m / NI ? s[m % NI] : Acc(0.f));
-        __builtin_amdgcn_sched_barrier(0);  // or all reads go first, into registers that are not there
+      };
+      const std::integral_constant<int, 0> at0;
+      const std::integral_constant<int, kN / 8> at1;
+      const std::integral_constant<int, kN / 2> at2;
+      const std::integral_constant<int, kN> at3;
+      products(at0, at1);
+      if (K) {
+        keys.Store(lds + ((t + 1 - t0) & 1) * kBuffer);
+        keys.Load(cp, cp.k_cache + head, stride, blocks, t + 2);
+        keys.Lookup(cp, table, j.len - 1, t + 3);
       }
+      products(at1, at2);
+      if (K) {
+        values.Store(lds + kValues + ((t - t0) & 1) * kBuffer, j.len - t * kTile);
+        values.Load(cp, stride, blocks, t + 1);
+        values.Lookup(cp, table, j.len - 1, t + 2);
+      }
+      products(at2, at3);
     };
     // Value n of a lane is token kOwn * g + n of the tile.
     auto softmax = [&](int t) __attribute__((always_inline)) {
@@ -1062,19 +1087,22 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     const bool whole = t0 == 0 && t1 == j.tiles;
     const int slot = me * 2 + part;
     constexpr int kQuads = DT * E / 4;
+    const bool alive = wrow < rows;  // the wave has a row
     if (!whole) {
       const int at = slot * kRowWaves + wave;
+      if (alive) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          const v4f x{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), Rsrc(p.part),
-                                                 ((at * kQuads + (d * E + e) / 4) * 64 + lane) * 16, 0, kDeviceScope);
+          for (int e = 0; e < E; e += 4) {
+            const v4f x{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), Rsrc(p.part),
+                                                   ((at * kQuads + (d * E + e) / 4) * 64 + lane) * 16, 0, kDeviceScope);
+          }
+        if (g == 0) {
+          PutStat(p, at * (W / 16) + c / 16, 0, c % 16, mo);
+          PutStat(p, at * (W / 16) + c / 16, 1, c % 16, sum);
         }
-      if (g == 0) {
-        PutStat(p, at * (W / 16) + c / 16, 0, c % 16, mo);
-        PutStat(p, at * (W / 16) + c / 16, 1, c % 16, sum);
       }
       const int w0 = Uniform((int)(j.first / piece)), w1 = Uniform((int)((j.first + j.tiles - 1) / piece));
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1092,18 +1120,25 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] = Acc(0.f);
       auto part_of = [&](int w) { return (w == w0 ? first : w * 2) * kRowWaves + wave; };
-      for (int w = w0; w <= w1; ++w) mo = fmaxf(mo, GetStat(p, part_of(w) * (W / 16) + c / 16, 0, c % 16));
-      for (int w = w0; w <= w1; ++w) {
+      for (int w = w0; alive && w <= w1; w += 8) {  // eight loads on their way at once
+        float m[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = GetStat(p, part_of(min(w + i, w1)) * (W / 16) + c / 16, 0, c % 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mo = fmaxf(mo, m[i]);
+      }
+      for (int w = w0; alive && w <= w1; ++w) {
         const int from = part_of(w);
-        const float f = __builtin_amdgcn_exp2f(GetStat(p, from * (W / 16) + c / 16, 0, c % 16) - mo);
-        sum += GetStat(p, from * (W / 16) + c / 16, 1, c % 16) * f;
+        const float f = GetStat(p, from * (W / 16) + c / 16, 0, c % 16), l = GetStat(p, from * (W / 16) + c / 16, 1, c % 16);
         v4u x[kQuads];
 #pragma unroll
         for (int i = 0; i < kQuads; ++i)
           x[i] = __builtin_amdgcn_raw_buffer_load_b128(Rsrc(p.part), ((from * kQuads + i) * 64 + lane) * 16, 0, kDeviceScope);
         __builtin_amdgcn_sched_barrier(0);  // all loads are on their way
+        const float by = __builtin_amdgcn_exp2f(f - mo);
+        sum += l * by;
 #pragma unroll
-        for (int i = 0; i < 4 * kQuads; ++i) o[i / E][i % E] += __builtin_bit_cast(v4f, x[i / 4])[i % 4] * f;
+        for (int i = 0; i < 4 * kQuads; ++i) o[i / E][i % E] += __builtin_bit_cast(v4f, x[i / 4])[i % 4] * by;
       }
     }
     if (wrow + c < rows) {
@@ -1152,13 +1187,18 @@ template <int HD, int W> void LaunchPrompt(const Plan &p, int64_t grid, hipStrea
           : KvPromptKernel<HD, W, false, false><<<g, kRowThreads, 0, s>>>(p);
 }
 
-// Sequences with at most this many rows (new tokens * heads of a group) take
-// the decoding kernel, the others the prompt kernel; a launch that no sequence
-// can need is left out.
-constexpr int kFewRows = 32;
+// Sequences with at most so many rows (new tokens * heads of a group) take the
+// decoding kernel, the others the prompt kernel; a launch that no sequence can
+// need is left out.  Per sequence of 8192 tokens, 8 kv heads of 128 dimensions,
+// decoding | prompt kernel: 8 sequences of 32 rows 49 | 84 us, of 64 rows 87 | 79,
+// of 128 rows 161 | 81.  Where all rows of the batch are few the parts of a
+// sequence are many, and the decoding kernel's are the smaller to join: one
+// sequence of 64 rows 21 | 38 us, of 128 rows 26 | 40, of 256 rows 37 | 56.
+constexpr int kFewRows = 32, kFewInAll = 128;
 
 struct Split {
   bool decode, prompt;
+  int few;  // the most rows of a sequence for the decoding kernel
   int64_t decode_grid, prompt_grid;
 };
 
@@ -1172,8 +1212,9 @@ Split SplitOf(const KvAttentionParams &p) {
   const int64_t most = known * group;
   const int64_t least = c.tokens - (c.batch - 1) * known;
   Split s;
-  s.prompt = c.batch > 0 && most > kFewRows;
-  s.decode = !s.prompt || least * group <= kFewRows;
+  s.few = c.tokens * group <= kFewInAll ? kFewInAll : kFewRows;
+  s.prompt = c.batch > 0 && most > s.few;
+  s.decode = !s.prompt || least * group <= s.few;
   s.decode_grid = DecodeGrid(p);
   const int64_t jobs = (c.tokens * group / PromptRows(p) + c.batch) * c.kv_heads;
   const int64_t tiles = ((int64_t)c.max_blocks * c.block_tokens + kTile - 1) / kTile;
@@ -1197,7 +1238,7 @@ void LaunchKvCacheAttention(const KvAttentionParams &a, void *scratch, hipStream
   p.a = a;
   p.group = a.heads / a.c.kv_heads;
   // a launch that stands alone has every sequence, also where max_query was wrong
-  p.rows_max = !sp.prompt ? 0x7fffffff : !sp.decode ? 0 : kFewRows;
+  p.rows_max = !sp.prompt ? 0x7fffffff : !sp.decode ? 0 : sp.few;
   p.fill = 1;
   p.done = Ctx().ws.Counters((size_t)std::max(sp.decode_grid, sp.prompt_grid));
   p.part = static_cast<float *>(scratch);
