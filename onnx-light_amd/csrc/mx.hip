@@ -163,12 +163,25 @@ bool LargeTiles(const MxMatMulParams &p) {
   return large * 29 <= small * 20;
 }
 
-// Few rows take the streaming kernel.
-constexpr int64_t kStreamRows = 64;
-bool Streams(const MxMatMulParams &p) { return p.M <= kStreamRows; }
+// Few rows take the streaming kernel, whose time goes with the weight's bytes and
+// the row tiles; the GEMM's one round of tiles goes with K alone, and a wide
+// weight fills it.  us, rows x K x N, stream | GEMM:
+//   MXFP4  32 x 4096 x 14336 15.0 | 18.9    48 x 4096 x 14336 17.9 | 19.0
+//          56 x 4096 x 14336 20.9 | 19.0    64 x 2048 x 16384 15.0 | 13.5
+//          64 x 8192 x 8192 28.0 | 28.4     64 x 11008 x 4096 21.4 | 34.0
+//   MXFP8  36 x 2048 x 8192 8.6 | 13.2      40 x 11008 x 8192 35.5 | 39.8
+//          40 x 4096 x 14336 27.6 | 21.2    33 x 8192 x 28672 82.4 | 51.4
+//          64 x 4096 x 6144 18.5 | 19.7     64 x 4096 x 8192 22.1 | 20.1
+bool Streams(const MxMatMulParams &p) {
+  if (p.M <= 32 || p.M > 64) return p.M <= 32;
+  if (p.a_fp4) return p.M <= 48 || p.N < 12288;
+  return p.N < (p.M <= 48 ? 11264 : 7168);
+}
 
 // Up to this many values every workgroup quantizes its activations itself
-// (eight at a time per thread); a launch for all costs about 4 us.
+// (eight at a time per thread); a launch for all costs about 4 us.  us, itself |
+// in a launch: 1 x 4096 x 14336 10.1 | 12.2, 4 x 4096 x 4096 6.6 | 8.1, 8 x 4096 x
+// 14336 24.3 | 13.8.
 constexpr int64_t kOwnQuant = 16384;
 bool OwnQuant(const MxMatMulParams &p) { return p.x && p.M <= 16 && p.M * Ceil(p.K, 512) * 512 <= kOwnQuant; }
 
@@ -186,10 +199,12 @@ StreamPlan PlanStream(const MxMatMulParams &p) {
   // Activations from memory are read by every wave for itself, all over the chip
   // the same ones at about the same time, and cost as much per 16 rows as the
   // weight: several row tiles share a read, while a wave for every CU's SIMD is
-  // left.  More than these do not fit the registers of two waves per SIMD.
+  // left.  More than these do not fit the registers of two waves per SIMD.  us,
+  // K = 4096, N = 14336, with these | with one: 8 rows 13.8 | 15.6, 16 rows 15.4 |
+  // 18.7, MXFP4 32 rows 15.0 | 19.8, 48 rows 17.9 | 24.5.
   s.nt = OwnQuant(p) ? 1 : s.mt == 1 ? 2 : s.mt <= (p.a_fp4 ? 3 : 2) ? 4 : 2;
   while (s.nt > 1 && Ceil(p.N, 16 * s.nt) * chunks < 4 * Ctx().num_cus) s.nt /= 2;
-  s.waves = s.nt == 4 ? 4 : s.nt == 1 && s.mt == 1 && chunks > 8 ? 16 : 8;
+  s.waves = s.nt == 4 ? 4 : 8;
   s.tiles = Ceil(p.N, 16 * s.nt);
   // as many as give every wave one chunk, while there are not more than about
   // two rounds of them

@@ -15,9 +15,13 @@
 // A workgroup has 16 NT rows of the weight; its waves take the chunks in turn
 // and add up in LDS.  Where rows are few and K is long several workgroups share
 // the chunks, so that all of a wave's loads are in flight at once; the last of
-// them to finish adds up their sums, in the order of the chunks whoever that is.  Activations of 16 bits that are few enough are quantized
-// by every workgroup for itself, into LDS, while its first weight bytes are on
-// their way: that costs less than a launch of its own.
+// them to finish adds up their sums, in the order of the chunks whoever that is.
+// Activations of 16 bits that are few enough are quantized by every workgroup for
+// itself, into LDS, while its first weight bytes are on their way: that costs less
+// than a launch of its own.
+//
+// One row of 4096 values by [14336, 4096]: 29.4 MB of codes and 1.8 of scales in
+// 10.1 us, 3.1 TB/s with the launch, which is a quarter of it.
 #pragma once
 
 #include <type_traits>
@@ -58,11 +62,11 @@ __device__ __forceinline__ int Scales4(const uint8_t *base, unsigned row, int at
   return (int)(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24);
 }
 
-// Most waves of a workgroup: what the registers of more rows and columns leave.
-template <int NT, int MT> constexpr int kStreamWaves = NT == 1 && MT == 1 ? 16 : NT == 4 ? 4 : 8;
+// Waves of a workgroup: what the registers of more rows and columns leave.
+template <int NT> constexpr int kStreamWaves = NT == 4 ? 4 : 8;
 
 template <bool A4, int NT, int MT, bool QUANT>
-__global__ __launch_bounds__((64 * kStreamWaves<NT, MT>), 2) void StreamKernel(const StreamArgs p) {
+__global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const StreamArgs p) {
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;

@@ -48,7 +48,6 @@ __device__ __forceinline__ BlockScale MxScaleOf(float top, int emax) {
 // Nearest codes, ties to even, of v = y * inv of a block with a FLOAT scale.
 // |v| is at most the largest code (and an ulp), which no rounding leaves.  In a
 // block whose scale is NaN v may be NaN: its codes mean nothing.
-__device__ __forceinline__ uint8_t Int8Code(float v) { return (uint8_t)(int8_t)(int)__builtin_rintf(v); }
 __device__ __forceinline__ unsigned Int8Codes4(float a, float b, float c, float d) {
   const unsigned lo = __builtin_amdgcn_perm((unsigned)(int)__builtin_rintf(b), (unsigned)(int)__builtin_rintf(a), 0x0c0c0400u);
   const unsigned hi = __builtin_amdgcn_perm((unsigned)(int)__builtin_rintf(d), (unsigned)(int)__builtin_rintf(c), 0x04000c0cu);
@@ -57,7 +56,6 @@ __device__ __forceinline__ unsigned Int8Codes4(float a, float b, float c, float 
 __device__ __forceinline__ unsigned Fp8Codes4(float a, float b, float c, float d) {
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
-__device__ __forceinline__ uint8_t Fp8Code(float v) { return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, 0.f, 0, false); }
 
 // MX blocks: v = x * 2^-e may pass the largest code, and the conversion gives
 // NaN past 464, so it is clamped.
