@@ -115,7 +115,7 @@ template <int G = 4> __device__ __forceinline__ float GroupSum(float v) {
 //
 // 64 sequences of 500 to 16384 tokens, 64 heads over 8 of 128 dimensions: 1.1 GB in
 // 207 us, 5.4 TB/s, what a large copy reaches.  One sequence of 8191 tokens: 17 MB
-// in 14 us, a chain of latencies (lengths, table, tile, parts, their join).
+// in 13.7 us, a chain of latencies (lengths, table, tile, parts, their join).
 
 struct Line {        // units before every thread's share of the sequences
   int64_t upto[kThreads];
@@ -233,7 +233,7 @@ __device__ __forceinline__ Job FindJob(const Plan &p, const Line &line, int64_t 
 
 // Up to 64 sequences: lane b of every wave keeps what there is to know of sequence
 // b, and nobody searches LDS or waits for another wave: one sequence of 8191
-// tokens 16.0 -> 15.2 us (with the join of parts below 14.2).
+// tokens 16.0 -> 15.2 us (with the join of parts below 13.7).
 struct Lanes {
   int64_t upto;       // units up to the end of the sequence
   int n, len, start;  // its rows' new tokens, length, first new token
@@ -398,51 +398,49 @@ template <typename SO> __device__ __forceinline__ v4f WaveSum(const SO &so, cons
 }
 
 // Joins the parts of a job: slot `first` of piece w0, slots 2 w of the others.
-// The waves take the parts in turn, several on their way at once, and join in LDS.
-template <int HD, typename SO, typename SM>
-__device__ __forceinline__ void JoinParts(const Plan &p, const Job &j, int w0, int w1, int first, SO &so, SM &sm) {
-  constexpr int DT = HD / 16;
+// Every wave has its share of the dimensions, so that nothing is joined between
+// waves, and kFly parts' loads on their way at once.
+template <int HD> __device__ __forceinline__ void JoinParts(const Plan &p, const Job &j, int w0, int w1, int first) {
+  constexpr int DT = HD / 16, kMine = DT / kWaves, kFly = kMine == 4 ? 4 : 8;
   const int lane = threadIdx.x % 64, c = lane % 16, wave = threadIdx.x / 64;
   const int parts = w1 - w0 + 1;
-  auto slot = [&](int i) { return i == 0 ? first : (w0 + i) * 2; };
-  constexpr int kFly = HD == 64 ? 4 : 2;  // parts whose loads are on their way at once
   float mo = kNone, sum = 0.f;
-  v4f a[DT];
+  v4f a[kMine];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) a[d] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int i = wave; i < parts; i += kWaves * kFly) {
+  for (int d = 0; d < kMine; ++d) a[d] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < parts; i += kFly) {
     float m[kFly], l[kFly];
-    v4u x[kFly][DT];
+    v4u x[kFly][kMine];
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
-      const int from = slot(min(i + k * kWaves, parts - 1));
+      const int part = min(i + k, parts - 1), from = part ? (w0 + part) * 2 : first;
       m[k] = GetStat(p, from, 0, c);
       l[k] = GetStat(p, from, 1, c);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-        x[k][d] = __builtin_amdgcn_raw_buffer_load_b128(Rsrc(p.part), ((from * DT + d) * 64 + lane) * 16, 0, kDeviceScope);
+      for (int d = 0; d < kMine; ++d)
+        x[k][d] = __builtin_amdgcn_raw_buffer_load_b128(Rsrc(p.part), ((from * DT + d * kWaves + wave) * 64 + lane) * 16, 0,
+                                                        kDeviceScope);
     }
     __builtin_amdgcn_sched_barrier(0);
+    float now = mo;
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) now = fmaxf(now, m[k]);
+    const float keep = __builtin_amdgcn_exp2f(mo - now);
+    mo = now;
+    sum *= keep;
+#pragma unroll
+    for (int d = 0; d < kMine; ++d) a[d] *= keep;
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
-      if (i + k * kWaves >= parts) continue;
-      const float now = fmaxf(mo, m[k]), keep = __builtin_amdgcn_exp2f(mo - now), by = __builtin_amdgcn_exp2f(m[k] - now);
-      mo = now;
-      sum = sum * keep + l[k] * by;
+      if (i + k >= parts) break;
+      const float by = __builtin_amdgcn_exp2f(m[k] - now);
+      sum += l[k] * by;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) a[d] = a[d] * keep + __builtin_bit_cast(v4f, x[k][d]) * by;
+      for (int d = 0; d < kMine; ++d) a[d] += __builtin_bit_cast(v4f, x[k][d]) * by;
     }
   }
 #pragma unroll
-  for (int d = 0; d < DT; ++d) so[wave][d][lane] = a[d];
-  if (lane < 16) {
-    sm[wave][0][c] = mo;
-    sm[wave][1][c] = sum;
-  }
-  __syncthreads();
-  float f[kWaves];
-  JoinWaves(sm, c, f, sum);
-  for (int d = wave; d < DT; d += kWaves) StoreRows(p, j, d, WaveSum(so, f, d, lane), sum);
+  for (int d = 0; d < kMine; ++d) StoreRows(p, j, d * kWaves + wave, a[d], sum);
 }
 
 template <int HD, bool FP8, bool EXACT>
@@ -585,7 +583,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
       if (before == (unsigned)(w1 - w0)) {
         if (tid == 0) p.done[w0] = 0;
         // a job that starts inside a piece is the last in it
-        JoinParts<HD>(p, j, w0, w1, w0 * 2 + (j.first > w0 * piece ? 1 : 0), so, sm);
+        JoinParts<HD>(p, j, w0, w1, w0 * 2 + (j.first > w0 * piece ? 1 : 0));
       }
     }
     u = j.first + t1;
