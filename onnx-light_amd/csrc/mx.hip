@@ -152,15 +152,20 @@ template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, hipStr
 }
 
 // Large tiles (256 x 256, 128 x 256 for E4M3 activations) feed more MFMAs per
-// byte, small ones (128 x 128) leave fewer CUs idle; a round of large ones takes
-// about 1.45 times a round of small ones (of which two fit a CU for E2M1).
+// byte, small ones (128 x 128) leave fewer CUs idle; E4M3 has 128 x 192 between
+// them.  A round of small, middle and large ones takes about 20, 24 and 29 parts of
+// time (of the small ones two fit a CU for E2M1), and the shortest sum is taken.
 // us, large / small: MXFP4 1000 x 4096 x 6144 40 / 27, 4096 x 8192 x 8192 174 /
-// 205; MXFP8 256 x 4096 x 4096 28 / 22, 1000 x 4096 x 6144 35 / 43.
-bool LargeTiles(const MxMatMulParams &p) {
+// 205.  Large / middle / small: MXFP8 256 x 4096 x 4096 29 / 25 / 22, 1000 x 4096 x
+// 6144 37 / 33 / 45, 2048 x 4096 x 4096 41 / 54 / 49, 4096 x 8192 x 8192 243 / 288 /
+// 326.
+enum class Tiles { kSmall, kMiddle, kLarge };
+Tiles TilesOf(const MxMatMulParams &p) {
   const int64_t cus = Ctx().num_cus;
-  const int64_t large = Ceil(Ceil(p.M, p.a_fp4 ? 256 : 128) * Ceil(p.N, 256), cus);
-  const int64_t small = Ceil(Ceil(p.M, 128) * Ceil(p.N, 128), p.a_fp4 ? 2 * cus : cus);
-  return large * 29 <= small * 20;
+  auto rounds = [&](int64_t m, int64_t n, int64_t at_once) { return Ceil(Ceil(p.M, m) * Ceil(p.N, n), at_once * cus); };
+  const int64_t small = 20 * rounds(128, 128, p.a_fp4 ? 2 : 1), large = 29 * rounds(p.a_fp4 ? 256 : 128, 256, 1);
+  if (!p.a_fp4 && 24 * rounds(128, 192, 1) < std::min(small, large)) return Tiles::kMiddle;
+  return large <= small ? Tiles::kLarge : Tiles::kSmall;
 }
 
 // Few rows take the streaming kernel, whose time goes with the weight's bytes and
@@ -300,8 +305,11 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
   }
   const mx::GemmArgs g{s.codes ? codes : p.a, p.b, a_tiles, b_tiles, static_cast<uint16_t *>(p.y), p.M, p.N, p.K, p.y_bf16,
                        p.N % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0};
-  if (LargeTiles(p))
+  const Tiles tiles = TilesOf(p);
+  if (tiles == Tiles::kLarge)
     p.a_fp4 ? LaunchGemm<true, 4, 4>(g, stream) : LaunchGemm<false, 2, 4>(g, stream);
+  else if (tiles == Tiles::kMiddle)
+    LaunchGemm<false, 2, 3>(g, stream);
   else
     p.a_fp4 ? LaunchGemm<true, 2, 2>(g, stream) : LaunchGemm<false, 2, 2>(g, stream);
 }

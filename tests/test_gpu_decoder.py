@@ -216,6 +216,17 @@ def test_mx_matmul_quantizes_its_activations(gpu, M, N, K, act, typ):
     check_mx_product(*dc.mx_quantize(x, act), b, bs, got, act)
 
 
+@pytest.mark.parametrize("M,N,K,act", [(1000, 6100, 96, "fp8"), (1900, 4000, 64, "fp8"), (2000, 4200, 64, "fp4"),
+                                       (40, 11300, 96, "fp8"), (61, 7200, 288, "fp8"), (50, 12301, 96, "fp4")])
+def test_mx_matmul_of_wide_products(gpu, M, N, K, act):
+    """Sizes that take each of the tiles, and wide weights of few rows."""
+    g = dc.gen(M + N + K)
+    x = dc.randn(g, (M, K), torch.bfloat16)
+    b, bs = dc.mx_weight(g, N, K)
+    got = gpu.mx_matmul(x.cuda(), b.cuda(), bs.cuda(), a_type=gpu.FLOAT8E4M3FN if act == "fp8" else gpu.FLOAT4E2M1)
+    check_mx_product(*dc.mx_quantize(x, act), b, bs, got, act)
+
+
 @pytest.mark.parametrize("M,N,K", MNK[3:])
 @pytest.mark.parametrize("act", ["fp8", "fp4"])
 def test_mx_matmul_of_codes(gpu, M, N, K, act):
