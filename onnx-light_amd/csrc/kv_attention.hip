@@ -21,7 +21,7 @@
 // but for what is below 2^-14 of that largest.  Sums, statistics and O are
 // fp32; P is rounded to fp16.  The weight of a token in O is its softmax weight
 // times its block's v scale, so P is taken relative to mo, the running maximum
-// of S + log2(v scale): P = 2^(S + log2 vs - mo) fills the fp16 range whatever
+// of S + log2(v scale): P = 2^(S + log2 vs - mo + kTop) fills the fp16 range whatever
 // the scales are.  The softmax sum takes the unrounded P / vs (one
 // multiplication per 16 tokens), and O / sum needs no other reference.
 #include <type_traits>
@@ -71,6 +71,11 @@ __device__ __forceinline__ uint2 Pack4(v4f v, int bf16) {
   const uint2 h = __builtin_bit_cast(uint2, __builtin_convertvector(v, v4h));
   return make_uint2(bf16 ? b.x : h.x, bf16 ? b.y : h.y);
 }
+
+// P is up to 2^kTop, near the largest fp16: its smallest is 2^-24, so a weight
+// keeps 11 bits down to 2^-29 of the row's largest (of weight times v scale), and
+// is lost below 2^-40.  O carries that power of two, the sum does not.
+constexpr float kTop = 15.f;
 
 // log2 of a token's weight in O: score (s * cs) plus log2 of its v scale, two
 // roundings, never fused, so that it is the same wherever it is computed.
@@ -277,7 +282,7 @@ __device__ __forceinline__ void StoreDims(const Plan &p, uint16_t *out, int d, v
 }
 __device__ __forceinline__ void StoreRows(const Plan &p, const Job &j, int t, v4f o, float sum) {
   const int row = j.row0 + threadIdx.x % 16;
-  if (row < j.n * p.group) StoreDims(p, OutRow(p, j, row), 16 * t + threadIdx.x % 64 / 16 * 4, o * (1.f / sum));
+  if (row < j.n * p.group) StoreDims(p, OutRow(p, j, row), 16 * t + threadIdx.x % 64 / 16 * 4, o * (0x1p-15f / sum));
 }
 
 // 16 bytes from any address.
@@ -499,7 +504,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
           s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Widen<FP8>(ld.k[i][h][2], ld.k[i][h][3]), q.q[h][1], s[i], 0, 0, 0);
         }
       }
-      const float cs = ld.ks * qf, lv = LogScale(ld.vs), inv = InvScale(ld.vs);
+      const float cs = ld.ks * qf, lv = LogScale(ld.vs), inv = InvScale(ld.vs) * 0x1p-15f;
       if constexpr (more) ld.LoadK(cp, j, t + kWaves, c, g);
       // tokens that the row does not see, in the tiles that have any
       const bool edge = base + kTile > j.len - j.n + 1;
@@ -516,7 +521,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
       v8h pr[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float w = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - now);
+        const float w = __builtin_amdgcn_exp2f((s[i / 4][i % 4] - now) + kTop);
         ps += w;
         pr[i / 8][i % 8] = (_Float16)w;
       }
@@ -615,8 +620,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
 // gave way to power from 2.4 to 2.05 GHz).  With the 16 x 16 products for 128
 // dimensions the issue slots that MFMAs take from the vector unit double.
 //
-// The reference mo moves only when it is exceeded by 2^8 or more, which P has
-// room for in fp16.
+// The reference mo moves only when it is exceeded by 2^kLag or more, which is left
+// free below kTop.
 
 // Q of one row for the prompt kernel: lane group g of G holds the dimensions
 // 8 (G k + g) + (0..7) at q[k], scaled to [1, 2); qf gives the scores in powers of two,
@@ -654,7 +659,7 @@ __device__ __forceinline__ void LoadQ(const KvAttentionParams &p, int64_t at, bo
 }
 
 constexpr int kRowWaves = 8, kRowThreads = 64 * kRowWaves;
-constexpr float kLag = 8.f;
+constexpr float kLag = 2.f;
 
 struct RowLine {                // over the row tiles of all sequences
   int64_t upto[kRowThreads];    // units before the end of every thread's share
@@ -1065,7 +1070,7 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
 #pragma unroll
       for (int e = 0; e < NS; ++e) {
         lv[e] = LogScale(scales.vs[e]);
-        inv[e] = InvScale(scales.vs[e]);
+        inv[e] = InvScale(scales.vs[e]) * 0x1p-13f;
         cs[e] = (scales.bad[e] ? __builtin_nanf("") : scales.ks[e]) * qf;
       }
       scales.Load(cp, j.head, blocks);
@@ -1103,12 +1108,13 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
       if (edge || __any(fabsf(mo) > 4096.f && mo > kNone)) {
 #pragma unroll
         for (int n = 0; n < kOwn; ++n) {
-          const float z = Weight(s[n / E][n % E], cs[n / 16], lv[n / 16]) - mo;
+          const float z = (Weight(s[n / E][n % E], cs[n / 16], lv[n / 16]) - mo) + (kTop - kLag);
           s[n / E][n % E] = n > seen ? -__builtin_huge_valf() : z;
         }
       } else {
 #pragma unroll
-        for (int n = 0; n < kOwn; ++n) s[n / E][n % E] = __builtin_fmaf(s[n / E][n % E], cs[n / 16], lv[n / 16] - mo);
+        for (int n = 0; n < kOwn; ++n)
+          s[n / E][n % E] = __builtin_fmaf(s[n / E][n % E], cs[n / 16], (lv[n / 16] - mo) + (kTop - kLag));
       }
 #pragma unroll
       for (int e = 0; e < NS; ++e) {
@@ -1206,7 +1212,7 @@ __global__ __launch_bounds__(kRowThreads, 1) void KvPromptKernel(const Plan p) {
     }
     if (wrow + c < rows) {
       uint16_t *out = OutRow(p, j, wrow + c);
-      const float f = 1.f / sum;
+      const float f = 0x1p-13f / sum;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll

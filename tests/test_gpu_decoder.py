@@ -487,6 +487,48 @@ def test_attention_with_a_wrong_hint(gpu, hint):
     check_attention(gpu, b, max_query=hint)
 
 
+@pytest.mark.parametrize("to", ["int8", "fp8"])
+def test_prompt_attention_scales_of_any_size(gpu, to):
+    """As above, with enough rows for the kernel of prompts."""
+    test_attention_scales_of_any_size(gpu, [100], [300], to)
+
+
+@pytest.mark.parametrize("typ", ["fp16", "bf16"])
+def test_prompt_attention_queries_of_any_size(gpu, typ):
+    test_attention_queries_of_any_size(gpu, typ, [60], [160])
+
+
+def test_prompt_attention_keeps_nan_to_its_row(gpu):
+    test_attention_keeps_nan_to_its_row(gpu, [90], [150])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [127, 128, 129, 255, 256, 257, 600])
+def test_attention_row_counts(gpu, D, rows):
+    """Rows beside the kernels' own counts, one sequence over many pieces."""
+    check_attention(gpu, dc.Batch(rows + D, [rows], [rows + 2300], 1, D, 64, "fp8", torch.bfloat16))
+
+
+@pytest.mark.parametrize("batch", [64, 65, 70, 300])
+def test_attention_of_many_sequences(gpu, batch):
+    """Single tokens of many sequences, among them prompts, empty sequences and ones without new tokens."""
+    new = [(1, 1, 0, 1, 2, 45, 1)[i % 7] for i in range(batch)]
+    total = [n + (37 * i) % 210 if n or i % 2 else 0 for i, n in enumerate(new)]
+    check_attention(gpu, dc.Batch(batch, new, total, 2, 64, 16, "int8", torch.float16, heads=4))
+
+
+def test_attention_of_many_sequences_of_which_some_do_not_fit(gpu):
+    b = dc.Batch(9, [2] * 70, [50] * 70, 2, 64, 16, "fp8", torch.bfloat16, heads=4)
+    want = check_attention(gpu, b)
+    table, start, lengths = b.index()
+    lengths[3] = 1
+    lengths[69] = 16 * table.shape[1] + 1
+    got = gpu.kv_cache_attention(b.q.cuda(), b.cache(gpu), table, start, lengths)
+    bad = torch.zeros(140, dtype=torch.bool)
+    bad[6:8] = bad[138:] = True
+    assert torch.isnan(got[bad.cuda()]).all() and torch.equal(got[~bad.cuda()], want[~bad.cuda()])
+
+
 def test_nothing_to_do(gpu):
     b = dc.Batch(2, [0, 0], [5, 0], 2, 64, 16, "int8", torch.float16, heads=2)
     assert gpu.kv_cache_attention(b.q.cuda(), b.cache(gpu), *b.index()).shape == (0, 2, 64)
