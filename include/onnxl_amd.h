@@ -736,8 +736,10 @@ int onnxl_amd_kv_cache_append(const onnxl_amd_tensor *k, const onnxl_amd_tensor 
  * kv_heads (consecutive heads share one).  The new token i of n of a sequence
  * of length L sees the tokens 0 .. L - n + i:
  *   out = sum_j softmax_j(scale * q . k_j) v_j,
- * statistics and sums in fp32.  What the cache holds past a sequence's length
- * is never used.  max_query: the most new tokens that a sequence has, where the
+ * statistics and sums in fp32.  Scales are not negative, and a v scale below
+ * 2^-100 counts as that (a block of zeros has 0).  What the cache holds past a
+ * sequence's length is never used; rows of q that belong to no sequence, and
+ * their output, are left alone.  max_query: the most new tokens that a sequence has, where the
  * caller knows it (0 otherwise); it only helps to choose the kernels. */
 int onnxl_amd_kv_cache_attention(const onnxl_amd_tensor *q, const onnxl_amd_tensor *k_cache,
                                  const onnxl_amd_tensor *v_cache, const onnxl_amd_tensor *k_scale,

@@ -529,6 +529,17 @@ def test_attention_of_many_sequences_of_which_some_do_not_fit(gpu):
     assert torch.isnan(got[bad.cuda()]).all() and torch.equal(got[~bad.cuda()], want[~bad.cuda()])
 
 
+@pytest.mark.parametrize("new,total", [([1, 2], [70, 9]), ([200, 3], [260, 40])])
+def test_attention_leaves_rows_of_no_sequence_alone(gpu, new, total):
+    b = dc.Batch(10, new, total, 2, 64, 16, "int8", torch.bfloat16, heads=4)
+    want = check_attention(gpu, b)
+    table, start, lengths = b.index()
+    q = torch.nn.functional.pad(b.q, (0, 0, 0, 0, 3, 5)).cuda()
+    out = torch.full_like(q, 7.0)
+    gpu.kv_cache_attention(q, b.cache(gpu), table, start + 3, lengths, out=out)
+    assert torch.equal(out[3:-5], want) and (out[:3] == 7).all() and (out[-5:] == 7).all()
+
+
 def test_nothing_to_do(gpu):
     b = dc.Batch(2, [0, 0], [5, 0], 2, 64, 16, "int8", torch.float16, heads=2)
     assert gpu.kv_cache_attention(b.q.cuda(), b.cache(gpu), *b.index()).shape == (0, 2, 64)
