@@ -65,9 +65,10 @@ template <bool FP8> __device__ __forceinline__ v8h Widen(int lo, int hi) {
 }
 
 __device__ __forceinline__ uint2 Pack4(v4f v, int bf16) {
-  typedef __bf16 v4b __attribute__((ext_vector_type(4)));
   typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-  const uint2 b = __builtin_bit_cast(uint2, __builtin_convertvector(v, v4b));
+  uint2 b;  // a conversion of vectors to bfloat16 has lost operands here
+  asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(b.x) : "v"(v[0]), "v"(v[1]));
+  asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(b.y) : "v"(v[2]), "v"(v[3]));
   const uint2 h = __builtin_bit_cast(uint2, __builtin_convertvector(v, v4h));
   return make_uint2(bf16 ? b.x : h.x, bf16 ? b.y : h.y);
 }
