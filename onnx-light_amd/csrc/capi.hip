@@ -3504,7 +3504,7 @@ int KvCacheAttention(const onnxl_amd_tensor *q, const onnxl_amd_tensor *k_cache,
   NeedShape(out, ShapeOf(*q), kKvtName, "out");
   OLA_ENFORCE(std::isfinite(scale), kKvtName, ": scale must be finite.");
   OLA_ENFORCE(max_query >= 0, kKvtName, ": max_query must not be negative.");
-  if (p.c.tokens == 0) return ONNXL_AMD_OK;
+  if (p.c.tokens == 0 || p.c.batch == 0) return ONNXL_AMD_OK;  // no sequence: its index tensors hold nothing to read
   Ctx();
   p.heads = (int)heads;
   p.bf16 = q->data_type == kBfloat16;
