@@ -346,7 +346,7 @@ template <int HD, bool EXACT> struct TileLoad {
     vb = table[min(t * kTile + 16 * g, j.len - 1) >> p.block_shift];
   }
   // Keys and scales of tile t.  A block outside the cache reads block 0 and gets
-  // a NaN score.
+  // a NaN k scale, so NaN scores; its values become zeros before they are used.
   __device__ __forceinline__ void LoadK(const KvCacheParams &p, const Job &j, int t, int c, int g) {
     const int kt = t * kTile + 16 * (c / 4), vt = t * kTile + 16 * g, D = EXACT ? HD : p.head_dim, bt = p.block_tokens;
     const bool bad = vb < 0 || vb >= p.num_blocks;
@@ -507,6 +507,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
         }
       }
       const float cs = ld.ks * qf, lv = LogScale(ld.vs), inv = InvScale(ld.vs) * 0x1p-15f;
+      const bool none = ld.ks != ld.ks;  // a row has a NaN score of these tokens, or does not see them
       if constexpr (more) ld.LoadK(cp, j, t + kWaves, c, g);
       // tokens that the row does not see, in the tiles that have any
       const bool edge = base + kTile > j.len - j.n + 1;
@@ -528,9 +529,10 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
         pr[i / 8][i % 8] = (_Float16)w;
       }
       sum = __builtin_fmaf(ps, inv, sum * keep);
-      if (edge) {
-        // what the cache holds past the end may be any code, NaN among them
-        const int left = j.len - vt;  // tokens of this lane that are there
+      if (edge || __any(none)) {
+        // what the cache holds past the end, or in the block that stands for one
+        // outside, may be any code, NaN among them, which a weight of 0 keeps
+        const int left = none ? 0 : j.len - vt;  // tokens of this lane that are there
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int n = left - 4 * w;
@@ -856,6 +858,7 @@ template <int HD, int W, bool FP8, bool EXACT> struct ValueStage {
   v4i r[kEach];
   const uint8_t *base;  // this thread's bytes of the tile's first tokens in block 0
   bool live[kEach];
+  bool bad;  // the codes in r stand for those of a block outside the cache
 
   __device__ __forceinline__ static int Token() { return 16 * (threadIdx.x % 4); }
   __device__ __forceinline__ static int Dim(int e) { return (int)(threadIdx.x + e * kRowThreads) / 4 % HD; }
@@ -868,7 +871,8 @@ template <int HD, int W, bool FP8, bool EXACT> struct ValueStage {
     blk = table[(unsigned)min(t * kTile + Token(), last) >> p.block_shift];
   }
   __device__ __forceinline__ void Load(const KvCacheParams &p, unsigned stride, unsigned blocks, int t) {
-    const unsigned u = (unsigned)blk < blocks ? (unsigned)blk : 0u;
+    bad = (unsigned)blk >= blocks;
+    const unsigned u = bad ? 0u : (unsigned)blk;
     const uint8_t *at = base + ((t * kTile) & (p.block_tokens - 1)) + (uint64_t)u * stride;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
@@ -876,14 +880,14 @@ template <int HD, int W, bool FP8, bool EXACT> struct ValueStage {
       r[e] = here ? *reinterpret_cast<const v4i *>(at + e * kRowThreads / 4 * p.block_tokens) : v4i{0, 0, 0, 0};
     }
   }
-  // Codes past the sequence's end (`left` tokens of the tile are there) may be
-  // any, NaN among them: as the second product multiplies them by zero, they
-  // become zero.
+  // Codes past the sequence's end (`left` tokens of the tile are there) or of a
+  // block outside the cache may be any, NaN among them: as the second product
+  // multiplies them by zero in rows that do not see them, they become zero.
   __device__ __forceinline__ void Store(char *lds, int left) {
-    if (left < kTile) {
+    if (left < kTile || __any(bad)) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const int n = left - Token() - 4 * w;
+        const int n = (bad ? 0 : left) - Token() - 4 * w;
         const int mask = (int)(n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) r[e][w] &= mask;

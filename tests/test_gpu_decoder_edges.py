@@ -1,0 +1,41 @@
+"""Edges of the decoder-layer operators on the GPU, against plain implementations in 64 bits: rows beside blocks that
+are not in the cache, values at the ends of fp32, sizes past one launch, a query_start that falls."""
+import pytest
+import torch
+
+import decoder_cases as dc
+from test_gpu_decoder import check_norm, same
+
+pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.fixture(scope="module")
+def gpu(olamd):
+    olamd.init(0)
+    return olamd
+
+
+# ---- attention beside a block outside the cache ---------------------------------
+
+@pytest.mark.parametrize("new,blocks", [(5, 2), (5, 70), (150, 0), (700, 3)])
+@pytest.mark.parametrize("to,typ,D,bt", [("fp8", "bf16", 64, 16), ("fp8", "fp16", 128, 64), ("fp8", "bf16", 80, 32),
+                                         ("fp8", "bf16", 256, 128), ("int8", "fp16", 128, 16)])
+@pytest.mark.parametrize("bad", [-7, 10 ** 9])
+def test_rows_before_a_bad_block_are_as_without_it(gpu, new, blocks, to, typ, D, bt, bad):
+    """The last block of a sequence is outside the cache.  Rows that see a token of it are NaN, and those before are
+    right, whatever block 0 of the cache holds (NaN codes and scales here, as memory that nobody wrote may)."""
+    total = (-(-new // bt) + blocks) * bt + 3
+    b = dc.Batch(new + D, [new], [total], 2, D, bt, to, dc.TYPE[typ], heads=4)
+    spare = next(i for i in range(1, len(b.k_scale)) if i not in b.table)
+    b.table[b.table == 0] = spare
+    out, mass, mag = dc.attention(b, D ** -0.5)
+    for t in (b.k_cache, b.v_cache):
+        t.view(torch.uint8)[0] = 0x7f
+    b.k_scale[0], b.v_scale[0] = NAN, INF
+    table, start, lengths = b.index()
+    table[0, -1] = bad
+    got = gpu.kv_cache_attention(b.q.cuda(), b.cache(gpu), table, start, lengths)
+    before = new - 3  # the three tokens of the last block come last
+    dc.near(got[:before], out[:before], dc.attention_bound(out, mass, mag, b.q.dtype)[:before])
+    assert torch.isnan(got[before:]).all()
