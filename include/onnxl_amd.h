@@ -716,8 +716,9 @@ int onnxl_amd_mx_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_sca
  *               block_tokens tokens of a sequence,
  *   query_start INT32 [batch + 1]: the first row of each sequence's new tokens,
  *   lengths     INT32 [batch]: its tokens in the cache, the new ones included.
- * No two sequences may append into one block.  Index tensors in host memory are
- * checked by the call; with device-resident ones a sequence whose numbers do
+ * No two sequences may append into one block.  query_start and lengths in host
+ * memory are checked by the call, and the block table where all three are there;
+ * what is on the device is looked at by the kernels: a sequence whose numbers do
  * not fit is not appended and its rows of the attention are NaN; new tokens of
  * a block outside the cache are dropped, and rows that see one are NaN.
  *

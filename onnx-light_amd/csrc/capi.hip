@@ -3421,21 +3421,21 @@ KvCacheParams PlanKvCache(const char *op, const onnxl_amd_tensor *k_cache, const
   NeedShape(start, {B + 1}, op, "query_start ([batch + 1])");
   OLA_ENFORCE(B < 65536 && most * bt <= (int64_t(1) << 31) - 4096 && tokens < (int64_t(1) << 31), op,
               ": more than 65535 sequences, or about 2^31 tokens.");
-  const bool host = start->location == ONNXL_AMD_HOST && lengths->location == ONNXL_AMD_HOST;
-  if (host) {
-    const int32_t *s = static_cast<const int32_t *>(start->data), *l = static_cast<const int32_t *>(lengths->data);
-    for (int64_t b = 0; b < B; ++b) {
-      OLA_ENFORCE(s[b] >= 0 && s[b + 1] >= s[b] && s[b + 1] <= tokens, op,
-                  ": query_start must rise from 0 to the number of tokens.");
-      OLA_ENFORCE(l[b] >= s[b + 1] - s[b] && l[b] <= most * bt, op,
-                  ": lengths must cover the new tokens and fit the block table.");
+  // each by itself, then what wants two or all three of them
+  auto on_host = [](const onnxl_amd_tensor *t) {
+    return t->location == ONNXL_AMD_HOST ? static_cast<const int32_t *>(t->data) : nullptr;
+  };
+  const int32_t *s = on_host(start), *l = on_host(lengths), *blocks_of = on_host(table);
+  for (int64_t b = 0; b < B; ++b) {
+    OLA_ENFORCE(!s || (s[b] >= 0 && s[b + 1] >= s[b] && s[b + 1] <= tokens), op,
+                ": query_start must rise from 0 to the number of tokens.");
+    OLA_ENFORCE(!l || (l[b] >= (s ? s[b + 1] - s[b] : 0) && l[b] <= most * bt), op,
+                ": lengths must cover the new tokens and fit the block table.");
+    // entries past a sequence's length, and of one without new tokens, are not read
+    for (int64_t j = 0; s && l && blocks_of && s[b + 1] > s[b] && j < (l[b] + bt - 1) / bt; ++j) {
+      const int32_t blk = blocks_of[b * most + j];
+      OLA_ENFORCE(blk >= 0 && blk < blocks, op, ": a block of block_table is outside the cache.");
     }
-    if (table->location == ONNXL_AMD_HOST)
-      for (int64_t b = 0; b < B; ++b)
-        for (int64_t j = 0; s[b + 1] > s[b] && j < (l[b] + bt - 1) / bt; ++j) {
-          const int32_t blk = static_cast<const int32_t *>(table->data)[b * most + j];
-          OLA_ENFORCE(blk >= 0 && blk < blocks, op, ": a block of block_table is outside the cache.");
-        }
   }
   KvCacheParams c{};
   c.k_cache = static_cast<uint8_t *>(k_cache->data);
