@@ -3296,7 +3296,7 @@ int MxQuantize(const onnxl_amd_tensor *x, onnxl_amd_tensor *y, onnxl_amd_tensor 
   Ctx();
   Staging st(stream, 0, {x}, {y, y_scale});
   MxQuantParams p{st.In(x), static_cast<uint8_t *>(st.Out(y)), static_cast<uint8_t *>(st.Out(y_scale)), n / K, K,
-                  x->data_type, y->data_type == kFloat4E2M1};
+                  x->data_type, y->data_type == kFloat4E2M1, 0};
   LaunchMxQuantize(p, stream);
   OLA_HIP(hipGetLastError());
   st.Finish();
@@ -3347,8 +3347,8 @@ int MxMatMul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t
   OLA_ENFORCE(Is16Bit(y->data_type) && (!quantise || y->data_type == a->data_type), kMxmName,
               ": y must be FLOAT16 or BFLOAT16, and a's type where a has 16 bits.");
   NeedShape(y, s, kMxmName, "y");
-  OLA_ENFORCE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 22), kMxmName,
-              ": M or N of 2^31 or more, or K of 2^22 or more.");
+  OLA_ENFORCE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) - 256 && K < (int64_t(1) << 22), kMxmName,
+              ": M of 2^31 or more, N of 2^31 - 256 or more, or K of 2^22 or more.");
   if (M == 0 || N == 0) return ONNXL_AMD_OK;
   Ctx();
   MxMatMulParams p{};
@@ -3500,7 +3500,8 @@ int KvCacheAttention(const onnxl_amd_tensor *q, const onnxl_amd_tensor *k_cache,
   const int64_t heads = q->dims[1];
   OLA_ENFORCE(heads > 0 && heads < 65536 && heads % p.c.kv_heads == 0, kKvtName,
               ": heads must be a multiple of the cache's kv_heads, up to 65535.");
-  OLA_ENFORCE(p.c.tokens * (heads / p.c.kv_heads) < (int64_t(1) << 31), kKvtName, ": 2^31 rows per kv head or more.");
+  OLA_ENFORCE(p.c.tokens * (heads / p.c.kv_heads) <= (int64_t(1) << 31) - 4096, kKvtName,
+              ": about 2^31 rows per kv head or more.");
   NeedShape(out, ShapeOf(*q), kKvtName, "out");
   OLA_ENFORCE(std::isfinite(scale), kKvtName, ": scale must be finite.");
   OLA_ENFORCE(max_query >= 0, kKvtName, ": max_query must not be negative.");

@@ -10,6 +10,14 @@
 
 namespace onnxl_amd {
 
+// A launch has fewer than 2^32 threads along x: a larger grid runs in part, and
+// nothing reports it.  launch(first, count) gets the workgroups piece by piece.
+template <typename F> void LaunchInPieces(int64_t groups, int threads, F launch) {
+  const int64_t most = (int64_t(1) << 31) / threads;
+  for (int64_t first = 0; first < groups; first += most)
+    launch(first, (unsigned)(groups - first < most ? groups - first : most));
+}
+
 // ---------------------------------------------------------------------------
 // RMS norm with the residual's addition and 8-bit output.
 //   h = round16(x + residual)  (x without a residual),  written to sum
@@ -32,6 +40,7 @@ struct RmsNormParams {
   int weight_f32;        // weight is FLOAT, else x's type
   int y_fp8;             // FLOAT8E4M3FN codes, else INT8
   int scale_kind;        // RmsNormScale
+  int64_t first;         // row of the launch's first workgroup
 };
 void LaunchRmsNormQuantize(const RmsNormParams &p, hipStream_t stream);
 
@@ -47,6 +56,7 @@ struct MxQuantParams {
   int64_t rows, K;
   int x_dtype;       // kFloat, kFloat16, kBfloat16
   int fp4;           // E2M1 codes, else E4M3
+  int64_t first;     // the launch's first workgroup of 2048 values
 };
 void LaunchMxQuantize(const MxQuantParams &p, hipStream_t stream);
 
@@ -95,6 +105,7 @@ struct KvAppendParams {
   KvCacheParams c;
   const void *k, *v;  // [tokens, kv_heads, head_dim]
   int bf16;           // BFLOAT16, else FLOAT16
+  int64_t first;      // new block of the launch's first workgroup
 };
 void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream);
 

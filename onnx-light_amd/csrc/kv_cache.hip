@@ -69,7 +69,7 @@ __global__ __launch_bounds__(THREADS) void KvAppendKernel(const KvAppendParams p
   const int head = blockIdx.y, tid = threadIdx.x, bt = c.block_tokens, D = c.head_dim, gd = D / 8;
   const bool is_v = blockIdx.z != 0, fp8 = c.fp8;
   int b, w;
-  if (!FindBlock(c, blockIdx.x, b, w)) return;
+  if (!FindBlock(c, p.first + blockIdx.x, b, w)) return;
   const int len = c.lengths[b], start = c.start[b], first = len - (c.start[b + 1] - start);
   const int j = (first >> c.block_shift) + w;
   const int64_t blk = c.table[(int64_t)b * c.max_blocks + j];
@@ -189,6 +189,14 @@ __global__ __launch_bounds__(THREADS) void KvAppendKernel(const KvAppendParams p
   }
 }
 
+template <int THREADS, int NG, bool KEPT> void LaunchBlocks(KvAppendParams p, int64_t blocks, hipStream_t s) {
+  LaunchInPieces(blocks, THREADS, [&](int64_t first, unsigned count) {
+    p.first = first;
+    const dim3 grid(count, (unsigned)p.c.kv_heads, 2);
+    KvAppendKernel<THREADS, NG, KEPT><<<grid, THREADS, p.c.block_tokens * p.c.head_dim, s>>>(p);
+  });
+}
+
 }  // namespace
 
 void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream) {
@@ -197,7 +205,6 @@ void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream) {
   // n new tokens of a sequence lie in at most (n - 1) / block_tokens + 2 blocks,
   // and in n; workgroups past the last block find none
   const int64_t most = std::min<int64_t>(c.tokens, c.tokens / c.block_tokens + 2 * (int64_t)c.batch);
-  const dim3 grid((unsigned)most, (unsigned)c.kv_heads, 2);
   const int values = c.block_tokens * c.head_dim;
   // A wave per block where a sequence has a token or two on average: there is
   // little to share, and no barrier.  64 sequences with a token each, 8 heads of
@@ -206,13 +213,13 @@ void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream) {
   // group a thread 20.9 us, four 23.3; of 64 tokens kept 16.8 us (3.0 TB/s), read
   // twice 17.3.
   if (c.tokens <= 2 * (int64_t)c.batch) {
-    KvAppendKernel<64, 1, false><<<grid, 64, values, stream>>>(p);
+    LaunchBlocks<64, 1, false>(p, most, stream);
   } else if (values <= 256 * 8) {
-    KvAppendKernel<256, 1, true><<<grid, 256, values, stream>>>(p);
+    LaunchBlocks<256, 1, true>(p, most, stream);
   } else if (values <= 4 * 256 * 8) {
-    KvAppendKernel<256, 4, true><<<grid, 256, values, stream>>>(p);
+    LaunchBlocks<256, 4, true>(p, most, stream);
   } else {
-    KvAppendKernel<256, 1, false><<<grid, 256, values, stream>>>(p);
+    LaunchBlocks<256, 1, false>(p, most, stream);
   }
 }
 

@@ -54,7 +54,7 @@ template <int DT, bool FP4> __device__ __forceinline__ void QuantizeRow8(const M
 }
 
 template <int DT> __global__ __launch_bounds__(256) void MxQuantizeKernel(const MxQuantParams p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (p.first + blockIdx.x) * 256 + threadIdx.x;
   if (i >= p.rows * (p.K / 8)) return;
   if (p.fp4)
     QuantizeRow8<DT, true>(p, nullptr, i);
@@ -90,16 +90,17 @@ struct MxOperands {
   uint8_t *a_tiles, *b_tiles;
   int64_t M, N, K;
   int64_t b_groups;           // workgroups of b's part
+  int64_t first;              // the launch's first workgroup
 };
 
 template <int DT> __global__ __launch_bounds__(256) void MxOperandsKernel(const MxOperands p) {
-  const int64_t steps = (p.K + 255) / 256;
-  if ((int64_t)blockIdx.x < p.b_groups) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t steps = (p.K + 255) / 256, group = p.first + blockIdx.x;
+  if (group < p.b_groups) {
+    const int64_t i = group * 256 + threadIdx.x;
     if (i < p.N * steps) TileScales(p.b_scale, p.b_tiles, p.N, p.K, i);
     return;
   }
-  const int64_t i = ((int64_t)blockIdx.x - p.b_groups) * 256 + threadIdx.x;
+  const int64_t i = (group - p.b_groups) * 256 + threadIdx.x;
   if (!p.q.x) {
     if (i < p.M * steps) TileScales(p.a_scale, p.a_tiles, p.M, p.K, i);
     if (!p.codes) return;
@@ -120,16 +121,17 @@ template <int DT> __global__ __launch_bounds__(256) void MxOperandsKernel(const 
 
 }  // namespace
 
-void LaunchMxQuantize(const MxQuantParams &p, hipStream_t stream) {
-  const int64_t n = p.rows * (p.K / 8);
-  if (n == 0) return;
-  const dim3 grid((unsigned)((n + 255) / 256));
-  if (p.x_dtype == kFloat)
-    MxQuantizeKernel<kFloat><<<grid, 256, 0, stream>>>(p);
-  else if (p.x_dtype == kFloat16)
-    MxQuantizeKernel<kFloat16><<<grid, 256, 0, stream>>>(p);
-  else
-    MxQuantizeKernel<kBfloat16><<<grid, 256, 0, stream>>>(p);
+void LaunchMxQuantize(const MxQuantParams &whole, hipStream_t stream) {
+  MxQuantParams p = whole;
+  LaunchInPieces((p.rows * (p.K / 8) + 255) / 256, 256, [&](int64_t first, unsigned count) {
+    p.first = first;
+    if (p.x_dtype == kFloat)
+      MxQuantizeKernel<kFloat><<<count, 256, 0, stream>>>(p);
+    else if (p.x_dtype == kFloat16)
+      MxQuantizeKernel<kFloat16><<<count, 256, 0, stream>>>(p);
+    else
+      MxQuantizeKernel<kBfloat16><<<count, 256, 0, stream>>>(p);
+  });
 }
 
 namespace {
@@ -221,7 +223,11 @@ template <bool A4, int NT, int MT, bool QUANT> void LaunchStream(const mx::Strea
   const int64_t chunks = Ceil(a.K, 512);
   const size_t codes = QUANT ? (size_t)(a.M * chunks * ((A4 ? 256 : 512) + 16)) : 0;
   const size_t lds = std::max(codes, (size_t)NT * MT * s.waves * 1024);
-  mx::StreamKernel<A4, NT, MT, QUANT><<<dim3((unsigned)s.tiles, (unsigned)s.split), 64 * s.waves, lds, st>>>(a);
+  LaunchInPieces(s.tiles, 64 * s.waves, [&](int64_t first, unsigned count) {
+    mx::StreamArgs p = a;
+    p.first = (int)first;
+    mx::StreamKernel<A4, NT, MT, QUANT><<<dim3(count, (unsigned)s.split), 64 * s.waves, lds, st>>>(p);
+  });
 }
 
 template <bool A4, int MT> void LaunchStreamRows(const mx::StreamArgs &a, const StreamPlan &s, hipStream_t st) {
@@ -263,7 +269,7 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
   if (Streams(p)) {
     const StreamPlan plan = PlanStream(p);
     mx::StreamArgs a{p.x, p.a, p.a_scale, p.b, p.b_scale, static_cast<uint16_t *>(p.y), (int)p.M, (int)p.N, (int)p.K,
-                     p.x_dtype == kBfloat16, p.y_bf16, plan.split, nullptr, nullptr};
+                     p.x_dtype == kBfloat16, p.y_bf16, plan.split, nullptr, nullptr, 0};
     const bool own = OwnQuant(p);
     uint8_t *codes = static_cast<uint8_t *>(scratch), *scales = codes + Scratch::Round((size_t)(p.M * p.K));
     if (a.split > 1) {
@@ -271,7 +277,7 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
       a.done = Ctx().ws.Counters((size_t)plan.tiles);
     }
     if (p.x && !own) {
-      LaunchMxQuantize(MxQuantParams{p.x, codes, scales, p.M, p.K, p.x_dtype, p.a_fp4}, stream);
+      LaunchMxQuantize(MxQuantParams{p.x, codes, scales, p.M, p.K, p.x_dtype, p.a_fp4, 0}, stream);
       a.a = codes;
       a.as = scales;
     }
@@ -290,19 +296,19 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
   o.N = p.N;
   o.K = p.K;
   o.b_groups = Ceil(p.N * steps, 256);
-  o.q = MxQuantParams{p.x, codes, nullptr, p.M, p.K, p.x_dtype, p.a_fp4};
+  o.q = MxQuantParams{p.x, codes, nullptr, p.M, p.K, p.x_dtype, p.a_fp4, 0};
   o.a = p.a;
   o.codes = s.codes ? codes : nullptr;
   // a thread per 8 values to quantize, or 16 bytes of codes to copy, or a step's scales
   const int64_t a_threads = p.M * steps * (p.x ? 32 : !s.codes ? 1 : p.a_fp4 ? 8 : 16);
-  const dim3 grid((unsigned)(o.b_groups + Ceil(a_threads, 256)));
-  if (grid.x == 0) {
-    // K = 0: no operands, sums of nothing
-  } else if (p.x_dtype == kFloat16) {
-    MxOperandsKernel<kFloat16><<<grid, 256, 0, stream>>>(o);
-  } else {
-    MxOperandsKernel<kBfloat16><<<grid, 256, 0, stream>>>(o);
-  }
+  // K = 0: no operands, no launch, sums of nothing
+  LaunchInPieces(o.b_groups + Ceil(a_threads, 256), 256, [&](int64_t first, unsigned count) {
+    o.first = first;
+    if (p.x_dtype == kFloat16)
+      MxOperandsKernel<kFloat16><<<count, 256, 0, stream>>>(o);
+    else
+      MxOperandsKernel<kBfloat16><<<count, 256, 0, stream>>>(o);
+  });
   const mx::GemmArgs g{s.codes ? codes : p.a, p.b, a_tiles, b_tiles, static_cast<uint16_t *>(p.y), p.M, p.N, p.K, p.y_bf16,
                        p.N % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0};
   const Tiles tiles = TilesOf(p);

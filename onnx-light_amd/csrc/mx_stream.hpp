@@ -42,6 +42,7 @@ struct StreamArgs {
   int split;                    // workgroups (grid.y) that share the chunks
   float *part;                  // their sums, [row tile][split][NT * MT][64] float4
   unsigned *done;               // [row tile] workgroups that are done, zero between launches
+  int first;                    // row tile of the launch's first workgroup
 };
 
 // Four block scales from `at` (a multiple of 4) on of the row of `blocks` at
@@ -71,7 +72,7 @@ __global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
   const int blocks = p.K / 32, chunks = (blocks + 15) / 16;
-  const int n0 = blockIdx.x * 16 * NT;
+  const int tile = p.first + (int)blockIdx.x, n0 = tile * 16 * NT;
   const int64_t pitch_b = p.K / 2, pitch_a = A4 ? p.K / 2 : p.K;
 
   // 32-bit offsets of this lane's rows (those past the last repeat it) from the
@@ -221,7 +222,7 @@ __global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const
   __syncthreads();
   constexpr int kScope = 16;  // sc1: past this XCD's L2, so that no fence is needed
   const __amdgpu_buffer_rsrc_t rs = Rsrc(p.part, 0x7fffffff);
-  auto slot = [&](int s, int i) { return (int)(((blockIdx.x * p.split + s) * (NT * MT) + i) * 64 + lane) * 16; };
+  auto slot = [&](int s, int i) { return (int)(((tile * p.split + s) * (NT * MT) + i) * 64 + lane) * 16; };
   auto store = [&](int i, v4f s) {
     const int row = i % MT * 16 + c, col = n0 + i / MT * 16 + 4 * g;
     if (row >= p.M) return;
@@ -247,10 +248,10 @@ __global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const
   __shared__ unsigned before;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this part is where every XCD sees it before it is counted
   __syncthreads();
-  if (tid == 0) before = atomicAdd(p.done + blockIdx.x, 1u);
+  if (tid == 0) before = atomicAdd(p.done + tile, 1u);
   __syncthreads();
   if (before != (unsigned)p.split - 1) return;
-  if (tid == 0) p.done[blockIdx.x] = 0;
+  if (tid == 0) p.done[tile] = 0;
   // up to kParts parts of all of a wave's tiles are on their way at once: one
   // after the other the six of 33 x 11008 x 4099 take 5.3 us of the launch's 15
   constexpr int kParts = 6, kMine = (NT * MT + kStreamWaves<NT> - 1) / kStreamWaves<NT>;

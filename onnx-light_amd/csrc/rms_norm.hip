@@ -144,7 +144,7 @@ __global__ __launch_bounds__(THREADS) void RmsNormKernel(const RmsNormParams p) 
   constexpr int WAVES = THREADS / 64, kStep = THREADS * 8;
   __shared__ float s_sum[WAVES];
   __shared__ unsigned s_top[WAVES];
-  const int64_t row = blockIdx.x, at = row * p.D, end = at + p.D;
+  const int64_t row = p.first + blockIdx.x, at = row * p.D, end = at + p.D;
   const int tid = threadIdx.x;
   float v[NG][8];
   // h of the group from i on (past the end: zeros)
@@ -259,22 +259,28 @@ __global__ __launch_bounds__(THREADS) void RmsNormKernel(const RmsNormParams p) 
   }
 }
 
+template <int DT, int THREADS, int NG, bool KEPT> void LaunchRows(RmsNormParams p, hipStream_t s) {
+  LaunchInPieces(p.rows, THREADS, [&](int64_t first, unsigned count) {
+    p.first = first;
+    RmsNormKernel<DT, THREADS, NG, KEPT><<<count, THREADS, 0, s>>>(p);
+  });
+}
+
 template <int DT> void Launch(const RmsNormParams &p, hipStream_t s) {
-  const dim3 grid((unsigned)p.rows);
   // As few threads as hold the row with one group of 8 values each, then more
   // groups; past the registers the row is read again.  4096 rows with residual,
   // bfloat16, us, the variant taken | the next: 512 values 5.7 | 8.4, 2048 14.3 |
   // 18.5, 8192 46.4 (5.1 TB/s) | 54.9, 16384 93.9 | 117.
   if (p.D <= 512)
-    RmsNormKernel<DT, 64, 1, true><<<grid, 64, 0, s>>>(p);
+    LaunchRows<DT, 64, 1, true>(p, s);
   else if (p.D <= 2048)
-    RmsNormKernel<DT, 256, 1, true><<<grid, 256, 0, s>>>(p);
+    LaunchRows<DT, 256, 1, true>(p, s);
   else if (p.D <= 8192)
-    RmsNormKernel<DT, 512, 2, true><<<grid, 512, 0, s>>>(p);
+    LaunchRows<DT, 512, 2, true>(p, s);
   else if (p.D <= 16384)
-    RmsNormKernel<DT, 512, 4, true><<<grid, 512, 0, s>>>(p);
+    LaunchRows<DT, 512, 4, true>(p, s);
   else
-    RmsNormKernel<DT, 512, 1, false><<<grid, 512, 0, s>>>(p);
+    LaunchRows<DT, 512, 1, false>(p, s);
 }
 
 }  // namespace

@@ -39,3 +39,27 @@ def test_rows_before_a_bad_block_are_as_without_it(gpu, new, blocks, to, typ, D,
     before = new - 3  # the three tokens of the last block come last
     dc.near(got[:before], out[:before], dc.attention_bound(out, mass, mag, b.q.dtype)[:before])
     assert torch.isnan(got[before:]).all()
+
+
+# ---- sizes past one launch (2^32 threads) ------------------------------------------
+
+def test_norm_of_more_rows_than_a_launch_takes(gpu):
+    rows = 2 ** 26 + 3
+    x = torch.randn((rows, 1), dtype=torch.float16, device="cuda")
+    w = torch.ones(1, dtype=torch.float16, device="cuda")
+    y, s, _ = gpu.rms_norm_quantize(x, w, output_dtype=gpu.INT8)
+    for part in range(0, rows, 2 ** 24):
+        rows_of = slice(part, min(rows, part + 2 ** 24))
+        want = gpu.rms_norm_quantize(x[rows_of], w, output_dtype=gpu.INT8)
+        assert torch.equal(y[rows_of], want[0]) and torch.equal(s[rows_of], want[1])
+
+
+def test_mx_product_with_more_columns_than_a_launch_takes(gpu):
+    N = 2 ** 27 + 40
+    x = dc.randn(dc.gen(1), (1, 32), torch.bfloat16).cuda()
+    b = torch.randint(0, 256, (N, 16), dtype=torch.uint8, device="cuda")
+    s = torch.randint(118, 124, (N, 1), dtype=torch.uint8, device="cuda")
+    y = gpu.mx_matmul(x, b, s)
+    for part in range(0, N, 2 ** 25):
+        cols = slice(part, min(N, part + 2 ** 25))
+        assert torch.equal(y[:, cols], gpu.mx_matmul(x, b[cols], s[cols]))
