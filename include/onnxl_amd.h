@@ -714,13 +714,17 @@ int onnxl_amd_mx_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_sca
  * tokens is described by
  *   block_table INT32 [batch, max_blocks]: the cache block of every
  *               block_tokens tokens of a sequence,
- *   query_start INT32 [batch + 1]: the first row of each sequence's new tokens,
+ *   query_start INT32 [batch + 1]: the first row of each sequence's new tokens;
+ *               it never falls,
  *   lengths     INT32 [batch]: its tokens in the cache, the new ones included.
  * No two sequences may append into one block.  query_start and lengths in host
  * memory are checked by the call, and the block table where all three are there;
  * what is on the device is looked at by the kernels: a sequence whose numbers do
  * not fit is not appended and its rows of the attention are NaN; new tokens of
  * a block outside the cache are dropped, and rows that see one are NaN.
+ * A query_start on the device that falls somewhere lets sequences claim the same
+ * rows: what such rows hold and which of the sequences are appended is not said,
+ * but nothing outside their rows and blocks is touched.
  *
  * Append: k, v FLOAT16 or BFLOAT16 [tokens, kv_heads, head_dim].  A block's
  * scale becomes the larger of that of the tokens it keeps (none: 0) and

@@ -89,6 +89,9 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream);
 // its length, a length beyond the table, rows past the last token) is not
 // appended and its attention is NaN; new tokens of a block outside the cache
 // are dropped, and rows that see one are NaN.
+// Each sequence is judged by its own numbers, so where query_start falls several
+// may claim the same rows: the last to write them wins, their NaN among it, and an
+// append, whose launch counts on no more new tokens than rows, may leave some out.
 
 struct KvCacheParams {
   uint8_t *k_cache, *v_cache;

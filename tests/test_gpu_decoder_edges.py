@@ -63,3 +63,26 @@ def test_mx_product_with_more_columns_than_a_launch_takes(gpu):
     for part in range(0, N, 2 ** 25):
         cols = slice(part, min(N, part + 2 ** 25))
         assert torch.equal(y[:, cols], gpu.mx_matmul(x, b[cols], s[cols]))
+
+
+# ---- a query_start that falls -----------------------------------------------------------
+
+@pytest.mark.parametrize("start", [[0, 9, 2, 4, 6], [0, 2, 100, 4, 8], [0, 8, 0, 8, 8], [8, 6, 4, 2, 0], [-3, 2, 4, 1, 8]])
+@pytest.mark.parametrize("n", [2, 40])
+def test_a_falling_query_start_stays_inside(gpu, start, n):
+    """Which results such a batch gives is not said, but it reads and writes nothing beyond its rows and blocks: blocks
+    of the cache that its table does not name and rows past `tokens` stay as they are."""
+    b = dc.Batch(8, [2 * n] * 4, [3 * n + 20] * 4, 2, 64, 16, "fp8", torch.bfloat16, heads=4)
+    start = torch.tensor(start, dtype=torch.int32) * n
+    tokens = 8 * n
+    c = b.cache(gpu)
+    table, _, lengths = b.index()
+    k, v, q = b.k[:tokens].cuda(), b.v[:tokens].cuda(), b.q[:tokens].cuda()
+    out = torch.full((tokens + 64, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    gpu.kv_cache_attention(q, c, table, start.cuda(), lengths, out=out[:tokens])
+    gpu.kv_cache_append(k, v, c, table, start.cuda(), lengths)
+    assert (out[tokens:] == 7).all()
+    free = [i for i in range(len(b.k_scale)) if i not in b.table]
+    assert len(free) == 3
+    for name in ("k_cache", "v_cache", "k_scale", "v_scale"):
+        assert same(getattr(c, name)[free], getattr(b, name)[free]), name
