@@ -671,7 +671,8 @@ int onnxl_amd_prepare_qqq(int64_t in_features, int64_t out_features, int64_t gro
  * x's shape and type:
  *   h = x + residual, rounded to x's type (written to `sum` if given, which
  *       may be x's or the residual's own buffer),
- *   v = h * (1 / sqrt(mean(h^2) + epsilon)) * weight, in fp32,
+ *   v = h * (1 / sqrt(mean(h^2) + epsilon)) * weight, in fp32, also where the
+ *       squares of finite values would leave its range,
  *   per block of block_size values (0: the row; 32, 64, 128 or 256):
  *   y_scale = max|v| / qmax, y = the nearest code of v / y_scale,
  * with y INT8 (qmax 127) or FLOAT8E4M3FN (qmax 448) and y_scale FLOAT

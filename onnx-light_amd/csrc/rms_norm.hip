@@ -158,6 +158,10 @@ __global__ __launch_bounds__(THREADS) void RmsNormKernel(const RmsNormParams p) 
       Round8<DT>(first ? p.sum : nullptr, i, end, h);
     }
   };
+  auto times = [](float (&h)[8], float by) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] *= by;
+  };
   float ss = 0.f;
   auto square = [&](const float (&h)[8]) __attribute__((always_inline)) {
     float t = 0.f;
@@ -184,7 +188,34 @@ __global__ __launch_bounds__(THREADS) void RmsNormKernel(const RmsNormParams p) 
       square(v[0]);
     }
   }
-  const float rstd = 1.f / sqrtf(Join<WAVES, false>(ss, s_sum) / (float)p.D + p.eps);
+  ss = Join<WAVES, false>(ss, s_sum);
+  // Squares of finite values may leave fp32.  The row is then multiplied by a power
+  // of two, which the norm does not see, and its squares are added again: by 2^-80
+  // where the sum is infinite (a square is below 2^96 then), by 2^90 where it is so
+  // small that squares may have been lost, unless epsilon is far above them (sum and
+  // epsilon are below 2^100 then).  No row of ordinary size comes here.
+  float by = 1.f, eps = p.eps;
+  if (!(ss < __builtin_huge_valf()) || (ss < 0x1p-80f && eps < 0x1p-80f)) {
+    by = ss < 1.f ? 0x1p90f : 0x1p-80f;
+    eps = p.eps * by * by;
+    ss = 0.f;
+    if constexpr (KEPT) {
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        times(v[k], by);
+        square(v[k]);
+      }
+    } else {
+      for (int64_t i = at + tid * 8; i < end; i += kStep) {
+        load(i, v[0], false);
+        times(v[0], by);
+        square(v[0]);
+      }
+    }
+    if constexpr (WAVES > 1) __syncthreads();  // the sums before were read
+    ss = Join<WAVES, false>(ss, s_sum);
+  }
+  const float rstd = 1.f / sqrtf(ss / (float)p.D + eps);
   auto scale_by_weight = [&](int64_t i, float (&h)[8]) __attribute__((always_inline)) {
     float w[8];
     if (p.weight_f32)
@@ -241,6 +272,7 @@ __global__ __launch_bounds__(THREADS) void RmsNormKernel(const RmsNormParams p) 
       for (int j = 0; j < 8; ++j) v[0][j] = 0.f;
       if (i < p.D) {
         load(at + i, v[0], false);
+        if (by != 1.f) times(v[0], by);
         scale_by_weight(i, v[0]);
       }
       if (per_row)
@@ -253,6 +285,7 @@ __global__ __launch_bounds__(THREADS) void RmsNormKernel(const RmsNormParams p) 
     if (tid == 0) put_scale(0, s);
     for (int64_t i = tid * 8; i < p.D; i += kStep) {
       load(at + i, v[0], false);
+      if (by != 1.f) times(v[0], by);
       scale_by_weight(i, v[0]);
       Store8(y, at + i, end, v[0], s, p);
     }

@@ -86,3 +86,22 @@ def test_a_falling_query_start_stays_inside(gpu, start, n):
     assert len(free) == 3
     for name in ("k_cache", "v_cache", "k_scale", "v_scale"):
         assert same(getattr(c, name)[free], getattr(b, name)[free]), name
+
+
+# ---- values at the ends of fp32 ------------------------------------------------------------
+
+@pytest.mark.parametrize("D", [64, 1000, 4096, 16384, 20011])
+@pytest.mark.parametrize("typ", ["bf16", "fp32"])
+@pytest.mark.parametrize("size,eps", [(1e20, 1e-5), (1e25, 1e-5), (3e36, 0.0), (1e-25, 0.0), (1e-33, 0.0), (1e-20, 1e-30)])
+def test_norm_of_rows_whose_squares_leave_fp32(gpu, D, typ, size, eps):
+    """Sums of squares above fp32's largest number and below its smallest, in rows beside ordinary ones."""
+    g = dc.gen(D)
+    x, r = dc.randn(g, (5, D), dc.TYPE[typ]), dc.randn(g, (5, D), dc.TYPE[typ])
+    x[1::2] *= size
+    r[1::2] *= size
+    w = dc.randn(g, (D,), torch.float32)
+    check_norm(gpu, x, w, r, "fp8", 0, eps=eps)
+    check_norm(gpu, x, w, None, "int8", 0, eps=eps)
+    if D % 32 == 0:
+        check_norm(gpu, x, w, r, "int8", 32, eps=eps)
+        check_norm(gpu, x, w, r, "fp8", 32, mx=True, eps=eps)
