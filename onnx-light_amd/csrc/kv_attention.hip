@@ -40,7 +40,7 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256, kWaves = 4, kTile = 64;
-constexpr float kNone = -1e30f;  // below every score: the maximum of no token
+constexpr float kNone = -0x1.fffffep127f;  // the maximum of no token: no finite score is below it
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Eight codes (two dwords) as fp16, exact.

@@ -105,3 +105,24 @@ def test_norm_of_rows_whose_squares_leave_fp32(gpu, D, typ, size, eps):
     if D % 32 == 0:
         check_norm(gpu, x, w, r, "int8", 32, eps=eps)
         check_norm(gpu, x, w, r, "fp8", 32, mx=True, eps=eps)
+
+
+@pytest.mark.parametrize("new,total", [([1], [1]), ([1], [100]), ([2, 1], [700, 9]), ([150], [150]), ([150], [700])])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_attention_of_scores_near_the_ends_of_fp32(gpu, new, total, sign):
+    """Every token of the cache has one key, so every weight is the same, at scores of 2^104 to 2^110 in size."""
+    b = dc.Batch(3, new, total, 1, 64, 16, "int8", torch.bfloat16, heads=2)
+    b.k_cache[:], b.k_scale[:], b.v_scale[:] = 64, 1.0, 2.0 ** -7
+    b.q[:] = sign * 2.0 ** 95
+    b.q[:, 1] *= 2.0 ** 6
+    got = gpu.kv_cache_attention(b.q.cuda(), b.cache(gpu), *b.index(), 0.125)
+    at = 0
+    for i, (n, t) in enumerate(zip(new, total)):
+        blk = b.table[i, :-(-t // 16)].long()
+        v = (b.v_cache[blk].double() * 2.0 ** -7).permute(1, 0, 3, 2).reshape(-1, 64)[:t]
+        for j in range(n):
+            seen = v[:t - n + j + 1]
+            want, mass = seen.mean(0), seen.abs().mean(0)
+            for h in range(2):
+                dc.near(got[at + j, h], want, dc.ROUND[torch.bfloat16] * want.abs() + 2.0 ** -10 * mass + 2.0 ** -24)
+        at += n
