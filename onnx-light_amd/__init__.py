@@ -938,19 +938,25 @@ def qlinear_conv(x, x_scale, x_zero_point, w, w_scale, w_zero_point, y_scale, y_
 
 # ---- decoder-layer operators (no reference kernels) --------------------------
 
+def _check_code_type(dtype: int, what: str) -> None:
+    if dtype not in (INT8, FLOAT8E4M3FN):
+        raise InvalidArgument(f"{what} must be INT8 or FLOAT8E4M3FN")
+
+
 def rms_norm_quantize(x, weight, residual=None, epsilon: float = 1e-5, block_size: int = 0,
                       output_dtype: int = FLOAT8E4M3FN, mx: bool = False, out=None):
     """RMS norm with the residual's addition and 8-bit output: returns (y,
     y_scale, sum), sum = x + residual in x's type (None without a residual).
     y is INT8 or FLOAT8E4M3FN with one float32 scale per block_size values of a
     row (0: one per row), or with ``mx`` MXFP8 (FLOAT8E4M3FN, blocks of 32,
-    uint8 E8M0 scales) for mx_matmul."""
+    uint8 E8M0 scales) for mx_matmul.  With ``out`` its tensors' types decide."""
     torch = _torch()
     shape, dev = _shape_of(x), _device_of(x)
-    if mx:
+    if mx and block_size == 0:
         block_size = 32
     if out is None:
-        blocks = shape[-1] // block_size if block_size else 1
+        _check_code_type(output_dtype, "output_dtype")
+        blocks = shape[-1] // block_size if block_size > 0 else 1
         out = (_empty(shape, torch.int8 if output_dtype == INT8 else torch.float8_e4m3fn, dev),
                _empty((*shape[:-1], blocks), torch.uint8 if mx else torch.float32, dev),
                torch.empty_like(x) if residual is not None else None)
@@ -980,13 +986,14 @@ def mx_matmul(a, b, b_scale, a_scale=None, a_type: int = FLOAT8E4M3FN, output_dt
     """a @ b^T in microscaled types: b packed FLOAT4E2M1 uint8 [N, K / 2] with
     b_scale uint8 E8M0 [N, K / 32] (the "mxfp4" checkpoint layout); a FLOAT16 /
     BFLOAT16 [.., K], quantized by the call to a_type (FLOAT8E4M3FN or
-    FLOAT4E2M1), or codes with a_scale as mx_quantize returns them, then with
-    output_dtype a torch type (bfloat16 by default)."""
+    FLOAT4E2M1), the output of its type; or codes with a_scale as mx_quantize
+    returns them (a_type is not looked at), the output of output_dtype, a torch
+    type (bfloat16 by default)."""
     torch = _torch()
     if a_scale is not None:
         a_type = 0
     if out is None:
-        dt = a.dtype if a_scale is None else output_dtype or torch.bfloat16
+        dt = output_dtype or (a.dtype if a_scale is None else torch.bfloat16)
         out = _empty((*_shape_of(a)[:-1], _shape_of(b)[0]), dt, _device_of(a, b))
     _check(lib().onnxl_amd_mx_matmul(describe(a), describe(a_scale), a_type, describe(b), describe(b_scale),
                                      describe(out), _stream_of(a, b, out)))
@@ -1002,6 +1009,7 @@ class KvCache:
     def __init__(self, blocks: int, kv_heads: int, block_tokens: int, head_dim: int, dtype: int = FLOAT8E4M3FN,
                  device="cuda"):
         torch = _torch()
+        _check_code_type(dtype, "the cache's dtype")
         dt = torch.int8 if dtype == INT8 else torch.float8_e4m3fn
         self.k_cache = torch.empty((blocks, kv_heads, block_tokens, head_dim), dtype=dt, device=device)
         self.v_cache = torch.empty((blocks, kv_heads, head_dim, block_tokens), dtype=dt, device=device)

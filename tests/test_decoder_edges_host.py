@@ -60,3 +60,31 @@ def test_host_index_tensors_that_fit_pass(olamd):
         q = torch.zeros(5, 3, 64, dtype=H16)
         rc, message = status(olamd, "kv_cache_attention", [dev(olamd, q)] + cache + [0.1, 0, dev(olamd, q)])
         assert rc == olamd.INVALID_ARGUMENT and "multiple" in message, (where, rc, message)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(output_dtype=10), "output_dtype"), (dict(output_dtype=2), "output_dtype"), (dict(output_dtype=23), "output_dtype"),
+    (dict(block_size=64, mx=True), "blocks of 32"), (dict(block_size=-1), "block_size"), (dict(block_size=-1, mx=True), "block_size"),
+    (dict(output_dtype=3, mx=True), "FLOAT8E4M3FN"),
+])
+def test_norm_front_end_refuses_what_it_does_not_do(olamd, kw, text):
+    """Types and block sizes that the caller names are taken or refused, never replaced."""
+    x = torch.zeros(2, 128, dtype=H16)
+    with pytest.raises(olamd.InvalidArgument, match=text):
+        olamd.rms_norm_quantize(x, x[0], **kw)
+
+
+@pytest.mark.parametrize("dtype", [10, 2, 0])
+def test_cache_of_another_type_is_refused(olamd, dtype):
+    with pytest.raises(olamd.InvalidArgument, match="INT8 or FLOAT8E4M3FN"):
+        olamd.KvCache(2, 1, 16, 64, dtype, "cpu")
+    assert olamd.KvCache(2, 1, 16, 64, olamd.INT8, "cpu").k_cache.dtype == torch.int8
+    assert olamd.KvCache(2, 1, 16, 64, device="cpu").v_cache.dtype == torch.float8_e4m3fn
+
+
+def test_product_front_end_refuses_another_output_type(olamd):
+    """16-bit activations give their own type: another one that the caller names is refused."""
+    w, s = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2, dtype=torch.uint8)
+    for dtype in (torch.bfloat16, torch.float32):
+        with pytest.raises(olamd.InvalidArgument, match="y must be"):
+            olamd.mx_matmul(torch.zeros(2, 64, dtype=H16), w, s, output_dtype=dtype)
