@@ -1639,14 +1639,15 @@ public:
     rt::RequireMinInputCount(node, 2);
     const onnxl_amd_tensor x = In(0, ctx), w = In(1, ctx), r = In(2, ctx);
     const bool mx = rt::GetAttributeIntOrDefault(node, "mx", 0) != 0;
-    const int64_t block = mx ? 32 : rt::GetAttributeIntOrDefault(node, "block_size", 0);
+    int64_t block = rt::GetAttributeIntOrDefault(node, "block_size", 0);
+    if (mx && block == 0) block = 32;
     const int32_t to = static_cast<int32_t>(rt::GetAttributeIntOrDefault(node, "output_dtype", kFloat8E4M3FN));
     if (x.rank < 1 || block < 0) throw std::invalid_argument("RmsNormQuantize: x must have a last dimension.");
     const rt::Shape shape = ShapeOf(x.dims, x.rank), scales = WithLast(x, block > 0 ? x.dims[x.rank - 1] / block : 1);
     rt::Tensor y = ctx.MakeOutputTensor(0, to, shape, static_cast<size_t>(Count(shape)));
     rt::Tensor s = ctx.MakeOutputTensor(1, mx ? kUint8 : kFloat, scales, static_cast<size_t>(Count(scales)) * (mx ? 1 : 4));
     onnxl_amd_tensor dy = DescribeOutput(y), ds = DescribeOutput(s), dt = Absent();
-    const bool total = r.rank >= 0 && node.output_size() > 2 && !node.output(2).empty();
+    const bool total = node.output_size() > 2 && !node.output(2).empty();  // refused without a residual
     rt::Tensor t;
     if (total) {
       t = ctx.MakeOutputTensor(2, x.data_type, shape, ByteSize(x.data_type, Count(shape)));
@@ -1673,7 +1674,10 @@ public:
     rt::RequireInputCount(node, 1);
     rt::RequireOutputCount(node, 2);
     const onnxl_amd_tensor x = In(0, ctx);
-    const bool fp4 = rt::GetAttributeIntOrDefault(node, "output_dtype", kFloat8E4M3FN) == kFloat4E2M1;
+    const int64_t to = rt::GetAttributeIntOrDefault(node, "output_dtype", kFloat8E4M3FN);
+    if (to != kFloat8E4M3FN && to != kFloat4E2M1)
+      throw std::invalid_argument("MxQuantize: output_dtype must be FLOAT8E4M3FN or FLOAT4E2M1.");
+    const bool fp4 = to == kFloat4E2M1;
     if (x.rank < 1) throw std::invalid_argument("MxQuantize: x must have a last dimension.");
     const int64_t K = x.dims[x.rank - 1];
     const rt::Shape codes = WithLast(x, fp4 ? K / 2 : K), scales = WithLast(x, K / 32);
