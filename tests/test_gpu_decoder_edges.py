@@ -126,3 +126,32 @@ def test_attention_of_scores_near_the_ends_of_fp32(gpu, new, total, sign):
             for h in range(2):
                 dc.near(got[at + j, h], want, dc.ROUND[torch.bfloat16] * want.abs() + 2.0 ** -10 * mass + 2.0 ** -24)
         at += n
+
+
+# ---- a cache past 4 GB ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new", [3, 200])
+@pytest.mark.parametrize("H,bt,D", [(8, 64, 128), (4, 256, 64)])
+def test_cache_whose_offsets_pass_32_bits(gpu, new, H, bt, D):
+    """Blocks on both sides of 2^32 bytes, appended to and attended over: as in a small cache."""
+    total = new + 5 * bt + 7
+    b = dc.Batch(new, [new], [total], H, D, bt, "fp8", torch.bfloat16, heads=2 * H)
+    line = 2 ** 32 // (H * bt * D)
+    blocks = line + len(b.k_scale)
+    order = torch.arange(b.table.shape[1], dtype=torch.int32) * (1 - 2 * (torch.arange(b.table.shape[1]) % 2)) + line
+    big = gpu.KvCache(blocks, H, bt, D)
+    for name in ("k_cache", "v_cache", "k_scale", "v_scale"):
+        small, large = getattr(b, name).cuda(), getattr(big, name)
+        large.view(torch.uint8).fill_(0x7f)
+        for i in range(b.table.shape[1]):
+            large[int(order[i])] = small[int(b.table[0, i])]
+    c, (table, start, lengths) = b.cache(gpu), b.index()
+    far = order.to(torch.int32)[None].cuda()
+    k, v, q = b.k.cuda(), b.v.cuda(), b.q.cuda()
+    gpu.kv_cache_append(k, v, c, table, start, lengths)
+    gpu.kv_cache_append(k, v, big, far, start, lengths)
+    for name in ("k_cache", "v_cache", "k_scale", "v_scale"):
+        for i in range(b.table.shape[1]):
+            assert same(getattr(big, name)[int(order[i])], getattr(c, name)[int(b.table[0, i])].cpu()), (name, i)
+    assert torch.equal(gpu.kv_cache_attention(q, big, far, start, lengths),
+                       gpu.kv_cache_attention(q, c, table, start, lengths))
