@@ -66,7 +66,7 @@ template <bool FP8> __device__ __forceinline__ v8h Widen(int lo, int hi) {
 
 __device__ __forceinline__ uint2 Pack4(v4f v, int bf16) {
   typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-  uint2 b;  // a conversion of vectors to bfloat16 has lost operands here
+  uint2 b;  // pairs by the instruction itself: one for two values, to nearest even
   asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(b.x) : "v"(v[0]), "v"(v[1]));
   asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(b.y) : "v"(v[2]), "v"(v[3]));
   const uint2 h = __builtin_bit_cast(uint2, __builtin_convertvector(v, v4h));
@@ -121,8 +121,8 @@ template <int G = 4> __device__ __forceinline__ float GroupSum(float v) {
 // whoever that is.
 //
 // 64 sequences of 500 to 16384 tokens, 64 heads over 8 of 128 dimensions: 1.1 GB in
-// 207 us, 5.4 TB/s, what a large copy reaches.  One sequence of 8191 tokens: 17 MB
-// in 13.7 us, a chain of latencies (lengths, table, tile, parts, their join).
+// 206 us, 5.4 TB/s (a copy of 1 GB reaches 5.1).  One sequence of 8191 tokens: 17 MB
+// in 13.2 us, a chain of latencies (lengths, table, tile, parts, their join).
 
 struct Line {        // units before every thread's share of the sequences
   int64_t upto[kThreads];
@@ -185,7 +185,6 @@ __device__ __forceinline__ int64_t MakeLine(const Plan &p, Line &line) {
   return Uniform(line.upto[kThreads - 1]);
 }
 
-// The job of unit u, the same in every lane.
 // NaN for the rows of sequences whose numbers do not fit.
 __device__ __forceinline__ void FillInvalid(const Plan &p) {
   const KvCacheParams &c = p.a.c;
@@ -204,7 +203,7 @@ __device__ __forceinline__ int64_t Over(int64_t a, int b) {
   return (uint64_t)a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
-// Unit u of sequence b, whose units start at `at`.
+// The job of unit u of sequence b, whose units start at `at`; the same in every lane.
 __device__ __forceinline__ Job JobOf(const Plan &p, int64_t u, int64_t at, int b, int n, int len, int start) {
   Job j;
   j.b = b;
@@ -240,7 +239,7 @@ __device__ __forceinline__ Job FindJob(const Plan &p, const Line &line, int64_t 
 
 // Up to 64 sequences: lane b of every wave keeps what there is to know of sequence
 // b, and nobody searches LDS or waits for another wave: one sequence of 8191
-// tokens 16.0 -> 15.2 us (with the join of parts below 13.7).
+// tokens 16.0 -> 15.2 us (with the join of parts below 13.2).
 struct Lanes {
   int64_t upto;       // units up to the end of the sequence
   int n, len, start;  // its rows' new tokens, length, first new token
@@ -271,7 +270,6 @@ __device__ __forceinline__ int64_t PieceOf(int64_t units) {
   return piece < kWaves ? kWaves : piece;
 }
 
-// Writes O / sum of the rows that there are.
 // Where a row's output goes, and the dimensions from d on of it.
 __device__ __forceinline__ uint16_t *OutRow(const Plan &p, const Job &j, int row) {
   const int64_t token = j.start + (int64_t)(row / p.group);
@@ -282,6 +280,7 @@ __device__ __forceinline__ void StoreDims(const Plan &p, uint16_t *out, int d, v
   const uint2 h = Pack4(o, p.a.bf16);
   __builtin_memcpy(out + d, &h, 8);
 }
+// O / sum of the rows that there are: 16 dimensions of 16 rows.
 __device__ __forceinline__ void StoreRows(const Plan &p, const Job &j, int t, v4f o, float sum) {
   const int row = j.row0 + threadIdx.x % 16;
   if (row < j.n * p.group) StoreDims(p, OutRow(p, j, row), 16 * t + threadIdx.x % 64 / 16 * 4, o * (0x1p-15f / sum));
@@ -622,7 +621,9 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void KvDecodeKernel(co
 // neighbouring pieces: the keys and values that they share stay in its L2, 617 ->
 // 586 us (930 TFLOP/s; a wave's part of a tile 5400 -> 4300 clocks, and the clock
 // gave way to power from 2.4 to 2.05 GHz).  With the 16 x 16 products for 128
-// dimensions the issue slots that MFMAs take from the vector unit double.
+// dimensions the issue slots that MFMAs take from the vector unit double.  Registers
+// are full: head dimensions above 64 other than 128 and 256, which look at every
+// dimension's end, keep up to 10 of them in memory.
 //
 // The reference mo moves only when it is exceeded by 2^kLag or more, which is left
 // free below kTop.
@@ -941,9 +942,11 @@ template <> struct Mfma<32> {
 
 constexpr int kAhead = 4;  // 6 and 8 want registers that are not there
 
-// Tiles that a workgroup takes at least.  One sequence of 256 rows, 8192 tokens:
-// pieces of 4, 8, 16 tiles 68, 56, 63 us; the parts of a job, 128 KB each, are
-// joined by one CU, at about 75 GB/s.
+// Tiles that a workgroup takes at least.  Pieces of 4 | 8 | 16 tiles, us, 8 kv heads
+// of 128, rows over tokens: one sequence 256 over 8192 69 | 56 | 63, 512 over 8192
+// 65 | 65 | 71, 256 over 2048 38 | 41 | 50; two 256 over 4096 49 | 48 | 58.  From
+// 1024 rows on pieces are longer by themselves.  The parts of a job, 128 KB each,
+// are joined by one CU, at about 75 GB/s.
 constexpr int kLeastPiece = 8;
 
 // LDS writes and reads of this wave are done; so for all waves.  Loads stay in
@@ -1265,10 +1268,16 @@ template <int HD, int W> void LaunchPrompt(const Plan &p, int64_t grid, hipStrea
 // Sequences with at most so many rows (new tokens * heads of a group) take the
 // decoding kernel, the others the prompt kernel; a launch that no sequence can
 // need is left out.  Per sequence of 8192 tokens, 8 kv heads of 128 dimensions,
-// decoding | prompt kernel: 8 sequences of 32 rows 49 | 84 us, of 64 rows 87 | 79,
-// of 128 rows 161 | 81.  Where all rows of the batch are few the parts of a
+// decoding | prompt kernel: 8 sequences of 32 rows 45 | 73 us, of 64 rows 80 | 75,
+// of 128 rows 149 | 81.  Where all rows of the batch are few the parts of a
 // sequence are many, and the decoding kernel's are the smaller to join: one
-// sequence of 64 rows 21 | 38 us, of 128 rows 26 | 40, of 256 rows 37 | 56.
+// sequence of 64 rows 17 | 36 us, of 128 rows 21 | 40.  The line could lie higher:
+// 256 rows in all are one sequence 31 | 56, two 32 | 41, four 31 | 46, and 512 in
+// eight 80 | 75.
+//
+// Without max_query every sequence may be the long one: 64 sequences of a token
+// with groups of 8 heads then pay the prompt kernel's launch, which finds nothing,
+// 52 -> 56 us and 118 -> 122, 17 of them 18 -> 21; up to 128 rows in all nothing.
 constexpr int kFewRows = 32, kFewInAll = 128;
 
 struct Split {

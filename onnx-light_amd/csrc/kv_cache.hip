@@ -208,10 +208,10 @@ void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream) {
   const int values = c.block_tokens * c.head_dim;
   // A wave per block where a sequence has a token or two on average: there is
   // little to share, and no barrier.  64 sequences with a token each, 8 heads of
-  // 128: 4.5 us, with 256 threads 5.3.  Else 256 threads, which keep a block in
+  // 128: at least 4.4 us, with 256 threads 5.0 (5.1 in the middle for both).  Else 256 threads, which keep a block in
   // registers while it fits: four times 2048 tokens, blocks of 16 tokens one
-  // group a thread 20.9 us, four 23.3; of 64 tokens kept 16.8 us (3.0 TB/s), read
-  // twice 17.3.
+  // group a thread 19.7 us, four 22.1; of 64 tokens kept 16.1 us (3.1 TB/s), read
+  // twice 15.8, no difference between runs.
   if (c.tokens <= 2 * (int64_t)c.batch) {
     LaunchBlocks<64, 1, false>(p, most, stream);
   } else if (values <= 256 * 8) {

@@ -157,10 +157,10 @@ template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, hipStr
 // byte, small ones (128 x 128) leave fewer CUs idle; E4M3 has 128 x 192 between
 // them.  A round of small, middle and large ones takes about 20, 24 and 29 parts of
 // time (of the small ones two fit a CU for E2M1), and the shortest sum is taken.
-// us, large / small: MXFP4 1000 x 4096 x 6144 40 / 27, 4096 x 8192 x 8192 174 /
-// 205.  Large / middle / small: MXFP8 256 x 4096 x 4096 29 / 25 / 22, 1000 x 4096 x
-// 6144 37 / 33 / 45, 2048 x 4096 x 4096 41 / 54 / 49, 4096 x 8192 x 8192 243 / 288 /
-// 326.
+// us, large / small: MXFP4 1000 x 4096 x 6144 38 / 25, 4096 x 8192 x 8192 156 /
+// 184.  Large / middle / small: MXFP8 256 x 4096 x 4096 27 / 24 / 21, 1000 x 4096 x
+// 6144 33 / 30 / 41, 2048 x 4096 x 4096 39 / 51 / 45, 4096 x 8192 x 8192 234 / 278 /
+// 311.
 enum class Tiles { kSmall, kMiddle, kLarge };
 Tiles TilesOf(const MxMatMulParams &p) {
   const int64_t cus = Ctx().num_cus;
@@ -173,12 +173,12 @@ Tiles TilesOf(const MxMatMulParams &p) {
 // Few rows take the streaming kernel, whose time goes with the weight's bytes and
 // the row tiles; the GEMM's one round of tiles goes with K alone, and a wide
 // weight fills it.  us, rows x K x N, stream | GEMM:
-//   MXFP4  32 x 4096 x 14336 15.0 | 18.9    48 x 4096 x 14336 17.9 | 19.0
-//          56 x 4096 x 14336 20.9 | 19.0    64 x 2048 x 16384 15.0 | 13.5
-//          64 x 8192 x 8192 28.0 | 28.4     64 x 11008 x 4096 21.4 | 34.0
-//   MXFP8  36 x 2048 x 8192 8.6 | 13.2      40 x 11008 x 8192 35.5 | 39.8
-//          40 x 4096 x 14336 27.6 | 21.2    33 x 8192 x 28672 82.4 | 51.4
-//          64 x 4096 x 6144 18.5 | 19.7     64 x 4096 x 8192 22.1 | 20.1
+//   MXFP4  32 x 4096 x 14336 14.7 | 18.6    48 x 4096 x 14336 18.1 | 18.5
+//          56 x 4096 x 14336 20.8 | 18.6    64 x 2048 x 16384 14.9 | 13.1
+//          64 x 8192 x 8192 27.1 | 28.2     64 x 11008 x 4096 20.9 | 33.9
+//   MXFP8  36 x 2048 x 8192 8.6 | 13.1      40 x 11008 x 8192 35.2 | 39.4
+//          40 x 4096 x 14336 27.3 | 20.7    33 x 8192 x 28672 81.4 | 51.5
+//          64 x 4096 x 6144 18.5 | 19.5     64 x 4096 x 8192 21.9 | 19.8
 bool Streams(const MxMatMulParams &p) {
   if (p.M <= 32 || p.M > 64) return p.M <= 32;
   if (p.a_fp4) return p.M <= 48 || p.N < 12288;
@@ -186,9 +186,19 @@ bool Streams(const MxMatMulParams &p) {
 }
 
 // Up to this many values every workgroup quantizes its activations itself
-// (eight at a time per thread); a launch for all costs about 4 us.  us, itself |
-// in a launch: 1 x 4096 x 14336 10.1 | 12.2, 4 x 4096 x 4096 6.6 | 8.1, 8 x 4096 x
-// 14336 24.3 | 13.8.
+// (eight at a time per thread); a launch for all costs 2 to 4 us.  us, MXFP8, itself |
+// in a launch, by N:
+//               2048        4096       8192        14336       28672
+//   1 x 4096    4.7 | 7.4   5.0 | 7.5   6.3 | 8.1    9.9 | 11.6  16.6 | 18.7
+//   2 x 4096    4.8 | 7.3   5.1 | 7.8   7.3 | 8.1   11.7 | 11.9  20.5 | 19.4
+//   4 x 4096    6.3 | 7.3   6.3 | 8.0   9.5 | 8.5   15.6 | 12.5  25.8 | 20.3
+//   8 x 4096    8.8 | 7.5   8.8 | 8.2  13.3 | 8.9   23.1 | 13.3  37.9 | 21.9
+//   8 x 2048    5.6 | 7.5   5.6 | 7.3   7.1 | 7.1   12.6 | 9.7   21.0 | 14.7
+//   1 x 8192    6.5 | 8.8   9.4 | 9.4  16.9 | 14.8  20.7 | 25.0  41.0 | 35.4
+//   2 x 8192    7.8 | 9.1  11.4 | 9.7  20.5 | 15.2  24.3 | 25.5  45.2 | 36.2
+// The rule does not look at N, with which the workgroups that repeat the work grow:
+// it holds up to 8192 values and for narrow weights, and loses up to 35 % between
+// that and its end by wide ones.
 constexpr int64_t kOwnQuant = 16384;
 bool OwnQuant(const MxMatMulParams &p) { return p.x && p.M <= 16 && p.M * Ceil(p.K, 512) * 512 <= kOwnQuant; }
 
@@ -207,8 +217,8 @@ StreamPlan PlanStream(const MxMatMulParams &p) {
   // the same ones at about the same time, and cost as much per 16 rows as the
   // weight: several row tiles share a read, while a wave for every CU's SIMD is
   // left.  More than these do not fit the registers of two waves per SIMD.  us,
-  // K = 4096, N = 14336, with these | with one: 8 rows 13.8 | 15.6, 16 rows 15.4 |
-  // 18.7, MXFP4 32 rows 15.0 | 19.8, 48 rows 17.9 | 24.5.
+  // K = 4096, N = 14336, with these | with one: 8 rows 13.3 | 15.0, 16 rows 15.0 |
+  // 18.3, MXFP4 32 rows 14.7 | 19.1, 48 rows 18.2 | 24.0.
   s.nt = OwnQuant(p) ? 1 : s.mt == 1 ? 2 : s.mt <= (p.a_fp4 ? 3 : 2) ? 4 : 2;
   while (s.nt > 1 && Ceil(p.N, 16 * s.nt) * chunks < 4 * Ctx().num_cus) s.nt /= 2;
   s.waves = s.nt == 4 ? 4 : 8;

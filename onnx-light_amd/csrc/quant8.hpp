@@ -11,7 +11,12 @@ namespace onnxl_amd {
 constexpr float kInt8Max = 127.f, kFp8Max = 448.f;
 constexpr float kMinNormal = 0x1p-126f;
 
-// The scale of a block: codes are round(y * inv) and stand for code * scale.
+// The scale of a block: codes are round(y * inv) and stand for code * scale.  With a
+// FLOAT scale inv and the product are rounded, to within 2^-23 of y / scale, so a
+// quotient that near the middle between two codes may take either of them; of
+// 16-bit values exact middles are no rarity (y qmax / max), and these roundings
+// decide them, not ties to even.  A division per value would take ten instructions
+// for one.
 struct BlockScale {
   float scale, inv;
   uint8_t e8m0;

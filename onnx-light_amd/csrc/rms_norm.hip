@@ -302,8 +302,8 @@ template <int DT, int THREADS, int NG, bool KEPT> void LaunchRows(RmsNormParams 
 template <int DT> void Launch(const RmsNormParams &p, hipStream_t s) {
   // As few threads as hold the row with one group of 8 values each, then more
   // groups; past the registers the row is read again.  4096 rows with residual,
-  // bfloat16, us, the variant taken | the next: 512 values 5.7 | 8.4, 2048 14.3 |
-  // 18.5, 8192 46.4 (5.1 TB/s) | 54.9, 16384 93.9 | 117.
+  // bfloat16, us, the variant taken | the next: 512 values 5.2 | 7.7, 2048 12.8 |
+  // 18.9, 8192 41.7 (5.6 TB/s) | 46.9, 16384 83.4 | 123.
   if (p.D <= 512)
     LaunchRows<DT, 64, 1, true>(p, s);
   else if (p.D <= 2048)
