@@ -22,7 +22,8 @@
 //    an encoded weight, ai.rt.amd:DequantizeLinearGroupedMatMul on quantized
 //    MoE experts) and, with no built-in counterpart, the operators of a decoder
 //    layer between them (ai.rt.amd:RmsNormQuantize, MxQuantize, MxMatMul,
-//    KvCacheAppend, KvCacheAttention),
+//    KvCacheAppend, KvCacheAttention, MxGatedMatMul, RotaryTables,
+//    RotaryEmbedding, RotaryKvCacheAppend, SampleTokens),
 //    registered with RegisterKernelFn(..., Device::kCPU, overwrite = true),
 //    the plain key the built-ins use (examples/register_custom_kernel/
 //    main.cc:105-114): a kGPU key would need RuntimeContextOptions.device =
@@ -77,7 +78,7 @@ using ONNX_LIGHT_NAMESPACE::NodeProto;
 namespace mi355x {
 
 // ONNX TensorProto data types used below.
-constexpr int32_t kFloat = 1, kUint8 = 2, kInt8 = 3, kInt32 = 6, kFloat16 = 10, kDouble = 11, kBfloat16 = 16,
+constexpr int32_t kFloat = 1, kUint8 = 2, kInt8 = 3, kInt32 = 6, kInt64 = 7, kFloat16 = 10, kDouble = 11, kBfloat16 = 16,
                   kFloat8E4M3FN = 17, kUint4 = 21, kInt4 = 22, kFloat4E2M1 = 23;
 constexpr const char *kFusedDomain = "ai.rt.amd";
 
@@ -1809,6 +1810,170 @@ template <typename K> void Register(const char *domain, const char *op_type) {
       /*overwrite=*/true);
 }
 
+// ---------------------------------------------------------------------------
+// Operators from a decoder layer's joint projection to the next token (ai.rt.amd; no
+// counterparts in the reference).
+
+// ai.rt.amd:MxGatedMatMul(a, gate, gate_scale, up, up_scale, a_scale | "";
+// activation = 0 (SiLU; 1 GELU, 2 GELU by tanh, 3 ReLU), a_type = FLOAT8E4M3FN (a of
+// 16 bits only), output_dtype = BFLOAT16 (codes only), mx = 0) = y[, y_scale].
+class Mi355xMxGatedMatMul : public Mi355xKernel {
+public:
+  static constexpr const char *name = "onnxl_amd:CPU:ai.rt.amd:MxGatedMatMul";
+  using Mi355xKernel::Mi355xKernel;
+  void Run(rt::RuntimeContext &ctx) override {
+    const NodeProto &node = *node_;
+    rt::RequireMinInputCount(node, 5);
+    const bool mx = rt::GetAttributeIntOrDefault(node, "mx", 0) != 0;
+    rt::RequireOutputCount(node, mx ? 2 : 1);
+    const onnxl_amd_tensor a = In(0, ctx), gate = In(1, ctx), gs = In(2, ctx), up = In(3, ctx), us = In(4, ctx), as = In(5, ctx);
+    const bool codes = as.rank >= 0;
+    const int32_t a_type = static_cast<int32_t>(rt::GetAttributeIntOrDefault(node, "a_type", kFloat8E4M3FN));
+    const int32_t to = mx      ? kFloat8E4M3FN
+                       : codes ? static_cast<int32_t>(rt::GetAttributeIntOrDefault(node, "output_dtype", kBfloat16))
+                               : a.data_type;
+    if (gate.rank != 2) throw std::invalid_argument("MxGatedMatMul: gate must be 2-D.");
+    const rt::Shape shape = WithLast(a, gate.dims[0]), scales = WithLast(a, gate.dims[0] / 32);
+    rt::Tensor y = ctx.MakeOutputTensor(0, to, shape, mx ? static_cast<size_t>(Count(shape)) : ByteSize(to, Count(shape)));
+    rt::Tensor s;
+    onnxl_amd_tensor dy = DescribeOutput(y), ds = Absent();
+    if (mx) {
+      s = ctx.MakeOutputTensor(1, kUint8, scales, static_cast<size_t>(Count(scales)));
+      ds = DescribeOutput(s);
+    }
+    Check(onnxl_amd_mx_gated_matmul(&a, &as, codes ? 0 : a_type, &gate, &gs, &up, &us,
+                                    static_cast<int32_t>(rt::GetAttributeIntOrDefault(node, "activation", 0)), &dy, &ds,
+                                    nullptr));
+    rt::SetOutput(node, 0, std::move(y), ctx);
+    if (mx) rt::SetOutput(node, 1, std::move(s), ctx);
+  }
+
+protected:
+  std::vector<int> ConstantInputs() const override { return {1, 2, 3, 4}; }
+};
+
+// ai.rt.amd:RotaryTables(base | "" (10000), factor | "" (1), turns_fast | "" (32),
+// turns_slow | "" (1), magnitude | "" (0), all FLOAT scalars; positions, rotary_dim,
+// scaling = 0 (none; 1 linear, 2 ntk, 3 by parts, 4 yarn), original_positions = 0) =
+// cos, sin, FLOAT.
+class Mi355xRotaryTables : public Mi355xKernel {
+public:
+  static constexpr const char *name = "onnxl_amd:CPU:ai.rt.amd:RotaryTables";
+  using Mi355xKernel::Mi355xKernel;
+  void Run(rt::RuntimeContext &ctx) override {
+    const NodeProto &node = *node_;
+    rt::RequireOutputCount(node, 2);
+    const int64_t positions = rt::GetAttributeIntOrDefault(node, "positions", -1);
+    const int64_t dims = rt::GetAttributeIntOrDefault(node, "rotary_dim", 0);
+    if (positions < 0 || dims < 2 || dims % 2 != 0)
+      throw std::invalid_argument("RotaryTables: positions must not be negative, rotary_dim even and at least 2.");
+    const rt::Shape shape(std::vector<int64_t>{positions, dims / 2});
+    rt::Tensor c = ctx.MakeOutputTensor(0, kFloat, shape, ByteSize(kFloat, Count(shape)));
+    rt::Tensor s = ctx.MakeOutputTensor(1, kFloat, shape, ByteSize(kFloat, Count(shape)));
+    onnxl_amd_tensor dc = DescribeOutput(c), ds = DescribeOutput(s);
+    Check(onnxl_amd_rotary_tables(ScalarInput(node, 0, ctx, 10000.f),
+                                  static_cast<int32_t>(rt::GetAttributeIntOrDefault(node, "scaling", 0)),
+                                  ScalarInput(node, 1, ctx, 1.f), rt::GetAttributeIntOrDefault(node, "original_positions", 0),
+                                  ScalarInput(node, 2, ctx, 32.f), ScalarInput(node, 3, ctx, 1.f),
+                                  ScalarInput(node, 4, ctx, 0.f), &dc, &ds, nullptr));
+    rt::SetOutput(node, 0, std::move(c), ctx);
+    rt::SetOutput(node, 1, std::move(s), ctx);
+  }
+};
+
+// ai.rt.amd:RotaryEmbedding(x, cos, sin, position_ids | ""; interleaved = 0,
+// num_heads = 0) = y.
+class Mi355xRotaryEmbedding : public Mi355xKernel {
+public:
+  static constexpr const char *name = "onnxl_amd:CPU:ai.rt.amd:RotaryEmbedding";
+  using Mi355xKernel::Mi355xKernel;
+  void Run(rt::RuntimeContext &ctx) override {
+    const NodeProto &node = *node_;
+    rt::RequireMinInputCount(node, 3);
+    rt::RequireOutputCount(node, 1);
+    const onnxl_amd_tensor x = In(0, ctx), cos = In(1, ctx), sin = In(2, ctx), ids = In(3, ctx);
+    if (x.rank < 1) throw std::invalid_argument("RotaryEmbedding: x has no dimensions.");
+    const rt::Shape shape = ShapeOf(x.dims, x.rank);
+    rt::Tensor y = ctx.MakeOutputTensor(0, x.data_type, shape, ByteSize(x.data_type, Count(shape)));
+    onnxl_amd_tensor dy = DescribeOutput(y);
+    Check(onnxl_amd_rotary_embedding(&x, &cos, &sin, &ids,
+                                     static_cast<int32_t>(rt::GetAttributeIntOrDefault(node, "interleaved", 0)),
+                                     rt::GetAttributeIntOrDefault(node, "num_heads", 0), &dy, nullptr));
+    rt::SetOutput(node, 0, std::move(y), ctx);
+  }
+
+protected:
+  std::vector<int> ConstantInputs() const override { return {1, 2}; }
+};
+
+// ai.rt.amd:RotaryKvCacheAppend(qkv, cos, sin, position_ids | "", k_cache, v_cache,
+// k_scale, v_scale, block_table, query_start, lengths; interleaved = 0) = q, the four
+// cache tensors with the new tokens.  Rows of q of no sequence are zeros.
+class Mi355xRotaryKvCacheAppend : public Mi355xKernel {
+public:
+  static constexpr const char *name = "onnxl_amd:CPU:ai.rt.amd:RotaryKvCacheAppend";
+  using Mi355xKernel::Mi355xKernel;
+  void Run(rt::RuntimeContext &ctx) override {
+    const NodeProto &node = *node_;
+    rt::RequireInputCount(node, 11);
+    rt::RequireOutputCount(node, 5);
+    const onnxl_amd_tensor qkv = In(0, ctx), cos = In(1, ctx), sin = In(2, ctx), ids = In(3, ctx), table = In(8, ctx),
+                           start = In(9, ctx), lengths = In(10, ctx);
+    CacheCopy c(node, 4, ctx);
+    const onnxl_amd_tensor &k = c.t[0]->desc;
+    if (qkv.rank != 3 || k.rank != 4 || qkv.dims[1] <= 2 * k.dims[1])
+      throw std::invalid_argument("RotaryKvCacheAppend: qkv must be [tokens, heads + 2 kv_heads, head_dim].");
+    const rt::Shape shape(std::vector<int64_t>{qkv.dims[0], qkv.dims[1] - 2 * k.dims[1], qkv.dims[2]});
+    rt::Tensor q = ctx.MakeOutputTensor(0, qkv.data_type, shape, ByteSize(qkv.data_type, Count(shape)));
+    if (q.size_bytes() > 0) std::memset(q.mutable_bytes(), 0, q.size_bytes());
+    std::shared_ptr<DeviceTensor> dq = UploadToHbm(q);
+    Check(onnxl_amd_rotary_kv_cache_append(&qkv, &cos, &sin, &ids,
+                                           static_cast<int32_t>(rt::GetAttributeIntOrDefault(node, "interleaved", 0)),
+                                           &dq->desc, &c.t[0]->desc, &c.t[1]->desc, &c.t[2]->desc, &c.t[3]->desc, &table,
+                                           &start, &lengths, nullptr));
+    Check(onnxl_amd_synchronize(nullptr));
+    if (q.size_bytes() > 0)
+      CheckHip(hipMemcpy(q.mutable_bytes(), dq->desc.data, q.size_bytes(), hipMemcpyDeviceToHost), "hipMemcpy");
+    rt::SetOutput(node, 0, std::move(q), ctx);
+    for (int i = 0; i < 4; ++i) {
+      const onnxl_amd_tensor &d = c.t[i]->desc;
+      rt::Tensor out = ctx.MakeOutputTensor(i + 1, d.data_type, ShapeOf(d.dims, d.rank), static_cast<size_t>(d.size_bytes));
+      if (d.size_bytes > 0)
+        CheckHip(hipMemcpy(out.mutable_bytes(), d.data, static_cast<size_t>(d.size_bytes), hipMemcpyDeviceToHost),
+                 "hipMemcpy");
+      rt::SetOutput(node, i + 1, std::move(out), ctx);
+    }
+  }
+
+protected:
+  std::vector<int> ConstantInputs() const override { return {1, 2}; }
+};
+
+// ai.rt.amd:SampleTokens(logits, uniform, temperature | "", top_k | "", top_p | "",
+// min_p | "") = token (INT64)[, probability].
+class Mi355xSampleTokens : public Mi355xKernel {
+public:
+  static constexpr const char *name = "onnxl_amd:CPU:ai.rt.amd:SampleTokens";
+  using Mi355xKernel::Mi355xKernel;
+  void Run(rt::RuntimeContext &ctx) override {
+    const NodeProto &node = *node_;
+    rt::RequireMinInputCount(node, 2);
+    const onnxl_amd_tensor x = In(0, ctx), u = In(1, ctx), t = In(2, ctx), k = In(3, ctx), p = In(4, ctx), m = In(5, ctx);
+    if (x.rank != 2) throw std::invalid_argument("SampleTokens: logits must be [rows, vocabulary].");
+    const rt::Shape shape(std::vector<int64_t>{x.dims[0]});
+    const bool wants = node.output_size() > 1 && !node.output(1).empty();
+    rt::Tensor token = ctx.MakeOutputTensor(0, kInt64, shape, ByteSize(kInt64, x.dims[0])), prob;
+    onnxl_amd_tensor dt = DescribeOutput(token), dp = Absent();
+    if (wants) {
+      prob = ctx.MakeOutputTensor(1, kFloat, shape, ByteSize(kFloat, x.dims[0]));
+      dp = DescribeOutput(prob);
+    }
+    Check(onnxl_amd_sample_tokens(&x, &u, &t, &k, &p, &m, &dt, &dp, nullptr));
+    rt::SetOutput(node, 0, std::move(token), ctx);
+    if (wants) rt::SetOutput(node, 1, std::move(prob), ctx);
+  }
+};
+
 std::once_flag g_registered;
 
 }  // namespace mi355x
@@ -1842,6 +2007,11 @@ const char *RegisterMi355xKernelFunctions(int device_ordinal = 0) {
     Register<Mi355xMxMatMul>(kFusedDomain, "MxMatMul");
     Register<Mi355xKvCacheAppend>(kFusedDomain, "KvCacheAppend");
     Register<Mi355xKvCacheAttention>(kFusedDomain, "KvCacheAttention");
+    Register<Mi355xMxGatedMatMul>(kFusedDomain, "MxGatedMatMul");
+    Register<Mi355xRotaryTables>(kFusedDomain, "RotaryTables");
+    Register<Mi355xRotaryEmbedding>(kFusedDomain, "RotaryEmbedding");
+    Register<Mi355xRotaryKvCacheAppend>(kFusedDomain, "RotaryKvCacheAppend");
+    Register<Mi355xSampleTokens>(kFusedDomain, "SampleTokens");
   });
   return onnxl_amd_version();
 }

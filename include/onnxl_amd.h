@@ -709,6 +709,53 @@ int onnxl_amd_mx_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_sca
                         const onnxl_amd_tensor *b, const onnxl_amd_tensor *b_scale, onnxl_amd_tensor *y,
                         void *stream);
 
+/* Gated feed-forward: y = act(a gate^T) * (a up^T), both products as
+ * onnxl_amd_mx_matmul's (a, a_scale and a_type as there), the activation and the
+ * product of the two in fp32.  gate and up [N, K] of one type with their scales
+ * [N, K / 32] of one type.  activation: 0 SiLU, 1 GELU (erf), 2 GELU by tanh, 3 ReLU.
+ * y [.., N] FLOAT16 or BFLOAT16, a's type where a has 16 bits, without y_scale; or
+ * FLOAT8E4M3FN with y_scale FLOAT8E8M0 or UINT8 [.., N / 32], N a multiple of 32: the
+ * MXFP8 that onnxl_amd_mx_quantize makes of the fp32 result, for the product that
+ * takes it back.  Codes, y's among them, must be 16-byte aligned. */
+int onnxl_amd_mx_gated_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type,
+                              const onnxl_amd_tensor *gate, const onnxl_amd_tensor *gate_scale,
+                              const onnxl_amd_tensor *up, const onnxl_amd_tensor *up_scale, int32_t activation,
+                              onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale, void *stream);
+
+/* Tables of rotary positions: cos[p, i] = m cos(p f_i), sin[p, i] = m sin(p f_i) for
+ * p = 0 .. positions - 1, FLOAT, FLOAT16 or BFLOAT16 [positions, d / 2], d the number
+ * of dimensions that turn (rotary_dim).  With f = base^(-2 i / d) and s = factor >= 1,
+ * f_i by `scaling`:
+ *   0 none      f (factor is not looked at)
+ *   1 linear    f / s
+ *   2 ntk       (base s^(d / (d - 2)))^(-2 i / d)
+ *   3 by parts  f k + f / s (1 - k), where k goes from 0 to 1 as a pair's turns in
+ *               original_positions, original_positions f / (2 pi), go from turns_slow
+ *               to turns_fast
+ *   4 yarn      the same with 1 - k going from 0 to 1 along i, from floor(i of
+ *               turns_fast) to ceil(i of turns_slow), these kept in 0 .. d - 1
+ * m = magnitude, or where that is 0: 1, for yarn 0.1 ln s + 1.  Angles are formed in
+ * 64 bits.  original_positions and the turns (32 and 1 are usual) are looked at by
+ * scalings 3 and 4 only. */
+int onnxl_amd_rotary_tables(double base, int32_t scaling, double factor, int64_t original_positions, double turns_fast,
+                            double turns_slow, double magnitude, onnxl_amd_tensor *cos, onnxl_amd_tensor *sin,
+                            void *stream);
+
+/* Rotary positions, as ONNX's RotaryEmbedding: of every head the pairs (a, b) of
+ * dimensions (i, d / 2 + i), or with `interleaved` (2 i, 2 i + 1), i < d / 2, become
+ *   (a cos - b sin, a sin + b cos)
+ * in fp32, rounded once to x's type; the dimensions from d on are copied.  x FLOAT,
+ * FLOAT16 or BFLOAT16: [batch, heads, seq, head_dim]; [batch, seq, num_heads *
+ * head_dim] with num_heads given; or, num_heads 0, [tokens, heads, head_dim].  cos and
+ * sin FLOAT or of x's type: [positions, d / 2] with position_ids INT32 or INT64
+ * [batch, seq] ([tokens]); without position_ids a row for each token, [batch, seq,
+ * d / 2] ([tokens, d / 2]).  y of x's type and shape, x's own buffer if wanted.
+ * position_ids in host memory are checked; the rotated dimensions of a token whose
+ * position on the device is outside the tables are NaN. */
+int onnxl_amd_rotary_embedding(const onnxl_amd_tensor *x, const onnxl_amd_tensor *cos, const onnxl_amd_tensor *sin,
+                               const onnxl_amd_tensor *position_ids, int32_t interleaved, int64_t num_heads,
+                               onnxl_amd_tensor *y, void *stream);
+
 /* A paged key / value cache in 8 bits with one scale for each block of tokens
  * and head:
  *   k_cache INT8 or FLOAT8E4M3FN [blocks, kv_heads, block_tokens, head_dim],
@@ -742,6 +789,24 @@ int onnxl_amd_kv_cache_append(const onnxl_amd_tensor *k, const onnxl_amd_tensor 
                               const onnxl_amd_tensor *block_table, const onnxl_amd_tensor *query_start,
                               const onnxl_amd_tensor *lengths, void *stream);
 
+/* The append of a joint projection's rows with rotary positions: qkv FLOAT16 or
+ * BFLOAT16 [tokens, heads + 2 kv_heads, head_dim], of every token the queries, then
+ * the keys, then the values.  Queries are rotated as onnxl_amd_rotary_embedding does
+ * into q [tokens, heads, head_dim] (device memory, as the cache); keys are rotated in
+ * fp32 and, unrounded between, appended, values appended as onnxl_amd_kv_cache_append
+ * does.  cos and sin FLOAT or of qkv's type [positions, d / 2], d a multiple of 16.  A
+ * token's position is its place in its sequence, length - new tokens + i, or that of
+ * position_ids INT32 or INT64 [tokens].  Positions in host memory are checked against
+ * the tables; on the device, one outside them makes the token's rotated queries NaN, and
+ * its key a value that is not finite.  Rows of q of no sequence, or of one whose numbers
+ * do not fit, are left alone. */
+int onnxl_amd_rotary_kv_cache_append(const onnxl_amd_tensor *qkv, const onnxl_amd_tensor *cos,
+                                     const onnxl_amd_tensor *sin, const onnxl_amd_tensor *position_ids,
+                                     int32_t interleaved, onnxl_amd_tensor *q, onnxl_amd_tensor *k_cache,
+                                     onnxl_amd_tensor *v_cache, onnxl_amd_tensor *k_scale, onnxl_amd_tensor *v_scale,
+                                     const onnxl_amd_tensor *block_table, const onnxl_amd_tensor *query_start,
+                                     const onnxl_amd_tensor *lengths, void *stream);
+
 /* Attention of the new tokens over the cache (which holds them already):
  * q and out FLOAT16 or BFLOAT16 [tokens, heads, head_dim], heads a multiple of
  * kv_heads (consecutive heads share one).  The new token i of n of a sequence
@@ -761,6 +826,28 @@ int onnxl_amd_kv_cache_attention(const onnxl_amd_tensor *q, const onnxl_amd_tens
                                  const onnxl_amd_tensor *v_scale, const onnxl_amd_tensor *block_table,
                                  const onnxl_amd_tensor *query_start, const onnxl_amd_tensor *lengths, float scale,
                                  int64_t max_query, onnxl_amd_tensor *out, void *stream);
+
+/* A token from each row of logits FLOAT, FLOAT16 or BFLOAT16 [rows, vocabulary]
+ * (vocabulary below 2^21) and a given random number, uniform FLOAT [rows] in [0, 1).
+ * The tokens of a row in order, larger logits first and the lower index first among
+ * equal ones, weigh w = exp((logit - largest) / temperature).  Kept are the first
+ * top_k; of those the ones before which the weights add up to less than top_p of
+ * their sum; of those the ones with w >= min_p.  The token is the first, in order of
+ * index, at which the kept weights add up to more than uniform times their sum.
+ * temperature, top_p, min_p FLOAT [rows], top_k INT32 or INT64 [rows]; each may be
+ * absent, or switched off in a row: top_k by 0 or less, top_p by 1 or more, min_p by 0
+ * or less (NaN switches off too).  At least the first token is kept.  A temperature
+ * that is not above 0 takes the first token of the order.  Logits of -inf and NaN are
+ * never taken; equal +inf share all the weight.  token INT32 or INT64 [rows], -1 where
+ * a row has no other logits; probability (optional) FLOAT [rows], the token's weight
+ * over the sum of the kept ones (1 at temperature 0, 0 with token -1).  A uniform below
+ * 0 or NaN counts as 0, of 1 or more as the number before 1.
+ * Weights are rounded to whole multiples of 2^-42 of the largest, and their sums
+ * exact: a border may fall to the other token only where it is that near. */
+int onnxl_amd_sample_tokens(const onnxl_amd_tensor *logits, const onnxl_amd_tensor *uniform,
+                            const onnxl_amd_tensor *temperature, const onnxl_amd_tensor *top_k,
+                            const onnxl_amd_tensor *top_p, const onnxl_amd_tensor *min_p, onnxl_amd_tensor *token,
+                            onnxl_amd_tensor *probability, void *stream);
 
 /* Waits for all work queued by this library on `stream`. */
 int onnxl_amd_synchronize(void *stream);

@@ -151,6 +151,12 @@ def lib() -> ctypes.CDLL:
         L.onnxl_amd_mx_matmul.argtypes = [TP, TP, I32, TP, TP, TP, ctypes.c_void_p]
         L.onnxl_amd_kv_cache_append.argtypes = [TP] * 9 + [ctypes.c_void_p]
         L.onnxl_amd_kv_cache_attention.argtypes = [TP] * 8 + [F32, I64, TP, ctypes.c_void_p]
+        F64 = ctypes.c_double
+        L.onnxl_amd_mx_gated_matmul.argtypes = [TP, TP, I32, TP, TP, TP, TP, I32, TP, TP, ctypes.c_void_p]
+        L.onnxl_amd_rotary_tables.argtypes = [F64, I32, F64, I64, F64, F64, F64, TP, TP, ctypes.c_void_p]
+        L.onnxl_amd_rotary_embedding.argtypes = [TP, TP, TP, TP, I32, I64, TP, ctypes.c_void_p]
+        L.onnxl_amd_rotary_kv_cache_append.argtypes = [TP, TP, TP, TP, I32] + [TP] * 8 + [ctypes.c_void_p]
+        L.onnxl_amd_sample_tokens.argtypes = [TP] * 8 + [ctypes.c_void_p]
         L.onnxl_amd_synchronize.argtypes = [ctypes.c_void_p]
         _lib = L
     return _lib
@@ -1000,6 +1006,73 @@ def mx_matmul(a, b, b_scale, a_scale=None, a_type: int = FLOAT8E4M3FN, output_dt
     return out
 
 
+ACTIVATIONS = ("silu", "gelu", "gelu_tanh", "relu")
+ROTARY_SCALINGS = ("none", "linear", "ntk", "by_parts", "yarn")
+
+
+def _number_of(name, names: tuple, what: str) -> int:
+    if name not in names:
+        raise InvalidArgument(f"{what} must be one of {', '.join(names)}")
+    return names.index(name)
+
+
+def mx_gated_matmul(a, gate, gate_scale, up, up_scale, activation: str = "silu", a_scale=None,
+                    a_type: int = FLOAT8E4M3FN, output_dtype=None, mx: bool = False, out=None):
+    """act(a @ gate^T) * (a @ up^T) in microscaled types: a, a_scale and a_type as
+    mx_matmul takes them, gate and up packed FLOAT4E2M1 uint8 [N, K / 2] with
+    uint8 E8M0 scales [N, K / 32]; activation "silu", "gelu", "gelu_tanh" or
+    "relu".  Returns y [.., N] in a's type (for codes output_dtype, bfloat16 by
+    default), or with ``mx`` (y, y_scale) as mx_quantize returns MXFP8, for
+    mx_matmul.  ``out`` is what is returned: a tensor, or with ``mx`` a pair."""
+    torch = _torch()
+    act = _number_of(activation, ACTIVATIONS, "activation")
+    if a_scale is not None:
+        a_type = 0
+    if out is None:
+        shape, N, dev = _shape_of(a)[:-1], _shape_of(gate)[0], _device_of(a, gate)
+        if mx:
+            out = (_empty((*shape, N), torch.float8_e4m3fn, dev), _empty((*shape, N // 32), torch.uint8, dev))
+        else:
+            out = _empty((*shape, N), output_dtype or (a.dtype if a_scale is None else torch.bfloat16), dev)
+    y, y_scale = out if mx else (out, None)
+    _check(lib().onnxl_amd_mx_gated_matmul(describe(a), describe(a_scale), a_type, describe(gate), describe(gate_scale),
+                                           describe(up), describe(up_scale), act, describe(y), describe(y_scale),
+                                           _stream_of(a, gate, y)))
+    return out
+
+
+def rotary_tables(positions: int, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                  original_positions: int = 0, turns_fast: float = 32.0, turns_slow: float = 1.0, magnitude: float = 0.0,
+                  dtype=None, out=None):
+    """(cos, sin) [positions, rotary_dim / 2] for rotary_embedding: angles
+    position * base^(-2 i / rotary_dim), for contexts longer than a model was
+    trained on scaled by "linear", "ntk", "by_parts" or "yarn" (onnxl_amd.h
+    has the formulas).  dtype is a torch type, float32 by default."""
+    torch = _torch()
+    how = _number_of(scaling, ROTARY_SCALINGS, "scaling")
+    if out is None:
+        if rotary_dim < 2 or rotary_dim % 2:
+            raise InvalidArgument("rotary_dim must be even and at least 2")
+        dev = torch.device("cuda", torch.cuda.current_device())
+        out = tuple(_empty((positions, rotary_dim // 2), dtype or torch.float32, dev) for _ in range(2))
+    cos, sin = out
+    _check(lib().onnxl_amd_rotary_tables(base, how, factor, original_positions, turns_fast, turns_slow, magnitude,
+                                         describe(cos), describe(sin), _stream_of(cos)))
+    return out
+
+
+def rotary_embedding(x, cos, sin, position_ids=None, interleaved: bool = False, num_heads: int = 0, out=None):
+    """ONNX's RotaryEmbedding: x [batch, heads, seq, head_dim], [batch, seq,
+    num_heads * head_dim] with num_heads, or [tokens, heads, head_dim]; the
+    first 2 * cos.shape[-1] dimensions of a head turn.  cos, sin [positions, ..]
+    with position_ids [batch, seq] or [tokens], else a row for every token."""
+    if out is None:
+        out = _torch().empty_like(x)
+    _check(lib().onnxl_amd_rotary_embedding(describe(x), describe(cos), describe(sin), describe(position_ids),
+                                            int(interleaved), num_heads, describe(out), _stream_of(x, cos, out)))
+    return out
+
+
 class KvCache:
     """A paged 8-bit key / value cache on the device, one scale for each block
     of tokens and head: k_cache [blocks, kv_heads, block_tokens, head_dim],
@@ -1030,6 +1103,27 @@ def kv_cache_append(k, v, cache: KvCache, block_table, query_start, lengths) -> 
     return cache
 
 
+def rotary_kv_cache_append(qkv, cos, sin, cache: KvCache, block_table, query_start, lengths, position_ids=None,
+                           interleaved: bool = False, out=None):
+    """The joint projection's rows qkv [tokens, heads + 2 * kv_heads, head_dim]:
+    keys rotated and values as they are into the cache, as kv_cache_append does;
+    returns the rotated queries [tokens, heads, head_dim], on the GPU.  A token's
+    position is its place in its sequence, or position_ids [tokens]."""
+    torch = _torch()
+    if out is None:
+        tokens, rows, D = _shape_of(qkv)
+        kv_heads = cache.k_cache.shape[1]
+        if rows <= 2 * kv_heads:
+            raise InvalidArgument("qkv has no queries beside the cache's keys and values")
+        out = _empty((tokens, rows - 2 * kv_heads, D), torch.from_numpy(qkv).dtype if isinstance(qkv, np.ndarray) else qkv.dtype,
+                     cache.k_cache.device)
+    _check(lib().onnxl_amd_rotary_kv_cache_append(describe(qkv), describe(cos), describe(sin), describe(position_ids),
+                                                  int(interleaved), describe(out), *(describe(t) for t in cache.tensors()),
+                                                  describe(block_table), describe(query_start), describe(lengths),
+                                                  _stream_of(qkv, cache.k_cache, out)))
+    return out
+
+
 def kv_cache_attention(q, cache: KvCache, block_table, query_start, lengths, scale=None, max_query: int = 0, out=None):
     """Causal attention of the new tokens q [tokens, heads, head_dim] over the
     cache, which holds them already; scale defaults to head_dim ** -0.5,
@@ -1041,6 +1135,24 @@ def kv_cache_attention(q, cache: KvCache, block_table, query_start, lengths, sca
     _check(lib().onnxl_amd_kv_cache_attention(describe(q), *(describe(t) for t in cache.tensors()),
                                               describe(block_table), describe(query_start), describe(lengths), scale,
                                               max_query, describe(out), _stream_of(q, cache.k_cache, out)))
+    return out
+
+
+def sample_tokens(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """(token int64 [rows], probability float32 [rows]) from logits [rows,
+    vocabulary] and random numbers uniform float32 [rows] in [0, 1): the kept
+    tokens of temperature, top_k, top_p and min_p (each a tensor [rows] or None;
+    onnxl_amd.h says what they keep) in order of index, and the one at which
+    their weights pass uniform times their sum.  ``out`` may have None for the
+    probability, and an int32 token."""
+    torch = _torch()
+    if out is None:
+        rows, dev = _shape_of(logits)[0], _device_of(logits, uniform)
+        out = _empty((rows,), torch.int64, dev), _empty((rows,), torch.float32, dev)
+    token, probability = out
+    _check(lib().onnxl_amd_sample_tokens(describe(logits), describe(uniform), describe(temperature), describe(top_k),
+                                         describe(top_p), describe(min_p), describe(token), describe(probability),
+                                         _stream_of(logits, uniform, token)))
     return out
 
 
@@ -1217,6 +1329,54 @@ class KvCacheAttention:
         return kv_cache_attention(q, cache, block_table, query_start, lengths, scale, max_query, out)
 
 
+class MxGatedMatMul:
+    """Gated feed-forward with MXFP4 weights (no reference kernel); attributes
+    activation, a_type, output_dtype and mx."""
+    name = "onnxl_amd:GPU:ai.rt.amd:MxGatedMatMul"
+
+    def __call__(self, a, gate, gate_scale, up, up_scale, a_scale=None, activation="silu", a_type=FLOAT8E4M3FN,
+                 output_dtype=None, mx=False, out=None):
+        return mx_gated_matmul(a, gate, gate_scale, up, up_scale, activation, a_scale, a_type, output_dtype, mx, out)
+
+
+class RotaryTables:
+    """Tables of rotary positions (no reference kernel); attributes as the
+    function's arguments."""
+    name = "onnxl_amd:GPU:ai.rt.amd:RotaryTables"
+
+    def __call__(self, positions, rotary_dim, **attributes):
+        return rotary_tables(positions, rotary_dim, **attributes)
+
+
+class RotaryEmbedding:
+    """ONNX's RotaryEmbedding; attributes interleaved and num_heads
+    (rotary_embedding_dim is the tables')."""
+    name = "onnxl_amd:GPU:ai.rt.amd:RotaryEmbedding"
+
+    def __call__(self, x, cos, sin, position_ids=None, interleaved=False, num_heads=0, out=None):
+        return rotary_embedding(x, cos, sin, position_ids, interleaved, num_heads, out)
+
+
+class RotaryKvCacheAppend:
+    """The joint projection's rows into a paged 8-bit cache, keys and queries
+    rotated (no reference kernel); attribute interleaved."""
+    name = "onnxl_amd:GPU:ai.rt.amd:RotaryKvCacheAppend"
+
+    def __call__(self, qkv, cos, sin, cache, block_table, query_start, lengths, position_ids=None, interleaved=False,
+                 out=None):
+        return rotary_kv_cache_append(qkv, cos, sin, cache, block_table, query_start, lengths, position_ids,
+                                      interleaved, out)
+
+
+class SampleTokens:
+    """A token from each row of logits and given random numbers (no reference
+    kernel)."""
+    name = "onnxl_amd:GPU:ai.rt.amd:SampleTokens"
+
+    def __call__(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+        return sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, out)
+
+
 # Dispatch keys "<domain>:<op_type>" as the reference table uses them
 # (core/runtime/kernels/kernel_dispatch_table.h:148-164).
 KERNELS = {"ai.onnx:MatMulInteger": MatMulInteger, "ai.onnx:QLinearMatMul": QLinearMatMul,
@@ -1231,7 +1391,10 @@ KERNELS = {"ai.onnx:MatMulInteger": MatMulInteger, "ai.onnx:QLinearMatMul": QLin
            "ai.rt.amd:DequantizeLinearGroupedMatMul": DequantizeLinearGroupedMatMul,
            "ai.rt.amd:RmsNormQuantize": RmsNormQuantize, "ai.rt.amd:MxQuantize": MxQuantize,
            "ai.rt.amd:MxMatMul": MxMatMul, "ai.rt.amd:KvCacheAppend": KvCacheAppend,
-           "ai.rt.amd:KvCacheAttention": KvCacheAttention}
+           "ai.rt.amd:KvCacheAttention": KvCacheAttention,
+           "ai.rt.amd:MxGatedMatMul": MxGatedMatMul, "ai.rt.amd:RotaryTables": RotaryTables,
+           "ai.rt.amd:RotaryEmbedding": RotaryEmbedding, "ai.rt.amd:RotaryKvCacheAppend": RotaryKvCacheAppend,
+           "ai.rt.amd:SampleTokens": SampleTokens}
 
 
 class Prepared:

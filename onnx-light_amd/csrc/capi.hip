@@ -3197,6 +3197,11 @@ constexpr const char *kMxqName = "MxQuantize";
 constexpr const char *kMxmName = "MxMatMul";
 constexpr const char *kKvaName = "KvCacheAppend";
 constexpr const char *kKvtName = "KvCacheAttention";
+constexpr const char *kMxgName = "MxGatedMatMul";
+constexpr const char *kRtbName = "RotaryTables";
+constexpr const char *kRotName = "RotaryEmbedding";
+constexpr const char *kRkvName = "RotaryKvCacheAppend";
+constexpr const char *kSmpName = "SampleTokens";
 
 bool Is16Bit(int32_t dt) { return dt == kFloat16 || dt == kBfloat16; }
 bool IsE8M0(int32_t dt) { return dt == kFloat8E8M0 || dt == kUint8; }
@@ -3309,58 +3314,53 @@ int64_t MxLength(const onnxl_amd_tensor *t) {
   return t->dims[t->rank - 1] * (t->data_type == kUint8 ? 2 : 1);
 }
 
-int MxMatMul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type, const onnxl_amd_tensor *b,
-             const onnxl_amd_tensor *b_scale, onnxl_amd_tensor *y, hipStream_t stream) {
-  OLA_ENFORCE(!Absent(a) && !Absent(b) && !Absent(b_scale) && !Absent(y), kMxmName,
-              ": a, b, b_scale and y are required.");
+// The activations a (codes with a_scale, or 16 bits to be quantized to a_type) and
+// the weight b of a product; fills the sizes and types, and returns y's shape.
+Shape PlanMxProduct(const char *op, const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type,
+                    const onnxl_amd_tensor *b, const onnxl_amd_tensor *b_scale, MxMatMulParams &p) {
   CheckDescriptor(a, "a");
   CheckDescriptor(a_scale, "a_scale");
   CheckDescriptor(b, "b");
   CheckDescriptor(b_scale, "b_scale");
-  CheckDescriptor(y, "y");
-  OLA_ENFORCE(b->data_type == kFloat4E2M1 || b->data_type == kUint8, kMxmName,
+  OLA_ENFORCE(b->data_type == kFloat4E2M1 || b->data_type == kUint8, op,
               ": b must be FLOAT4E2M1 [N, K] or its packed UINT8 [N, K / 2].");
-  OLA_ENFORCE(b->rank == 2 && a->rank >= 1, kMxmName, ": b must be 2-D and a at least 1-D.");
+  OLA_ENFORCE(b->rank == 2 && a->rank >= 1, op, ": b must be 2-D and a at least 1-D.");
   const bool quantise = Absent(a_scale);
   Shape as = ShapeOf(*a);
   if (quantise) {
-    OLA_ENFORCE(Is16Bit(a->data_type), kMxmName, ": a without a_scale must be FLOAT16 or BFLOAT16.");
-    OLA_ENFORCE(a_type == kFloat8E4M3FN || a_type == kFloat4E2M1, kMxmName,
+    OLA_ENFORCE(Is16Bit(a->data_type), op, ": a without a_scale must be FLOAT16 or BFLOAT16.");
+    OLA_ENFORCE(a_type == kFloat8E4M3FN || a_type == kFloat4E2M1, op,
                 ": a_type must be FLOAT8E4M3FN or FLOAT4E2M1, the type a is quantized to.");
   } else {
-    OLA_ENFORCE(a->data_type == kFloat8E4M3FN || a->data_type == kFloat4E2M1 || a->data_type == kUint8, kMxmName,
+    OLA_ENFORCE(a->data_type == kFloat8E4M3FN || a->data_type == kFloat4E2M1 || a->data_type == kUint8, op,
                 ": a with a_scale must be FLOAT8E4M3FN, FLOAT4E2M1 or packed UINT8.");
-    OLA_ENFORCE(a_type == 0, kMxmName, ": a_type is for a 16-bit a; a is quantized already.");
-    OLA_ENFORCE(IsE8M0(a_scale->data_type), kMxmName, ": a_scale must be FLOAT8E8M0 or UINT8.");
+    OLA_ENFORCE(a_type == 0, op, ": a_type is for a 16-bit a; a is quantized already.");
+    OLA_ENFORCE(IsE8M0(a_scale->data_type), op, ": a_scale must be FLOAT8E8M0 or UINT8.");
   }
-  OLA_ENFORCE(IsE8M0(b_scale->data_type), kMxmName, ": b_scale must be FLOAT8E8M0 or UINT8.");
-  const int64_t K = MxLength(b), N = b->dims[0];
-  OLA_ENFORCE(K % 32 == 0, kMxmName, ": K must be a multiple of the block size 32.");
-  OLA_ENFORCE((quantise ? as.back() : MxLength(a)) == K, kMxmName, ": a and b have different lengths of K.");
-  NeedShape(b_scale, {N, K / 32}, kMxmName, "b_scale");
+  OLA_ENFORCE(IsE8M0(b_scale->data_type), op, ": b_scale must be FLOAT8E8M0 or UINT8.");
+  p.K = MxLength(b);
+  p.N = b->dims[0];
+  OLA_ENFORCE(p.K % 32 == 0, op, ": K must be a multiple of the block size 32.");
+  OLA_ENFORCE((quantise ? as.back() : MxLength(a)) == p.K, op, ": a and b have different lengths of K.");
+  NeedShape(b_scale, {p.N, p.K / 32}, op, "b_scale");
   Shape s = as;
-  s.back() = K / 32;
-  if (!quantise) NeedShape(a_scale, s, kMxmName, "a_scale");
-  int64_t M = 1;
-  for (size_t i = 0; i + 1 < as.size(); ++i) M *= as[i];
-  s.back() = N;
-  OLA_ENFORCE(Is16Bit(y->data_type) && (!quantise || y->data_type == a->data_type), kMxmName,
-              ": y must be FLOAT16 or BFLOAT16, and a's type where a has 16 bits.");
-  NeedShape(y, s, kMxmName, "y");
-  OLA_ENFORCE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) - 256 && K < (int64_t(1) << 22), kMxmName,
+  s.back() = p.K / 32;
+  if (!quantise) NeedShape(a_scale, s, op, "a_scale");
+  p.M = 1;
+  for (size_t i = 0; i + 1 < as.size(); ++i) p.M *= as[i];
+  OLA_ENFORCE(p.M < (int64_t(1) << 31) && p.N < (int64_t(1) << 31) - 256 && p.K < (int64_t(1) << 22), op,
               ": M of 2^31 or more, N of 2^31 - 256 or more, or K of 2^22 or more.");
-  if (M == 0 || N == 0) return ONNXL_AMD_OK;
-  Ctx();
-  MxMatMulParams p{};
-  p.M = M;
-  p.N = N;
-  p.K = K;
   p.x = quantise ? a->data : nullptr;
   p.x_dtype = a->data_type;
   p.a_fp4 = quantise ? a_type == kFloat4E2M1 : a->data_type != kFloat8E4M3FN;
-  p.y_bf16 = y->data_type == kBfloat16;
-  Staging st(stream, MxMatMulScratchBytes(p), {a, quantise ? nullptr : a_scale, b, b_scale}, {y});
-  if (quantise) {
+  s.back() = p.N;
+  return s;
+}
+
+// The device addresses of a product's operands.
+void TakeMxOperands(const char *op, const Staging &st, const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale,
+                    const onnxl_amd_tensor *b, const onnxl_amd_tensor *b_scale, MxMatMulParams &p) {
+  if (Absent(a_scale)) {
     p.x = st.In(a);
   } else {
     p.a = static_cast<const uint8_t *>(st.In(a));
@@ -3368,9 +3368,76 @@ int MxMatMul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t
   }
   p.b = static_cast<const uint8_t *>(st.In(b));
   p.b_scale = static_cast<const uint8_t *>(st.In(b_scale));
-  p.y = st.Out(y);
-  OLA_ENFORCE(reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0, kMxmName,
+  OLA_ENFORCE(reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0, op,
               ": the codes must be 16-byte aligned.");
+}
+
+int MxMatMul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type, const onnxl_amd_tensor *b,
+             const onnxl_amd_tensor *b_scale, onnxl_amd_tensor *y, hipStream_t stream) {
+  OLA_ENFORCE(!Absent(a) && !Absent(b) && !Absent(b_scale) && !Absent(y), kMxmName,
+              ": a, b, b_scale and y are required.");
+  MxMatMulParams p{};
+  const Shape want = PlanMxProduct(kMxmName, a, a_scale, a_type, b, b_scale, p);
+  CheckDescriptor(y, "y");
+  OLA_ENFORCE(Is16Bit(y->data_type) && (!Absent(a_scale) || y->data_type == a->data_type), kMxmName,
+              ": y must be FLOAT16 or BFLOAT16, and a's type where a has 16 bits.");
+  NeedShape(y, want, kMxmName, "y");
+  if (p.M == 0 || p.N == 0) return ONNXL_AMD_OK;
+  Ctx();
+  p.y_bf16 = y->data_type == kBfloat16;
+  Staging st(stream, MxMatMulScratchBytes(p), {a, Absent(a_scale) ? nullptr : a_scale, b, b_scale}, {y});
+  TakeMxOperands(kMxmName, st, a, a_scale, b, b_scale, p);
+  p.y = st.Out(y);
+  LaunchMxMatMul(p, st.Extra(), stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+int MxGatedMatMul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type,
+                  const onnxl_amd_tensor *gate, const onnxl_amd_tensor *gate_scale, const onnxl_amd_tensor *up,
+                  const onnxl_amd_tensor *up_scale, int32_t activation, onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale,
+                  hipStream_t stream) {
+  OLA_ENFORCE(!Absent(a) && !Absent(gate) && !Absent(gate_scale) && !Absent(up) && !Absent(up_scale) && !Absent(y),
+              kMxgName, ": a, gate, gate_scale, up, up_scale and y are required.");
+  MxMatMulParams p{};
+  Shape want = PlanMxProduct(kMxgName, a, a_scale, a_type, gate, gate_scale, p);
+  CheckDescriptor(up, "up");
+  CheckDescriptor(up_scale, "up_scale");
+  CheckDescriptor(y, "y");
+  CheckDescriptor(y_scale, "y_scale");
+  OLA_ENFORCE(up->data_type == gate->data_type && up_scale->data_type == gate_scale->data_type, kMxgName,
+              ": up and up_scale must have gate's and gate_scale's types.");
+  NeedShape(up, ShapeOf(*gate), kMxgName, "up (gate's)");
+  NeedShape(up_scale, ShapeOf(*gate_scale), kMxgName, "up_scale (gate_scale's)");
+  OLA_ENFORCE(activation >= kSilu && activation <= kRelu, kMxgName, ": activation must be 0 (SiLU) to 3 (ReLU).");
+  OLA_ENFORCE(p.N < (int64_t(1) << 30) - 256, kMxgName, ": N of 2^30 - 256 or more.");
+  const bool mx = !Absent(y_scale);
+  if (mx) {
+    OLA_ENFORCE(y->data_type == kFloat8E4M3FN && IsE8M0(y_scale->data_type), kMxgName,
+                ": y with y_scale must be FLOAT8E4M3FN, y_scale FLOAT8E8M0 or UINT8.");
+    OLA_ENFORCE(p.N % 32 == 0, kMxgName, ": N must be a multiple of the block size 32 of y_scale.");
+  } else {
+    OLA_ENFORCE(Is16Bit(y->data_type) && (!Absent(a_scale) || y->data_type == a->data_type), kMxgName,
+                ": y without y_scale must be FLOAT16 or BFLOAT16, and a's type where a has 16 bits.");
+  }
+  NeedShape(y, want, kMxgName, "y");
+  want.back() = p.N / 32;
+  if (mx) NeedShape(y_scale, want, kMxgName, "y_scale");
+  if (p.M == 0 || p.N == 0) return ONNXL_AMD_OK;
+  Ctx();
+  p.y_bf16 = y->data_type == kBfloat16;
+  p.activation = activation;
+  p.output = mx ? kGatedMx : kGated;
+  Staging st(stream, MxMatMulScratchBytes(p), {a, Absent(a_scale) ? nullptr : a_scale, gate, gate_scale, up, up_scale},
+             {y, mx ? y_scale : nullptr});
+  TakeMxOperands(kMxgName, st, a, a_scale, gate, gate_scale, p);
+  p.up = static_cast<const uint8_t *>(st.In(up));
+  p.up_scale = static_cast<const uint8_t *>(st.In(up_scale));
+  p.y = st.Out(y);
+  p.y_scale = mx ? static_cast<uint8_t *>(st.Out(y_scale)) : nullptr;
+  OLA_ENFORCE(reinterpret_cast<uintptr_t>(p.up) % 16 == 0 && (!mx || reinterpret_cast<uintptr_t>(p.y) % 16 == 0),
+              kMxgName, ": the codes must be 16-byte aligned.");
   LaunchMxMatMul(p, st.Extra(), stream);
   OLA_HIP(hipGetLastError());
   st.Finish();
@@ -3479,6 +3546,238 @@ int KvCacheAppend(const onnxl_amd_tensor *k, const onnxl_amd_tensor *v, onnxl_am
   p.v = st.In(v);
   p.bf16 = k->data_type == kBfloat16;
   LaunchKvCacheAppend(p, stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+int RotaryTables(double base, int32_t scaling, double factor, int64_t original, double turns_fast, double turns_slow,
+                 double magnitude, onnxl_amd_tensor *cos, onnxl_amd_tensor *sin, hipStream_t stream) {
+  OLA_ENFORCE(!Absent(cos) && !Absent(sin), kRtbName, ": cos and sin are required.");
+  CheckDescriptor(cos, "cos");
+  CheckDescriptor(sin, "sin");
+  OLA_ENFORCE((cos->data_type == kFloat || Is16Bit(cos->data_type)) && sin->data_type == cos->data_type, kRtbName,
+              ": cos and sin must be FLOAT, FLOAT16 or BFLOAT16, both the same.");
+  OLA_ENFORCE(cos->rank == 2, kRtbName, ": cos must be [positions, rotary_dim / 2].");
+  NeedShape(sin, ShapeOf(*cos), kRtbName, "sin (cos's)");
+  const int64_t P = cos->dims[0], half = cos->dims[1];
+  OLA_ENFORCE(half >= 1 && half < 32768 && P < (int64_t(1) << 31), kRtbName,
+              ": rotary_dim / 2 must be from 1 to 32767, positions below 2^31.");
+  OLA_ENFORCE(std::isfinite(base) && base > 1.0, kRtbName, ": base must be finite and above 1.");
+  OLA_ENFORCE(scaling >= kRotaryNone && scaling <= kRotaryYarn, kRtbName, ": scaling must be 0 (none) to 4 (yarn).");
+  OLA_ENFORCE(std::isfinite(factor) && factor >= 1.0, kRtbName, ": factor must be finite and at least 1.");
+  OLA_ENFORCE(scaling != kRotaryNtk || half > 1, kRtbName, ": ntk scaling needs a rotary_dim above 2.");
+  if (scaling == kRotaryByParts || scaling == kRotaryYarn) {
+    OLA_ENFORCE(original > 0, kRtbName, ": original_positions must be above 0.");
+    OLA_ENFORCE(turns_slow > 0.0 && turns_slow < turns_fast && std::isfinite(turns_fast), kRtbName,
+                ": the slow number of turns must be above 0 and below the fast one.");
+  }
+  OLA_ENFORCE(std::isfinite(magnitude) && magnitude >= 0.0, kRtbName, ": magnitude must be finite and not negative.");
+  if (P == 0) return ONNXL_AMD_OK;
+  Ctx();
+  if (magnitude == 0.0) magnitude = scaling == kRotaryYarn ? 0.1 * std::log(factor) + 1.0 : 1.0;
+  Staging st(stream, 0, {}, {cos, sin});
+  LaunchRotaryTables(RotaryTablesParams{st.Out(cos), st.Out(sin), P, (int)half, cos->data_type, scaling, base,
+                                        scaling == kRotaryNone ? 1.0 : factor, (double)original, turns_fast, turns_slow,
+                                        magnitude},
+                     stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+// The tables that rotate x, for one row of them a token or by position ids.
+RotaryTable PlanRotary(const char *op, const onnxl_amd_tensor *x, const onnxl_amd_tensor *cos,
+                       const onnxl_amd_tensor *sin, const onnxl_amd_tensor *ids, int32_t interleaved, int64_t D) {
+  CheckDescriptor(cos, "cos");
+  CheckDescriptor(sin, "sin");
+  CheckDescriptor(ids, "position_ids");
+  OLA_ENFORCE((cos->data_type == kFloat || cos->data_type == x->data_type) && sin->data_type == cos->data_type, op,
+              ": cos and sin must be FLOAT or of x's type, both the same.");
+  OLA_ENFORCE(cos->rank >= 2, op, ": cos must be [positions, rotary_dim / 2].");
+  NeedShape(sin, ShapeOf(*cos), op, "sin (cos's)");
+  const int64_t half = cos->dims[cos->rank - 1];
+  OLA_ENFORCE(half >= 1 && 2 * half <= D, op, ": rotary_dim, twice the tables' last dimension, must be from 2 to head_dim.");
+  OLA_ENFORCE(interleaved == 0 || interleaved == 1, op, ": interleaved must be 0 or 1.");
+  RotaryTable t{};
+  t.half = (int)half;
+  t.positions = NumElements(*cos) / half;
+  t.f32 = cos->data_type == kFloat;
+  t.interleaved = interleaved;
+  if (!Absent(ids)) {
+    OLA_ENFORCE(ids->data_type == kInt32 || ids->data_type == kInt64, op, ": position_ids must be INT32 or INT64.");
+    t.ids64 = ids->data_type == kInt64;
+    if (ids->location == ONNXL_AMD_HOST) {
+      for (int64_t i = 0, n = NumElements(*ids); i < n; ++i) {
+        const int64_t at = t.ids64 ? static_cast<const int64_t *>(ids->data)[i] : static_cast<const int32_t *>(ids->data)[i];
+        OLA_ENFORCE(at >= 0 && at < t.positions, op, ": a position of position_ids is outside the tables.");
+      }
+    }
+  }
+  return t;
+}
+
+int RotaryEmbedding(const onnxl_amd_tensor *x, const onnxl_amd_tensor *cos, const onnxl_amd_tensor *sin,
+                    const onnxl_amd_tensor *ids, int32_t interleaved, int64_t num_heads, onnxl_amd_tensor *y,
+                    hipStream_t stream) {
+  OLA_ENFORCE(!Absent(x) && !Absent(cos) && !Absent(sin) && !Absent(y), kRotName, ": x, cos, sin and y are required.");
+  CheckDescriptor(x, "x");
+  CheckDescriptor(y, "y");
+  OLA_ENFORCE(x->data_type == kFloat || Is16Bit(x->data_type), kRotName, ": x must be FLOAT, FLOAT16 or BFLOAT16.");
+  OLA_ENFORCE(y->data_type == x->data_type, kRotName, ": y must have x's type.");
+  const Shape xs = ShapeOf(*x);
+  OLA_ENFORCE(xs.size() == 3 || xs.size() == 4, kRotName,
+              ": x must be [batch, heads, seq, head_dim], [batch, seq, heads * head_dim] or [tokens, heads, head_dim].");
+  OLA_ENFORCE(num_heads >= 0, kRotName, ": num_heads must not be negative.");
+  RotaryParams p{};
+  const bool joint = xs.size() == 3 && num_heads > 0;
+  p.by_head = xs.size() == 4;
+  int64_t B = 1, H, D;
+  if (p.by_head) {
+    B = xs[0], H = xs[1], p.seq = xs[2], D = xs[3];
+    OLA_ENFORCE(num_heads == 0 || num_heads == H, kRotName, ": num_heads is not x's number of heads.");
+  } else if (joint) {
+    OLA_ENFORCE(xs[2] % num_heads == 0, kRotName, ": num_heads must divide x's last dimension.");
+    B = xs[0], p.seq = xs[1], H = num_heads, D = xs[2] / num_heads;
+  } else {
+    p.seq = xs[0], H = xs[1], D = xs[2];
+  }
+  OLA_ENFORCE(D >= 2 && D < (int64_t(1) << 24) && H < (int64_t(1) << 24), kRotName,
+              ": head_dim must be from 2, and it and the heads below 2^24.");
+  p.t = PlanRotary(kRotName, x, cos, sin, ids, interleaved, D);
+  const Shape per_token = p.by_head || joint ? Shape{B, p.seq} : Shape{p.seq};
+  if (Absent(ids)) {
+    Shape s = per_token;
+    s.push_back(p.t.half);
+    NeedShape(cos, s, kRotName, "cos without position_ids ([batch, seq] or [tokens], rotary_dim / 2)");
+  } else {
+    OLA_ENFORCE(cos->rank == 2, kRotName, ": cos with position_ids must be [positions, rotary_dim / 2].");
+    NeedShape(ids, per_token, kRotName, "position_ids ([batch, seq] or [tokens])");
+  }
+  NeedShape(y, xs, kRotName, "y");
+  p.tokens = B * p.seq;
+  p.heads = (int)H;
+  p.D = (int)D;
+  p.dtype = x->data_type;
+  if (p.tokens == 0 || H == 0) return ONNXL_AMD_OK;
+  Ctx();
+  const onnxl_amd_tensor *on = Absent(ids) ? nullptr : ids;
+  Staging st(stream, 0, {x, cos, sin, on}, {y});
+  p.t.cos = st.In(cos);
+  p.t.sin = st.In(sin);
+  p.t.ids = st.In(on);
+  p.x = st.In(x);
+  p.y = st.Out(y);
+  LaunchRotaryEmbedding(p, stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+int RotaryKvCacheAppend(const onnxl_amd_tensor *qkv, const onnxl_amd_tensor *cos, const onnxl_amd_tensor *sin,
+                        const onnxl_amd_tensor *ids, int32_t interleaved, onnxl_amd_tensor *q,
+                        onnxl_amd_tensor *k_cache, onnxl_amd_tensor *v_cache, onnxl_amd_tensor *k_scale,
+                        onnxl_amd_tensor *v_scale, const onnxl_amd_tensor *table, const onnxl_amd_tensor *start,
+                        const onnxl_amd_tensor *lengths, hipStream_t stream) {
+  OLA_ENFORCE(!Absent(qkv) && !Absent(cos) && !Absent(sin) && !Absent(q), kRkvName, ": qkv, cos, sin and q are required.");
+  CheckDescriptor(qkv, "qkv");
+  CheckDescriptor(q, "q");
+  OLA_ENFORCE(qkv->rank == 3 && q->rank == 3, kRkvName,
+              ": qkv must be [tokens, heads + 2 kv_heads, head_dim], q [tokens, heads, head_dim].");
+  RotaryAppendParams p{};
+  p.a.c = PlanKvCache(kRkvName, k_cache, v_cache, k_scale, v_scale, table, start, lengths, qkv->dims[0]);
+  const KvCacheParams &c = p.a.c;
+  OLA_ENFORCE(Is16Bit(qkv->data_type) && q->data_type == qkv->data_type, kRkvName,
+              ": qkv and q must be FLOAT16 or BFLOAT16, both the same.");
+  const int64_t heads = q->dims[1];
+  OLA_ENFORCE(heads > 0 && heads < 65536 && heads % c.kv_heads == 0, kRkvName,
+              ": heads must be a multiple of the cache's kv_heads, up to 65535.");
+  NeedShape(qkv, {c.tokens, heads + 2 * (int64_t)c.kv_heads, c.head_dim}, kRkvName,
+            "qkv ([tokens, heads + 2 kv_heads, head_dim])");
+  NeedShape(q, {c.tokens, heads, c.head_dim}, kRkvName, "q ([tokens, heads, head_dim])");
+  OLA_ENFORCE(q->location == ONNXL_AMD_DEVICE, kRkvName, ": q must be device memory, as the cache.");
+  p.t = PlanRotary(kRkvName, qkv, cos, sin, ids, interleaved, c.head_dim);
+  OLA_ENFORCE(cos->rank == 2, kRkvName, ": cos must be [positions, rotary_dim / 2].");
+  OLA_ENFORCE(p.t.half % 8 == 0, kRkvName, ": rotary_dim must be a multiple of 16.");
+  if (!Absent(ids)) NeedShape(ids, {c.tokens}, kRkvName, "position_ids ([tokens])");
+  const int32_t *held = lengths->location == ONNXL_AMD_HOST && Absent(ids) ? static_cast<const int32_t *>(lengths->data) : nullptr;
+  for (int b = 0; held && b < c.batch; ++b)
+    OLA_ENFORCE(held[b] <= p.t.positions, kRkvName, ": a sequence of lengths is longer than the tables.");
+  if (c.tokens == 0 || c.batch == 0) return ONNXL_AMD_OK;
+  Ctx();
+  const onnxl_amd_tensor *on = Absent(ids) ? nullptr : ids;
+  Staging st(stream, 0, {qkv, cos, sin, on, table, start, lengths}, {});
+  p.a.c.table = static_cast<const int32_t *>(st.In(table));
+  p.a.c.start = static_cast<const int32_t *>(st.In(start));
+  p.a.c.lengths = static_cast<const int32_t *>(st.In(lengths));
+  p.a.k = st.In(qkv);
+  p.a.bf16 = qkv->data_type == kBfloat16;
+  p.t.cos = st.In(cos);
+  p.t.sin = st.In(sin);
+  p.t.ids = st.In(on);
+  p.q = q->data;
+  p.heads = (int)heads;
+  LaunchRotaryKvCacheAppend(p, stream);
+  OLA_HIP(hipGetLastError());
+  st.Finish();
+  return ONNXL_AMD_OK;
+}
+
+int SampleTokens(const onnxl_amd_tensor *x, const onnxl_amd_tensor *uniform, const onnxl_amd_tensor *temperature,
+                 const onnxl_amd_tensor *top_k, const onnxl_amd_tensor *top_p, const onnxl_amd_tensor *min_p,
+                 onnxl_amd_tensor *token, onnxl_amd_tensor *probability, hipStream_t stream) {
+  OLA_ENFORCE(!Absent(x) && !Absent(uniform) && !Absent(token), kSmpName, ": logits, uniform and token are required.");
+  CheckDescriptor(x, "logits");
+  CheckDescriptor(uniform, "uniform");
+  CheckDescriptor(temperature, "temperature");
+  CheckDescriptor(top_k, "top_k");
+  CheckDescriptor(top_p, "top_p");
+  CheckDescriptor(min_p, "min_p");
+  CheckDescriptor(token, "token");
+  CheckDescriptor(probability, "probability");
+  OLA_ENFORCE(x->data_type == kFloat || Is16Bit(x->data_type), kSmpName, ": logits must be FLOAT, FLOAT16 or BFLOAT16.");
+  OLA_ENFORCE(x->rank == 2, kSmpName, ": logits must be [rows, vocabulary].");
+  const int64_t rows = x->dims[0], vocab = x->dims[1];
+  OLA_ENFORCE(vocab >= 1 && vocab < (int64_t(1) << 21) && rows < (int64_t(1) << 31), kSmpName,
+              ": the vocabulary must be from 1 to 2^21 - 1, rows below 2^31.");
+  for (const onnxl_amd_tensor *t : {uniform, temperature, top_p, min_p}) {
+    if (Absent(t)) continue;
+    OLA_ENFORCE(t->data_type == kFloat, kSmpName, ": uniform, temperature, top_p and min_p must be FLOAT.");
+    NeedShape(t, {rows}, kSmpName, "uniform, temperature, top_p or min_p ([rows])");
+  }
+  auto whole = [&](const onnxl_amd_tensor *t, const char *what) {
+    OLA_ENFORCE(t->data_type == kInt32 || t->data_type == kInt64, kSmpName, ": ", what, " must be INT32 or INT64.");
+    NeedShape(t, {rows}, kSmpName, what);
+  };
+  if (!Absent(top_k)) whole(top_k, "top_k");
+  whole(token, "token");
+  if (!Absent(probability)) {
+    OLA_ENFORCE(probability->data_type == kFloat, kSmpName, ": probability must be FLOAT.");
+    NeedShape(probability, {rows}, kSmpName, "probability ([rows])");
+  }
+  if (rows == 0) return ONNXL_AMD_OK;
+  Ctx();
+  auto there = [](const onnxl_amd_tensor *t) { return Absent(t) ? nullptr : t; };
+  SampleParams p{};
+  p.rows = rows;
+  p.vocab = (int)vocab;
+  p.dtype = x->data_type;
+  p.k64 = !Absent(top_k) && top_k->data_type == kInt64;
+  p.token64 = token->data_type == kInt64;
+  p.top_k = there(top_k) ? top_k->data : nullptr;
+  p.top_p = static_cast<const float *>(there(top_p) ? top_p->data : nullptr);
+  onnxl_amd_tensor *prob = Absent(probability) ? nullptr : probability;
+  Staging st(stream, SampleScratchBytes(p), {x, uniform, there(temperature), there(top_k), there(top_p), there(min_p)},
+             {token, prob});
+  p.x = st.In(x);
+  p.uniform = static_cast<const float *>(st.In(uniform));
+  p.temperature = static_cast<const float *>(st.In(there(temperature)));
+  p.top_k = st.In(there(top_k));
+  p.top_p = static_cast<const float *>(st.In(there(top_p)));
+  p.min_p = static_cast<const float *>(st.In(there(min_p)));
+  p.token = st.Out(token);
+  p.probability = static_cast<float *>(st.Out(prob));
+  LaunchSampleTokens(p, st.Extra(), stream);
   OLA_HIP(hipGetLastError());
   st.Finish();
   return ONNXL_AMD_OK;
@@ -4059,6 +4358,55 @@ int onnxl_amd_mx_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_sca
                         const onnxl_amd_tensor *b, const onnxl_amd_tensor *b_scale, onnxl_amd_tensor *y,
                         void *stream) {
   return Guard([&] { return MxMatMul(a, a_scale, a_type, b, b_scale, y, static_cast<hipStream_t>(stream)); });
+}
+
+int onnxl_amd_mx_gated_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type,
+                              const onnxl_amd_tensor *gate, const onnxl_amd_tensor *gate_scale,
+                              const onnxl_amd_tensor *up, const onnxl_amd_tensor *up_scale, int32_t activation,
+                              onnxl_amd_tensor *y, onnxl_amd_tensor *y_scale, void *stream) {
+  return Guard([&] {
+    return MxGatedMatMul(a, a_scale, a_type, gate, gate_scale, up, up_scale, activation, y, y_scale,
+                         static_cast<hipStream_t>(stream));
+  });
+}
+
+int onnxl_amd_rotary_tables(double base, int32_t scaling, double factor, int64_t original_positions, double turns_fast,
+                            double turns_slow, double magnitude, onnxl_amd_tensor *cos, onnxl_amd_tensor *sin,
+                            void *stream) {
+  return Guard([&] {
+    return RotaryTables(base, scaling, factor, original_positions, turns_fast, turns_slow, magnitude, cos, sin,
+                        static_cast<hipStream_t>(stream));
+  });
+}
+
+int onnxl_amd_rotary_embedding(const onnxl_amd_tensor *x, const onnxl_amd_tensor *cos, const onnxl_amd_tensor *sin,
+                               const onnxl_amd_tensor *position_ids, int32_t interleaved, int64_t num_heads,
+                               onnxl_amd_tensor *y, void *stream) {
+  return Guard([&] {
+    return RotaryEmbedding(x, cos, sin, position_ids, interleaved, num_heads, y, static_cast<hipStream_t>(stream));
+  });
+}
+
+int onnxl_amd_rotary_kv_cache_append(const onnxl_amd_tensor *qkv, const onnxl_amd_tensor *cos,
+                                     const onnxl_amd_tensor *sin, const onnxl_amd_tensor *position_ids,
+                                     int32_t interleaved, onnxl_amd_tensor *q, onnxl_amd_tensor *k_cache,
+                                     onnxl_amd_tensor *v_cache, onnxl_amd_tensor *k_scale, onnxl_amd_tensor *v_scale,
+                                     const onnxl_amd_tensor *block_table, const onnxl_amd_tensor *query_start,
+                                     const onnxl_amd_tensor *lengths, void *stream) {
+  return Guard([&] {
+    return RotaryKvCacheAppend(qkv, cos, sin, position_ids, interleaved, q, k_cache, v_cache, k_scale, v_scale,
+                               block_table, query_start, lengths, static_cast<hipStream_t>(stream));
+  });
+}
+
+int onnxl_amd_sample_tokens(const onnxl_amd_tensor *logits, const onnxl_amd_tensor *uniform,
+                            const onnxl_amd_tensor *temperature, const onnxl_amd_tensor *top_k,
+                            const onnxl_amd_tensor *top_p, const onnxl_amd_tensor *min_p, onnxl_amd_tensor *token,
+                            onnxl_amd_tensor *probability, void *stream) {
+  return Guard([&] {
+    return SampleTokens(logits, uniform, temperature, top_k, top_p, min_p, token, probability,
+                        static_cast<hipStream_t>(stream));
+  });
 }
 
 int onnxl_amd_kv_cache_append(const onnxl_amd_tensor *k, const onnxl_amd_tensor *v, onnxl_amd_tensor *k_cache,

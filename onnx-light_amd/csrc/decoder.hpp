@@ -1,7 +1,7 @@
 // Launch parameters and launcher declarations of the decoder-layer operators
 // that stand between the quantized products: RMS norm with 8-bit output,
-// microscaled (MX) quantization and product, the paged 8-bit key / value cache
-// and its attention.
+// microscaled (MX) quantization, product and gated feed-forward, rotary
+// positions, the paged 8-bit key / value cache and its attention, and sampling.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -60,7 +60,11 @@ struct MxQuantParams {
 };
 void LaunchMxQuantize(const MxQuantParams &p, hipStream_t stream);
 
-// y[m, n] = sum over blocks of 2^(sa + sb) * sum of a[m, k] b[n, k]; M, N > 0
+// y[m, n] = sum over blocks of 2^(sa + sb) * sum of a[m, k] b[n, k]; M, N > 0.
+// Gated: y = act(a . b^T) * (a . up^T), both weights [N, K], in 16 bits or as MXFP8
+// (codes y and E8M0 scales y_scale [M, N / 32], N % 32 == 0).
+enum MxOutput : int { kPlain = 0, kGated = 1, kGatedMx = 2 };
+enum Activation : int { kSilu = 0, kGelu = 1, kGeluTanh = 2, kRelu = 3 };
 struct MxMatMulParams {
   const void *x;           // [M, K] FLOAT16 or BFLOAT16, quantized by the call; or nullptr and
   const uint8_t *a;        // [M, K] E4M3 or E2M1 codes with
@@ -72,6 +76,10 @@ struct MxMatMulParams {
   int x_dtype;             // of x
   int a_fp4;               // a's codes are (or x's become) E2M1, else E4M3
   int y_bf16;
+  int output;              // MxOutput
+  const uint8_t *up, *up_scale;  // the second weight of a gated product
+  int activation;
+  uint8_t *y_scale;
 };
 size_t MxMatMulScratchBytes(const MxMatMulParams &p);
 void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream);
@@ -112,6 +120,54 @@ struct KvAppendParams {
 };
 void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream);
 
+// ---------------------------------------------------------------------------
+// Rotary positions: pairs (a, b) of a head's first 2 half dimensions, (i, half + i)
+// or (2 i, 2 i + 1), become (a c - b s, a s + b c) with row `position` of the
+// tables cos and sin [positions, half]; the other dimensions stay.
+
+enum RotaryScaling : int { kRotaryNone = 0, kRotaryLinear = 1, kRotaryNtk = 2, kRotaryByParts = 3, kRotaryYarn = 4 };
+
+struct RotaryTablesParams {
+  void *cos, *sin;      // [positions, half]
+  int64_t positions;
+  int half;
+  int dtype;            // kFloat, kFloat16, kBfloat16
+  int scaling;          // RotaryScaling
+  double base, factor, original, turns_fast, turns_slow, magnitude;
+};
+void LaunchRotaryTables(const RotaryTablesParams &p, hipStream_t stream);
+
+struct RotaryTable {
+  const void *cos, *sin;  // [positions, half], FLOAT or the rotated tensor's type
+  int64_t positions;
+  int half, f32, interleaved;
+  const void *ids;        // INT32 or INT64 position of every token, or nullptr
+  int ids64;
+};
+
+struct RotaryParams {
+  RotaryTable t;          // ids nullptr: row `token` of the tables
+  const void *x;
+  void *y;                // the same layout; may be x
+  int64_t tokens, seq;    // tokens: batch * seq
+  int heads, D;
+  int by_head;            // [batch, heads, seq, D], else [tokens, heads, D]
+  int dtype;              // kFloat, kFloat16, kBfloat16
+  int64_t first;          // the launch's first workgroup
+};
+void LaunchRotaryEmbedding(const RotaryParams &p, hipStream_t stream);
+
+// The append of a joint projection's rows [tokens, heads + 2 kv_heads, head_dim]:
+// queries rotated into q, keys rotated and values as they are into the cache.
+struct RotaryAppendParams {
+  KvAppendParams a;       // k: the joint rows; v is not looked at
+  RotaryTable t;          // ids nullptr: a token's place in its sequence
+  void *q;                // [tokens, heads, head_dim]
+  int heads;
+  int64_t groups;         // the launcher's: workgroups of all launches for a head
+};
+void LaunchRotaryKvCacheAppend(const RotaryAppendParams &p, hipStream_t stream);
+
 struct KvAttentionParams {
   KvCacheParams c;
   const void *q;      // [tokens, heads, head_dim]
@@ -122,6 +178,27 @@ struct KvAttentionParams {
 };
 size_t KvAttentionScratchBytes(const KvAttentionParams &p);
 void LaunchKvCacheAttention(const KvAttentionParams &p, void *scratch, hipStream_t stream);
+
+// ---------------------------------------------------------------------------
+// A token from each row of logits and a given random number.
+
+struct SampleParams {
+  const void *x;             // [rows, vocab]
+  const float *uniform;      // [rows]
+  const float *temperature;  // [rows], or nullptr: 1
+  const void *top_k;         // INT32 or INT64 [rows], or nullptr: all
+  const float *top_p;        // [rows], or nullptr: 1
+  const float *min_p;        // [rows], or nullptr: 0
+  void *token;               // INT32 or INT64 [rows]
+  float *probability;        // [rows], or nullptr
+  int64_t rows;
+  int vocab;
+  int dtype;                 // kFloat, kFloat16, kBfloat16
+  int k64, token64;
+  int64_t first;             // row of the launch's first workgroup
+};
+size_t SampleScratchBytes(const SampleParams &p);
+void LaunchSampleTokens(const SampleParams &p, void *scratch, hipStream_t stream);
 
 #ifdef __HIPCC__
 // New tokens of sequence b, or -1 where its numbers do not fit.

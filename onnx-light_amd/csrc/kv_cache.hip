@@ -8,10 +8,13 @@
 // the kept codes rounded again by s / s' where the scale grew, the new codes.
 // Nothing else touches that block and head, so there are no atomics.  Values go
 // through LDS, which turns 16 tokens of a dimension into one 16-byte store.
+#include <type_traits>
+
 #include "common.hpp"
 #include "decoder.hpp"
 #include "device_codecs.hpp"
 #include "quant8.hpp"
+#include "rotary.hpp"
 
 namespace onnxl_amd {
 namespace {
@@ -60,14 +63,83 @@ __device__ __forceinline__ bool FindBlock(const KvCacheParams &c, int64_t w, int
   return false;
 }
 
+// Eight values of a row of the joint projection: of a key, turned to the row's
+// position, or as they are.
+struct Wide8 {
+  float v[8];
+};
+template <int DT>
+__device__ __forceinline__ Wide8 JointValues(const RotaryTable &t, const uint16_t *row, int d, bool turn, int64_t pos) {
+  Wide8 r;
+  Widen<DT, 8>(row, d, r.v);
+  if (!turn || d >= 2 * t.half) return r;
+  if (t.interleaved) {
+    float c[4], s[4];
+    TableValues<DT, 4>(t, pos, d / 2, c, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = r.v[2 * i], b = r.v[2 * i + 1];
+      r.v[2 * i] = a * c[i] - b * s[i];
+      r.v[2 * i + 1] = a * s[i] + b * c[i];
+    }
+    return r;
+  }
+  const bool upper = d >= t.half;
+  float o[8], c[8], s[8];
+  Widen<DT, 8>(row, upper ? d - t.half : d + t.half, o);
+  TableValues<DT, 8>(t, pos, upper ? d - t.half : d, c, s);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = upper ? o[i] * s[i] + r.v[i] * c[i] : r.v[i] * c[i] - o[i] * s[i];
+  return r;
+}
+
+// Queries of the joint rows: a token a wave.
+template <int DT> __device__ __forceinline__ void RotateQueries(const RotaryAppendParams &p, int64_t wave, int64_t waves) {
+  const KvCacheParams &c = p.a.c;
+  const int lane = threadIdx.x % 64, D = c.head_dim, gd = D / 8;
+  for (int64_t t = wave; t < c.tokens; t += waves) {
+    int b = -1;  // the first sequence that ends past the row
+    for (int base = 0; base < c.batch && b < 0; base += 64) {
+      const bool ends = base + lane < c.batch && c.start[base + lane + 1] > t;
+      const uint64_t past = __ballot(ends);
+      if (past) b = base + __builtin_ctzll(past);
+    }
+    if (b < 0 || c.start[b] > t || KvNewTokens(c, b) < 0) continue;
+    const int64_t pos = RotaryRow(p.t, t, (int64_t)c.lengths[b] - (c.start[b + 1] - t));
+    const uint16_t *row = static_cast<const uint16_t *>(p.a.k) + t * (p.heads + 2 * c.kv_heads) * (int64_t)D;
+    uint16_t *q = static_cast<uint16_t *>(p.q) + t * p.heads * (int64_t)D;
+    for (int i = lane; i < p.heads * gd; i += 64) {
+      const Wide8 w = JointValues<DT>(p.t, row + i / gd * D, i % gd * 8, true, pos);
+      uint16_t out[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[j] = DT == kFloat16 ? F32ToF16(w.v[j]) : F32ToBf16(w.v[j]);
+      __builtin_memcpy(q + (int64_t)i * 8, out, 16);
+    }
+  }
+}
+
+__device__ __forceinline__ const KvAppendParams &Append(const KvAppendParams &p) { return p; }
+__device__ __forceinline__ const KvAppendParams &Append(const RotaryAppendParams &p) { return p.a; }
+
 // NG groups of 8 values per thread are kept; KEPT: they are all there can be.
-template <int THREADS, int NG, bool KEPT>
-__global__ __launch_bounds__(THREADS) void KvAppendKernel(const KvAppendParams p) {
+// JOINT: the rows of a joint projection, p.k, whose keys are rotated on the way.
+template <int THREADS, int NG, bool KEPT, int JOINT = 0>
+__global__ __launch_bounds__(THREADS) void KvAppendKernel(
+    const std::conditional_t<JOINT != 0, RotaryAppendParams, KvAppendParams> all) {
   extern __shared__ __align__(16) uint8_t codes[];  // [token][dimension] of the new values
   __shared__ unsigned s_top[THREADS / 64];
+  const KvAppendParams &p = Append(all);
   const KvCacheParams &c = p.c;
   const int head = blockIdx.y, tid = threadIdx.x, bt = c.block_tokens, D = c.head_dim, gd = D / 8;
   const bool is_v = blockIdx.z != 0, fp8 = c.fp8;
+  if constexpr (JOINT != 0) {
+    if (blockIdx.z == 2) {
+      constexpr int W = THREADS / 64;
+      const int64_t group = (p.first + blockIdx.x) * c.kv_heads + head;
+      RotateQueries<JOINT>(all, group * W + __builtin_amdgcn_readfirstlane(tid / 64), all.groups * c.kv_heads * W);
+      return;
+    }
+  }
   int b, w;
   if (!FindBlock(c, p.first + blockIdx.x, b, w)) return;
   const int len = c.lengths[b], start = c.start[b], first = len - (c.start[b + 1] - start);
@@ -76,24 +148,42 @@ __global__ __launch_bounds__(THREADS) void KvAppendKernel(const KvAppendParams p
   if (blk < 0 || blk >= c.num_blocks) return;
   const int lo = max(first - j * bt, 0), hi = min(len - j * bt, bt);  // tokens kept before lo, new from lo on
   const int groups = (hi - lo) * gd;
-  const uint16_t *src = static_cast<const uint16_t *>(is_v ? p.v : p.k) +
-                        ((int64_t)start + j * bt + lo - first) * c.kv_heads * D + (int64_t)head * D;
+  int64_t pitch = (int64_t)c.kv_heads * D;
+  const uint16_t *src = static_cast<const uint16_t *>(JOINT == 0 && is_v ? p.v : p.k);
+  const int row0 = start + j * bt + lo - first;  // row of the block's first new token
+  if constexpr (JOINT != 0) {
+    pitch = (all.heads + 2 * (int64_t)c.kv_heads) * D;
+    src += row0 * pitch + (all.heads + (is_v ? c.kv_heads : 0) + (int64_t)head) * D;
+  } else {
+    src += row0 * pitch + (int64_t)head * D;
+  }
   uint8_t *dst = (is_v ? c.v_cache : c.k_cache) + (blk * c.kv_heads + head) * (int64_t)bt * D;
   float *scale = (is_v ? c.v_scale : c.k_scale) + blk * c.kv_heads + head;
   const float was = lo ? *scale : 0.f;
 
-  v4u raw[NG];
+  typedef std::conditional_t<JOINT != 0, Wide8, v4u> Group;
+  Group raw[NG];
   auto load = [&](int q) __attribute__((always_inline)) {
-    v4u r;
-    __builtin_memcpy(&r, src + (int64_t)(q / gd) * c.kv_heads * D + q % gd * 8, 16);
-    return r;
+    if constexpr (JOINT != 0) {
+      const int64_t pos = is_v ? 0 : RotaryRow(all.t, row0 + q / gd, j * bt + lo + q / gd);
+      return JointValues<JOINT>(all.t, src + q / gd * pitch, q % gd * 8, !is_v, pos);
+    } else {
+      v4u r;
+      __builtin_memcpy(&r, src + q / gd * pitch + q % gd * 8, 16);
+      return r;
+    }
   };
-  // the largest magnitude as bits (both 16-bit types order like whole numbers; a
-  // NaN is above every number)
+  // the largest magnitude as bits (both 16-bit types, and 32-bit ones, order like
+  // whole numbers; a NaN is above every number)
   unsigned top = 0;
-  auto look = [&](const v4u &r) __attribute__((always_inline)) {
+  auto look = [&](const Group &r) __attribute__((always_inline)) {
+    if constexpr (JOINT != 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(r[i] & 0x7fffu, r[i] >> 16 & 0x7fffu));
+      for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(unsigned, r.v[i]) & 0x7fffffffu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = max(top, max(r[i] & 0x7fffu, r[i] >> 16 & 0x7fffu));
+    }
   };
   if constexpr (KEPT) {
 #pragma unroll
@@ -113,7 +203,7 @@ __global__ __launch_bounds__(THREADS) void KvAppendKernel(const KvAppendParams p
     for (int i = 0; i < THREADS / 64; ++i) top = max(top, s_top[i]);
   }
   auto widen = [&](unsigned u) { return p.bf16 ? __builtin_bit_cast(float, u << 16) : F16ToF32((uint16_t)u); };
-  BlockScale s = ScaleOf(widen(top), fp8 ? kFp8Max : kInt8Max);
+  BlockScale s = ScaleOf(JOINT != 0 ? __builtin_bit_cast(float, top) : widen(top), fp8 ? kFp8Max : kInt8Max);
   // a larger or NaN scale of the kept tokens stays; a NaN of the new ones too
   if (s.scale == s.scale && !(was <= s.scale)) s = BlockScale{was, was == was ? 1.f / was : 0.f, 0};
   const bool nan = s.scale != s.scale;
@@ -140,10 +230,15 @@ __global__ __launch_bounds__(THREADS) void KvAppendKernel(const KvAppendParams p
     if constexpr (THREADS > 64) __syncthreads();
   }
   if (tid == 0) *scale = s.scale;
-  auto encode = [&](int q, const v4u &r) __attribute__((always_inline)) {
+  auto encode = [&](int q, const Group &r) __attribute__((always_inline)) {
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = widen(r[i / 2] >> (16 * (i % 2)) & 0xffffu) * s.inv;
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (JOINT != 0)
+        v[i] = r.v[i] * s.inv;
+      else
+        v[i] = widen(r[i / 2] >> (16 * (i % 2)) & 0xffffu) * s.inv;
+    }
     uint2 w = fp8 ? make_uint2(Fp8Codes4(v[0], v[1], v[2], v[3]), Fp8Codes4(v[4], v[5], v[6], v[7]))
                   : make_uint2(Int8Codes4(v[0], v[1], v[2], v[3]), Int8Codes4(v[4], v[5], v[6], v[7]));
     if (nan) w = make_uint2(0, 0);
@@ -197,10 +292,20 @@ template <int THREADS, int NG, bool KEPT> void LaunchBlocks(KvAppendParams p, in
   });
 }
 
-}  // namespace
+template <int THREADS, int NG, bool KEPT> void LaunchBlocks(RotaryAppendParams p, int64_t blocks, hipStream_t s) {
+  p.groups = blocks;
+  LaunchInPieces(blocks, THREADS, [&](int64_t first, unsigned count) {
+    p.a.first = first;
+    const dim3 grid(count, (unsigned)p.a.c.kv_heads, 3);
+    const int lds = p.a.c.block_tokens * p.a.c.head_dim;
+    if (p.a.bf16)
+      KvAppendKernel<THREADS, NG, KEPT, kBfloat16><<<grid, THREADS, lds, s>>>(p);
+    else
+      KvAppendKernel<THREADS, NG, KEPT, kFloat16><<<grid, THREADS, lds, s>>>(p);
+  });
+}
 
-void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream) {
-  const KvCacheParams &c = p.c;
+template <typename P> void LaunchAppend(const KvCacheParams &c, const P &p, hipStream_t stream) {
   if (c.tokens == 0 || c.batch == 0) return;
   // n new tokens of a sequence lie in at most (n - 1) / block_tokens + 2 blocks,
   // and in n; workgroups past the last block find none
@@ -222,5 +327,10 @@ void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream) {
     LaunchBlocks<256, 1, false>(p, most, stream);
   }
 }
+
+}  // namespace
+
+void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream) { LaunchAppend(p.c, p, stream); }
+void LaunchRotaryKvCacheAppend(const RotaryAppendParams &p, hipStream_t stream) { LaunchAppend(p.a.c, p, stream); }
 
 }  // namespace onnxl_amd

@@ -1,5 +1,6 @@
 // Microscaled 4-bit products: quantization of 16-bit activations to MXFP8 or
-// MXFP4 and the product with MXFP4 weights on the block-scaled matrix cores.
+// MXFP4 and the product, plain or gated, with MXFP4 weights on the block-scaled
+// matrix cores.
 #include "common.hpp"
 #include "decoder.hpp"
 #include "device_codecs.hpp"
@@ -86,8 +87,9 @@ __device__ __forceinline__ void TileScales(const uint8_t *scale, uint8_t *tiles,
 struct MxOperands {
   MxQuantParams q;            // a to be quantized: x set
   const uint8_t *a, *a_scale, *b_scale;
+  const uint8_t *up_scale;    // of the second weight of a gated product, or nullptr
   uint8_t *codes;             // a's codes with padded rows, where K is not whole steps
-  uint8_t *a_tiles, *b_tiles;
+  uint8_t *a_tiles, *b_tiles, *up_tiles;
   int64_t M, N, K;
   int64_t b_groups;           // workgroups of b's part
   int64_t first;              // the launch's first workgroup
@@ -97,7 +99,10 @@ template <int DT> __global__ __launch_bounds__(256) void MxOperandsKernel(const 
   const int64_t steps = (p.K + 255) / 256, group = p.first + blockIdx.x;
   if (group < p.b_groups) {
     const int64_t i = group * 256 + threadIdx.x;
-    if (i < p.N * steps) TileScales(p.b_scale, p.b_tiles, p.N, p.K, i);
+    if (i < p.N * steps)
+      TileScales(p.b_scale, p.b_tiles, p.N, p.K, i);
+    else if (p.up_scale && i < 2 * p.N * steps)
+      TileScales(p.up_scale, p.up_tiles, p.N, p.K, i - p.N * steps);
     return;
   }
   const int64_t i = (group - p.b_groups) * 256 + threadIdx.x;
@@ -138,8 +143,11 @@ namespace {
 
 int64_t Ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Rows of a product's weight, or of both weights of a gated one.
+int64_t WeightRows(const MxMatMulParams &p) { return p.output ? 2 * p.N : p.N; }
+
 // Scratch: codes (where they are not a's own) and scale tiles of a, scale tiles
-// of b.
+// of b and of the second weight.
 struct MxScratch {
   size_t codes, a_tiles, b_tiles;
   explicit MxScratch(const MxMatMulParams &p)
@@ -148,9 +156,16 @@ struct MxScratch {
         b_tiles(Scratch::Round((size_t)mx::ScaleTileBytes(p.N, p.K))) {}
 };
 
-template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, hipStream_t s) {
+template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, int output, hipStream_t s) {
   using S = mx::Shape<A4, MB, NB>;
-  mx::GemmKernel<A4, MB, NB><<<dim3((unsigned)(Ceil(g.M, S::BM) * Ceil(g.N, S::BN))), 256, 0, s>>>(g);
+  const dim3 grid((unsigned)(Ceil(g.M, S::BM) * Ceil(g.N, output ? S::BN / 2 : S::BN)));
+  if constexpr (NB % 2 == 0) {
+    if (output == kGatedMx)
+      mx::GemmKernel<A4, MB, NB, kGatedMx><<<grid, 256, 0, s>>>(g);
+    else if (output == kGated)
+      mx::GemmKernel<A4, MB, NB, kGated><<<grid, 256, 0, s>>>(g);
+  }
+  if (output == kPlain) mx::GemmKernel<A4, MB, NB><<<grid, 256, 0, s>>>(g);
 }
 
 // Large tiles (256 x 256, 128 x 256 for E4M3 activations) feed more MFMAs per
@@ -164,9 +179,12 @@ template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, hipStr
 enum class Tiles { kSmall, kMiddle, kLarge };
 Tiles TilesOf(const MxMatMulParams &p) {
   const int64_t cus = Ctx().num_cus;
-  auto rounds = [&](int64_t m, int64_t n, int64_t at_once) { return Ceil(Ceil(p.M, m) * Ceil(p.N, n), at_once * cus); };
+  // a gated tile has half the columns, of two weights
+  auto rounds = [&](int64_t m, int64_t n, int64_t at_once) {
+    return Ceil(Ceil(p.M, m) * Ceil(p.N, p.output ? n / 2 : n), at_once * cus);
+  };
   const int64_t small = 20 * rounds(128, 128, p.a_fp4 ? 2 : 1), large = 29 * rounds(p.a_fp4 ? 256 : 128, 256, 1);
-  if (!p.a_fp4 && 24 * rounds(128, 192, 1) < std::min(small, large)) return Tiles::kMiddle;
+  if (!p.a_fp4 && !p.output && 24 * rounds(128, 192, 1) < std::min(small, large)) return Tiles::kMiddle;
   return large <= small ? Tiles::kLarge : Tiles::kSmall;
 }
 
@@ -181,8 +199,11 @@ Tiles TilesOf(const MxMatMulParams &p) {
 //          64 x 4096 x 6144 18.5 | 19.5     64 x 4096 x 8192 21.9 | 19.8
 bool Streams(const MxMatMulParams &p) {
   if (p.M <= 32 || p.M > 64) return p.M <= 32;
-  if (p.a_fp4) return p.M <= 48 || p.N < 12288;
-  return p.N < (p.M <= 48 ? 11264 : 7168);
+  // MXFP8 output takes four row tiles, which more rows leave no registers for
+  if (p.output == kGatedMx) return false;
+  const int64_t rows = WeightRows(p);
+  if (p.a_fp4) return p.M <= 48 || rows < 12288;
+  return rows < (p.M <= 48 ? 11264 : 7168);
 }
 
 // Up to this many values every workgroup quantizes its activations itself
@@ -219,48 +240,58 @@ StreamPlan PlanStream(const MxMatMulParams &p) {
   // left.  More than these do not fit the registers of two waves per SIMD.  us,
   // K = 4096, N = 14336, with these | with one: 8 rows 13.3 | 15.0, 16 rows 15.0 |
   // 18.3, MXFP4 32 rows 14.7 | 19.1, 48 rows 18.2 | 24.0.
-  s.nt = OwnQuant(p) ? 1 : s.mt == 1 ? 2 : s.mt <= (p.a_fp4 ? 3 : 2) ? 4 : 2;
-  while (s.nt > 1 && Ceil(p.N, 16 * s.nt) * chunks < 4 * Ctx().num_cus) s.nt /= 2;
+  // A gated product's row tiles come in pairs, for MXFP8 blocks in two.
+  const int least = p.output == kGatedMx ? 4 : p.output ? 2 : 1;
+  s.nt = OwnQuant(p) ? least : s.mt == 1 ? 2 : s.mt <= (p.a_fp4 ? 3 : 2) ? 4 : 2;
+  while (s.nt > 1 && Ceil(WeightRows(p), 16 * s.nt) * chunks < 4 * Ctx().num_cus) s.nt /= 2;
+  s.nt = std::max(s.nt, least);
   s.waves = s.nt == 4 ? 4 : 8;
-  s.tiles = Ceil(p.N, 16 * s.nt);
+  s.tiles = Ceil(WeightRows(p), 16 * s.nt);
   // as many as give every wave one chunk, while there are not more than about
   // two rounds of them
   s.split = (int)std::max<int64_t>(1, std::min<int64_t>(Ceil(chunks, s.waves), 32 * Ctx().num_cus / (s.waves * s.tiles)));
   return s;
 }
 
-template <bool A4, int NT, int MT, bool QUANT> void LaunchStream(const mx::StreamArgs &a, const StreamPlan &s, hipStream_t st) {
+template <bool A4, int NT, int MT, bool QUANT, int OUT> void LaunchStream(const mx::StreamArgs &a, const StreamPlan &s, hipStream_t st) {
   const int64_t chunks = Ceil(a.K, 512);
   const size_t codes = QUANT ? (size_t)(a.M * chunks * ((A4 ? 256 : 512) + 16)) : 0;
   const size_t lds = std::max(codes, (size_t)NT * MT * s.waves * 1024);
   LaunchInPieces(s.tiles, 64 * s.waves, [&](int64_t first, unsigned count) {
     mx::StreamArgs p = a;
     p.first = (int)first;
-    mx::StreamKernel<A4, NT, MT, QUANT><<<dim3(count, (unsigned)s.split), 64 * s.waves, lds, st>>>(p);
+    mx::StreamKernel<A4, NT, MT, QUANT, OUT><<<dim3(count, (unsigned)s.split), 64 * s.waves, lds, st>>>(p);
   });
 }
 
-template <bool A4, int MT> void LaunchStreamRows(const mx::StreamArgs &a, const StreamPlan &s, hipStream_t st) {
+template <bool A4, int MT, int OUT> void LaunchStreamRows(const mx::StreamArgs &a, const StreamPlan &s, hipStream_t st) {
   constexpr bool kFour = MT == 2 || (A4 && MT == 3);
-  if (kFour && s.nt == 4)
-    LaunchStream<A4, kFour ? 4 : 2, MT, false>(a, s, st);
-  else if (s.nt == 2)
-    LaunchStream<A4, 2, MT, false>(a, s, st);
-  else
-    LaunchStream<A4, 1, MT, false>(a, s, st);
+  if constexpr (OUT == kGatedMx) {
+    if constexpr (MT <= 2) LaunchStream<A4, 4, MT, false, OUT>(a, s, st);
+  } else if (kFour && s.nt == 4) {
+    LaunchStream<A4, kFour ? 4 : 2, MT, false, OUT>(a, s, st);
+  } else if (OUT == kGated || s.nt == 2) {
+    LaunchStream<A4, 2, MT, false, OUT>(a, s, st);
+  } else {
+    LaunchStream<A4, OUT == kPlain ? 1 : 2, MT, false, OUT>(a, s, st);
+  }
 }
 
-template <bool A4> void LaunchStreamOf(const mx::StreamArgs &a, bool own, const StreamPlan &s, hipStream_t st) {
+template <bool A4, int OUT> void LaunchStreamOf(const mx::StreamArgs &a, bool own, const StreamPlan &s, hipStream_t st) {
   if (own)
-    LaunchStream<A4, 1, 1, true>(a, s, st);
+    LaunchStream<A4, OUT == kPlain ? 1 : OUT == kGated ? 2 : 4, 1, true, OUT>(a, s, st);
   else if (s.mt == 1)
-    LaunchStreamRows<A4, 1>(a, s, st);
+    LaunchStreamRows<A4, 1, OUT>(a, s, st);
   else if (s.mt == 2)
-    LaunchStreamRows<A4, 2>(a, s, st);
+    LaunchStreamRows<A4, 2, OUT>(a, s, st);
   else if (s.mt == 3)
-    LaunchStreamRows<A4, 3>(a, s, st);
+    LaunchStreamRows<A4, 3, OUT>(a, s, st);
   else
-    LaunchStreamRows<A4, 4>(a, s, st);
+    LaunchStreamRows<A4, 4, OUT>(a, s, st);
+}
+
+template <int OUT> void LaunchStreams(const mx::StreamArgs &a, bool a_fp4, bool own, const StreamPlan &s, hipStream_t st) {
+  a_fp4 ? LaunchStreamOf<true, OUT>(a, own, s, st) : LaunchStreamOf<false, OUT>(a, own, s, st);
 }
 
 }  // namespace
@@ -272,14 +303,15 @@ size_t MxMatMulScratchBytes(const MxMatMulParams &p) {
     return codes + (s.split > 1 ? (size_t)s.tiles * s.split * s.nt * s.mt * 1024 : 0);
   }
   const MxScratch s(p);
-  return s.codes + s.a_tiles + s.b_tiles;
+  return s.codes + s.a_tiles + (p.output ? 2 : 1) * s.b_tiles;
 }
 
 void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) {
   if (Streams(p)) {
     const StreamPlan plan = PlanStream(p);
     mx::StreamArgs a{p.x, p.a, p.a_scale, p.b, p.b_scale, static_cast<uint16_t *>(p.y), (int)p.M, (int)p.N, (int)p.K,
-                     p.x_dtype == kBfloat16, p.y_bf16, plan.split, nullptr, nullptr, 0};
+                     p.x_dtype == kBfloat16, p.y_bf16, plan.split, nullptr, nullptr, 0, p.up, p.up_scale, p.activation,
+                     p.y_scale};
     const bool own = OwnQuant(p);
     uint8_t *codes = static_cast<uint8_t *>(scratch), *scales = codes + Scratch::Round((size_t)(p.M * p.K));
     if (a.split > 1) {
@@ -291,21 +323,29 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
       a.a = codes;
       a.as = scales;
     }
-    p.a_fp4 ? LaunchStreamOf<true>(a, own, plan, stream) : LaunchStreamOf<false>(a, own, plan, stream);
+    if (p.output == kGatedMx)
+      LaunchStreams<kGatedMx>(a, p.a_fp4, own, plan, stream);
+    else if (p.output)
+      LaunchStreams<kGated>(a, p.a_fp4, own, plan, stream);
+    else
+      LaunchStreams<kPlain>(a, p.a_fp4, own, plan, stream);
     return;
   }
   const MxScratch s(p);
   uint8_t *codes = static_cast<uint8_t *>(scratch), *a_tiles = codes + s.codes, *b_tiles = a_tiles + s.a_tiles;
+  uint8_t *up_tiles = b_tiles + s.b_tiles;
   const int64_t steps = Ceil(p.K, 256);
   MxOperands o{};
   o.a_scale = p.a_scale;
   o.b_scale = p.b_scale;
   o.a_tiles = a_tiles;
   o.b_tiles = b_tiles;
+  o.up_scale = p.up_scale;
+  o.up_tiles = up_tiles;
   o.M = p.M;
   o.N = p.N;
   o.K = p.K;
-  o.b_groups = Ceil(p.N * steps, 256);
+  o.b_groups = Ceil(WeightRows(p) * steps, 256);
   o.q = MxQuantParams{p.x, codes, nullptr, p.M, p.K, p.x_dtype, p.a_fp4, 0};
   o.a = p.a;
   o.codes = s.codes ? codes : nullptr;
@@ -320,14 +360,15 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
       MxOperandsKernel<kBfloat16><<<count, 256, 0, stream>>>(o);
   });
   const mx::GemmArgs g{s.codes ? codes : p.a, p.b, a_tiles, b_tiles, static_cast<uint16_t *>(p.y), p.M, p.N, p.K, p.y_bf16,
-                       p.N % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0};
+                       (p.output == kGatedMx || p.N % 8 == 0) && reinterpret_cast<uintptr_t>(p.y) % 16 == 0, p.up, up_tiles,
+                       p.activation, p.y_scale};
   const Tiles tiles = TilesOf(p);
   if (tiles == Tiles::kLarge)
-    p.a_fp4 ? LaunchGemm<true, 4, 4>(g, stream) : LaunchGemm<false, 2, 4>(g, stream);
+    p.a_fp4 ? LaunchGemm<true, 4, 4>(g, p.output, stream) : LaunchGemm<false, 2, 4>(g, p.output, stream);
   else if (tiles == Tiles::kMiddle)
-    LaunchGemm<false, 2, 3>(g, stream);
+    LaunchGemm<false, 2, 3>(g, p.output, stream);
   else
-    p.a_fp4 ? LaunchGemm<true, 2, 2>(g, stream) : LaunchGemm<false, 2, 2>(g, stream);
+    p.a_fp4 ? LaunchGemm<true, 2, 2>(g, p.output, stream) : LaunchGemm<false, 2, 2>(g, p.output, stream);
 }
 
 }  // namespace onnxl_amd

@@ -23,6 +23,10 @@
 // One row of 4096 values by [14336, 4096]: 29.4 MB of codes and 1.8 of scales in
 // 9.8 us, 3.2 TB/s with the launch, which is a quarter of it.
 //
+// A gated product (MxOutput) takes row tiles of both weights in turn, so that a wave
+// has a column's two sums in the same lanes and registers; everything else is the
+// same.  MXFP8 output has 32 columns, a block, in a workgroup.
+//
 // What the instruction does with E4M3 products is said at the GEMM (mx_gemm.hpp).
 // With four row tiles and three of activations (E2M1, 33 to 48 rows) the registers
 // of two waves per SIMD do not hold everything: 4 are kept in memory.
@@ -30,6 +34,7 @@
 
 #include <type_traits>
 
+#include "mx_gate.hpp"
 #include "mx_gemm.hpp"
 #include "quant8.hpp"
 
@@ -47,6 +52,9 @@ struct StreamArgs {
   float *part;                  // their sums, [row tile][split][NT * MT][64] float4
   unsigned *done;               // [row tile] workgroups that are done, zero between launches
   int first;                    // row tile of the launch's first workgroup
+  const uint8_t *up = nullptr, *ups = nullptr;  // gated: the second weight, of which N counts no rows
+  int activation = 0;
+  uint8_t *y_scale = nullptr;   // kGatedMx: [M, N / 32]
 };
 
 // Four block scales from `at` (a multiple of 4) on of the row of `blocks` at
@@ -70,21 +78,24 @@ __device__ __forceinline__ int Scales4(const uint8_t *base, unsigned row, int at
 // Waves of a workgroup: what the registers of more rows and columns leave.
 template <int NT> constexpr int kStreamWaves = NT == 4 ? 4 : 8;
 
-template <bool A4, int NT, int MT, bool QUANT>
+template <bool A4, int NT, int MT, bool QUANT, int OUT = kPlain>
 __global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const StreamArgs p) {
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
   const int blocks = p.K / 32, chunks = (blocks + 15) / 16;
-  const int tile = p.first + (int)blockIdx.x, n0 = tile * 16 * NT;
+  constexpr int NW = OUT == kPlain ? 1 : 2, NO = NT / NW;  // weights, tiles of y's columns
+  static_assert(NT % NW == 0 && (OUT != kGatedMx || NO == 2), "whole pairs, and a block of 32 columns");
+  const int tile = p.first + (int)blockIdx.x, n0 = tile * 16 * NO;
   const int64_t pitch_b = p.K / 2, pitch_a = A4 ? p.K / 2 : p.K;
 
   // 32-bit offsets of this lane's rows (those past the last repeat it) from the
   // tile's first
-  const uint8_t *tile_b = p.b + n0 * pitch_b, *tile_s = p.bs + (int64_t)n0 * blocks;
-  unsigned row_b[NT], row_s[NT];
+  const uint8_t *tile_b[2] = {p.b + n0 * pitch_b, p.up + n0 * pitch_b};
+  const uint8_t *tile_s[2] = {p.bs + (int64_t)n0 * blocks, p.ups + (int64_t)n0 * blocks};
+  unsigned row_b[NO], row_s[NO];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+  for (int n = 0; n < NO; ++n) {
     const unsigned row = (unsigned)(min(n0 + 16 * n + c, p.N - 1) - n0);
     row_b[n] = row * (unsigned)pitch_b;
     row_s[n] = row * (unsigned)blocks;
@@ -100,8 +111,8 @@ __global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        w[n][j] = *reinterpret_cast<const v4i *>(tile_b + (row_b[n] + 16u * (unsigned)(blk + j < blocks ? blk + j : 0)));
-      ws[n] = Scales4(tile_s, row_s[n], blk, blocks, tail);
+        w[n][j] = *reinterpret_cast<const v4i *>(tile_b[n % NW] + (row_b[n / NW] + 16u * (unsigned)(blk + j < blocks ? blk + j : 0)));
+      ws[n] = Scales4(tile_s[n % NW], row_s[n / NW], blk, blocks, tail);
     }
   };
 
@@ -227,26 +238,54 @@ __global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const
   constexpr int kScope = 16;  // sc1: past this XCD's L2, so that no fence is needed
   const __amdgpu_buffer_rsrc_t rs = Rsrc(p.part, 0x7fffffff);
   auto slot = [&](int s, int i) { return (int)(((tile * p.split + s) * (NT * MT) + i) * 64 + lane) * 16; };
-  auto store = [&](int i, v4f s) {
-    const int row = i % MT * 16 + c, col = n0 + i / MT * 16 + 4 * g;
-    if (row >= p.M) return;
-    uint16_t *y = p.y + (int64_t)row * p.N + col;
-    uint16_t v[4];
+  // Units of the output, of a wave each: a tile of 16 x 16, or for MXFP8 two side by
+  // side; unit u has row tile u % MT, and part tiles PU from PU (u / MT) on.
+  constexpr int CU = OUT == kGatedMx ? 2 : 1, PU = CU * NW, U = NO / CU * MT;
+  auto tile_of = [&](int u, int e) { return (u / MT * PU + e) * MT + u % MT; };
+  auto store = [&](int u, const v4f(&s)[PU]) __attribute__((always_inline)) {
+    const int row = u % MT * 16 + c, col = n0 + u / MT * CU * 16 + 4 * g;
+    if constexpr (OUT == kGatedMx) {
+      float v[8];
+      unsigned top = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = Half(s[e], p.bf16);
-    if (col + 4 <= p.N) {
-      __builtin_memcpy(y, v, 8);
+      for (int e = 0; e < 8; ++e) {
+        v[e] = Activate(s[e / 4 * 2][e % 4], p.activation) * s[e / 4 * 2 + 1][e % 4];
+        top = max(top, __builtin_bit_cast(unsigned, v[e]) & 0x7fffffffu);
+      }
+      // the block's other columns are in the lanes of the same row
+      top = max(top, (unsigned)__shfl_xor((int)top, 16));
+      top = max(top, (unsigned)__shfl_xor((int)top, 32));
+      const BlockScale b = MxScaleOf(__builtin_bit_cast(float, top), 8);
+      const uint2 w = MxFp8Codes8(v, b);
+      if (row >= p.M || col >= p.N) return;  // N % 32 == 0
+      uint8_t *y = reinterpret_cast<uint8_t *>(p.y) + (int64_t)row * p.N + col;
+      *reinterpret_cast<unsigned *>(y) = w.x;
+      *reinterpret_cast<unsigned *>(y + 16) = w.y;
+      if (g == 0) p.y_scale[(int64_t)row * (p.N / 32) + col / 32] = b.e8m0;
     } else {
-      for (int e = 0; col + e < p.N; ++e) y[e] = v[e];
+      if (row >= p.M) return;
+      uint16_t *y = p.y + (int64_t)row * p.N + col;
+      uint16_t v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = Half(OUT == kPlain ? s[0][e] : Activate(s[0][e], p.activation) * s[PU - 1][e], p.bf16);
+      if (col + 4 <= p.N) {
+        __builtin_memcpy(y, v, 8);
+      } else {
+        for (int e = 0; col + e < p.N; ++e) y[e] = v[e];
+      }
     }
   };
-  for (int i = wave; i < NT * MT; i += waves) {
-    v4f s = part[i * waves * 64 + lane];
-    for (int v = 1; v < waves; ++v) s += part[(i * waves + v) * 64 + lane];
-    if (p.split == 1)
-      store(i, s);
-    else
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, s), rs, slot(blockIdx.y, i), 0, kScope);
+  for (int u = wave; u < U; u += waves) {
+    v4f s[PU];
+#pragma unroll
+    for (int e = 0; e < PU; ++e) {
+      const int i = tile_of(u, e);
+      s[e] = part[i * waves * 64 + lane];
+      for (int v = 1; v < waves; ++v) s[e] += part[(i * waves + v) * 64 + lane];
+      if (p.split > 1) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, s[e]), rs, slot(blockIdx.y, i), 0, kScope);
+    }
+    if (p.split == 1) store(u, s);
   }
   if (p.split == 1) return;
   __shared__ unsigned before;
@@ -258,29 +297,35 @@ __global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const
   if (tid == 0) p.done[tile] = 0;
   // up to kParts parts of all of a wave's tiles are on their way at once: one
   // after the other the six of 33 x 11008 x 4099 take 5.3 us of the launch's 15
-  constexpr int kParts = 6, kMine = (NT * MT + kStreamWaves<NT> - 1) / kStreamWaves<NT>;
-  v4f sum[kMine];
+  constexpr int kParts = 6, kMine = (U + kStreamWaves<NT> - 1) / kStreamWaves<NT>;
+  v4f sum[kMine][PU];
 #pragma unroll
-  for (int t = 0; t < kMine; ++t) sum[t] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < kMine; ++t)
+#pragma unroll
+    for (int e = 0; e < PU; ++e) sum[t][e] = v4f{0.f, 0.f, 0.f, 0.f};
   for (int v0 = 0; v0 < p.split; v0 += kParts) {
-    v4u x[kMine][kParts];
+    v4u x[kMine][PU][kParts];
 #pragma unroll
     for (int t = 0; t < kMine; ++t)
 #pragma unroll
-      for (int v = 0; v < kParts; ++v)
-        x[t][v] = __builtin_amdgcn_raw_buffer_load_b128(
-            rs, slot(min(v0 + v, p.split - 1), min(wave + t * waves, NT * MT - 1)), 0, kScope);
+      for (int e = 0; e < PU; ++e)
+#pragma unroll
+        for (int v = 0; v < kParts; ++v)
+          x[t][e][v] = __builtin_amdgcn_raw_buffer_load_b128(
+              rs, slot(min(v0 + v, p.split - 1), tile_of(min(wave + t * waves, U - 1), e)), 0, kScope);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int v = 0; v < kParts; ++v) {
       if (v0 + v >= p.split) break;
 #pragma unroll
-      for (int t = 0; t < kMine; ++t) sum[t] += __builtin_bit_cast(v4f, x[t][v]);
+      for (int t = 0; t < kMine; ++t)
+#pragma unroll
+        for (int e = 0; e < PU; ++e) sum[t][e] += __builtin_bit_cast(v4f, x[t][e][v]);
     }
   }
 #pragma unroll
   for (int t = 0; t < kMine; ++t)
-    if (wave + t * waves < NT * MT) store(wave + t * waves, sum[t]);
+    if (wave + t * waves < U) store(wave + t * waves, sum[t]);
 }
 
 }  // namespace mx
