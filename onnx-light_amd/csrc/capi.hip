@@ -3576,11 +3576,28 @@ int RotaryTables(double base, int32_t scaling, double factor, int64_t original, 
   if (P == 0) return ONNXL_AMD_OK;
   Ctx();
   if (magnitude == 0.0) magnitude = scaling == kRotaryYarn ? 0.1 * std::log(factor) + 1.0 : 1.0;
+  const double d = 2.0 * half, two_pi = 6.283185307179586476925;
   Staging st(stream, 0, {}, {cos, sin});
-  LaunchRotaryTables(RotaryTablesParams{st.Out(cos), st.Out(sin), P, (int)half, cos->data_type, scaling, base,
-                                        scaling == kRotaryNone ? 1.0 : factor, (double)original, turns_fast, turns_slow,
-                                        magnitude},
-                     stream);
+  RotaryTablesParams p{};
+  p.cos = st.Out(cos);
+  p.sin = st.Out(sin);
+  p.positions = P;
+  p.half = (int)half;
+  p.dtype = cos->data_type;
+  p.scaling = scaling;
+  p.log_base = std::log(base) + (scaling == kRotaryNtk ? d / (d - 2.0) * std::log(factor) : 0.0);
+  p.factor = factor;
+  p.original = (double)original;
+  p.turns_fast = turns_fast;
+  p.turns_slow = turns_slow;
+  if (scaling == kRotaryYarn) {
+    // the pair that makes so many turns in the original positions
+    auto pair_of = [&](double turns) { return d * std::log(p.original / (turns * two_pi)) / (2.0 * std::log(base)); };
+    p.low = std::max(std::floor(pair_of(turns_fast)), 0.0);
+    p.high = std::min(std::ceil(pair_of(turns_slow)), d - 1.0);
+  }
+  p.magnitude = (float)magnitude;
+  LaunchRotaryTables(p, stream);
   OLA_HIP(hipGetLastError());
   st.Finish();
   return ONNXL_AMD_OK;

@@ -133,7 +133,10 @@ struct RotaryTablesParams {
   int half;
   int dtype;            // kFloat, kFloat16, kBfloat16
   int scaling;          // RotaryScaling
-  double base, factor, original, turns_fast, turns_slow, magnitude;
+  double log_base;      // of the base, ntk's growth included
+  double factor, original, turns_fast, turns_slow;
+  double low, high;     // yarn: pairs up to low keep their frequency, from high on 1 / factor of it
+  float magnitude;
 };
 void LaunchRotaryTables(const RotaryTablesParams &p, hipStream_t stream);
 
