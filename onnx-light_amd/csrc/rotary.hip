@@ -25,7 +25,7 @@ __device__ __forceinline__ void CosSin(double turns, float &c, float &s) {
   const float x = (float)((turns - 0.25 * quarters) * kTwoPi), z = x * x;
   const float si = x + x * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
   const float co = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 - z * (1.f / 3628800)))));
-  const int q = (int)(long long)quarters & 3;
+  const int q = (int)quarters & 3;  // positions are below 2^31, a position at most 1 / (2 pi) turns
   const float a = q & 1 ? si : co, b = q & 1 ? co : si;
   c = q == 1 || q == 2 ? -a : a;
   s = q >= 2 ? -b : b;
@@ -68,12 +68,13 @@ template <int DT, int N> __global__ __launch_bounds__(256) void RotaryTablesKern
   double turns[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) turns[j] = TurnsPerPosition(p, i + j);
-  const int64_t step = (int64_t)gridDim.x * rows;
-  for (int64_t pos = (int64_t)blockIdx.x * rows + r; pos < p.positions; pos += step) {
+  const int64_t step = (int64_t)gridDim.x * rows, first = (int64_t)blockIdx.x * rows + r;
+  double place = (double)first;
+  for (int64_t pos = first; pos < p.positions; pos += step, place += (double)step) {
     float c[N], s[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      CosSin(pos * turns[j], c[j], s[j]);
+      CosSin(place * turns[j], c[j], s[j]);
       c[j] *= p.magnitude;
       s[j] *= p.magnitude;
     }
