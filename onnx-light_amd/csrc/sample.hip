@@ -2,7 +2,7 @@
 // top-p and min-p, then the first token, in order of index, at which the kept
 // weights add up to more than the random number's share of their sum.
 //
-// A weight exp((x - max) / T) is a whole number of 2^-kUnit: sums of them have no
+// A weight exp((x - max) / T) is a whole number of 2^-42: sums of them have no
 // order, so they are the same from run to run and however the work is split, and
 // a row's tokens and the borders of top-p are decided exactly on them.  2^-42 of
 // the largest weight is far below what separates two tokens' places, and a row of
@@ -15,6 +15,8 @@
 // by its bits.  The kept weights are added up in chunks of consecutive tokens, the
 // chunk of the random number's share is found, and its token.  A row whose list
 // would not fit has its border found by the bits of all its logits.
+#include <type_traits>
+
 #include "common.hpp"
 #include "decoder.hpp"
 #include "device_codecs.hpp"
@@ -22,15 +24,17 @@
 namespace onnxl_amd {
 namespace {
 
-constexpr int kUnit = 42, kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048, kList = 4096, kChunks = 1024;
 constexpr float kOctaves = 44.f;  // of weights that the bins span; the last bin has the rest
+constexpr float kMaxFloat = 0x1.fffffep127f, kMinFloat = 0x1p-126f;
 typedef unsigned long long u64;
 
 // Whole numbers in the order of the logits: NaN and -inf, which are never
 // chosen, 0; the zeros equal.
+__device__ __forceinline__ bool IsLogit(float x) { return x > -__builtin_huge_valf(); }
 __device__ __forceinline__ unsigned KeyOf(float x) {
-  if (!(x > -__builtin_huge_valf())) return 0;
+  if (!IsLogit(x)) return 0;
   const unsigned u = __builtin_bit_cast(unsigned, x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
@@ -44,25 +48,77 @@ struct Shared {
   u64 digit[256];
   u64 chunk[kChunks];
   u64 bin[kBins];
-  u64 list[kList];  // key << 32 | index
+  u64 list[kList];         // key << 32 | index
+  u64 queue[kWaves][128];  // of a wave: logit << 32 | index, kept for certain
   u64 out[2];
   unsigned n, at;
 };
 
-// A row, and what its weights go by.
+// ---- sums over lanes and threads ----------------------------------------------
+
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 AddFrom(u64 v) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xf, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((u64)hi << 32 | lo);
+}
+// Sums of the lanes up to and with this one: inside rows of 16, then the last lane of a
+// row to the next row, of the second to the third and fourth.
+__device__ __forceinline__ u64 WaveScan(u64 v) {
+  v = AddFrom<0x111, 0xf>(v);
+  v = AddFrom<0x112, 0xf>(v);
+  v = AddFrom<0x114, 0xf>(v);
+  v = AddFrom<0x118, 0xf>(v);
+  v = AddFrom<0x142, 0xa>(v);
+  return AddFrom<0x143, 0xc>(v);
+}
+// Sums of all threads up to and with this one; `all` of all.
+__device__ __forceinline__ u64 GroupScan(Shared &s, u64 v, u64 &all) {
+  v = WaveScan(v);
+  __syncthreads();
+  if (threadIdx.x % 64 == 63) s.wave[threadIdx.x / 64] = v;
+  __syncthreads();
+  u64 before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    before += w < (int)threadIdx.x / 64 ? s.wave[w] : 0;
+    all += s.wave[w];
+  }
+  return v + before;
+}
+__device__ __forceinline__ u64 GroupMax(Shared &s, u64 v) {
+  for (int o = 32; o > 0; o >>= 1) {
+    const u64 w = __shfl_xor(v, o);
+    v = w > v ? w : v;
+  }
+  __syncthreads();
+  if (threadIdx.x % 64 == 0) s.wave[threadIdx.x / 64] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) v = s.wave[w] > v ? s.wave[w] : v;
+  return v;
+}
+
+// ---- a row ----------------------------------------------------------------------
+
 template <int DT> struct Row {
   const void *x;
   int64_t base;
   int vocab;
-  float top, per_bin;  // the largest logit; bins a unit of it
-  double octaves;      // log2(e) / T
-  double least;        // min_p, 0: none
+  int shift;       // log2 of a chunk's tokens
+  // what weights go by, from the largest logit on
+  float top, per_bin;
+  double high, octaves;  // the largest logit (past all others where it is infinite); log2(e) / T
+  double least;          // min_p, 0: none
   const double *power;
 
-  __device__ float At(int i) const {
-    float v[1];
-    Load<1>(i, v);
-    return v[0];
+  __device__ __forceinline__ void Weigh(float largest, float T, float min_p) {
+    top = fminf(largest, kMaxFloat);
+    high = largest > kMaxFloat ? 0x1p1000 : (double)largest;
+    octaves = largest > kMaxFloat ? 1.0 : 1.4426950408889634074 / (double)T;
+    // any positive number keeps the order of the bins
+    per_bin = fminf(fmaxf((float)(octaves * (kBins / kOctaves)), kMinFloat), kMaxFloat);
+    least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
   }
   template <int N> __device__ __forceinline__ void Load(int i, float (&v)[N]) const {
     if constexpr (DT == kFloat) {
@@ -74,87 +130,269 @@ template <int DT> struct Row {
       for (int j = 0; j < N; ++j) v[j] = DT == kFloat16 ? F16ToF32(u[j]) : Bf16ToF32(u[j]);
     }
   }
-  // 2^-t by a table of the 32nds and the series of the rest, |r| <= ln 2 / 64, to
-  // about 2^-48
-  __device__ __forceinline__ double Weight(float v) const {
-    if (v == top) return 1.0;
-    const double t = ((double)top - (double)v) * octaves;
-    if (!(t < 1000.0)) return 0.0;
-    const double k = rint(32.0 * t), r = (k * 0.03125 - t) * 0.6931471805599453094;
-    double p = fma(r, 1.0 / 120, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    const int i = (int)k;
-    return ldexp(power[i & 31] * p, -(i >> 5));
+  __device__ __forceinline__ float At(int i) const {
+    float v[1];
+    Load<1>(i, v);
+    return v[0];
   }
-  __device__ static __forceinline__ u64 Whole(double w) { return (u64)rint(w * (double)(u64(1) << kUnit)); }
+  // 2^-t by a table of the 32nds, whose number stands in the low bits of a sum with 1.5
+  // 2^47, and the series of the rest, at most 1/64, to about 2^-48.  A difference past
+  // 1000 octaves counts as that, one of infinities as the largest logit itself.
+  __device__ __forceinline__ double Weight(float v) const {
+    const double t = fmax(fmin((high - (double)v) * octaves, 1000.0), 0.0);
+    const double sum = t + 0x1.8p47, r = (sum - 0x1.8p47) - t;
+    double p = fma(r, 0x1.5d87fe78a6731p-10, 0x1.3b2ab6fba4e77p-7);
+    p = fma(p, r, 0x1.c6b08d704a0c0p-5);
+    p = fma(p, r, 0x1.ebfbdff82c58fp-3);
+    p = fma(p, r, 0x1.62e42fefa39efp-1);
+    p = fma(p, r, 1.0);
+    const unsigned k = (unsigned)__builtin_bit_cast(u64, sum);
+    const u64 w = __builtin_bit_cast(u64, power[k & 31] * p);
+    return __builtin_bit_cast(double, w - ((u64)(k >> 5) << 52));
+  }
+  // in units of 2^-42, the last place of numbers from 1024 to 2048
+  __device__ static __forceinline__ u64 Whole(double w) {
+    return __builtin_bit_cast(u64, w + 1024.0) - __builtin_bit_cast(u64, 1024.0);
+  }
   // what min_p leaves of a token's weight
   __device__ __forceinline__ u64 Kept(float v) const {
     const double w = Weight(v);
     return w >= least ? Whole(w) : 0;
   }
+  // falls with v, as every rounding in it does
   __device__ __forceinline__ int Bin(float v) const {
-    const float b = (top - v) * per_bin;  // falls with v, as every rounding in it does
-    return v == top ? 0 : b < (float)(kBins - 1) ? (int)b : kBins - 1;
+    return (int)__builtin_amdgcn_fmed3f((top - v) * per_bin, 0.f, (float)(kBins - 1));
   }
-  // f(logits, first index, how many) for 16 bytes at a time, four of them on their way;
-  // every thread of the workgroup comes by the same number of times
-  template <typename F> __device__ __forceinline__ void Each(F &&f) const {
+  // f(logits, first index) for 16 bytes at a time of the tokens from..to - 1, four of them
+  // on their way; what is past the end is -inf
+  template <typename F> __device__ __forceinline__ void Each(int from, int to, F &&f) const {
     constexpr int N = DT == kFloat ? 4 : 8, U = 4;
-    for (int i0 = 0; i0 < vocab; i0 += U * N * kThreads) {
+    for (int i0 = from; i0 < to; i0 += U * N * kThreads) {
       float v[U][N];
+      const int wave = i0 + (int)(threadIdx.x & ~63u) * N;  // the wave's first
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + (u * kThreads + (int)threadIdx.x) * N;
-        if (i + N <= vocab) {
+        if (i + N <= to) {
           Load<N>(i, v[u]);
-        } else {
+        } else if (wave + u * kThreads * N < to) {
 #pragma unroll
-          for (int j = 0; j < N; ++j) v[u][j] = i + j < vocab ? At(i + j) : -__builtin_huge_valf();
+          for (int j = 0; j < N; ++j) v[u][j] = i + j < to ? At(i + j) : -__builtin_huge_valf();
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) f(v[u], i0 + (u * kThreads + (int)threadIdx.x) * N, std::integral_constant<int, N>{});
+      for (int u = 0; u < U; ++u)
+        if (wave + u * kThreads * N < to) f(v[u], i0 + (u * kThreads + (int)threadIdx.x) * N);
     }
+  }
+  // f(logit, index) for each that can be chosen
+  template <typename F> __device__ __forceinline__ void EachLogit(int from, int to, F &&f) const {
+    Each(from, to, [&](const auto &v, int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < (int)(sizeof(v) / 4); ++j)
+        if (IsLogit(v[j])) f(v[j], i + j);
+    });
   }
 };
 
-template <typename T> __device__ __forceinline__ T WaveSum(T v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// What a row asks for, and which token that is where nothing has to be weighed: the first
+// in order, -1 of none.
+struct Wish {
+  float T, top_p, min_p;
+  int64_t k;
+  bool cuts;  // top_p does
+};
+__device__ __forceinline__ Wish WishOf(const SampleParams &p, int64_t row) {
+  Wish w;
+  w.T = p.temperature ? p.temperature[row] : 1.f;
+  w.top_p = p.top_p ? p.top_p[row] : 1.f;
+  w.min_p = p.min_p ? p.min_p[row] : 0.f;
+  w.k = 0;
+  if (p.top_k) w.k = p.k64 ? static_cast<const int64_t *>(p.top_k)[row] : (int64_t) static_cast<const int32_t *>(p.top_k)[row];
+  if (w.k < 0 || w.k >= p.vocab) w.k = 0;
+  w.cuts = w.top_p < 1.f;
+  return w;
 }
-// Sums of all threads up to and with this one; `all` of all.
-__device__ __forceinline__ u64 GroupScan(Shared &s, u64 v, u64 &all) {
-  const int lane = threadIdx.x % 64;
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 w = __shfl_up(v, o);
-    if (lane >= o) v += w;
-  }
-  __syncthreads();
-  if (lane == 63) s.wave[threadIdx.x / 64] = v;
-  __syncthreads();
-  all = 0;
-  u64 before = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < (int)threadIdx.x / 64) before += s.wave[w];
-    all += s.wave[w];
-  }
-  return v + before;
+__device__ __forceinline__ void Answer(const SampleParams &p, int64_t row, int64_t token, float probability) {
+  if (p.token64)
+    static_cast<int64_t *>(p.token)[row] = token;
+  else
+    static_cast<int32_t *>(p.token)[row] = (int32_t)token;
+  if (p.probability) p.probability[row] = probability;
+}
+// `best`: the largest key, and the complement of the lowest index that has it
+__device__ __forceinline__ bool Plain(const Wish &w, u64 best) { return best >> 32 == 0 || !(w.T > 0.f) || w.k == 1; }
+__device__ __forceinline__ void AnswerPlain(const SampleParams &p, int64_t row, u64 best) {
+  const bool none = best >> 32 == 0;
+  Answer(p, row, none ? -1 : (int64_t)(0xffffffffu - (unsigned)best), none ? 0.f : 1.f);
+}
+// The token at which the weights up to it reach this is the last that top_p keeps.
+__device__ __forceinline__ u64 WantOf(float top_p, u64 total) {
+  const u64 w = (u64)ceil((double)fmaxf(top_p, 0.f) * (double)total);
+  return w ? w : 1;
 }
 
-// The 32-bit number at which units, counted from the largest numbers down, reach
-// `want` (the smallest number, where they do not); `above`: the units of larger ones.
-// visit(f) calls f(number, unit) for the workgroup's numbers.
-template <typename V> __device__ unsigned Border(Shared &s, u64 want, u64 &above, V &&visit) {
-  unsigned prefix = 0;
-  above = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
+// ---- the steps -------------------------------------------------------------------
+
+template <int DT> __device__ __forceinline__ u64 Best(Shared &s, const Row<DT> &r, int from, int to) {
+  u64 best = 0;
+  r.Each(from, to, [&](const auto &v, int i) __attribute__((always_inline)) {
+    // the largest of the 16 bytes, and where it stands first
+    constexpr int N = sizeof(v) / 4;
+    float top = v[0];
+    int at = 0;
+#pragma unroll
+    for (int j = 1; j < N; ++j)
+      if (!(top >= v[j]) && v[j] == v[j]) top = v[j], at = j;
+    const u64 k = (u64)KeyOf(top) << 32 | (0xffffffffu - (unsigned)(i + at));
+    best = k > best ? k : best;
+  });
+  return GroupMax(s, best);
+}
+
+__device__ __forceinline__ void Clear(Shared &s) {
+  const int tid = threadIdx.x;
+  s.bin[2 * tid] = s.bin[2 * tid + 1] = 0;
+  s.chunk[tid] = 0;
+  if (tid < 32) s.power[tid] = exp2(-tid / 32.0);
+  if (tid == 0) s.n = 0;
+  __syncthreads();
+}
+
+// Counts, or weights, of the tokens in bins.
+template <int DT, bool WEIGHTS> __device__ __forceinline__ void FillBins(Shared &s, const Row<DT> &r, int from, int to) {
+  r.EachLogit(from, to, [&](float v, int) __attribute__((always_inline)) {
+    atomicAdd(&s.bin[r.Bin(v)], WEIGHTS ? r.Whole(r.Weight(v)) : 1ull);
+  });
+  __syncthreads();
+}
+
+// Where the border is: the bin with it, and how much there is in the bins above and in
+// it.  What is in bins above the border's is kept for certain, if `sure`; the tokens of
+// the border's bin, or (not `sure`) of it and all above, are listed, if `listed`.
+struct Place {
+  int bin;
+  int sure, listed, by_bits;
+  unsigned k;       // of top_k, 0 where it leaves nothing out
+  u64 above, want;  // top_p's
+};
+
+__device__ __forceinline__ int BinOf(Shared &s, u64 upto, u64 a, u64 b, u64 want, u64 &above, u64 &in) {
+  const int tid = threadIdx.x;
+  if (upto >= want && upto - a - b < want) {
+    const bool second = upto - b < want;
+    s.at = 2 * tid + second;
+    s.out[0] = second ? upto - b : upto - a - b;
+    s.out[1] = second ? b : a;
+  }
+  __syncthreads();
+  above = s.out[0];
+  in = s.out[1];
+  return (int)s.at;
+}
+// From bins of counts; `again`: top_k leaves nothing out and the list would not hold
+// all, so that top_p needs bins of weights.
+__device__ __forceinline__ Place PlaceOfCounts(Shared &s, const Wish &w, bool &again) {
+  const u64 a = s.bin[2 * threadIdx.x], b = s.bin[2 * threadIdx.x + 1];
+  u64 all, above, in;
+  const u64 upto = GroupScan(s, a + b, all);
+  again = false;
+  Place q{kBins - 1, 0, 1, 0, 0, 0, 0};
+  if (all <= kList) {  // list them all
+    q.k = all <= (u64)w.k ? 0 : (unsigned)w.k;
+    return q;
+  }
+  if (all <= (u64)w.k) {
+    again = w.cuts;
+    return Place{kBins, 1, 0, 0, 0, 0, 0};
+  }
+  q.bin = BinOf(s, upto, a, b, (u64)w.k, above, in);
+  q.k = (unsigned)w.k;
+  if (above + in > kList) q.listed = 0, q.by_bits = 1;
+  return q;
+}
+__device__ __forceinline__ Place PlaceOfWeights(Shared &s, const Wish &w) {
+  const u64 a = s.bin[2 * threadIdx.x], b = s.bin[2 * threadIdx.x + 1];
+  u64 all, in;
+  const u64 upto = GroupScan(s, a + b, all);
+  Place q{0, 1, 1, 0, 0, 0, 0};
+  q.want = WantOf(w.top_p, all);
+  q.bin = BinOf(s, upto, a, b, q.want, q.above, in);
+  return q;
+}
+
+// Lists what is to be listed, and adds what is kept for certain to its chunks.
+template <int DT> __device__ __forceinline__ void Take(Shared &s, const Row<DT> &r, const Place &q, int from, int to) {
+  const int lane = threadIdx.x % 64;
+  if (!q.listed) {  // all of it is kept, or nothing known
+    if (q.sure)
+      r.Each(from, to, [&](const auto &v, int i) __attribute__((always_inline)) {
+        u64 sum = 0;
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(v) / 4); ++j) sum += IsLogit(v[j]) ? r.Kept(v[j]) : 0;
+        if (sum) atomicAdd(&s.chunk[i >> r.shift], sum);
+      });
+    __syncthreads();
+    return;
+  }
+  // Few of a wave's tokens are kept: they wait in a queue until there is one for each lane.
+  u64 *queue = s.queue[threadIdx.x / 64];
+  int queued = 0;
+  auto weigh = [&](int count) __attribute__((always_inline)) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const u64 e = queue[lane], more = queue[64 + lane];
+    if (lane < count) {
+      const u64 kept = r.Kept(__builtin_bit_cast(float, (unsigned)(e >> 32)));
+      if (kept) atomicAdd(&s.chunk[(unsigned)e >> r.shift], kept);
+    }
+    queue[lane] = more;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  r.Each(from, to, [&](const auto &v, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(v) / 4); ++j) {
+      const int b = r.Bin(v[j]);
+      const bool is = IsLogit(v[j]), mine = is && (b == q.bin || (!q.sure && b < q.bin));
+      const u64 vote = __ballot(mine);
+      if (vote) {
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(&s.n, (unsigned)__popcll(vote));
+        at = __builtin_amdgcn_readfirstlane(at) + __builtin_amdgcn_mbcnt_hi((unsigned)(vote >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)vote, 0));
+        if (mine && at < kList) s.list[at] = (u64)KeyOf(v[j]) << 32 | (unsigned)(i + j);
+      }
+      if (q.sure) {
+        const bool sure = is && b < q.bin;
+        const u64 kept = __ballot(sure);
+        if (kept) {
+          const int at = queued + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(kept >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)kept, 0));
+          if (sure) queue[at] = (u64)__builtin_bit_cast(unsigned, v[j]) << 32 | (unsigned)(i + j);
+          queued += __popcll(kept);
+          if (queued >= 64) {
+            weigh(64);
+            queued -= 64;
+          }
+        }
+      }
+    }
+  });
+  if (queued) weigh(queued);
+  __syncthreads();
+}
+
+// The number at which units, counted from the largest numbers down, reach `want` (the
+// smallest number, where they do not); `above` and `in`: the units of larger ones and of
+// it.  visit(f) calls f(number, unit) for the workgroup's numbers, from lo to hi.
+template <typename V>
+__device__ unsigned Border(Shared &s, unsigned lo, unsigned hi, u64 want, u64 &above, u64 &in, V &&visit) {
+  const int bits = hi > lo ? 32 - __builtin_clz(hi - lo) : 0;
+  unsigned prefix = 0;  // of the number less lo
+  above = in = 0;
+  for (int shift = (bits + 7) / 8 * 8 - 8 < 0 ? 0 : (bits + 7) / 8 * 8 - 8; shift >= 0; shift -= 8) {
     __syncthreads();
     if (threadIdx.x < 256) s.digit[threadIdx.x] = 0;
     __syncthreads();
     visit([&](unsigned number, u64 unit) __attribute__((always_inline)) {
+      number -= lo;
       if (shift == 24 || number >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s.digit[number >> shift & 255], unit);
     });
     __syncthreads();
@@ -164,303 +402,198 @@ template <typename V> __device__ unsigned Border(Shared &s, u64 want, u64 &above
       u64 d[4], sum = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum += d[j] = s.digit[255 - 4 * lane - j];
-      u64 upto = sum;
-      for (int o = 1; o < 64; o <<= 1) {
-        const u64 w = __shfl_up(upto, o);
-        if (lane >= o) upto += w;
-      }
-      const u64 reach = __ballot(above + upto >= want);
+      const u64 upto = WaveScan(sum), reach = __ballot(above + upto >= want);
       if (lane == (reach ? __builtin_ctzll(reach) : 63)) {
         u64 a = above + upto - sum;
         int j = 0;
         for (; j < 3 && a + d[j] < want; ++j) a += d[j];
         s.out[0] = a;
+        s.out[1] = d[j];
         s.at = 255 - 4 * lane - j;
       }
     }
     __syncthreads();
     above = s.out[0];
+    in = s.out[1];
     prefix |= s.at << shift;
   }
-  return prefix;
+  return lo + prefix;
 }
 
-// The token at which the weights up to it reach this is the last that top_p keeps.
-__device__ __forceinline__ u64 WantOf(float top_p, u64 total) {
-  const u64 w = (u64)ceil((double)fmaxf(top_p, 0.f) * (double)total);
-  return w ? w : 1;
+// Kept are the tokens with a larger key, and of those with this key the ones up to an
+// index.
+struct Edge {
+  unsigned key, last;
+};
+
+// The border among tokens that visit(f) gives as f(key, weight, index), their keys from lo to
+// hi: of top_k, then of top_p.
+template <int DT, typename V>
+__device__ __forceinline__ Edge EdgeOf(Shared &s, const Row<DT> &r, const Wish &w, const Place &q, unsigned lo, unsigned hi, V &&visit) {
+  Edge e{0, 0};
+  u64 over, in, ties = 0, equal = 0, want = q.want - q.above;
+  if (q.k) {
+    e.key = Border(s, lo, hi, q.k, over, in, [&](auto &&f) { visit([&](unsigned key, float, int) { f(key, 1ull); }); });
+    ties = q.k - over;
+    equal = in;
+    lo = e.key;
+  }
+  if (w.cuts) {
+    auto weights = [&](auto &&f) {
+      visit([&](unsigned key, float v, int) {
+        if (key >= e.key) f(key, r.Whole(r.Weight(v)));
+      });
+    };
+    if (!q.want) {
+      // the sum of what top_k leaves
+      u64 mine = 0, total;
+      weights([&](unsigned key, u64 one) { mine += key > e.key ? one : 0; });
+      GroupScan(s, mine, total);
+      want = WantOf(w.top_p, total + (e.key ? ties * r.Whole(r.Weight(LogitOf(e.key))) : 0));
+    }
+    const unsigned b = Border(s, lo, hi, want, over, in, weights);
+    const u64 one = r.Whole(r.Weight(LogitOf(b))), left = want > over ? want - over : 0;
+    const u64 n = one ? (left + one - 1) / one : 1;
+    if (!q.k || b != e.key || n < ties) ties = n;
+    equal = one ? in / one : ~u64(0);
+    e.key = b;
+  }
+  e.last = ~0u;
+  if (ties < equal)
+    e.last = ~Border(s, ~(unsigned)(r.vocab - 1), ~0u, ties, over, in, [&](auto &&f) {
+      visit([&](unsigned key, float, int i) {
+        if (key == e.key) f(~(unsigned)i, 1ull);
+      });
+    });
+  return e;
 }
 
-template <int DT> __global__ __launch_bounds__(kThreads) void SampleRowKernel(const SampleParams p) {
-  __shared__ Shared s;
-  const int tid = threadIdx.x, lane = tid % 64;
-  const int64_t row = p.first + blockIdx.x;
-  Row<DT> r{p.x, row * p.vocab, p.vocab, 0.f, 0.f, 0.0, 0.0, s.power};
-  auto answer = [&](int64_t token, float probability) {
-    if (p.token64)
-      static_cast<int64_t *>(p.token)[row] = token;
-    else
-      static_cast<int32_t *>(p.token)[row] = (int32_t)token;
-    if (p.probability) p.probability[row] = probability;
-  };
-  if (tid < 32) s.power[tid] = exp2(-tid / 32.0);
-
-  // the largest logit, and the lowest index that has it
-  u64 best = 0;
-  r.Each([&](const auto &v, int i, auto n) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < n; ++j) {
-      const u64 k = (u64)KeyOf(v[j]) << 32 | (0xffffffffu - (unsigned)(i + j));
-      best = k > best ? k : best;
-    }
-  });
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 k = __shfl_xor(best, o);
-    best = k > best ? k : best;
-  }
-  if (lane == 0) s.wave[tid / 64] = best;
-  __syncthreads();
-  for (int i = 0; i < kWaves; ++i) best = s.wave[i] > best ? s.wave[i] : best;
-  const unsigned top = (unsigned)(best >> 32);
-  const float T = p.temperature ? p.temperature[row] : 1.f;
-  int64_t k = 0;
-  if (p.top_k) k = p.k64 ? static_cast<const int64_t *>(p.top_k)[row] : (int64_t) static_cast<const int32_t *>(p.top_k)[row];
-  if (k >= p.vocab) k = 0;
-  if (top == 0 || !(T > 0.f) || k == 1) {
-    if (tid == 0) answer(top == 0 ? -1 : (int64_t)(0xffffffffu - (unsigned)best), top == 0 ? 0.f : 1.f);
-    return;
-  }
-  const float tp = p.top_p ? p.top_p[row] : 1.f, mp = p.min_p ? p.min_p[row] : 0.f;
-  const bool cuts = tp < 1.f;
-  r.top = LogitOf(top);
-  r.octaves = 1.4426950408889634074 / (double)T;
-  r.per_bin = (float)(r.octaves * (kBins / kOctaves));
-  r.least = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
-
-  // the bin with the border, and how much is in those above: counts for top-k, weights
-  // for top-p
-  auto bin_of = [&](u64 want, u64 &above, u64 &in, u64 &all) {
-    const u64 a = s.bin[2 * tid], b = s.bin[2 * tid + 1], upto = GroupScan(s, a + b, all);
-    if (want > all) want = all;
-    __syncthreads();
-    if (upto >= want && upto - a - b < want) {
-      const bool second = upto - b < want;
-      s.at = 2 * tid + second;
-      s.out[0] = second ? upto - b : upto - a - b;
-      s.out[1] = second ? b : a;
-    }
-    __syncthreads();
-    above = s.out[0];
-    in = s.out[1];
-    return (int)s.at;
-  };
-  auto clear = [&] {
-    s.bin[2 * tid] = s.bin[2 * tid + 1] = 0;
-    s.chunk[tid] = 0;
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-  };
-  clear();
-  int border_bin = kBins;  // all below it in number is kept
-  u64 above = 0, in = 0, all = 0, want = 0;
-  if (k > 0) {
-    r.Each([&](const auto &v, int, auto n) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < n; ++j)
-        if (KeyOf(v[j])) atomicAdd(&s.bin[r.Bin(v[j])], 1ull);
-    });
-    __syncthreads();
-    border_bin = bin_of((u64)k, above, in, all);
-    if (all <= (u64)k) {
-      k = 0;  // nothing to leave out
-      border_bin = kBins;
-      __syncthreads();
-      clear();
-    }
-  }
-  if (k <= 0 && cuts) {
-    r.Each([&](const auto &v, int, auto n) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < n; ++j)
-        if (KeyOf(v[j])) atomicAdd(&s.bin[r.Bin(v[j])], r.Whole(r.Weight(v[j])));
-    });
-    __syncthreads();
-    u64 none;
-    const u64 total = (bin_of(~u64(0), above, none, all), all);
-    want = WantOf(tp, total);
-    __syncthreads();
-    border_bin = bin_of(want, above, none, all);
-  }
-  // top-k lists its bin and all above it, top-p its bin alone; what is kept for certain
-  // goes to its chunk
-  const int size = (p.vocab + kChunks * 8 - 1) / (kChunks * 8) * 8;  // tokens of a chunk
-  const bool few = k > 0 && above + in <= kList;
-  auto take = [&](bool listed, float v, int i) __attribute__((always_inline)) {
-    const u64 vote = __ballot(listed);
-    if (!vote) return;
-    unsigned at = 0;
-    if (lane == (int)__builtin_ctzll(vote)) at = atomicAdd(&s.n, (unsigned)__popcll(vote));
-    at = __shfl(at, (int)__builtin_ctzll(vote)) + (unsigned)__popcll(vote & ((u64(1) << lane) - 1));
-    if (listed && at < kList) s.list[at] = (u64)KeyOf(v) << 32 | (unsigned)i;
-  };
-  const bool by_list = k > 0 ? few : cuts;
-  if (k <= 0 || few) {
-    r.Each([&](const auto &v, int i, auto n) __attribute__((always_inline)) {
-      u64 sum = 0;
-#pragma unroll
-      for (int j = 0; j < n; ++j) {
-        const bool is = KeyOf(v[j]) != 0;
-        const int b = r.Bin(v[j]);
-        if (by_list) take(is && (k > 0 ? b <= border_bin : b == border_bin), v[j], i + j);
-        if (k <= 0 && is && b < border_bin) sum += r.Kept(v[j]);
-      }
-      if (sum) atomicAdd(&s.chunk[i / size], sum);
-    });
-    __syncthreads();
-  }
-  // kept are the tokens with a larger key than `border`, and of those with that key the
-  // ones up to index `last`
-  unsigned border = 0, last = 0;
+// The border, and the chunks' weights with what was listed.
+template <int DT> __device__ __forceinline__ Edge Resolve(Shared &s, const Row<DT> &r, const Wish &w, const Place &q) {
+  Edge edge{0, ~0u};
   const unsigned n = s.n;
-  if (by_list && n <= kList) {
+  if (q.listed && n <= kList) {
     constexpr int E = kList / kThreads;
-    u64 e[E], w[E];
+    u64 e[E];
+    unsigned lo = ~0u, hi = 0;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const unsigned i = j * kThreads + tid;
+      const unsigned i = j * kThreads + threadIdx.x;
       e[j] = i < n ? s.list[i] : 0;
-      w[j] = e[j] ? r.Whole(r.Weight(LogitOf((unsigned)(e[j] >> 32)))) : 0;
+      if (!e[j]) continue;
+      lo = min(lo, (unsigned)(e[j] >> 32));
+      hi = max(hi, (unsigned)(e[j] >> 32));
     }
-    auto counts = [&](auto &&f) {
+    auto listed = [&](auto &&f) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if (e[j]) f((unsigned)(e[j] >> 32), 1ull);
+        if (e[j]) f((unsigned)(e[j] >> 32), LogitOf((unsigned)(e[j] >> 32)), (int)(unsigned)e[j]);
     };
-    u64 over = 0, ties = ~u64(0);
-    if (k > 0) {
-      border = Border(s, (u64)k, over, counts);
-      ties = (u64)k - over;
-      if (cuts) {
-        u64 mine = 0, total = 0;
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if ((unsigned)(e[j] >> 32) > border) mine += w[j];
-        GroupScan(s, mine, total);
-        want = WantOf(tp, total + ties * r.Whole(r.Weight(LogitOf(border))));
-      }
-      above = 0;
+    if (q.k || w.cuts) {
+      // the largest and the complement of the smallest, at once: neither is 0
+      hi = (unsigned)(GroupMax(s, hi));
+      lo = ~(unsigned)GroupMax(s, ~lo);
+      edge = EdgeOf(s, r, w, q, lo, hi, listed);
     }
-    if (cuts) {
-      const unsigned floor = border;
-      const unsigned b = Border(s, want - above, over, [&](auto &&f) {
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (e[j] && (unsigned)(e[j] >> 32) >= floor) f((unsigned)(e[j] >> 32), w[j]);
-      });
-      const u64 one = r.Whole(r.Weight(LogitOf(b))), left = want - above > over ? want - above - over : 0;
-      const u64 m = one ? (left + one - 1) / one : 1;
-      ties = b == border && ties < m ? ties : m;
-      border = b;
-    }
-    // the first `ties` of the equal ones: the largest numbers ~index
-    u64 none;
-    last = ~Border(s, ties, none, [&](auto &&f) {
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (e[j] && (unsigned)(e[j] >> 32) == border) f(~(unsigned)e[j], 1ull);
-    });
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const unsigned key = (unsigned)(e[j] >> 32), i = (unsigned)e[j];
-      if (key > border || (e[j] && key == border && i <= last)) {
-        const u64 kept = r.Kept(LogitOf(key));
-        if (kept) atomicAdd(&s.chunk[i / size], kept);
-      }
-    }
-    __syncthreads();
-  } else if (k > 0 || cuts) {
-    // by the bits of all logits
-    auto each = [&](auto &&f) {
-      r.Each([&](const auto &v, int i, auto m) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < m; ++j) {
-          const unsigned key = KeyOf(v[j]);
-          if (key) f(key, v[j], i + j);
-        }
-      });
-    };
-    u64 over = 0, ties = ~u64(0), total = 0;
-    if (k > 0) {
-      border = Border(s, (u64)k, over, [&](auto &&f) { each([&](unsigned key, float, int) { f(key, 1ull); }); });
-      ties = (u64)k - over;
-      if (cuts) {
-        u64 mine = 0;
-        each([&](unsigned key, float v, int) {
-          if (key > border) mine += r.Whole(r.Weight(v));
-        });
-        GroupScan(s, mine, total);
-        want = WantOf(tp, total + ties * r.Whole(r.Weight(LogitOf(border))));
-      }
-    }
-    if (cuts) {
-      const unsigned floor = border;
-      const unsigned b = Border(s, want, over, [&](auto &&f) {
-        each([&](unsigned key, float v, int) {
-          if (key >= floor) f(key, r.Whole(r.Weight(v)));
-        });
-      });
-      const u64 one = r.Whole(r.Weight(LogitOf(b))), left = want > over ? want - over : 0;
-      const u64 m = one ? (left + one - 1) / one : 1;
-      ties = b == border && ties < m ? ties : m;
-      border = b;
-    }
-    u64 none;
-    last = ~Border(s, ties, none, [&](auto &&f) {
-      each([&](unsigned key, float, int i) {
-        if (key == border) f(~(unsigned)i, 1ull);
-      });
-    });
-    __syncthreads();
-    s.chunk[tid] = 0;
-    __syncthreads();
-    each([&](unsigned key, float v, int i) {
-      if (key > border || (key == border && (unsigned)i <= last)) {
+    listed([&](unsigned key, float v, int i) {
+      if (key > edge.key || (key == edge.key && (unsigned)i <= edge.last)) {
         const u64 kept = r.Kept(v);
-        if (kept) atomicAdd(&s.chunk[i / size], kept);
+        if (kept) atomicAdd(&s.chunk[i >> r.shift], kept);
+      }
+    });
+    __syncthreads();
+  } else if (q.listed || q.by_bits) {
+    auto logits = [&](auto &&f) { r.EachLogit(0, r.vocab, [&](float v, int i) { f(KeyOf(v), v, i); }); };
+    Place whole = q;  // among all tokens
+    whole.above = 0;
+    edge = EdgeOf(s, r, w, whole, 1, ~0u, logits);
+    __syncthreads();
+    s.chunk[threadIdx.x] = 0;
+    __syncthreads();
+    logits([&](unsigned key, float v, int i) {
+      if (key > edge.key || (key == edge.key && (unsigned)i <= edge.last)) {
+        const u64 kept = r.Kept(v);
+        if (kept) atomicAdd(&s.chunk[i >> r.shift], kept);
       }
     });
     __syncthreads();
   }
+  return edge;
+}
 
-  // the chunk, then the token, at which the kept weights pass the share
+// The chunk, then the token, at which the kept weights pass the share.
+template <int DT> __device__ __forceinline__ void Choose(Shared &s, const Row<DT> &r, const SampleParams &p, int64_t row, const Edge &edge) {
   u64 total;
-  const u64 mine = s.chunk[tid], upto = GroupScan(s, mine, total);
+  const u64 mine = s.chunk[threadIdx.x], upto = GroupScan(s, mine, total);
   float u = p.uniform[row];
   u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
   u64 share = (u64)((double)u * (double)total);
   if (share >= total) share = total - 1;
   if (upto > share && upto - mine <= share) {
-    s.at = tid;
+    s.at = threadIdx.x;
     s.out[0] = share - (upto - mine);
   }
   __syncthreads();
-  const int from = (int)s.at * size;
+  const int size = 1 << r.shift, from = (int)s.at << r.shift;
   u64 left = s.out[0];
   for (int i0 = 0; i0 < size; i0 += kThreads) {
-    const int i = from + i0 + tid;
-    u64 kept = 0;
+    const int i = from + i0 + (int)threadIdx.x;
+    u64 kept = 0, sum;
     float v = 0.f;
-    if (i0 + tid < size && i < p.vocab) {
+    if (i0 + (int)threadIdx.x < size && i < r.vocab) {
       v = r.At(i);
       const unsigned key = KeyOf(v);
-      if (key > border || (key != 0 && key == border && (unsigned)i <= last)) kept = r.Kept(v);
+      if (key > edge.key || (key != 0 && key == edge.key && (unsigned)i <= edge.last)) kept = r.Kept(v);
     }
-    u64 sum;
     const u64 incl = GroupScan(s, kept, sum);
-    if (incl > left && incl - kept <= left) answer(i, (float)(r.Weight(v) / ((double)total * 0x1p-42)));
+    if (incl > left && incl - kept <= left) Answer(p, row, i, (float)(r.Weight(v) / ((double)total * 0x1p-42)));
     if (sum > left) return;
     left -= sum;
   }
+}
+
+// ---- a workgroup a row --------------------------------------------------------------
+
+template <int DT> __device__ __forceinline__ Row<DT> RowOf(const SampleParams &p, int64_t row, const Shared &s) {
+  Row<DT> r{};
+  r.x = p.x;
+  r.base = row * p.vocab;
+  r.vocab = p.vocab;
+  // chunks of at least the 8 tokens of a load
+  r.shift = 3;
+  while ((p.vocab - 1) >> r.shift >= kChunks) ++r.shift;
+  r.power = s.power;
+  return r;
+}
+
+template <int DT> __global__ __launch_bounds__(kThreads) void SampleRowKernel(const SampleParams p) {
+  __shared__ Shared s;
+  const int64_t row = p.first + blockIdx.x;
+  Row<DT> r = RowOf<DT>(p, row, s);
+  Clear(s);
+  const u64 best = Best(s, r, 0, p.vocab);
+  const Wish w = WishOf(p, row);
+  if (Plain(w, best)) {
+    if (threadIdx.x == 0) AnswerPlain(p, row, best);
+    return;
+  }
+  r.Weigh(LogitOf((unsigned)(best >> 32)), w.T, w.min_p);
+  Place q{kBins, 1, 0, 0, 0, 0, 0};
+  bool again = w.k == 0 && w.cuts;
+  if (w.k > 0) {
+    FillBins<DT, false>(s, r, 0, p.vocab);
+    q = PlaceOfCounts(s, w, again);
+    if (again) {
+      __syncthreads();
+      Clear(s);
+    }
+  }
+  if (again) {
+    FillBins<DT, true>(s, r, 0, p.vocab);
+    q = PlaceOfWeights(s, w);
+  }
+  Take(s, r, q, 0, p.vocab);
+  Choose(s, r, p, row, Resolve(s, r, w, q));
 }
 
 }  // namespace
