@@ -157,11 +157,11 @@ template <int DT> struct Row {
   // what min_p leaves of a token's weight
   __device__ __forceinline__ u64 Kept(float v) const {
     const double w = Weight(v);
-    return w >= least ? Whole(w) : 0;
+    return Whole(w >= least ? w : 0.0);
   }
-  // falls with v, as every rounding in it does
+  // falls with v, as every rounding in it does; anything for a NaN
   __device__ __forceinline__ int Bin(float v) const {
-    return (int)__builtin_amdgcn_fmed3f((top - v) * per_bin, 0.f, (float)(kBins - 1));
+    return (int)__builtin_amdgcn_fmed3f((top - v) * per_bin, 0.f, (float)(kBins - 1)) & (kBins - 1);
   }
   // f(logits, first index) for 16 bytes at a time of the tokens from..to - 1, four of them
   // on their way; what is past the end is -inf
@@ -185,7 +185,7 @@ template <int DT> struct Row {
         if (wave + u * kThreads * N < to) f(v[u], i0 + (u * kThreads + (int)threadIdx.x) * N);
     }
   }
-  // f(logit, index) for each that can be chosen
+  // f(logit, index) for each that can be chosen, one after the other
   template <typename F> __device__ __forceinline__ void EachLogit(int from, int to, F &&f) const {
     Each(from, to, [&](const auto &v, int i) __attribute__((always_inline)) {
 #pragma unroll
@@ -234,7 +234,15 @@ __device__ __forceinline__ u64 WantOf(float top_p, u64 total) {
 
 // ---- the steps -------------------------------------------------------------------
 
-template <int DT> __device__ __forceinline__ u64 Best(Shared &s, const Row<DT> &r, int from, int to) {
+// The values are made where they stand, not where they are used: one after the other,
+// behind a branch each, they wait for themselves (a row of 131072 42 us in place of 16).
+template <int N> __device__ __forceinline__ void Made(u64 (&w)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(w[j]));
+}
+
+// Of the workgroup; `own` of the thread.
+template <int DT> __device__ __forceinline__ u64 Best(Shared &s, const Row<DT> &r, int from, int to, u64 &own) {
   u64 best = 0;
   r.Each(from, to, [&](const auto &v, int i) __attribute__((always_inline)) {
     // the largest of the 16 bytes, and where it stands first
@@ -247,6 +255,7 @@ template <int DT> __device__ __forceinline__ u64 Best(Shared &s, const Row<DT> &
     const u64 k = (u64)KeyOf(top) << 32 | (0xffffffffu - (unsigned)(i + at));
     best = k > best ? k : best;
   });
+  own = best;
   return GroupMax(s, best);
 }
 
@@ -261,21 +270,32 @@ __device__ __forceinline__ void Clear(Shared &s) {
 
 // Counts, or weights, of the tokens in bins.
 template <int DT, bool WEIGHTS> __device__ __forceinline__ void FillBins(Shared &s, const Row<DT> &r, int from, int to) {
-  r.EachLogit(from, to, [&](float v, int) __attribute__((always_inline)) {
-    atomicAdd(&s.bin[r.Bin(v)], WEIGHTS ? r.Whole(r.Weight(v)) : 1ull);
+  r.Each(from, to, [&](const auto &v, int) __attribute__((always_inline)) {
+    constexpr int N = sizeof(v) / 4;
+    u64 w[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = WEIGHTS ? r.Whole(r.Weight(v[j])) : IsLogit(v[j]);
+    Made(w);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (w[j]) atomicAdd(&s.bin[r.Bin(v[j])], w[j]);
   });
   __syncthreads();
 }
 
-// Where the border is: the bin with it, and how much there is in the bins above and in
-// it.  What is in bins above the border's is kept for certain, if `sure`; the tokens of
-// the border's bin, or (not `sure`) of it and all above, are listed, if `listed`.
+// Where the border is.  If `sure`, the tokens in bins above the border's are kept for
+// certain, and those of its bin are listed, if `listed`; else it is among the tokens of
+// bins up to `bin` that are at least `least`, and those are listed.
 struct Place {
   int bin;
   int sure, listed, by_bits;
   unsigned k;       // of top_k, 0 where it leaves nothing out
-  u64 above, want;  // top_p's
+  u64 above, want;  // top_p's: weights of the bins above, and up to the border
+  float least;
 };
+
+__device__ __forceinline__ Place KeepAll() { return Place{kBins, 1, 0, 0, 0, 0, 0, -__builtin_huge_valf()}; }
+__device__ __forceinline__ Place ListAll(unsigned k) { return Place{kBins - 1, 0, 1, 0, k, 0, 0, -__builtin_huge_valf()}; }
 
 __device__ __forceinline__ int BinOf(Shared &s, u64 upto, u64 a, u64 b, u64 want, u64 &above, u64 &in) {
   const int tid = threadIdx.x;
@@ -297,28 +317,34 @@ __device__ __forceinline__ Place PlaceOfCounts(Shared &s, const Wish &w, bool &a
   u64 all, above, in;
   const u64 upto = GroupScan(s, a + b, all);
   again = false;
-  Place q{kBins - 1, 0, 1, 0, 0, 0, 0};
-  if (all <= kList) {  // list them all
-    q.k = all <= (u64)w.k ? 0 : (unsigned)w.k;
-    return q;
-  }
+  if (all <= kList) return ListAll(all <= (u64)w.k ? 0 : (unsigned)w.k);
   if (all <= (u64)w.k) {
     again = w.cuts;
-    return Place{kBins, 1, 0, 0, 0, 0, 0};
+    return KeepAll();
   }
-  q.bin = BinOf(s, upto, a, b, (u64)w.k, above, in);
-  q.k = (unsigned)w.k;
-  if (above + in > kList) q.listed = 0, q.by_bits = 1;
-  return q;
+  const int bin = BinOf(s, upto, a, b, (u64)w.k, above, in);
+  if (above + in > kList) return Place{0, 0, 0, 1, (unsigned)w.k, 0, 0, 0.f};
+  return Place{bin, 0, 1, 0, (unsigned)w.k, 0, 0, -__builtin_huge_valf()};
 }
 __device__ __forceinline__ Place PlaceOfWeights(Shared &s, const Wish &w) {
   const u64 a = s.bin[2 * threadIdx.x], b = s.bin[2 * threadIdx.x + 1];
   u64 all, in;
   const u64 upto = GroupScan(s, a + b, all);
-  Place q{0, 1, 1, 0, 0, 0, 0};
+  Place q{0, 1, 1, 0, 0, 0, 0, 0.f};
   q.want = WantOf(w.top_p, all);
   q.bin = BinOf(s, upto, a, b, q.want, q.above, in);
   return q;
+}
+
+// Voting lanes before this one.
+__device__ __forceinline__ int Before(u64 vote) {
+  return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(vote >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)vote, 0));
+}
+__device__ __forceinline__ void List(Shared &s, u64 vote, bool mine, float v, int i) {
+  unsigned at = 0;
+  if (threadIdx.x % 64 == 0) at = atomicAdd(&s.n, (unsigned)__popcll(vote));
+  at = __builtin_amdgcn_readfirstlane(at) + Before(vote);
+  if (mine && at < kList) s.list[at] = (u64)KeyOf(v) << 32 | (unsigned)i;
 }
 
 // Lists what is to be listed, and adds what is kept for certain to its chunks.
@@ -327,9 +353,10 @@ template <int DT> __device__ __forceinline__ void Take(Shared &s, const Row<DT> 
   if (!q.listed) {  // all of it is kept, or nothing known
     if (q.sure)
       r.Each(from, to, [&](const auto &v, int i) __attribute__((always_inline)) {
+        // -inf and NaN weigh 2^-1000, which is 0 in whole units
         u64 sum = 0;
 #pragma unroll
-        for (int j = 0; j < (int)(sizeof(v) / 4); ++j) sum += IsLogit(v[j]) ? r.Kept(v[j]) : 0;
+        for (int j = 0; j < (int)(sizeof(v) / 4); ++j) sum += r.Kept(v[j]);
         if (sum) atomicAdd(&s.chunk[i >> r.shift], sum);
       });
     __syncthreads();
@@ -352,25 +379,17 @@ template <int DT> __device__ __forceinline__ void Take(Shared &s, const Row<DT> 
 #pragma unroll
     for (int j = 0; j < (int)(sizeof(v) / 4); ++j) {
       const int b = r.Bin(v[j]);
-      const bool is = IsLogit(v[j]), mine = is && (b == q.bin || (!q.sure && b < q.bin));
-      const u64 vote = __ballot(mine);
-      if (vote) {
-        unsigned at = 0;
-        if (lane == 0) at = atomicAdd(&s.n, (unsigned)__popcll(vote));
-        at = __builtin_amdgcn_readfirstlane(at) + __builtin_amdgcn_mbcnt_hi((unsigned)(vote >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)vote, 0));
-        if (mine && at < kList) s.list[at] = (u64)KeyOf(v[j]) << 32 | (unsigned)(i + j);
-      }
-      if (q.sure) {
-        const bool sure = is && b < q.bin;
-        const u64 kept = __ballot(sure);
-        if (kept) {
-          const int at = queued + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(kept >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)kept, 0));
-          if (sure) queue[at] = (u64)__builtin_bit_cast(unsigned, v[j]) << 32 | (unsigned)(i + j);
-          queued += __popcll(kept);
-          if (queued >= 64) {
-            weigh(64);
-            queued -= 64;
-          }
+      const bool is = IsLogit(v[j]);
+      const bool mine = is && (q.sure ? b == q.bin : b <= q.bin && v[j] >= q.least), sure = is && q.sure && b < q.bin;
+      const u64 vote = __ballot(mine), kept = __ballot(sure);
+      if (vote) List(s, vote, mine, v[j], i + j);
+      if (kept) {
+        const int at = queued + Before(kept);
+        if (sure) queue[at] = (u64)__builtin_bit_cast(unsigned, v[j]) << 32 | (unsigned)(i + j);
+        queued += __popcll(kept);
+        if (queued >= 64) {
+          weigh(64);
+          queued -= 64;
         }
       }
     }
@@ -382,12 +401,14 @@ template <int DT> __device__ __forceinline__ void Take(Shared &s, const Row<DT> 
 // The number at which units, counted from the largest numbers down, reach `want` (the
 // smallest number, where they do not); `above` and `in`: the units of larger ones and of
 // it.  visit(f) calls f(number, unit) for the workgroup's numbers, from lo to hi.
-template <typename V>
+// LAST: the shift of the last digit looked at; with more than 0 the result is the
+// smallest number with the digits before.
+template <int LAST = 0, typename V>
 __device__ unsigned Border(Shared &s, unsigned lo, unsigned hi, u64 want, u64 &above, u64 &in, V &&visit) {
   const int bits = hi > lo ? 32 - __builtin_clz(hi - lo) : 0;
   unsigned prefix = 0;  // of the number less lo
   above = in = 0;
-  for (int shift = (bits + 7) / 8 * 8 - 8 < 0 ? 0 : (bits + 7) / 8 * 8 - 8; shift >= 0; shift -= 8) {
+  for (int shift = (bits + 7) / 8 * 8 - 8 < 0 ? 0 : (bits + 7) / 8 * 8 - 8; shift >= LAST; shift -= 8) {
     __syncthreads();
     if (threadIdx.x < 256) s.digit[threadIdx.x] = 0;
     __syncthreads();
@@ -420,6 +441,20 @@ __device__ unsigned Border(Shared &s, unsigned lo, unsigned hi, u64 want, u64 &a
   return lo + prefix;
 }
 
+// From every thread's largest key: where the k-th of those stands, at least k tokens do,
+// and hardly more while k is well below the number of threads.
+constexpr int kFew = 512;
+__device__ __forceinline__ bool PlaceOfLargest(Shared &s, const Wish &w, u64 best, u64 own, Place &q) {
+  u64 above, in;
+  const unsigned key = Border<16>(s, 1, (unsigned)(best >> 32), (u64)w.k, above, in, [&](auto &&f) {
+    if (own >> 32) f((unsigned)(own >> 32), 1ull);
+  });
+  if (above + in < (u64)w.k) return false;
+  q = ListAll((unsigned)w.k);
+  q.least = LogitOf(max(key, KeyOf(-kMaxFloat)));  // smaller keys are no logits
+  return true;
+}
+
 // Kept are the tokens with a larger key, and of those with this key the ones up to an
 // index.
 struct Edge {
@@ -434,7 +469,7 @@ __device__ __forceinline__ Edge EdgeOf(Shared &s, const Row<DT> &r, const Wish &
   u64 over, in, ties = 0, equal = 0, want = q.want - q.above;
   if (q.k) {
     e.key = Border(s, lo, hi, q.k, over, in, [&](auto &&f) { visit([&](unsigned key, float, int) { f(key, 1ull); }); });
-    ties = q.k - over;
+    ties = q.k - over < in ? q.k - over : in;  // fewer tokens than k may be there
     equal = in;
     lo = e.key;
   }
@@ -569,30 +604,40 @@ template <int DT> __device__ __forceinline__ Row<DT> RowOf(const SampleParams &p
 template <int DT> __global__ __launch_bounds__(kThreads) void SampleRowKernel(const SampleParams p) {
   __shared__ Shared s;
   const int64_t row = p.first + blockIdx.x;
+  const Wish w = WishOf(p, row);
   Row<DT> r = RowOf<DT>(p, row, s);
   Clear(s);
-  const u64 best = Best(s, r, 0, p.vocab);
-  const Wish w = WishOf(p, row);
+  u64 own;
+  const u64 best = Best(s, r, 0, p.vocab, own);
   if (Plain(w, best)) {
     if (threadIdx.x == 0) AnswerPlain(p, row, best);
     return;
   }
   r.Weigh(LogitOf((unsigned)(best >> 32)), w.T, w.min_p);
-  Place q{kBins, 1, 0, 0, 0, 0, 0};
-  bool again = w.k == 0 && w.cuts;
-  if (w.k > 0) {
-    FillBins<DT, false>(s, r, 0, p.vocab);
-    q = PlaceOfCounts(s, w, again);
-    if (again) {
+  Place q = KeepAll();
+  bool taken = false, weights = w.k == 0 && w.cuts;
+  if (p.vocab <= kList && (w.k > 0 || w.cuts)) {
+    q = ListAll((unsigned)w.k);
+    weights = false;
+  } else if (w.k > 0) {
+    if (w.k <= kFew && PlaceOfLargest(s, w, best, own, q)) {
+      Take(s, r, q, 0, p.vocab);
+      taken = s.n <= kList;
       __syncthreads();
-      Clear(s);
+      if (!taken) Clear(s);
+    }
+    if (!taken) {
+      FillBins<DT, false>(s, r, 0, p.vocab);
+      q = PlaceOfCounts(s, w, weights);
+      __syncthreads();
+      if (weights) Clear(s);
     }
   }
-  if (again) {
+  if (weights) {
     FillBins<DT, true>(s, r, 0, p.vocab);
     q = PlaceOfWeights(s, w);
   }
-  Take(s, r, q, 0, p.vocab);
+  if (!taken) Take(s, r, q, 0, p.vocab);
   Choose(s, r, p, row, Resolve(s, r, w, q));
 }
 
