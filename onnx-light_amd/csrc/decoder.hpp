@@ -167,7 +167,8 @@ struct RotaryAppendParams {
   RotaryTable t;          // ids nullptr: a token's place in its sequence
   void *q;                // [tokens, heads, head_dim]
   int heads;
-  int64_t groups;         // the launcher's: workgroups of all launches for a head
+  int64_t groups, blocks; // the launcher's: workgroups for queries, and for keys of a head,
+  bool stream;            // and whether q is written past the caches
 };
 void LaunchRotaryKvCacheAppend(const RotaryAppendParams &p, hipStream_t stream);
 

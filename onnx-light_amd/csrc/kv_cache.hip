@@ -93,11 +93,14 @@ __device__ __forceinline__ Wide8 JointValues(const RotaryTable &t, const uint16_
   return r;
 }
 
-// Queries of the joint rows: a token a wave.
+// Queries of the joint rows, by waves: a lane has 16 dimensions of a head, the wave as many
+// heads at once as that makes.
 template <int DT> __device__ __forceinline__ void RotateQueries(const RotaryAppendParams &p, int64_t wave, int64_t waves) {
   const KvCacheParams &c = p.a.c;
-  const int lane = threadIdx.x % 64, D = c.head_dim, gd = D / 8;
-  for (int64_t t = wave; t < c.tokens; t += waves) {
+  const int lane = threadIdx.x % 64, D = c.head_dim, parts = D / 16, at_once = 64 / parts;
+  const int units = (p.heads + at_once - 1) / at_once;  // of a token
+  for (int64_t u = wave; u < c.tokens * units; u += waves) {
+    const int64_t t = u / units;
     int b = -1;  // the first sequence that ends past the row
     for (int base = 0; base < c.batch && b < 0; base += 64) {
       const bool ends = base + lane < c.batch && c.start[base + lane + 1] > t;
@@ -105,16 +108,14 @@ template <int DT> __device__ __forceinline__ void RotateQueries(const RotaryAppe
       if (past) b = base + __builtin_ctzll(past);
     }
     if (b < 0 || c.start[b] > t || KvNewTokens(c, b) < 0) continue;
+    const int first = (int)(u % units) * at_once + lane / parts;
+    if (lane >= at_once * parts || first >= p.heads) continue;
     const int64_t pos = RotaryRow(p.t, t, (int64_t)c.lengths[b] - (c.start[b + 1] - t));
-    const uint16_t *row = static_cast<const uint16_t *>(p.a.k) + t * (p.heads + 2 * c.kv_heads) * (int64_t)D;
-    uint16_t *q = static_cast<uint16_t *>(p.q) + t * p.heads * (int64_t)D;
-    for (int i = lane; i < p.heads * gd; i += 64) {
-      const Wide8 w = JointValues<DT>(p.t, row + i / gd * D, i % gd * 8, true, pos);
-      uint16_t out[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) out[j] = DT == kFloat16 ? F32ToF16(w.v[j]) : F32ToBf16(w.v[j]);
-      __builtin_memcpy(q + (int64_t)i * 8, out, 16);
-    }
+    const int64_t from = t * (p.heads + 2 * c.kv_heads) * (int64_t)D, to = t * p.heads * (int64_t)D;
+    if (p.t.interleaved)
+      RotateHeads<DT, 1, true>(p.t, p.a.k, from, D, p.q, to, D, first, 1, p.heads, D, lane % parts, pos, p.stream);
+    else
+      RotateHeads<DT, 1, false>(p.t, p.a.k, from, D, p.q, to, D, first, 1, p.heads, D, lane % parts, pos, p.stream);
   }
 }
 
@@ -130,18 +131,26 @@ __global__ __launch_bounds__(THREADS) void KvAppendKernel(
   __shared__ unsigned s_top[THREADS / 64];
   const KvAppendParams &p = Append(all);
   const KvCacheParams &c = p.c;
-  const int head = blockIdx.y, tid = threadIdx.x, bt = c.block_tokens, D = c.head_dim, gd = D / 8;
-  const bool is_v = blockIdx.z != 0, fp8 = c.fp8;
+  const int tid = threadIdx.x, bt = c.block_tokens, D = c.head_dim, gd = D / 8;
+  int head = blockIdx.y;
+  bool is_v = blockIdx.z != 0;
+  int64_t block = p.first + blockIdx.x;
   if constexpr (JOINT != 0) {
-    if (blockIdx.z == 2) {
+    // the queries' workgroups first: they are the most, and what the others wait for, their
+    // block's maximum, is then waited for beside the last of them
+    if (block < all.groups) {
       constexpr int W = THREADS / 64;
-      const int64_t group = (p.first + blockIdx.x) * c.kv_heads + head;
-      RotateQueries<JOINT>(all, group * W + __builtin_amdgcn_readfirstlane(tid / 64), all.groups * c.kv_heads * W);
+      RotateQueries<JOINT>(all, block * W + __builtin_amdgcn_readfirstlane(tid / 64), all.groups * W);
       return;
     }
+    const unsigned rest = (unsigned)(block - all.groups), blocks = (unsigned)all.blocks;
+    block = rest % blocks;
+    head = (int)(rest / blocks % (unsigned)c.kv_heads);
+    is_v = rest / blocks >= (unsigned)c.kv_heads;
   }
+  const bool fp8 = c.fp8;
   int b, w;
-  if (!FindBlock(c, p.first + blockIdx.x, b, w)) return;
+  if (!FindBlock(c, block, b, w)) return;
   const int len = c.lengths[b], start = c.start[b], first = len - (c.start[b + 1] - start);
   const int j = (first >> c.block_shift) + w;
   const int64_t blk = c.table[(int64_t)b * c.max_blocks + j];
@@ -293,15 +302,22 @@ template <int THREADS, int NG, bool KEPT> void LaunchBlocks(KvAppendParams p, in
 }
 
 template <int THREADS, int NG, bool KEPT> void LaunchBlocks(RotaryAppendParams p, int64_t blocks, hipStream_t s) {
-  p.groups = blocks;
-  LaunchInPieces(blocks, THREADS, [&](int64_t first, unsigned count) {
+  const KvCacheParams &c = p.a.c;
+  const int D = c.head_dim, half = p.t.half, at_once = 64 / (D / 16);
+  // whole lines of an aligned q: its stores go past the caches (rotary.hip); not those of a few
+  // tokens, which the attention reads at once
+  p.stream = (p.t.interleaved ? D % 128 == 0 : half % 64 == 0 && (D / 2 - half) % 64 == 0) &&
+             reinterpret_cast<uintptr_t>(p.q) % 128 == 0 && THREADS > 64;
+  p.blocks = blocks;
+  // a piece a wave, and rounds past what the chip holds at once
+  p.groups = std::min<int64_t>((c.tokens * ((p.heads + at_once - 1) / at_once) + THREADS / 64 - 1) / (THREADS / 64), 1280);
+  LaunchInPieces(p.groups + 2 * blocks * c.kv_heads, THREADS, [&](int64_t first, unsigned count) {
     p.a.first = first;
-    const dim3 grid(count, (unsigned)p.a.c.kv_heads, 3);
-    const int lds = p.a.c.block_tokens * p.a.c.head_dim;
+    const int lds = c.block_tokens * D;
     if (p.a.bf16)
-      KvAppendKernel<THREADS, NG, KEPT, kBfloat16><<<grid, THREADS, lds, s>>>(p);
+      KvAppendKernel<THREADS, NG, KEPT, kBfloat16><<<count, THREADS, lds, s>>>(p);
     else
-      KvAppendKernel<THREADS, NG, KEPT, kFloat16><<<grid, THREADS, lds, s>>>(p);
+      KvAppendKernel<THREADS, NG, KEPT, kFloat16><<<count, THREADS, lds, s>>>(p);
   });
 }
 

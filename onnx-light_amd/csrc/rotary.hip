@@ -31,35 +31,6 @@ __device__ __forceinline__ void CosSin(double turns, float &c, float &s) {
   s = q >= 2 ? -b : b;
 }
 
-template <int DT, int N> __device__ __forceinline__ void Narrow(void *base, int64_t at, const float (&v)[N]) {
-  if constexpr (DT == kFloat) {
-    __builtin_memcpy(static_cast<float *>(base) + at, v, 4 * N);
-  } else {
-    uint16_t u[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) u[i] = DT == kFloat16 ? F32ToF16(v[i]) : F32ToBf16(v[i]);
-    __builtin_memcpy(static_cast<uint16_t *>(base) + at, u, 2 * N);
-  }
-}
-
-// The same past the caches: only for whole lines at a time.
-template <int DT> __device__ __forceinline__ void NarrowStream(void *base, int64_t at, const float (&v)[8]) {
-  constexpr int W = DT == kFloat ? 2 : 1;
-  typedef unsigned w4u __attribute__((ext_vector_type(4), aligned(2)));
-  w4u r[W];
-#pragma unroll
-  for (int i = 0; i < 4 * W; ++i) {
-    if constexpr (DT == kFloat)
-      r[i / 4][i % 4] = __builtin_bit_cast(unsigned, v[i]);
-    else
-      r[0][i] = DT == kFloat16 ? F32ToF16(v[2 * i]) | (unsigned)F32ToF16(v[2 * i + 1]) << 16
-                               : F32ToBf16(v[2 * i]) | (unsigned)F32ToBf16(v[2 * i + 1]) << 16;
-  }
-  char *y = static_cast<char *>(base) + at * (DT == kFloat ? 4 : 2);
-#pragma unroll
-  for (int i = 0; i < W; ++i) __builtin_nontemporal_store(r[i], reinterpret_cast<w4u *>(y + 16 * i));
-}
-
 // Bound by the stores.  A thread has N pairs of every step-th position and their
 // frequencies in registers; the threads of a position write its rows in one piece.
 template <int DT, int N> __global__ __launch_bounds__(256) void RotaryTablesKernel(const RotaryTablesParams p, int per_row) {
@@ -108,86 +79,24 @@ template <int DT> __global__ __launch_bounds__(256) void RotaryAnyKernel(const R
   Narrow<DT, 1>(p.y, ib, yb);
 }
 
-// Sixteen values a thread and head: eight pairs (i, d / 2 + i) or as many dimensions
-// that stay; where pairs are neighbours two eights half the head apart, each of which
-// turns or stays, so that the loads and the stores of neighbouring threads are one
-// piece.  Bound by memory: a thread takes its part of the token's table rows once for
-// HEADS heads, whose values are all on their way before the first is turned.
+// Sixteen values a thread and head (RotateHeads).  Bound by memory.
 // 2 x 40 x 8191 x 128 fp16, us, one head a thread | two | four | eight: 77 | 71 | 73 | 77.
 // Stores go past the caches where each is of whole lines (`stream`), past them | not:
 // 62.9 | 69.1 interleaved, half of the head turning, 65.2 | 71.5 in halves, all of it; not
 // where half of it turns in halves, lines in two pieces: 77.2 | 72.0.
-struct Sixteen {
-  float a[8], b[8];
-};
-__device__ __forceinline__ void Turn(float &a, float &b, float c, float s) {
-  const float t = a * c - b * s;
-  b = a * s + b * c;
-  a = t;
-}
-// four neighbouring pairs, from dimension `dim` on
-template <int DT, int HEADS, bool B>
-__device__ __forceinline__ void TurnEight(const RotaryTable &t, int64_t pos, int dim, Sixteen (&v)[HEADS]) {
-  if (dim >= 2 * t.half) return;
-  float c[4], s[4];
-  TableValues<DT, 4>(t, pos, dim / 2, c, s);
-#pragma unroll
-  for (int h = 0; h < HEADS; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float *x = B ? v[h].b : v[h].a;
-      Turn(x[2 * i], x[2 * i + 1], c[i], s[i]);
-    }
-}
 template <int DT, int HEADS, bool INTER>
 __global__ __launch_bounds__(256) void RotaryKernel(const RotaryParams p, int groups, int per_block, bool stream) {
   const int r = threadIdx.x / groups, g = threadIdx.x % groups;
   const int64_t token = (p.first + blockIdx.x) * per_block + r;
   if (r >= per_block || token >= p.tokens) return;
-  const int turning = p.t.half / 8, h0 = blockIdx.y * HEADS;
-  const bool turns = INTER ? 8 * g < 2 * p.t.half : g < turning;  // the first eight, and so anything
-  if (!turns && p.x == p.y) return;
-  const int da = INTER || turns ? 8 * g : 2 * p.t.half + 8 * (g - turning);
-  const int db = da + (INTER ? p.D / 2 : turns ? p.t.half : p.D / 2 - p.t.half);
   int64_t at = token * p.heads * p.D, pitch = p.D;
   if (p.by_head) {
     const int64_t b = p.tokens <= 0x7fffffff ? (unsigned)token / (unsigned)p.seq : token / p.seq;
     at = (b * p.heads * p.seq + (token - b * p.seq)) * p.D;
     pitch = p.seq * p.D;
   }
-  Sixteen v[HEADS];
-#pragma unroll
-  for (int h = 0; h < HEADS; ++h) {
-    const int64_t row = at + min(h0 + h, p.heads - 1) * pitch;
-    Widen<DT, 8>(p.x, row + da, v[h].a);
-    Widen<DT, 8>(p.x, row + db, v[h].b);
-  }
-  if (turns) {
-    const int64_t pos = RotaryRow(p.t, token, token);
-    if constexpr (INTER) {
-      TurnEight<DT, HEADS, false>(p.t, pos, da, v);
-      TurnEight<DT, HEADS, true>(p.t, pos, db, v);
-    } else {
-      float c[8], s[8];
-      TableValues<DT, 8>(p.t, pos, 8 * g, c, s);
-#pragma unroll
-      for (int h = 0; h < HEADS; ++h)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) Turn(v[h].a[i], v[h].b[i], c[i], s[i]);
-    }
-  }
-#pragma unroll
-  for (int h = 0; h < HEADS; ++h) {
-    if (h0 + h >= p.heads) break;
-    const int64_t row = at + (h0 + h) * pitch;
-    if (stream) {
-      NarrowStream<DT>(p.y, row + da, v[h].a);
-      NarrowStream<DT>(p.y, row + db, v[h].b);
-    } else {
-      Narrow<DT, 8>(p.y, row + da, v[h].a);
-      Narrow<DT, 8>(p.y, row + db, v[h].b);
-    }
-  }
+  RotateHeads<DT, HEADS, INTER>(p.t, p.x, at, pitch, p.y, at, pitch, blockIdx.y * HEADS, 1, p.heads, p.D, g,
+                                RotaryRow(p.t, token, token), stream);
 }
 
 template <int DT, int HEADS> void LaunchHeads(RotaryParams p, int groups, hipStream_t st) {
