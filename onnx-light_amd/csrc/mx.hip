@@ -197,12 +197,16 @@ Tiles TilesOf(const MxMatMulParams &p) {
 //   MXFP8  36 x 2048 x 8192 8.6 | 13.1      40 x 11008 x 8192 35.2 | 39.4
 //          40 x 4096 x 14336 27.3 | 20.7    33 x 8192 x 28672 81.4 | 51.5
 //          64 x 4096 x 6144 18.5 | 19.5     64 x 4096 x 8192 21.9 | 19.8
+// Gated (N of each weight), MXFP4:
+//          33 x 4096 x 8192 18.0 | 21.8     33 x 4096 x 10240 24.1 | 22.6
+//          33 x 5120 x 13001 32.1 | 30.8    48 x 8192 x 14336 56.9 | 52.2
+//          33 x 2048 x 14336 14.7 | 17.2    33 x 8192 x 8192 28.3 | 33.5
 bool Streams(const MxMatMulParams &p) {
   if (p.M <= 32 || p.M > 64) return p.M <= 32;
   // MXFP8 output takes four row tiles, which more rows leave no registers for
   if (p.output == kGatedMx) return false;
   const int64_t rows = WeightRows(p);
-  if (p.a_fp4) return p.M <= 48 || rows < 12288;
+  if (p.a_fp4) return rows < (p.M > 48 ? 12288 : p.output ? 20480 : INT64_MAX);
   return rows < (p.M <= 48 ? 11264 : 7168);
 }
 

@@ -78,8 +78,14 @@ __device__ __forceinline__ int Scales4(const uint8_t *base, unsigned row, int at
 // Waves of a workgroup: what the registers of more rows and columns leave.
 template <int NT> constexpr int kStreamWaves = NT == 4 ? 4 : 8;
 
+// Waves of a SIMD that the registers have to suffice for.  The gated product of up to
+// 16 rows would take 130 of them by itself, and one workgroup per CU: held to
+// 128 it has two.  us, MXFP8, 1 x 4096 x 14336 gated 18.5 -> 15.0, 2 x 4096 x 14336
+// 21.3 -> 17.4, 16 x 4096 x 14336 25.9 -> 24.0.
+template <int NT, int MT, int OUT> constexpr int kStreamFit = OUT == kGated && NT == 2 && MT == 1 ? 4 : 2;
+
 template <bool A4, int NT, int MT, bool QUANT, int OUT = kPlain>
-__global__ __launch_bounds__((64 * kStreamWaves<NT>), 2) void StreamKernel(const StreamArgs p) {
+__global__ __launch_bounds__((64 * kStreamWaves<NT>), (kStreamFit<NT, MT, OUT>)) void StreamKernel(const StreamArgs p) {
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
