@@ -799,7 +799,8 @@ int onnxl_amd_kv_cache_append(const onnxl_amd_tensor *k, const onnxl_amd_tensor 
  * position_ids INT32 or INT64 [tokens].  Positions in host memory are checked against
  * the tables; on the device, one outside them makes the token's rotated queries NaN, and
  * its key a value that is not finite.  Rows of q of no sequence, or of one whose numbers
- * do not fit, are left alone. */
+ * do not fit, are left alone.  q may not overlap qkv; the blocks of the new tokens times
+ * kv_heads have to stay below 2^31. */
 int onnxl_amd_rotary_kv_cache_append(const onnxl_amd_tensor *qkv, const onnxl_amd_tensor *cos,
                                      const onnxl_amd_tensor *sin, const onnxl_amd_tensor *position_ids,
                                      int32_t interleaved, onnxl_amd_tensor *q, onnxl_amd_tensor *k_cache,

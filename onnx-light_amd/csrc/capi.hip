@@ -3716,6 +3716,8 @@ int RotaryKvCacheAppend(const onnxl_amd_tensor *qkv, const onnxl_amd_tensor *cos
   p.t = PlanRotary(kRkvName, qkv, cos, sin, ids, interleaved, c.head_dim);
   OLA_ENFORCE(cos->rank == 2, kRkvName, ": cos must be [positions, rotary_dim / 2].");
   OLA_ENFORCE(p.t.half % 8 == 0, kRkvName, ": rotary_dim must be a multiple of 16.");
+  // the kernel counts blocks, heads, keys and values in 32 bits
+  OLA_ENFORCE(MostNewBlocks(c) * c.kv_heads < (int64_t(1) << 31), kRkvName, ": more than 2^31 blocks and heads.");
   if (!Absent(ids)) NeedShape(ids, {c.tokens}, kRkvName, "position_ids ([tokens])");
   const int32_t *held = lengths->location == ONNXL_AMD_HOST && Absent(ids) ? static_cast<const int32_t *>(lengths->data) : nullptr;
   for (int b = 0; held && b < c.batch; ++b)

@@ -119,6 +119,10 @@ struct KvAppendParams {
   int64_t first;      // new block of the launch's first workgroup
 };
 void LaunchKvCacheAppend(const KvAppendParams &p, hipStream_t stream);
+// n new tokens of a sequence lie in at most (n - 1) / block_tokens + 2 blocks, and in n.
+inline int64_t MostNewBlocks(const KvCacheParams &c) {
+  return std::min<int64_t>(c.tokens, c.tokens / c.block_tokens + 2 * (int64_t)c.batch);
+}
 
 // ---------------------------------------------------------------------------
 // Rotary positions: pairs (a, b) of a head's first 2 half dimensions, (i, half + i)

@@ -90,6 +90,23 @@ def test_rotary_append_refuses(olamd, kw, text):
     refused(olamd, "rotary_kv_cache_append", append_args(olamd, kw), text)
 
 
+def test_rotary_append_refuses_more_blocks_and_heads_than_its_grid_counts(olamd):
+    # 65535 sequences and 65536 tokens: up to 65536 blocks of 32768 heads; shapes without memory
+    def shaped(dtype, *dims):
+        d = dev(olamd, z(*[1] * len(dims), dtype=dtype))
+        for i, n in enumerate(dims):
+            d.dims[i] = n
+        d.size_bytes = math.prod(dims) * dtype.itemsize
+        return d
+
+    for kv, text in [(32768, "more than 2^31 blocks and heads"), (32767, "interleaved")]:
+        # (the second is refused for another reason: nothing is launched)
+        args = [shaped(H16, 65536, 3 * kv, 16), shaped(F32, 9, 8), shaped(F32, 9, 8), olamd.describe(None), 0 if kv == 32768 else 7,
+                shaped(H16, 65536, kv, 16), shaped(E4, 9, kv, 16, 16), shaped(E4, 9, kv, 16, 16), shaped(F32, 9, kv), shaped(F32, 9, kv),
+                shaped(I32, 65535, 4), shaped(I32, 65536), shaped(I32, 65535)]
+        refused(olamd, "rotary_kv_cache_append", args, text)
+
+
 def test_rotary_append_checks_what_is_on_the_host(olamd):
     args = append_args(olamd, {})
     args[5].location = olamd.HOST
