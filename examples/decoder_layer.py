@@ -1,11 +1,12 @@
 """A decoder layer with MXFP4 weights, MXFP8 activations and an 8-bit paged
 cache: two prompts of different lengths enter it, then both sequences go on one
-token at a time.
+token at a time, each token drawn from the logits of the one before.
 
     python examples/decoder_layer.py [--hidden 2048] [--prompt 700] [--tokens 8]
 
-The quantized products, the norms, the cache and its attention are the
-framework's; the rotation of q and k by position and the gate are torch's.
+The quantized products, plain and gated, the norms, the rotation by position, the
+cache and its attention, and the choice of a token are the framework's; the sum
+behind the layer and the embeddings' lookup are torch's.
 Prints how far the outputs are from the same layer in 64 bits on the CPU, and on
 a GPU the time of a step.
 """
@@ -55,7 +56,7 @@ def random_weights(shape: Shape, seed=0) -> dict:
 
 def rotate(x, positions):
     """Rotates pairs of dimensions (i, i + D / 2) of x [tokens, heads, D] by
-    position * 10000^(-2 i / D)."""
+    position * 10000^(-2 i / D): the plain layer's form of the rotary tables."""
     half = x.shape[-1] // 2
     wide = torch.float64 if x.dtype == torch.float64 else torch.float32
     turn = positions.to(wide)[:, None] * 10000.0 ** (-torch.arange(half, device=x.device, dtype=wide) / half)
@@ -79,24 +80,25 @@ class Sequences:
 
     def grow(self, new):
         """Room for new[b] tokens of every sequence: (block_table, query_start,
-        lengths, positions of the new tokens), on the GPU."""
-        positions = []
+        lengths) on the GPU."""
         for b, n in enumerate(new):
-            positions += range(self.length[b], self.length[b] + n)
             self.length[b] += n
             while self.held[b] * self.block_tokens < self.length[b]:
                 self.table[b, self.held[b]] = self.free.pop()
                 self.held[b] += 1
         start = [sum(new[:b]) for b in range(len(new) + 1)]
         return (self.table.cuda(), torch.tensor(start, dtype=torch.int32, device="cuda"),
-                torch.tensor(self.length, dtype=torch.int32, device="cuda"), torch.tensor(positions, device="cuda"))
+                torch.tensor(self.length, dtype=torch.int32, device="cuda"))
 
 
 class DecoderLayer:
-    def __init__(self, ola, shape: Shape, weights: dict):
+    def __init__(self, ola, shape: Shape, weights: dict, longest=8192):
         self.ola, self.shape = ola, shape
+        self.tables = ola.rotary_tables(longest, shape.head_dim)  # cos, sin
         self.norm1, self.norm2 = weights["norm1"].cuda(), weights["norm2"].cuda()
         self.w = {n: ola.mx_quantize(weights[n].cuda(), ola.FLOAT4E2M1) for n in shape.matrices()}
+        # codes and scales of the gate's rows, then of those it is multiplied by
+        self.gate, self.up = zip(*(t.split(shape.inner) for t in self.w["gate_up"]))
 
     def dense(self) -> dict:
         """The weights that the quantized ones stand for, in 64 bits on the CPU."""
@@ -119,18 +121,35 @@ class DecoderLayer:
     def __call__(self, x, sequences: Sequences, new):
         """x bfloat16 [tokens, hidden], the new[b] new tokens of sequence b one
         sequence after the other."""
+        return self.step(x, sequences.cache, *sequences.grow(new), max(new))
+
+    def step(self, x, cache, table, start, lengths, most):
+        """The same on the GPU alone; no sequence has more than `most` new tokens."""
         s, ola = self.shape, self.ola
-        table, start, lengths, positions = sequences.grow(new)
         y, scale, x = self.norm(x, self.norm1)
         qkv = self.product("qkv", y, scale).view(len(x), -1, s.head_dim)
-        q, k, v = qkv.split([s.heads, s.kv_heads, s.kv_heads], 1)
-        q, k, v = rotate(q, positions).contiguous(), rotate(k, positions).contiguous(), v.contiguous()
-        ola.kv_cache_append(k, v, sequences.cache, table, start, lengths)
-        o = ola.kv_cache_attention(q, sequences.cache, table, start, lengths, max_query=max(new))
+        q = ola.rotary_kv_cache_append(qkv, *self.tables, cache, table, start, lengths)
+        o = ola.kv_cache_attention(q, cache, table, start, lengths, max_query=most)
         o = self.product("o", o.view(len(x), -1))  # 16-bit rows, quantized by the product
         y, scale, x = self.norm(o, self.norm2, x)  # x + o, and its norm
-        gate, up = self.product("gate_up", y, scale).chunk(2, -1)
-        return x + self.product("down", torch.nn.functional.silu(gate) * up)
+        h, h_scale = ola.mx_gated_matmul(y, *self.gate, *self.up, a_scale=scale, mx=True)
+        return x + self.product("down", h, h_scale)
+
+
+class Vocabulary:
+    """Embeddings of tokens, and from the layer's outputs the next ones."""
+
+    def __init__(self, ola, hidden: int, size=32000, seed=2):
+        g = torch.Generator().manual_seed(seed)
+        self.ola = ola
+        self.rows = torch.randn((size, hidden), generator=g).bfloat16().cuda()
+        head = torch.randn((size, hidden), generator=g).mul_(2 * hidden ** -0.5).bfloat16()
+        self.w = ola.mx_quantize(head.cuda(), ola.FLOAT4E2M1)
+
+    def next(self, y, start, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+        """(token, probability) after each sequence's last row of y."""
+        logits = self.ola.mx_matmul(y[start[1:].long() - 1], *self.w)
+        return self.ola.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
 
 
 def plain_layer(shape: Shape, w: dict, x, length: int):
@@ -170,6 +189,24 @@ def run(ola, shape: Shape, prompts, tokens: int, dtype=None, seed=0):
     return layer, inputs, [torch.cat(o) for o in outputs]
 
 
+def generate(layer: DecoderLayer, words: Vocabulary, prompts, tokens: int, seed=0):
+    """Lets prompts (lists of tokens) go on by `tokens` drawn ones each, at temperature
+    0.8 of the 50 likeliest and 95 % of their weight; returns the drawn tokens."""
+    batch = len(prompts)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rules = (torch.full((batch,), 0.8, device="cuda"), torch.full((batch,), 50, dtype=torch.int32, device="cuda"),
+             torch.full((batch,), 0.95, device="cuda"))
+    sequences = Sequences(layer.ola, layer.shape, batch, max(map(len, prompts)) + tokens)
+    ids, new, drawn = torch.tensor(sum(prompts, []), device="cuda"), [len(p) for p in prompts], []
+    for _ in range(tokens):
+        table, start, lengths = sequences.grow(new)
+        y = layer.step(words.rows[ids], sequences.cache, table, start, lengths, max(new))
+        ids, _ = words.next(y, start, torch.rand(batch, generator=g, device="cuda"), *rules)
+        drawn.append(ids)
+        new = [1] * batch
+    return torch.stack(drawn, 1).tolist()
+
+
 def error(layer: DecoderLayer, x, y) -> float:
     """How far y is from the layer in 64 bits, of what the layer adds to x (root
     mean squares)."""
@@ -191,6 +228,9 @@ def main():
     for b, (x, y) in enumerate(zip(inputs, outputs)):
         print(f"sequence {b}: {prompts[b]} tokens of prompt and {a.tokens} single ones, "
               f"error {error(layer, x, y):.3f} of what the layer adds")
+    words = Vocabulary(ola, shape.hidden)
+    for b, drawn in enumerate(generate(layer, words, [list(range(n)) for n in prompts], a.tokens)):
+        print(f"sequence {b} goes on with tokens {drawn}")
     for name, new in (("prompt", prompts), ("token", [1] * len(prompts))):
         x = torch.randn(sum(new), shape.hidden, device="cuda").bfloat16()
         times = []
