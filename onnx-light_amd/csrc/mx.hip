@@ -156,16 +156,16 @@ struct MxScratch {
         b_tiles(Scratch::Round((size_t)mx::ScaleTileBytes(p.N, p.K))) {}
 };
 
-template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, int output, hipStream_t s) {
+template <bool A4, int MB, int NB, int STAGES> void LaunchGemm(const mx::GemmArgs &g, int output, hipStream_t s) {
   using S = mx::Shape<A4, MB, NB>;
   const dim3 grid((unsigned)(Ceil(g.M, S::BM) * Ceil(g.N, output ? S::BN / 2 : S::BN)));
   if constexpr (NB % 2 == 0) {
     if (output == kGatedMx)
-      mx::GemmKernel<A4, MB, NB, kGatedMx><<<grid, 256, 0, s>>>(g);
+      mx::GemmKernel<A4, MB, NB, STAGES, kGatedMx><<<grid, 256, 0, s>>>(g);
     else if (output == kGated)
-      mx::GemmKernel<A4, MB, NB, kGated><<<grid, 256, 0, s>>>(g);
+      mx::GemmKernel<A4, MB, NB, STAGES, kGated><<<grid, 256, 0, s>>>(g);
   }
-  if (output == kPlain) mx::GemmKernel<A4, MB, NB><<<grid, 256, 0, s>>>(g);
+  if (output == kPlain) mx::GemmKernel<A4, MB, NB, STAGES><<<grid, 256, 0, s>>>(g);
 }
 
 // Large tiles (256 x 256, 128 x 256 for E4M3 activations) feed more MFMAs per
@@ -176,6 +176,12 @@ template <bool A4, int MB, int NB> void LaunchGemm(const mx::GemmArgs &g, int ou
 // 184.  Large / middle / small: MXFP8 256 x 4096 x 4096 27 / 24 / 21, 1000 x 4096 x
 // 6144 33 / 30 / 41, 2048 x 4096 x 4096 39 / 51 / 45, 4096 x 8192 x 8192 234 / 278 /
 // 311.
+// A small tile has as many stages as LDS has room for, since a step of its own takes
+// less time than a load: three for E4M3, and for E2M1 four, where there are no more tiles
+// than CUs, else two, so that two workgroups share a CU.  us, two stages | more: MXFP8
+// 128 x 4096 x 4096 20.5 | 18.2, 1000 x 14336 x 4096 66.9 | 61.7; MXFP4 128 x 4096 x
+// 4096 18.5 | 14.4, 1000 x 14336 x 4096 53.6 | 45.0, but 1000 x 4096 x 6144 25.7 | 30.3,
+// 2000 x 4096 x 4096 30.4 | 35.9.
 enum class Tiles { kSmall, kMiddle, kLarge };
 Tiles TilesOf(const MxMatMulParams &p) {
   const int64_t cus = Ctx().num_cus;
@@ -190,23 +196,31 @@ Tiles TilesOf(const MxMatMulParams &p) {
 
 // Few rows take the streaming kernel, whose time goes with the weight's bytes and
 // the row tiles; the GEMM's one round of tiles goes with K alone, and a wide
-// weight fills it.  us, rows x K x N, stream | GEMM:
-//   MXFP4  32 x 4096 x 14336 14.7 | 18.6    48 x 4096 x 14336 18.1 | 18.5
-//          56 x 4096 x 14336 20.8 | 18.6    64 x 2048 x 16384 14.9 | 13.1
-//          64 x 8192 x 8192 27.1 | 28.2     64 x 11008 x 4096 20.9 | 33.9
-//   MXFP8  36 x 2048 x 8192 8.6 | 13.1      40 x 11008 x 8192 35.2 | 39.4
-//          40 x 4096 x 14336 27.3 | 20.7    33 x 8192 x 28672 81.4 | 51.5
-//          64 x 4096 x 6144 18.5 | 19.5     64 x 4096 x 8192 21.9 | 19.8
-// Gated (N of each weight), MXFP4:
-//          33 x 4096 x 8192 18.0 | 21.8     33 x 4096 x 10240 24.1 | 22.6
-//          33 x 5120 x 13001 32.1 | 30.8    48 x 8192 x 14336 56.9 | 52.2
-//          33 x 2048 x 14336 14.7 | 17.2    33 x 8192 x 8192 28.3 | 33.5
+// weight fills it.  us, rows x K x N, stream | GEMM (gated: N of each weight):
+//   MXFP4  32 x 4096 x 14336 14.9 | 15.1    36 x 2048 x 8192 7.8 | 10.9
+//          40 x 4096 x 14336 16.9 | 15.2    40 x 11008 x 8192 22.2 | 25.5
+//          56 x 4096 x 11008 20.3 | 16.0    64 x 4096 x 8192 12.8 | 14.5
+//          64 x 8192 x 8192 27.2 | 21.4     64 x 11008 x 4096 21.0 | 25.2
+//   MXFP8  36 x 2048 x 8192 8.6 | 12.5      40 x 11008 x 8192 35.2 | 32.9
+//          48 x 4096 x 6144 15.7 | 17.2     64 x 4096 x 4096 15.9 | 17.3
+//          64 x 11008 x 4096 28.7 | 32.7    33 x 8192 x 28672 81 | 44.1
+//   gated, MXFP4
+//          20 x 4096 x 14336 22.7 | 21.9    32 x 4096 x 14336 24.0 | 21.9
+//          32 x 4096 x 8192 15.1 | 18.4     48 x 2048 x 5632 12.7 | 14.2
+//          33 x 4096 x 8192 18.0 | 18.5     33 x 8192 x 8192 28.3 | 25.6
+//          33 x 5120 x 13001 32.1 | 27.4    64 x 4096 x 4096 13.7 | 17.6
+//          64 x 8192 x 5632 40.0 | 25.2
+//   gated, MXFP8
+//          20 x 4096 x 14336 24.8 | 23.0    32 x 4096 x 14336 29.3 | 23.0
+//          24 x 4096 x 10240 21.6 | 21.6    20 x 8192 x 8192 25.6 | 31.0
 bool Streams(const MxMatMulParams &p) {
-  if (p.M <= 32 || p.M > 64) return p.M <= 32;
+  if (p.M <= 16 || p.M > 64) return p.M <= 16;
+  const int64_t rows = WeightRows(p), K = std::max<int64_t>(p.K, 1);
+  if (p.M <= 32) return p.output != kGated || rows < 24576;
   // MXFP8 output takes four row tiles, which more rows leave no registers for
   if (p.output == kGatedMx) return false;
-  const int64_t rows = WeightRows(p);
-  if (p.a_fp4) return rows < (p.M > 48 ? 12288 : p.output ? 20480 : INT64_MAX);
+  // where rows * K of the one takes as long as K and a launch of the other
+  if (p.a_fp4) return rows < (p.M > 48 ? 4500 + 16500000 / K : 9000 + 20000000 / K);
   return rows < (p.M <= 48 ? 11264 : 7168);
 }
 
@@ -368,11 +382,15 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
                        p.activation, p.y_scale};
   const Tiles tiles = TilesOf(p);
   if (tiles == Tiles::kLarge)
-    p.a_fp4 ? LaunchGemm<true, 4, 4>(g, p.output, stream) : LaunchGemm<false, 2, 4>(g, p.output, stream);
+    p.a_fp4 ? LaunchGemm<true, 4, 4, 2>(g, p.output, stream) : LaunchGemm<false, 2, 4, 2>(g, p.output, stream);
   else if (tiles == Tiles::kMiddle)
-    LaunchGemm<false, 2, 3>(g, p.output, stream);
+    LaunchGemm<false, 2, 3, 2>(g, p.output, stream);
+  else if (!p.a_fp4)
+    LaunchGemm<false, 2, 2, 3>(g, p.output, stream);
+  else if (Ceil(p.M, 128) * Ceil(p.N, p.output ? 64 : 128) <= Ctx().num_cus)
+    LaunchGemm<true, 2, 2, 4>(g, p.output, stream);
   else
-    p.a_fp4 ? LaunchGemm<true, 2, 2>(g, p.output, stream) : LaunchGemm<false, 2, 2>(g, p.output, stream);
+    LaunchGemm<true, 2, 2, 2>(g, p.output, stream);
 }
 
 }  // namespace onnxl_amd

@@ -10,8 +10,8 @@
 // Workgroup: 4 waves (2 x 2), tile 64 MB x 64 NB outputs, each wave MB x NB
 // blocks of 32 x 32.  A K step is 256 values: 128 bytes of an E2M1 row, 256 of
 // an E4M3 row, two 16-byte chunks (four) per 64-value sub-step and lane.  Two
-// stages in LDS, filled by direct loads (16 bytes a lane, nothing held in
-// registers) while the other is multiplied; a row's chunks are XOR-swizzled by
+// or more stages in LDS, filled by direct loads (16 bytes a lane, nothing held in
+// registers) while another is multiplied; a row's chunks are XOR-swizzled by
 // the row, so that a fragment read meets no bank twice.  Scales are read through
 // LDS as well, from tiles that a first kernel wrote (ScaleTileAt): the four
 // bytes of a lane's register are its blocks of the four sub-steps, so a step
@@ -28,8 +28,9 @@
 //
 // What bounds it: the matrix cores work half of the time.  A product takes 61 cycles
 // of its SIMD where the instruction needs 32 (MXFP4, 4096 rows; with MXFP8 and 1000
-// rows 175 and 64), since a step waits for loads that left half a step before, and
-// the one wave of a SIMD has nothing else to do meanwhile.
+// rows 175 and 64), since a step waits for loads that left half a step before (with
+// more than two stages, steps before), and the one wave of a SIMD has nothing else to do
+// meanwhile.
 //
 // A gated product (MxOutput) has the 32-row blocks of both weights in turn in the
 // tile's b, so that a wave's blocks 2 j and 2 j + 1 are gate and up of the same 32
@@ -97,9 +98,9 @@ __device__ __forceinline__ void DirectLoad4(__amdgpu_buffer_rsrc_t rs, const cha
   const unsigned m0 = (unsigned)(size_t)(lds_ptr_t)lds;
   asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voffset), "s"(rs), "{m0}"(m0));
 }
-// This wave's loads have landed and its LDS reads are done; so for all waves.
-__device__ __forceinline__ void StepBarrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// This wave's loads but the last LEFT have landed and its LDS reads are done; so for all waves.
+template <int LEFT = 0> __device__ __forceinline__ void StepBarrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
 __device__ __forceinline__ uint16_t Half(float v, int bf16) {
@@ -115,17 +116,17 @@ __device__ __forceinline__ uint16_t Half(float v, int bf16) {
 __device__ __forceinline__ v8i Operand(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 __device__ __forceinline__ v8i Operand(v8i v) { return v; }
 
-template <bool A4, int MB, int NB> struct Shape {
+template <bool A4, int MB, int NB, int STAGES = 2> struct Shape {
   static constexpr int BM = 64 * MB, BN = 64 * NB;
   static constexpr int kRowA = A4 ? 128 : 256;  // bytes of an a row per step
   static constexpr int kA = BM * kRowA, kB = BN * 128, kS = (BM + BN) * 8;
   static constexpr int kStage = kA + kB + kS;
-  static constexpr int kLds = 2 * kStage;
+  static constexpr int kLds = STAGES * kStage;
 };
 
-template <bool A4, int MB, int NB, int OUT = kPlain>
-__global__ __launch_bounds__(256, (Shape<A4, MB, NB>::kLds > 80 * 1024 ? 1 : 2)) void GemmKernel(const GemmArgs p) {
-  using S = Shape<A4, MB, NB>;
+template <bool A4, int MB, int NB, int STAGES, int OUT = kPlain>
+__global__ __launch_bounds__(256, (Shape<A4, MB, NB, STAGES>::kLds > 80 * 1024 ? 1 : 2)) void GemmKernel(const GemmArgs p) {
+  using S = Shape<A4, MB, NB, STAGES>;
   constexpr int NW = OUT == kPlain ? 1 : 2, NO = NB / NW;  // weights, a wave's blocks of y's columns
   static_assert(NB % NW == 0, "gate and up in pairs");
   constexpr int BM = S::BM, BN = S::BN / NW, kRowA = S::kRowA;  // rows and columns of y
@@ -205,9 +206,9 @@ __global__ __launch_bounds__(256, (Shape<A4, MB, NB>::kLds > 80 * 1024 ? 1 : 2))
   int sa[2][MB], sb[2][NB];
   // fragment x (a's blocks, then b's) of sub-step kk of stage s: 32 rows are 32
   // LDS rows further, a sub-step other bits of the chunk
-  int a_rd[2], b_rd[2];
+  int a_rd[STAGES], b_rd[STAGES];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
+  for (int s = 0; s < STAGES; ++s) {
     const int row = wm * 32 * MB + r;
     a_rd[s] = s * S::kStage + row * kRowA + 16 * (A4 ? h ^ (r & 7) ^ (r >> 3 & 1) : h ^ (r & 15));
     b_rd[s] = s * S::kStage + S::kA + (wn * 32 * NB + r) * 128 + 16 * (h ^ (r & 7) ^ (r >> 3 & 1));
@@ -249,61 +250,71 @@ __global__ __launch_bounds__(256, (Shape<A4, MB, NB>::kLds > 80 * 1024 ? 1 : 2))
   constexpr int NM = MB * NB, NR = MB + NB;
   // A sub-step: every MFMA with its share of the next sub-step's reads before
   // it and of the direct loads [l0, l1) after it, pinned in that order.
-  auto sub = [&](auto kk, int t, int s, int buf, int l0, int l1) __attribute__((always_inline)) {
+  auto sub = [&](auto kk, int t, int s, int sbuf, int buf, int l0, int l1) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < NM; ++x) {
 #pragma unroll
       for (int y = x * NR / NM; y < (x + 1) * NR / NM; ++y) read(buf ^ 1, s, kk + 1, y);
-      mma(kk, buf, s, x);
+      mma(kk, buf, sbuf, x);
 #pragma unroll
-      for (int y = l0 + (l1 - l0) * x / NM; y < l0 + (l1 - l0) * (x + 1) / NM; ++y) issue(t + 1, s ^ 1, y);
+      for (int y = l0 + (l1 - l0) * x / NM; y < l0 + (l1 - l0) * (x + 1) / NM; ++y) issue(t + STAGES - 1, (s + STAGES - 1) % STAGES, y);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   constexpr int kEarly = L / 3, kMid = 2 * L / 3;  // loads issued in the last sub-step of the step before
   // step t in stage s; its fragments of sub-step 0 and its scales are in
   // registers and the first kEarly loads of step t + 1 are out
-  auto step = [&](int t, int s) __attribute__((always_inline)) {
+  auto step = [&](int t, int s, int sbuf) __attribute__((always_inline)) {
     // the loads' and reads' addresses are made where they are used: all of them
     // kept across the loop do not fit beside 256 accumulators
-    asm volatile("" : "+v"(a_g), "+v"(b_g0), "+v"(b_g1), "+v"(a_rd[0]), "+v"(a_rd[1]), "+v"(b_rd[0]), "+v"(b_rd[1]));
-    sub(std::integral_constant<int, 0>{}, t, s, 0, kEarly, kMid);
-    sub(std::integral_constant<int, 1>{}, t, s, 1, kMid, L);
-    sub(std::integral_constant<int, 2>{}, t, s, 0, 0, 0);
+    asm volatile("" : "+v"(a_g), "+v"(b_g0), "+v"(b_g1));
 #pragma unroll
-    for (int x = 0; x < NM / 2; ++x) mma(std::integral_constant<int, 3>{}, 1, s, x);
+    for (int i = 0; i < STAGES; ++i) asm volatile("" : "+v"(a_rd[i]), "+v"(b_rd[i]));
+    sub(std::integral_constant<int, 0>{}, t, s, sbuf, 0, kEarly, kMid);
+    sub(std::integral_constant<int, 1>{}, t, s, sbuf, 1, kMid, L);
+    sub(std::integral_constant<int, 2>{}, t, s, sbuf, 0, 0, 0);
+#pragma unroll
+    for (int x = 0; x < NM / 2; ++x) mma(std::integral_constant<int, 3>{}, 1, sbuf, x);
     __builtin_amdgcn_sched_barrier(0);
-    StepBarrier();
+    StepBarrier<(STAGES - 2) * L>();
 #pragma unroll
     for (int x = 0; x < NM / 2; ++x) {
       constexpr int H = NM / 2 > 0 ? NM / 2 : 1;
 #pragma unroll
       for (int y = x * NR / H; y < (x + 1) * NR / H; ++y) {
-        read(0, s ^ 1, 0, y);
-        read_scale(s ^ 1, s ^ 1, y);
+        read(0, (s + 1) % STAGES, 0, y);
+        read_scale(sbuf ^ 1, (s + 1) % STAGES, y);
       }
-      mma(std::integral_constant<int, 3>{}, 1, s, NM / 2 + x);
+      mma(std::integral_constant<int, 3>{}, 1, sbuf, NM / 2 + x);
 #pragma unroll
-      for (int y = kEarly * x / H; y < kEarly * (x + 1) / H; ++y) issue(t + 2, s, y);
+      for (int y = kEarly * x / H; y < kEarly * (x + 1) / H; ++y) issue(t + STAGES, s, y);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
 #pragma unroll
-  for (int x = 0; x < L; ++x) issue(0, 0, x);
-  StepBarrier();
+  for (int i = 0; i < STAGES - 1; ++i)
 #pragma unroll
-  for (int x = 0; x < kEarly; ++x) issue(1, 1, x);
+    for (int x = 0; x < L; ++x) issue(i, i, x);
+  StepBarrier<(STAGES - 2) * L>();
+#pragma unroll
+  for (int x = 0; x < kEarly; ++x) issue(STAGES - 1, STAGES - 1, x);
 #pragma unroll
   for (int x = 0; x < NR; ++x) {
     read(0, 0, 0, x);
     read_scale(0, 0, x);
   }
+  // (the scales' two buffers take turns as well)
+  constexpr int kUnroll = STAGES % 2 ? 2 * STAGES : STAGES;
   int t = 0;
   do {  // K = 0 runs one step of zeros
-    step(t, 0);
-    if (t + 1 < nk) step(t + 1, 1);
-    t += 2;
+    step(t, 0, 0);
+#pragma unroll
+    for (int i = 1; i < kUnroll; ++i) {
+      if (t + i >= nk) break;
+      step(t + i, i % STAGES, i % 2);
+    }
+    t += kUnroll;
   } while (t < nk);
   StepBarrier();  // the loads past the last step, before the LDS is used again
 
