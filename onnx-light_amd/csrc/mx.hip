@@ -156,16 +156,16 @@ struct MxScratch {
         b_tiles(Scratch::Round((size_t)mx::ScaleTileBytes(p.N, p.K))) {}
 };
 
-template <bool A4, int MB, int NB, int STAGES> void LaunchGemm(const mx::GemmArgs &g, int output, hipStream_t s) {
-  using S = mx::Shape<A4, MB, NB>;
+template <bool A4, int MB, int NB, int STAGES, int WN = 2> void LaunchGemm(const mx::GemmArgs &g, int output, hipStream_t s) {
+  using S = mx::Shape<A4, MB, NB, STAGES, WN>;
   const dim3 grid((unsigned)(Ceil(g.M, S::BM) * Ceil(g.N, output ? S::BN / 2 : S::BN)));
-  if constexpr (NB % 2 == 0) {
+  if constexpr (NB == 2) {
     if (output == kGatedMx)
-      mx::GemmKernel<A4, MB, NB, STAGES, kGatedMx><<<grid, 256, 0, s>>>(g);
+      mx::GemmKernel<A4, MB, NB, STAGES, WN, kGatedMx><<<grid, 128 * WN, 0, s>>>(g);
     else if (output == kGated)
-      mx::GemmKernel<A4, MB, NB, STAGES, kGated><<<grid, 256, 0, s>>>(g);
+      mx::GemmKernel<A4, MB, NB, STAGES, WN, kGated><<<grid, 128 * WN, 0, s>>>(g);
   }
-  if (output == kPlain) mx::GemmKernel<A4, MB, NB, STAGES><<<grid, 256, 0, s>>>(g);
+  if (output == kPlain) mx::GemmKernel<A4, MB, NB, STAGES, WN><<<grid, 128 * WN, 0, s>>>(g);
 }
 
 // Large tiles (256 x 256, 128 x 256 for E4M3 activations) feed more MFMAs per
@@ -182,6 +182,12 @@ template <bool A4, int MB, int NB, int STAGES> void LaunchGemm(const mx::GemmArg
 // 128 x 4096 x 4096 20.5 | 18.2, 1000 x 14336 x 4096 66.9 | 61.7; MXFP4 128 x 4096 x
 // 4096 18.5 | 14.4, 1000 x 14336 x 4096 53.6 | 45.0, but 1000 x 4096 x 6144 25.7 | 30.3,
 // 2000 x 4096 x 4096 30.4 | 35.9.
+// A large tile has eight waves, two a SIMD, of which one multiplies while the other waits
+// or stores; four read less of LDS, which wins in the end along a long K of E4M3.  us,
+// four waves | eight: MXFP4 4096 x 8192 x 8192 153 | 149, 1000 x 4096 x 14336 44.4 | 39.8,
+// gated 4096 x 8192 x 14336 572 | 472; MXFP8 1000 x 4096 x 14336 62 | 58, 16384 x 4096 x
+// 4096 278 | 270, 2000 x 8192 x 8192 118 | 117, 4096 x 8192 x 8192 234 | 243, 1000 x 14336 x
+// 14336 181 | 193, gated 500 x 4096 x 14336 72.6 | 63.0, 4096 x 8192 x 14336 821 | 811.
 enum class Tiles { kSmall, kMiddle, kLarge };
 Tiles TilesOf(const MxMatMulParams &p) {
   const int64_t cus = Ctx().num_cus;
@@ -381,8 +387,12 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
                        (p.output == kGatedMx || p.N % 8 == 0) && reinterpret_cast<uintptr_t>(p.y) % 16 == 0, p.up, up_tiles,
                        p.activation, p.y_scale};
   const Tiles tiles = TilesOf(p);
-  if (tiles == Tiles::kLarge)
-    p.a_fp4 ? LaunchGemm<true, 4, 4, 2>(g, p.output, stream) : LaunchGemm<false, 2, 4, 2>(g, p.output, stream);
+  if (tiles == Tiles::kLarge && p.a_fp4)
+    LaunchGemm<true, 4, 2, 2, 4>(g, p.output, stream);
+  else if (tiles == Tiles::kLarge && (p.output || p.K < 8192))
+    LaunchGemm<false, 2, 2, 2, 4>(g, p.output, stream);
+  else if (tiles == Tiles::kLarge)
+    LaunchGemm<false, 2, 4, 2>(g, kPlain, stream);
   else if (tiles == Tiles::kMiddle)
     LaunchGemm<false, 2, 3, 2>(g, p.output, stream);
   else if (!p.a_fp4)

@@ -7,8 +7,8 @@
 // E8M0 scale of k block h comes from the same lane, one byte of a register that
 // the instruction selects.
 //
-// Workgroup: 4 waves (2 x 2), tile 64 MB x 64 NB outputs, each wave MB x NB
-// blocks of 32 x 32.  A K step is 256 values: 128 bytes of an E2M1 row, 256 of
+// Workgroup: 4 waves (2 x 2) or 8 (2 x 4), tile 64 MB x 64 NB outputs or 64 MB x 128 NB,
+// each wave MB x NB blocks of 32 x 32.  A K step is 256 values: 128 bytes of an E2M1 row, 256 of
 // an E4M3 row, two 16-byte chunks (four) per 64-value sub-step and lane.  Two
 // or more stages in LDS, filled by direct loads (16 bytes a lane, nothing held in
 // registers) while another is multiplied; a row's chunks are XOR-swizzled by
@@ -33,7 +33,7 @@
 // meanwhile.
 //
 // A gated product (MxOutput) has the 32-row blocks of both weights in turn in the
-// tile's b, so that a wave's blocks 2 j and 2 j + 1 are gate and up of the same 32
+// tile's b, so that a wave's two blocks of b are gate and up of the same 32
 // columns of y and meet in the registers.
 //
 // Sums are fp32, but not all of a product enters them: with E4M3 activations the
@@ -116,25 +116,25 @@ __device__ __forceinline__ uint16_t Half(float v, int bf16) {
 __device__ __forceinline__ v8i Operand(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 __device__ __forceinline__ v8i Operand(v8i v) { return v; }
 
-template <bool A4, int MB, int NB, int STAGES = 2> struct Shape {
-  static constexpr int BM = 64 * MB, BN = 64 * NB;
+template <bool A4, int MB, int NB, int STAGES = 2, int WN = 2> struct Shape {
+  static constexpr int BM = 64 * MB, BN = 32 * NB * WN;
   static constexpr int kRowA = A4 ? 128 : 256;  // bytes of an a row per step
   static constexpr int kA = BM * kRowA, kB = BN * 128, kS = (BM + BN) * 8;
   static constexpr int kStage = kA + kB + kS;
   static constexpr int kLds = STAGES * kStage;
 };
 
-template <bool A4, int MB, int NB, int STAGES, int OUT = kPlain>
-__global__ __launch_bounds__(256, (Shape<A4, MB, NB, STAGES>::kLds > 80 * 1024 ? 1 : 2)) void GemmKernel(const GemmArgs p) {
-  using S = Shape<A4, MB, NB, STAGES>;
+template <bool A4, int MB, int NB, int STAGES, int WN, int OUT = kPlain>
+__global__ __launch_bounds__(128 * WN, (Shape<A4, MB, NB, STAGES, WN>::kLds > 80 * 1024 && WN == 2 ? 1 : 2)) void GemmKernel(const GemmArgs p) {
+  using S = Shape<A4, MB, NB, STAGES, WN>;
   constexpr int NW = OUT == kPlain ? 1 : 2, NO = NB / NW;  // weights, a wave's blocks of y's columns
   static_assert(NB % NW == 0, "gate and up in pairs");
   constexpr int BM = S::BM, BN = S::BN / NW, kRowA = S::kRowA;  // rows and columns of y
-  constexpr int LA = S::kA / 4096, LB = S::kB / 4096;  // 1 KB loads per wave and step
-  constexpr int LS = MB > NB ? MB : NB;                // 256-byte scale loads per wave and step
+  constexpr int LA = S::kA / (2048 * WN), LB = S::kB / (2048 * WN);  // 1 KB loads per wave and step
+  constexpr int LS = WN > 2 ? 2 : MB > NB ? MB : NB;   // 256-byte scale loads per wave and step
   __shared__ __align__(1024) char lds[S::kLds];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 1, wn = wave & 1, r = lane & 31, h = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN, r = lane & 31, h = lane >> 5;
 
   // each XCD a contiguous run of tiles, kGroupM tile rows high, so that tiles
   // sharing rows of a and b share an L2
@@ -149,18 +149,19 @@ __global__ __launch_bounds__(256, (Shape<A4, MB, NB, STAGES>::kLds > 80 * 1024 ?
   const int nk = (int)((p.K + 255) / 256);
   const int64_t pitch_a = (int64_t)nk * kRowA, pitch_b = p.K / 2;
   const int64_t rows_a = p.M - row0 < BM ? p.M - row0 : BM, rows_b = p.N - col0 < BN ? p.N - col0 : BN;
-  const __amdgpu_buffer_rsrc_t rsA = Rsrc(p.a + row0 * pitch_a, rows_a * pitch_a), rsB = Rsrc(p.b + col0 * pitch_b, rows_b * pitch_b);
-  // gated: of the second weight, and what a wave whose pieces are all of one takes
-  const __amdgpu_buffer_rsrc_t rsU = Rsrc(p.up + col0 * pitch_b, OUT == kPlain ? 0 : rows_b * pitch_b);
-  const __amdgpu_buffer_rsrc_t rsW = Rsrc((wave & 1 ? p.up : p.b) + col0 * pitch_b, OUT == kPlain ? 0 : rows_b * pitch_b);
-  // scale tiles: waves 0 and 1 load those of a's 32-row blocks, 2 and 3 of b's;
-  // blocks past the last are not read
+  const __amdgpu_buffer_rsrc_t rsA = Rsrc(p.a + row0 * pitch_a, rows_a * pitch_a), rsB = Rsrc((OUT != kPlain && wave & 1 ? p.up : p.b) + col0 * pitch_b, rows_b * pitch_b);
+  // scale tiles, blocks past the last are not read.  Four waves: 0 and 1 load those of a's
+  // 32-row blocks, 2 and 3 of b's; eight: one of b's each, and one of a's, which some load
+  // twice where there are four.  Gated: odd blocks of b are the second weight's
+  static_assert(WN == 2 || (WN == 4 && NB == 2 && MB <= 4), "a scale block of b a wave");
   const int sblk = wave < 2 ? MB : NB;
-  const uint8_t *scales = wave < 2 ? p.as + row0 / 32 * nk * 256 : p.bs + col0 / 32 * nk * 256;
-  const __amdgpu_buffer_rsrc_t rsS = Rsrc(scales, ((wave < 2 ? rows_a : rows_b) + 31) / 32 * nk * 256);
-  // gated: odd blocks of waves 2 and 3 are the second weight's
-  const uint8_t *scales2 = wave < 2 ? scales : p.ups + col0 / 32 * nk * 256;
-  const __amdgpu_buffer_rsrc_t rsT = Rsrc(scales2, OUT == kPlain ? 0 : ((wave < 2 ? rows_a : rows_b) + 31) / 32 * nk * 256);
+  const uint8_t *bs = p.bs + col0 / 32 * nk * 256, *ups = p.ups + col0 / 32 * nk * 256;
+  const unsigned as_bytes = (unsigned)((rows_a + 31) / 32 * nk * 256), bs_bytes = (unsigned)((rows_b + 31) / 32 * nk * 256);
+  const bool for_a = WN > 2 || wave < 2;
+  const __amdgpu_buffer_rsrc_t rsS = Rsrc(for_a ? p.as + row0 / 32 * nk * 256 : bs, for_a ? as_bytes : bs_bytes);
+  const __amdgpu_buffer_rsrc_t rsT = WN > 2 ? Rsrc(OUT != kPlain && wave & 1 ? ups : bs, bs_bytes)
+                                            : Rsrc(OUT != kPlain && wave >= 2 ? ups : p.as + row0 / 32 * nk * 256,
+                                                   OUT == kPlain ? 0 : wave < 2 ? as_bytes : bs_bytes);
   const __amdgpu_buffer_rsrc_t rs0 = Rsrc(p.a, 0);  // loads past the last step: every access out of range
 
   // A piece is 1 KB: 8 rows of 128 bytes or 4 of 256; lane -> (row, position),
@@ -169,10 +170,9 @@ __global__ __launch_bounds__(256, (Shape<A4, MB, NB, STAGES>::kLds > 80 * 1024 ?
   static_assert(LA % 4 == 0 && LB % 2 == 0, "keys repeat within a wave's pieces");
   unsigned a_g = A4 ? (unsigned)((8 * wave * LA + (lane >> 3)) * pitch_a + 16 * ((lane & 7) ^ (lane >> 3)))
                           : (unsigned)((4 * wave * LA + (lane >> 4)) * pitch_a + 16 * ((lane & 15) ^ (lane >> 4)));
-  // gated: a piece is in the block of 32 tile rows wave LB / 4 + x / 4, and that is
-  // every other one of a weight's
-  constexpr int kPieces = OUT == kPlain ? LB : LB / 2;  // of a weight, of a wave's LB
-  const unsigned b_row = (unsigned)((8 * (OUT == kPlain || LB >= 8 ? wave * kPieces : wave / 2 * 4) + (lane >> 3)) * pitch_b);
+  // gated: a wave's pieces are a block of 32 tile rows, every other one a weight's
+  static_assert(OUT == kPlain || LB == 4, "a block a wave");
+  const unsigned b_row = (unsigned)((8 * (OUT == kPlain ? wave * LB : wave / 2 * LB) + (lane >> 3)) * pitch_b);
   unsigned b_g0 = b_row + 16 * ((lane & 7) ^ (lane >> 3)), b_g1 = b_row + 16 * ((lane & 7) ^ (lane >> 3) ^ 1);
   const unsigned a_piece = (unsigned)(A4 ? 8 * pitch_a : 4 * pitch_a), b_piece = (unsigned)(8 * pitch_b);
 
@@ -186,11 +186,17 @@ __global__ __launch_bounds__(256, (Shape<A4, MB, NB, STAGES>::kLds > 80 * 1024 ?
                    (a_g ^ (A4 ? 16 * (x & 1) : 64 * (x & 3))) + ((unsigned)x * a_piece + (unsigned)t * kRowA));
     } else if (x < LA + LB) {
       const int piece = x - LA;
-      const __amdgpu_buffer_rsrc_t rs = OUT == kPlain ? rsB : LB < 8 ? rsW : piece / 4 & 1 ? rsU : rsB;
-      const int mine = OUT == kPlain || LB < 8 ? piece : piece / 8 * 4 + piece % 4;  // rows 8 mine of the wave's of that weight
-      DirectLoad16(live ? rs : rs0, st + S::kA + (wave * LB + piece) * 1024,
-                   (piece & 1 ? b_g1 : b_g0) + ((unsigned)mine * b_piece + (unsigned)t * 128));
+      DirectLoad16(live ? rsB : rs0, st + S::kA + (wave * LB + piece) * 1024,
+                   (piece & 1 ? b_g1 : b_g0) + ((unsigned)piece * b_piece + (unsigned)t * 128));
     } else {
+      if constexpr (WN > 2) {
+        const bool is_a = x == LA + LB;
+        const int blk = is_a ? wave % (2 * MB) : wave;
+        const int from = OUT != kPlain && !is_a ? blk / 2 : blk;
+        DirectLoad4(live ? is_a ? rsS : rsT : rs0, st + S::kA + S::kB + ((is_a ? 0 : 2 * MB) + blk) * 256,
+                    (unsigned)((from * nk + t) * 256 + lane * 4));
+        return;
+      }
       const int blk = (wave & 1) * sblk + (x - LA - LB) % sblk;
       // (the parity of blk is that of x's place, 4 or 2 to a wave)
       const __amdgpu_buffer_rsrc_t rs = OUT != kPlain && (x - LA - LB) % 2 ? rsT : rsS;

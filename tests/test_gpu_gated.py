@@ -98,6 +98,22 @@ def test_gated_of_codes(gpu, M, N, K, act):
     check(gpu, None, gate, up, act, "silu", codes=(codes, s, values))
 
 
+@pytest.mark.parametrize("M,N,K,act", [(1000, 3050, 288, "fp8"), (1000, 3050, 1056, "fp8"), (2000, 4200, 800, "fp4"), (2000, 4200, 1024, "fp4")])
+def test_large_tiles_over_several_steps(gpu, M, N, K, act):
+    check(gpu, *operands(M, N, K, "bf16"), act, "silu")
+
+
+@pytest.mark.parametrize("M,N,K,act", [(1000, 6100, 1056, "fp8"), (2000, 8400, 800, "fp4"), (100, 4000, 1312, "fp8"), (100, 4000, 2592, "fp4"),
+                                       (1000, 6100, 8480, "fp8")])
+def test_plain_products_by_tiles_over_several_steps(gpu, M, N, K, act):
+    """(the last on four waves; its rows and columns are looked at by a sample)"""
+    x, w, _ = operands(M, N, K, "bf16")
+    got = gpu.mx_matmul(x.cuda(), w[0].cuda(), w[1].cuda(), a_type=gpu.FLOAT8E4M3FN if act == "fp8" else gpu.FLOAT4E2M1)
+    rows, cols = torch.arange(0, M, 1 if K < 3000 else 17), torch.arange(0, N, 1 if K < 3000 else 23)
+    want, off = ts.product(dc.mx_values(*dc.mx_quantize(x, act))[rows], dense(w)[cols], act)
+    dc.near(got.cpu()[rows][:, cols], want, dc.ROUND[got.dtype] * want.abs() + off + 2.0 ** -25)
+
+
 @pytest.mark.parametrize("M,N,K,act", [(1000, 3050, 96, "fp8"), (1900, 4000, 64, "fp8"), (2000, 4200, 64, "fp4"), (40, 5700, 96, "fp8"),
                                        (61, 3600, 288, "fp8"), (50, 6301, 96, "fp4")])
 def test_wide(gpu, M, N, K, act):
