@@ -156,16 +156,16 @@ struct MxScratch {
         b_tiles(Scratch::Round((size_t)mx::ScaleTileBytes(p.N, p.K))) {}
 };
 
-template <bool A4, int MB, int NB, int STAGES, int WN = 2> void LaunchGemm(const mx::GemmArgs &g, int output, hipStream_t s) {
-  using S = mx::Shape<A4, MB, NB, STAGES, WN>;
+template <bool A4, int MB, int NB, int STAGES, int WM, int WN> void LaunchGemm(const mx::GemmArgs &g, int output, hipStream_t s) {
+  using S = mx::Shape<A4, MB, NB, STAGES, WM, WN>;
   const dim3 grid((unsigned)(Ceil(g.M, S::BM) * Ceil(g.N, output ? S::BN / 2 : S::BN)));
-  if constexpr (NB == 2) {
+  if constexpr (WM * WN == 8) {
     if (output == kGatedMx)
-      mx::GemmKernel<A4, MB, NB, STAGES, WN, kGatedMx><<<grid, 128 * WN, 0, s>>>(g);
+      mx::GemmKernel<A4, MB, NB, STAGES, WM, WN, kGatedMx><<<grid, 512, 0, s>>>(g);
     else if (output == kGated)
-      mx::GemmKernel<A4, MB, NB, STAGES, WN, kGated><<<grid, 128 * WN, 0, s>>>(g);
+      mx::GemmKernel<A4, MB, NB, STAGES, WM, WN, kGated><<<grid, 512, 0, s>>>(g);
   }
-  if (output == kPlain) mx::GemmKernel<A4, MB, NB, STAGES, WN><<<grid, 128 * WN, 0, s>>>(g);
+  if (output == kPlain) mx::GemmKernel<A4, MB, NB, STAGES, WM, WN><<<grid, 64 * WM * WN, 0, s>>>(g);
 }
 
 // Large tiles (256 x 256, 128 x 256 for E4M3 activations) feed more MFMAs per
@@ -182,12 +182,16 @@ template <bool A4, int MB, int NB, int STAGES, int WN = 2> void LaunchGemm(const
 // 128 x 4096 x 4096 20.5 | 18.2, 1000 x 14336 x 4096 66.9 | 61.7; MXFP4 128 x 4096 x
 // 4096 18.5 | 14.4, 1000 x 14336 x 4096 53.6 | 45.0, but 1000 x 4096 x 6144 25.7 | 30.3,
 // 2000 x 4096 x 4096 30.4 | 35.9.
-// A large tile has eight waves, two a SIMD, of which one multiplies while the other waits
-// or stores; four read less of LDS, which wins in the end along a long K of E4M3.  us,
-// four waves | eight: MXFP4 4096 x 8192 x 8192 153 | 149, 1000 x 4096 x 14336 44.4 | 39.8,
-// gated 4096 x 8192 x 14336 572 | 472; MXFP8 1000 x 4096 x 14336 62 | 58, 16384 x 4096 x
-// 4096 278 | 270, 2000 x 8192 x 8192 118 | 117, 4096 x 8192 x 8192 234 | 243, 1000 x 14336 x
-// 14336 181 | 193, gated 500 x 4096 x 14336 72.6 | 63.0, 4096 x 8192 x 14336 821 | 811.
+// Tiles have eight waves, two a SIMD, of which one multiplies while the other waits or
+// stores.  Four read less of LDS, which wins along a long K of E4M3 by large tiles.
+// us, four waves | eight, large tiles: MXFP4 4096 x 8192 x 8192 153 | 149, 1000 x 4096 x
+// 14336 44.4 | 39.8, gated 4096 x 8192 x 14336 572 | 472; MXFP8 1000 x 4096 x 14336 62 | 58,
+// 16384 x 4096 x 4096 278 | 270, 2000 x 8192 x 8192 118 | 117, 4096 x 8192 x 8192 234 | 243,
+// 1000 x 14336 x 14336 181 | 193, gated 500 x 4096 x 14336 72.6 | 63.0, 4096 x 8192 x 14336
+// 821 | 811.  Small ones: MXFP8 128 x 4096 x 4096 18.2 | 16.5, 1000 x 14336 x 4096 60.7 |
+// 60.6; MXFP4 128 x 4096 x 4096 14.4 | 13.1, 2000 x 4096 x 4096 30.7 | 31.1, gated 33 x 5120 x
+// 13001 27.6 | 23.7.  (Three blocks of 32 columns, the middle tile's, are not two waves' to
+// share.)
 enum class Tiles { kSmall, kMiddle, kLarge };
 Tiles TilesOf(const MxMatMulParams &p) {
   const int64_t cus = Ctx().num_cus;
@@ -388,19 +392,19 @@ void LaunchMxMatMul(const MxMatMulParams &p, void *scratch, hipStream_t stream) 
                        p.activation, p.y_scale};
   const Tiles tiles = TilesOf(p);
   if (tiles == Tiles::kLarge && p.a_fp4)
-    LaunchGemm<true, 4, 2, 2, 4>(g, p.output, stream);
+    LaunchGemm<true, 4, 2, 2, 2, 4>(g, p.output, stream);
   else if (tiles == Tiles::kLarge && (p.output || p.K < 8192))
-    LaunchGemm<false, 2, 2, 2, 4>(g, p.output, stream);
+    LaunchGemm<false, 2, 2, 2, 2, 4>(g, p.output, stream);
   else if (tiles == Tiles::kLarge)
-    LaunchGemm<false, 2, 4, 2>(g, kPlain, stream);
+    LaunchGemm<false, 2, 4, 2, 2, 2>(g, kPlain, stream);
   else if (tiles == Tiles::kMiddle)
-    LaunchGemm<false, 2, 3, 2>(g, p.output, stream);
+    LaunchGemm<false, 2, 3, 2, 2, 2>(g, kPlain, stream);
   else if (!p.a_fp4)
-    LaunchGemm<false, 2, 2, 3>(g, p.output, stream);
+    LaunchGemm<false, 1, 2, 3, 4, 2>(g, p.output, stream);
   else if (Ceil(p.M, 128) * Ceil(p.N, p.output ? 64 : 128) <= Ctx().num_cus)
-    LaunchGemm<true, 2, 2, 4>(g, p.output, stream);
+    LaunchGemm<true, 1, 2, 4, 4, 2>(g, p.output, stream);
   else
-    LaunchGemm<true, 2, 2, 2>(g, p.output, stream);
+    LaunchGemm<true, 1, 2, 2, 4, 2>(g, p.output, stream);
 }
 
 }  // namespace onnxl_amd

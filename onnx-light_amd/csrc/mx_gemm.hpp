@@ -7,8 +7,8 @@
 // E8M0 scale of k block h comes from the same lane, one byte of a register that
 // the instruction selects.
 //
-// Workgroup: 4 waves (2 x 2) or 8 (2 x 4), tile 64 MB x 64 NB outputs or 64 MB x 128 NB,
-// each wave MB x NB blocks of 32 x 32.  A K step is 256 values: 128 bytes of an E2M1 row, 256 of
+// Workgroup: WM x WN waves, 4 (2 x 2) or 8 (2 x 4, 4 x 2), each with MB x NB
+// blocks of 32 x 32.  A K step is 256 values: 128 bytes of an E2M1 row, 256 of
 // an E4M3 row, two 16-byte chunks (four) per 64-value sub-step and lane.  Two
 // or more stages in LDS, filled by direct loads (16 bytes a lane, nothing held in
 // registers) while another is multiplied; a row's chunks are XOR-swizzled by
@@ -116,22 +116,27 @@ __device__ __forceinline__ uint16_t Half(float v, int bf16) {
 __device__ __forceinline__ v8i Operand(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 __device__ __forceinline__ v8i Operand(v8i v) { return v; }
 
-template <bool A4, int MB, int NB, int STAGES = 2, int WN = 2> struct Shape {
-  static constexpr int BM = 64 * MB, BN = 32 * NB * WN;
+template <bool A4, int MB, int NB, int STAGES, int WM, int WN> struct Shape {
+  static constexpr int BM = 32 * MB * WM, BN = 32 * NB * WN;
   static constexpr int kRowA = A4 ? 128 : 256;  // bytes of an a row per step
   static constexpr int kA = BM * kRowA, kB = BN * 128, kS = (BM + BN) * 8;
   static constexpr int kStage = kA + kB + kS;
   static constexpr int kLds = STAGES * kStage;
 };
 
-template <bool A4, int MB, int NB, int STAGES, int WN, int OUT = kPlain>
-__global__ __launch_bounds__(128 * WN, (Shape<A4, MB, NB, STAGES, WN>::kLds > 80 * 1024 && WN == 2 ? 1 : 2)) void GemmKernel(const GemmArgs p) {
-  using S = Shape<A4, MB, NB, STAGES, WN>;
+// Waves of a SIMD that the registers have to suffice for: those of one workgroup, or of two
+// where LDS has room for them.
+template <typename S, int W> constexpr int kGemmFit = W / 4 * (S::kLds > 80 * 1024 ? 1 : 2);
+
+template <bool A4, int MB, int NB, int STAGES, int WM, int WN, int OUT = kPlain>
+__global__ __launch_bounds__(64 * WM * WN, (kGemmFit<Shape<A4, MB, NB, STAGES, WM, WN>, WM * WN>)) void GemmKernel(const GemmArgs p) {
+  using S = Shape<A4, MB, NB, STAGES, WM, WN>;
+  constexpr int W = WM * WN;
   constexpr int NW = OUT == kPlain ? 1 : 2, NO = NB / NW;  // weights, a wave's blocks of y's columns
   static_assert(NB % NW == 0, "gate and up in pairs");
   constexpr int BM = S::BM, BN = S::BN / NW, kRowA = S::kRowA;  // rows and columns of y
-  constexpr int LA = S::kA / (2048 * WN), LB = S::kB / (2048 * WN);  // 1 KB loads per wave and step
-  constexpr int LS = WN > 2 ? 2 : MB > NB ? MB : NB;   // 256-byte scale loads per wave and step
+  constexpr int LA = S::kA / (1024 * W), LB = S::kB / (1024 * W);  // 1 KB loads per wave and step
+  constexpr int LS = W == 4 ? (MB > NB ? MB : NB) : WN == 4 ? 2 : 1;  // 256-byte scale loads per wave and step
   __shared__ __align__(1024) char lds[S::kLds];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, r = lane & 31, h = lane >> 5;
@@ -149,30 +154,30 @@ __global__ __launch_bounds__(128 * WN, (Shape<A4, MB, NB, STAGES, WN>::kLds > 80
   const int nk = (int)((p.K + 255) / 256);
   const int64_t pitch_a = (int64_t)nk * kRowA, pitch_b = p.K / 2;
   const int64_t rows_a = p.M - row0 < BM ? p.M - row0 : BM, rows_b = p.N - col0 < BN ? p.N - col0 : BN;
-  const __amdgpu_buffer_rsrc_t rsA = Rsrc(p.a + row0 * pitch_a, rows_a * pitch_a), rsB = Rsrc((OUT != kPlain && wave & 1 ? p.up : p.b) + col0 * pitch_b, rows_b * pitch_b);
-  // scale tiles, blocks past the last are not read.  Four waves: 0 and 1 load those of a's
-  // 32-row blocks, 2 and 3 of b's; eight: one of b's each, and one of a's, which some load
-  // twice where there are four.  Gated: odd blocks of b are the second weight's
-  static_assert(WN == 2 || (WN == 4 && NB == 2 && MB <= 4), "a scale block of b a wave");
-  const int sblk = wave < 2 ? MB : NB;
-  const uint8_t *bs = p.bs + col0 / 32 * nk * 256, *ups = p.ups + col0 / 32 * nk * 256;
-  const unsigned as_bytes = (unsigned)((rows_a + 31) / 32 * nk * 256), bs_bytes = (unsigned)((rows_b + 31) / 32 * nk * 256);
-  const bool for_a = WN > 2 || wave < 2;
-  const __amdgpu_buffer_rsrc_t rsS = Rsrc(for_a ? p.as + row0 / 32 * nk * 256 : bs, for_a ? as_bytes : bs_bytes);
-  const __amdgpu_buffer_rsrc_t rsT = WN > 2 ? Rsrc(OUT != kPlain && wave & 1 ? ups : bs, bs_bytes)
-                                            : Rsrc(OUT != kPlain && wave >= 2 ? ups : p.as + row0 / 32 * nk * 256,
-                                                   OUT == kPlain ? 0 : wave < 2 ? as_bytes : bs_bytes);
+  // gated: a wave's pieces of b are one of the weights', blocks of 32 rows in turn
+  const bool b_up = OUT != kPlain && (LB == 2 ? wave / 2 : wave) % 2;
+  const __amdgpu_buffer_rsrc_t rsA = Rsrc(p.a + row0 * pitch_a, rows_a * pitch_a);
+  const __amdgpu_buffer_rsrc_t rsB = Rsrc((b_up ? p.up : p.b) + col0 * pitch_b, rows_b * pitch_b);
+  // scale tiles, blocks of 32 rows, those past the last not read.  Four waves: 0 and 1 load
+  // those of a, 2 and 3 of b; 4 x 2: each one, the first four of a; 2 x 4: each one of b's
+  // and one of a's, which two load where there are four.  Gated: odd blocks of b are the
+  // second weight's
+  static_assert(W == 4 ? OUT == kPlain : NB == 2 && (WN == 4 ? MB <= 4 : MB == 1), "scale blocks by waves");
+  const uint8_t *as = p.as + row0 / 32 * nk * 256, *bs = (OUT != kPlain && wave % 2 ? p.ups : p.bs) + col0 / 32 * nk * 256;
+  const int64_t as_bytes = (rows_a + 31) / 32 * nk * 256, bs_bytes = (rows_b + 31) / 32 * nk * 256;
+  const bool for_a = WN == 4 || wave < W / 2;
+  const __amdgpu_buffer_rsrc_t rsS = Rsrc(for_a ? as : bs, for_a ? as_bytes : bs_bytes), rsT = Rsrc(bs, WN == 4 ? bs_bytes : 0);
   const __amdgpu_buffer_rsrc_t rs0 = Rsrc(p.a, 0);  // loads past the last step: every access out of range
 
   // A piece is 1 KB: 8 rows of 128 bytes or 4 of 256; lane -> (row, position),
   // position c of row x holding chunk c ^ key(x).  Piece q of a wave is some rows
   // further and differs in the key by q's low bits alone.
-  static_assert(LA % 4 == 0 && LB % 2 == 0, "keys repeat within a wave's pieces");
+  static_assert(LA % (A4 ? 2 : 4) == 0 && LB % 2 == 0, "keys repeat within a wave's pieces");
   unsigned a_g = A4 ? (unsigned)((8 * wave * LA + (lane >> 3)) * pitch_a + 16 * ((lane & 7) ^ (lane >> 3)))
                           : (unsigned)((4 * wave * LA + (lane >> 4)) * pitch_a + 16 * ((lane & 15) ^ (lane >> 4)));
-  // gated: a wave's pieces are a block of 32 tile rows, every other one a weight's
-  static_assert(OUT == kPlain || LB == 4, "a block a wave");
-  const unsigned b_row = (unsigned)((8 * (OUT == kPlain ? wave * LB : wave / 2 * LB) + (lane >> 3)) * pitch_b);
+  static_assert(OUT == kPlain || LB == 4 || LB == 2, "a block a wave, or half of one");
+  const int b_first = OUT == kPlain ? wave * LB : LB == 4 ? wave / 2 * 4 : wave / 4 * 4 + wave % 2 * 2;  // in eights, of the weight
+  const unsigned b_row = (unsigned)((8 * b_first + (lane >> 3)) * pitch_b);
   unsigned b_g0 = b_row + 16 * ((lane & 7) ^ (lane >> 3)), b_g1 = b_row + 16 * ((lane & 7) ^ (lane >> 3) ^ 1);
   const unsigned a_piece = (unsigned)(A4 ? 8 * pitch_a : 4 * pitch_a), b_piece = (unsigned)(8 * pitch_b);
 
@@ -189,19 +194,12 @@ __global__ __launch_bounds__(128 * WN, (Shape<A4, MB, NB, STAGES, WN>::kLds > 80
       DirectLoad16(live ? rsB : rs0, st + S::kA + (wave * LB + piece) * 1024,
                    (piece & 1 ? b_g1 : b_g0) + ((unsigned)piece * b_piece + (unsigned)t * 128));
     } else {
-      if constexpr (WN > 2) {
-        const bool is_a = x == LA + LB;
-        const int blk = is_a ? wave % (2 * MB) : wave;
-        const int from = OUT != kPlain && !is_a ? blk / 2 : blk;
-        DirectLoad4(live ? is_a ? rsS : rsT : rs0, st + S::kA + S::kB + ((is_a ? 0 : 2 * MB) + blk) * 256,
-                    (unsigned)((from * nk + t) * 256 + lane * 4));
-        return;
-      }
-      const int blk = (wave & 1) * sblk + (x - LA - LB) % sblk;
-      // (the parity of blk is that of x's place, 4 or 2 to a wave)
-      const __amdgpu_buffer_rsrc_t rs = OUT != kPlain && (x - LA - LB) % 2 ? rsT : rsS;
-      const int from = OUT != kPlain && wave >= 2 ? blk / 2 : blk;
-      DirectLoad4(live ? rs : rs0, st + S::kA + S::kB + ((wave < 2 ? 0 : 2 * MB) + blk) * 256,
+      const int i = x - LA - LB;
+      const bool of_a = WN == 4 ? i == 0 : wave < W / 2;
+      const int blocks = of_a ? WM * MB : WN * NB;  // of the tile
+      const int blk = W == 4 ? wave % 2 * (blocks / 2) + i % (blocks / 2) : wave % blocks;
+      const int from = OUT != kPlain && !of_a ? blk / 2 : blk;  // of the matrix
+      DirectLoad4(live ? (WN == 4 && i ? rsT : rsS) : rs0, st + S::kA + S::kB + ((of_a ? 0 : WM * MB) + blk) * 256,
                   (unsigned)((from * nk + t) * 256 + lane * 4));
     }
   };
@@ -237,7 +235,7 @@ __global__ __launch_bounds__(128 * WN, (Shape<A4, MB, NB, STAGES, WN>::kLds > 80
     if (x < MB)
       sa[buf][x] = *reinterpret_cast<const int *>(st + (wm * MB + x) * 256 + lane * 4);
     else
-      sb[buf][x - MB] = *reinterpret_cast<const int *>(st + (2 * MB + wn * NB + x - MB) * 256 + lane * 4);
+      sb[buf][x - MB] = *reinterpret_cast<const int *>(st + (WM * MB + wn * NB + x - MB) * 256 + lane * 4);
   };
 
   v16f acc[MB][NB];
