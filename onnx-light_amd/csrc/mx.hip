@@ -207,31 +207,34 @@ Tiles TilesOf(const MxMatMulParams &p) {
 // Few rows take the streaming kernel, whose time goes with the weight's bytes and
 // the row tiles; the GEMM's one round of tiles goes with K alone, and a wide
 // weight fills it.  us, rows x K x N, stream | GEMM (gated: N of each weight):
-//   MXFP4  32 x 4096 x 14336 14.9 | 15.1    36 x 2048 x 8192 7.8 | 10.9
-//          40 x 4096 x 14336 16.9 | 15.2    40 x 11008 x 8192 22.2 | 25.5
-//          56 x 4096 x 11008 20.3 | 16.0    64 x 4096 x 8192 12.8 | 14.5
-//          64 x 8192 x 8192 27.2 | 21.4     64 x 11008 x 4096 21.0 | 25.2
-//   MXFP8  36 x 2048 x 8192 8.6 | 12.5      40 x 11008 x 8192 35.2 | 32.9
-//          48 x 4096 x 6144 15.7 | 17.2     64 x 4096 x 4096 15.9 | 17.3
-//          64 x 11008 x 4096 28.7 | 32.7    33 x 8192 x 28672 81 | 44.1
+//   MXFP4  32 x 4096 x 14336 14.8 | 13.7    20 x 8192 x 28672 45.6 | 38.2
+//          36 x 2048 x 8192 8.1 | 9.5       40 x 8192 x 8192 18.1 | 19.7
+//          40 x 11008 x 8192 22.1 | 24.0    48 x 4096 x 11008 17.7 | 14.4
+//          64 x 2048 x 8192 8.6 | 9.7       64 x 4096 x 6144 12.5 | 12.9
+//          64 x 4096 x 8192 12.9 | 13.1     52 x 8192 x 5632 22.0 | 19.6
+//          64 x 11008 x 4096 21.0 | 23.4
+//   MXFP8  20 x 8192 x 28672 45.5 | 42.1    32 x 4096 x 14336 18.1 | 16.7
+//          36 x 2048 x 8192 8.9 | 11.1      48 x 4096 x 6144 15.6 | 15.8
+//          48 x 4096 x 8192 18.3 | 16.1     40 x 11008 x 8192 35.2 | 31.8
+//          64 x 4096 x 4096 15.8 | 15.7     64 x 4096 x 6144 18.7 | 15.9
+//          64 x 11008 x 4096 28.7 | 31.4
 //   gated, MXFP4
-//          20 x 4096 x 14336 22.7 | 21.9    32 x 4096 x 14336 24.0 | 21.9
-//          32 x 4096 x 8192 15.1 | 18.4     48 x 2048 x 5632 12.7 | 14.2
-//          33 x 4096 x 8192 18.0 | 18.5     33 x 8192 x 8192 28.3 | 25.6
-//          33 x 5120 x 13001 32.1 | 27.4    64 x 4096 x 4096 13.7 | 17.6
-//          64 x 8192 x 5632 40.0 | 25.2
+//          32 x 4096 x 8192 15.2 | 15.4     24 x 4096 x 11008 21.6 | 18.2
+//          33 x 2048 x 8192 11.1 | 11.7     33 x 4096 x 8192 18.0 | 15.5
+//          48 x 4096 x 5632 18.3 | 15.2     33 x 5120 x 13001 32.1 | 23.7
+//          64 x 4096 x 4096 13.6 | 14.7
 //   gated, MXFP8
-//          20 x 4096 x 14336 24.8 | 23.0    32 x 4096 x 14336 29.3 | 23.0
-//          24 x 4096 x 10240 21.6 | 21.6    20 x 8192 x 8192 25.6 | 31.0
+//          32 x 4096 x 8192 19.5 | 18.7     24 x 4096 x 11008 21.7 | 20.8
+//          20 x 8192 x 11008 36.0 | 35.7
 bool Streams(const MxMatMulParams &p) {
   if (p.M <= 16 || p.M > 64) return p.M <= 16;
   const int64_t rows = WeightRows(p), K = std::max<int64_t>(p.K, 1);
-  if (p.M <= 32) return p.output != kGated || rows < 24576;
-  // MXFP8 output takes four row tiles, which more rows leave no registers for
-  if (p.output == kGatedMx) return false;
+  // MXFP8 output takes four row tiles, which more than 32 rows leave no registers for
+  if (p.output == kGatedMx) return p.M <= 32;
+  if (p.M <= 32) return rows < 14336;
   // where rows * K of the one takes as long as K and a launch of the other
-  if (p.a_fp4) return rows < (p.M > 48 ? 4500 + 16500000 / K : 9000 + 20000000 / K);
-  return rows < (p.M <= 48 ? 11264 : 7168);
+  if (p.a_fp4) return rows < (p.M > 48 ? 3000 + 19000000 / K : 7000 + 16000000 / K);
+  return rows < 3500 + 10000000 / K;
 }
 
 // Up to this many values every workgroup quantizes its activations itself
