@@ -172,16 +172,20 @@ template <bool A4, int MB, int NB, int STAGES, int WM, int WN> void LaunchGemm(c
 // byte, small ones (128 x 128) leave fewer CUs idle; E4M3 has 128 x 192 between
 // them.  A round of small, middle and large ones takes about 20, 24 and 29 parts of
 // time (of the small ones two fit a CU for E2M1), and the shortest sum is taken.
-// us, large / small: MXFP4 1000 x 4096 x 6144 38 / 25, 4096 x 8192 x 8192 156 /
-// 184.  Large / middle / small: MXFP8 256 x 4096 x 4096 27 / 24 / 21, 1000 x 4096 x
-// 6144 33 / 30 / 41, 2048 x 4096 x 4096 39 / 51 / 45, 4096 x 8192 x 8192 234 / 278 /
-// 311.
+// us, large / small: MXFP4 4096 x 4096 x 4096 47 / 56, 4096 x 8192 x 8192 149 / 190, gated
+// 1000 x 4096 x 14336 89 / 94; MXFP8 2000 x 4096 x 4096 37.5 / 44.6, 4096 x 4096 x 4096 72 / 81,
+// 700 x 8192 x 8192 51 / 60, gated 1000 x 4096 x 14336 131 / 134, 1000 x 2048 x 5632 40.6 / 38.3
+// (the rule's loss).  Middle / small: 1000 x 4096 x 6144 31.4 / 37.2.  With four waves large /
+// small MXFP4 1000 x 4096 x 6144 38 / 25, large / middle / small MXFP8 256 x 4096 x 4096 27 /
+// 24 / 21, 1000 x 4096 x 6144 33 / 30 / 41.
+//
 // A small tile has as many stages as LDS has room for, since a step of its own takes
 // less time than a load: three for E4M3, and for E2M1 four, where there are no more tiles
 // than CUs, else two, so that two workgroups share a CU.  us, two stages | more: MXFP8
 // 128 x 4096 x 4096 20.5 | 18.2, 1000 x 14336 x 4096 66.9 | 61.7; MXFP4 128 x 4096 x
 // 4096 18.5 | 14.4, 1000 x 14336 x 4096 53.6 | 45.0, but 1000 x 4096 x 6144 25.7 | 30.3,
 // 2000 x 4096 x 4096 30.4 | 35.9.
+//
 // Tiles have eight waves, two a SIMD, of which one multiplies while the other waits or
 // stores.  Four read less of LDS, which wins along a long K of E4M3 by large tiles.
 // us, four waves | eight, large tiles: MXFP4 4096 x 8192 x 8192 153 | 149, 1000 x 4096 x
