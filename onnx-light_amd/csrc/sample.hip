@@ -488,8 +488,8 @@ template <int DT> __device__ __forceinline__ float BinsFrom(Shared &s, const Row
   __syncthreads();
   return from;
 }
-// Weights of the tokens from..to - 1 in bins, of those that are at least `least`; the sum of
-// this thread's, all of them.
+// Weights of the tokens from..to - 1 in bins, of those that are at least `least`, there for
+// every thread when it returns; the sum of this thread's, all of them.
 template <int DT> __device__ __forceinline__ u64 FillBins(Shared &s, const Row<DT> &r, float least, int from, int to) {
   u64 sum = 0;
   r.Each(from, to, [&](const auto &x, int, int) __attribute__((always_inline)) {
@@ -502,6 +502,7 @@ template <int DT> __device__ __forceinline__ u64 FillBins(Shared &s, const Row<D
       if (x[j] >= least) atomicAdd(&s.bin[r.Bin(x[j])], e[j]);
     }
   });
+  __syncthreads();
   return sum;
 }
 // The border of top_p from bins, or from sums of `width` of them that stand in the last; by_bits
