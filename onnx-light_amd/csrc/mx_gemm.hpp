@@ -104,13 +104,10 @@ template <int LEFT = 0> __device__ __forceinline__ void StepBarrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
+// To nearest even, by conversions that the compiler knows: v may be a matrix product's register, for which it puts
+// in the wait states (behind an assembly statement it does not).
 __device__ __forceinline__ uint16_t Half(float v, int bf16) {
-  unsigned r;
-  if (bf16) {
-    asm("v_cvt_pk_bf16_f32 %0, %1, %1" : "=v"(r) : "v"(v));
-    return (uint16_t)r;
-  }
-  return __builtin_bit_cast(uint16_t, (_Float16)v);
+  return bf16 ? __builtin_bit_cast(uint16_t, (__bf16)v) : __builtin_bit_cast(uint16_t, (_Float16)v);
 }
 
 // E2M1 operands take the first four registers.
