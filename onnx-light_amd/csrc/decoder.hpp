@@ -8,6 +8,8 @@
 
 #include <cstdint>
 
+#include "mx_plan.hpp"
+
 namespace onnxl_amd {
 
 // A launch has fewer than 2^32 threads along x: a larger grid runs in part, and
@@ -63,7 +65,6 @@ void LaunchMxQuantize(const MxQuantParams &p, hipStream_t stream);
 // y[m, n] = sum over blocks of 2^(sa + sb) * sum of a[m, k] b[n, k]; M, N > 0.
 // Gated: y = act(a . b^T) * (a . up^T), both weights [N, K], in 16 bits or as MXFP8
 // (codes y and E8M0 scales y_scale [M, N / 32], N % 32 == 0).
-enum MxOutput : int { kPlain = 0, kGated = 1, kGatedMx = 2 };
 enum Activation : int { kSilu = 0, kGelu = 1, kGeluTanh = 2, kRelu = 3 };
 struct MxMatMulParams {
   const void *x;           // [M, K] FLOAT16 or BFLOAT16, quantized by the call; or nullptr and
