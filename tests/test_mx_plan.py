@@ -5,6 +5,8 @@ import subprocess
 
 import pytest
 
+from mx_kernel_cases import BOTH, CASES
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "onnx-light_amd", "csrc")
 OUTPUT = {"plain": 0, "gated": 1, "gated mx": 2}
 CUS = 256
@@ -62,3 +64,16 @@ MEASURED = [
 def test_few_rows_take_the_faster_kernel(plan, form, act, M, K, N, stream, tiles):
     """Sizes on both sides of the rule's lines, each more than a tenth apart (a few less)."""
     assert plan(form, act, M, K, N).startswith("stream" if stream < tiles else "tiles")
+
+
+def test_every_kernel_that_a_size_takes_is_tested(plan):
+    """Of a sweep of sizes, each kernel (and for the streaming one, K shared by workgroups or not) is a size's of the GPU
+    tests too; sizes that take a kernel in fewer than three of its steps do not count there."""
+    rows = [1, 2, 3, 4, 8, 16, 17, 24, 31, 32, 33, 40, 48, 49, 56, 64, 65, 100, 128, 129, 200, 256, 300, 513, 700, 1000, 2000, 4096, 10000]
+    widths = [1, 16, 33, 64, 100, 257, 512, 1000, 1056, 2048, 2600, 3050, 4096, 5700, 6100, 8192, 9000, 11008, 14336, 20000, 28672, 60000]
+    lengths = [32, 96, 256, 288, 512, 544, 800, 1056, 1312, 2048, 2080, 2592, 4096, 6016, 8192, 8480, 14336, 28672]
+    met = {(form, act, plan(form, act, M, K, N, x)) for form in OUTPUT for act in BOTH for M in rows for N in widths for K in lengths
+           for x in (True, False) if form != "gated mx" or N % 32 == 0}
+    tested = {(form, act, plan(form, act, M, K, N, x)) for form, act, M, K, N, x in CASES
+              if K >= 768 or plan(form, act, M, K, N, x).startswith("stream")}
+    assert len(met) > 80 and not met - tested, met - tested
