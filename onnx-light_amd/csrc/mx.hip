@@ -162,14 +162,18 @@ struct MxScratch {
 template <bool A4, int MB, int NB, int STAGES, int WM, int WN> bool LaunchGemm(const mx::GemmArgs &g, const mx::GemmPlan &t, int output, hipStream_t s) {
   if (t.mb != MB || t.nb != NB || t.stages != STAGES || t.wm != WM || t.wn != WN) return false;
   using S = mx::Shape<A4, MB, NB, STAGES, WM, WN>;
-  const dim3 grid((unsigned)(Ceil(g.M, S::BM) * Ceil(g.N, output ? S::BN / 2 : S::BN)));
-  if constexpr (WM * WN == 8) {
-    if (output == kGatedMx)
-      mx::GemmKernel<A4, MB, NB, STAGES, WM, WN, kGatedMx><<<grid, 512, 0, s>>>(g);
-    else if (output == kGated)
-      mx::GemmKernel<A4, MB, NB, STAGES, WM, WN, kGated><<<grid, 512, 0, s>>>(g);
-  }
-  if (output == kPlain) mx::GemmKernel<A4, MB, NB, STAGES, WM, WN><<<grid, 64 * WM * WN, 0, s>>>(g);
+  constexpr int kThreads = 64 * WM * WN;
+  LaunchInPieces(Ceil(g.M, S::BM) * Ceil(g.N, output ? S::BN / 2 : S::BN), kThreads, [&](int64_t first, unsigned count) {
+    mx::GemmArgs p = g;
+    p.first = (int)first;
+    if constexpr (WM * WN == 8) {
+      if (output == kGatedMx)
+        mx::GemmKernel<A4, MB, NB, STAGES, WM, WN, kGatedMx><<<count, kThreads, 0, s>>>(p);
+      else if (output == kGated)
+        mx::GemmKernel<A4, MB, NB, STAGES, WM, WN, kGated><<<count, kThreads, 0, s>>>(p);
+    }
+    if (output == kPlain) mx::GemmKernel<A4, MB, NB, STAGES, WM, WN><<<count, kThreads, 0, s>>>(p);
+  });
   return true;
 }
 

@@ -83,6 +83,7 @@ struct GemmArgs {
   const uint8_t *up = nullptr, *ups = nullptr;  // gated: the second weight [N, K], its scale tiles
   int activation = 0;
   uint8_t *y_scale = nullptr;                   // kGatedMx: y is codes, these their scales [M, N / 32]
+  int first = 0;           // the launch's first workgroup
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t Rsrc(const void *p, int64_t bytes) {
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(64 * WM * WN, (kGemmFit<Shape<A4, MB, NB, STAGES, W
   // each XCD a contiguous run of tiles, kGroupM tile rows high, so that tiles
   // sharing rows of a and b share an L2
   const int nbm = (int)((p.M + BM - 1) / BM), nbn = (int)((p.N + BN - 1) / BN), total = nbm * nbn;
-  const int pid = (int)blockIdx.x, xcd = pid % kXcds, per = total / kXcds, extra = total % kXcds;
+  const int pid = p.first + (int)blockIdx.x, xcd = pid % kXcds, per = total / kXcds, extra = total % kXcds;
   const int t_all = xcd * per + (xcd < extra ? xcd : extra) + pid / kXcds;
   const int first_m = t_all / (kGroupM * nbn) * kGroupM;
   const int gsize = nbm - first_m < kGroupM ? nbm - first_m : kGroupM;
