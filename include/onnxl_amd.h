@@ -843,8 +843,9 @@ int onnxl_amd_kv_cache_attention(const onnxl_amd_tensor *q, const onnxl_amd_tens
  * a row has no other logits; probability (optional) FLOAT [rows], the token's weight
  * over the sum of the kept ones (1 at temperature 0, 0 with token -1).  A uniform below
  * 0 or NaN counts as 0, of 1 or more as the number before 1.
- * Weights are rounded to whole multiples of 2^-42 of the largest, and their sums
- * exact: a border may fall to the other token only where it is that near. */
+ * Weights are rounded to whole multiples of 2^-42 of the largest; their sums, and the
+ * shares top_p and uniform of those, are exact.  A border may fall to the other token
+ * only where it is nearer than those roundings add up to, 2^-43 for each token. */
 int onnxl_amd_sample_tokens(const onnxl_amd_tensor *logits, const onnxl_amd_tensor *uniform,
                             const onnxl_amd_tensor *temperature, const onnxl_amd_tensor *top_k,
                             const onnxl_amd_tensor *top_p, const onnxl_amd_tensor *min_p, onnxl_amd_tensor *token,

@@ -4,7 +4,7 @@
 //
 // A weight exp((x - max) / T) is a whole number of 2^-42: sums of them have no
 // order, so they are the same from run to run and however the work is split, and
-// a row's tokens and the borders of top-p are decided exactly on them.  2^-42 of
+// a row's tokens and the borders of top-p are decided exactly on them, by whole shares.  2^-42 of
 // the largest weight is far below what separates two tokens' places, and a row of
 // 2^21 tokens still adds up in 63 bits.
 //
@@ -345,9 +345,25 @@ __device__ __forceinline__ void AnswerPlain(const SampleParams &p, int64_t row, 
   const bool none = best >> 32 == 0;
   Answer(p, row, none ? -1 : (int64_t)(0xffffffffu - (unsigned)best), none ? 0.f : 1.f);
 }
+// floor(f n) of f from 0 to 1, which is m 2^-shift with m of 24 bits, and a sum n below 2^63;
+// `rest`: whether that leaves anything.  In whole numbers: the product has 87 bits.
+__device__ __forceinline__ u64 ShareOf(float f, u64 n, bool &rest) {
+  const unsigned u = __builtin_bit_cast(unsigned, f), e = max(u >> 23, 1u);
+  const u64 m = u < 0x800000u ? u : (u & 0x7fffffu) | 0x800000u;
+  const u64 hi = __umul64hi(m, n), lo = m * n;
+  const unsigned shift = 150 - e;  // 23 and more
+  if (shift < 64) {
+    rest = lo << (64 - shift) != 0;
+    return hi << (64 - shift) | lo >> shift;
+  }
+  const unsigned s = min(shift - 64, 63u);  // hi has 23 bits
+  rest = lo != 0 || (hi & ((u64(1) << s) - 1)) != 0;
+  return hi >> s;
+}
 // The token at which the weights up to it reach this is the last that top_p keeps.
 __device__ __forceinline__ u64 WantOf(float top_p, u64 total) {
-  const u64 w = (u64)ceil((double)fmaxf(top_p, 0.f) * (double)total);
+  bool rest;
+  const u64 w = ShareOf(fmaxf(top_p, 0.f), total, rest) + rest;
   return w ? w : 1;
 }
 
@@ -791,8 +807,8 @@ template <int DT> __device__ __forceinline__ void Choose(Shared &s, const Row<DT
   u64 total;
   const u64 mine = s.chunk[threadIdx.x], upto = GroupScan(s, mine, total);
   u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
-  u64 share = (u64)((double)u * (double)total);
-  if (share >= total) share = total - 1;
+  bool rest;
+  const u64 share = ShareOf(u, total, rest);
   if (upto > share && upto - mine <= share) {
     s.at = threadIdx.x;
     s.out[0] = share - (upto - mine);
