@@ -92,6 +92,8 @@ class Sequences:
 
 
 class DecoderLayer:
+    """Weights, and tables of positions for sequences of up to `longest` tokens."""
+
     def __init__(self, ola, shape: Shape, weights: dict, longest=8192):
         self.ola, self.shape = ola, shape
         self.tables = ola.rotary_tables(longest, shape.head_dim)  # cos, sin
@@ -121,7 +123,14 @@ class DecoderLayer:
     def __call__(self, x, sequences: Sequences, new):
         """x bfloat16 [tokens, hidden], the new[b] new tokens of sequence b one
         sequence after the other."""
-        return self.step(x, sequences.cache, *sequences.grow(new), max(new))
+        return self.step(x, sequences.cache, *self.grow(sequences, new), max(new))
+
+    def grow(self, sequences: Sequences, new):
+        """Sequences.grow inside the tables of positions: lengths on the GPU are not checked
+        against them by the library, and a position outside makes NaN."""
+        if max(held + n for held, n in zip(sequences.length, new)) > len(self.tables[0]):
+            raise ValueError(f"a sequence has more tokens than the layer's {len(self.tables[0])} positions")
+        return sequences.grow(new)
 
     def step(self, x, cache, table, start, lengths, most):
         """The same on the GPU alone; no sequence has more than `most` new tokens."""
@@ -174,7 +183,7 @@ def plain_layer(shape: Shape, w: dict, x, length: int):
 def run(ola, shape: Shape, prompts, tokens: int, dtype=None, seed=0):
     """Runs prompts and then `tokens` single tokens of every sequence; returns the
     layer, the inputs and the outputs of each sequence in order of position."""
-    layer = DecoderLayer(ola, shape, random_weights(shape, seed))
+    layer = DecoderLayer(ola, shape, random_weights(shape, seed), max(prompts) + tokens)
     g = torch.Generator().manual_seed(seed + 1)
     inputs = [torch.randn(n + tokens, shape.hidden, generator=g).bfloat16() for n in prompts]
     sequences = Sequences(ola, shape, len(prompts), max(prompts) + tokens, dtype=dtype)
@@ -199,7 +208,7 @@ def generate(layer: DecoderLayer, words: Vocabulary, prompts, tokens: int, seed=
     sequences = Sequences(layer.ola, layer.shape, batch, max(map(len, prompts)) + tokens)
     ids, new, drawn = torch.tensor(sum(prompts, []), device="cuda"), [len(p) for p in prompts], []
     for _ in range(tokens):
-        table, start, lengths = sequences.grow(new)
+        table, start, lengths = layer.grow(sequences, new)
         y = layer.step(words.rows[ids], sequences.cache, table, start, lengths, max(new))
         ids, _ = words.next(y, start, torch.rand(batch, generator=g, device="cuda"), *rules)
         drawn.append(ids)
