@@ -213,7 +213,7 @@ def generate(layer: DecoderLayer, words: Vocabulary, prompts, tokens: int, seed=
         ids, _ = words.next(y, start, torch.rand(batch, generator=g, device="cuda"), *rules)
         drawn.append(ids)
         new = [1] * batch
-    return torch.stack(drawn, 1).tolist()
+    return torch.stack(drawn, 1).tolist() if drawn else [[] for _ in prompts]
 
 
 def error(layer: DecoderLayer, x, y) -> float:
@@ -238,7 +238,7 @@ def main():
         print(f"sequence {b}: {prompts[b]} tokens of prompt and {a.tokens} single ones, "
               f"error {error(layer, x, y):.3f} of what the layer adds")
     words = Vocabulary(ola, shape.hidden)
-    for b, drawn in enumerate(generate(layer, words, [list(range(n)) for n in prompts], a.tokens)):
+    for b, drawn in enumerate(generate(layer, words, [[i % len(words.rows) for i in range(n)] for n in prompts], a.tokens)):
         print(f"sequence {b} goes on with tokens {drawn}")
     for name, new in (("prompt", prompts), ("token", [1] * len(prompts))):
         x = torch.randn(sum(new), shape.hidden, device="cuda").bfloat16()

@@ -40,3 +40,12 @@ def test_prompt_past_eight_thousand_tokens(olamd):
     assert [len(d) for d in drawn] == [4, 4] and all(0 <= t < 500 for d in drawn for t in d)
     with pytest.raises(ValueError, match="8194 positions"):
         ex.generate(layer, words, [[i % 500 for i in range(8190)]], 6)
+
+
+@pytest.mark.gpu
+def test_nothing_to_draw(olamd):
+    olamd.init(0)
+    ex = example()
+    shape = ex.Shape(hidden=128, heads=2, kv_heads=1, head_dim=64, inner=192)
+    layer = ex.DecoderLayer(olamd, shape, ex.random_weights(shape), 64)
+    assert ex.generate(layer, ex.Vocabulary(olamd, 128, 500), [[1, 2], [3]], 0) == [[], []]
