@@ -3783,8 +3783,6 @@ int SampleTokens(const onnxl_amd_tensor *x, const onnxl_amd_tensor *uniform, con
   p.dtype = x->data_type;
   p.k64 = !Absent(top_k) && top_k->data_type == kInt64;
   p.token64 = token->data_type == kInt64;
-  p.top_k = there(top_k) ? top_k->data : nullptr;
-  p.top_p = static_cast<const float *>(there(top_p) ? top_p->data : nullptr);
   onnxl_amd_tensor *prob = Absent(probability) ? nullptr : probability;
   Staging st(stream, SampleScratchBytes(p), {x, uniform, there(temperature), there(top_k), there(top_p), there(min_p)},
              {token, prob});
