@@ -3722,6 +3722,10 @@ int RotaryKvCacheAppend(const onnxl_amd_tensor *qkv, const onnxl_amd_tensor *cos
   const int32_t *held = lengths->location == ONNXL_AMD_HOST && Absent(ids) ? static_cast<const int32_t *>(lengths->data) : nullptr;
   for (int b = 0; held && b < c.batch; ++b)
     OLA_ENFORCE(held[b] <= p.t.positions, kRkvName, ": a sequence of lengths is longer than the tables.");
+  // keys and values are read by other workgroups than those that write q
+  const char *from = static_cast<const char *>(qkv->data), *to = static_cast<const char *>(q->data);
+  OLA_ENFORCE(qkv->location != ONNXL_AMD_DEVICE || c.tokens == 0 || to + NumElements(*q) * 2 <= from || from + NumElements(*qkv) * 2 <= to,
+              kRkvName, ": q may not overlap qkv.");
   if (c.tokens == 0 || c.batch == 0) return ONNXL_AMD_OK;
   Ctx();
   const onnxl_amd_tensor *on = Absent(ids) ? nullptr : ids;

@@ -68,3 +68,20 @@ def test_append(gpu, new, total, heads, D, d, interleaved, to, typ):
     waves = 1 if sum(new) <= 2 * len(new) else 4
     assert sum(new) * -(-heads // at_once) > 1280 * waves  # past one round
     check_append(gpu, b, heads, d, interleaved, dc.TYPE[typ])
+
+
+def test_append_with_q_beside_qkv(gpu):
+    """One piece of memory: queries to be, rows, queries to be again."""
+    b = dc.Batch(3, [1, 40], [9, 70], 2, 64, 16, "fp8", torch.bfloat16)
+    rows = dc.randn(dc.gen(4), (41, 6 + 4, 64), torch.bfloat16).cuda()
+    c, s = gpu.rotary_tables(70, 64)
+    want = gpu.rotary_kv_cache_append(rows, c, s, b.cache(gpu), *b.index())
+    n = want.numel()
+    for at in (0, n + rows.numel()):
+        memory = torch.empty(2 * n + rows.numel(), dtype=torch.bfloat16, device="cuda")
+        qkv, q = memory[n:n + rows.numel()].view(rows.shape), memory[at:at + n].view(want.shape)
+        qkv.copy_(rows)
+        gpu.rotary_kv_cache_append(qkv, c, s, b.cache(gpu), *b.index(), out=q)
+        assert torch.equal(q, want) and torch.equal(qkv, rows)
+    with pytest.raises(gpu.InvalidArgument, match="overlap"):
+        gpu.rotary_kv_cache_append(qkv, c, s, b.cache(gpu), *b.index(), out=memory[n - 8:2 * n - 8].view(want.shape))
