@@ -687,6 +687,11 @@ def _empty(shape, torch_dtype, device):
     return _torch().empty(shape, dtype=torch_dtype, device=device)
 
 
+def _type_of(t):
+    """A tensor's torch type, a numpy array's among them."""
+    return _torch().from_numpy(np.empty(0, t.dtype)).dtype if isinstance(t, np.ndarray) else t.dtype
+
+
 # ---- kernels (reference operator() overloads) ------------------------------
 
 def matmul_integer(a, b, a_zero_point=None, b_zero_point=None, out=None):
@@ -965,7 +970,7 @@ def rms_norm_quantize(x, weight, residual=None, epsilon: float = 1e-5, block_siz
         blocks = shape[-1] // block_size if block_size > 0 else 1
         out = (_empty(shape, torch.int8 if output_dtype == INT8 else torch.float8_e4m3fn, dev),
                _empty((*shape[:-1], blocks), torch.uint8 if mx else torch.float32, dev),
-               torch.empty_like(x) if residual is not None else None)
+               _empty(shape, _type_of(x), dev) if residual is not None else None)
     y, y_scale, total = out
     _check(lib().onnxl_amd_rms_norm_quantize(describe(x), describe(weight), describe(residual), epsilon, block_size,
                                              describe(y), describe(y_scale), describe(total), _stream_of(x, y)))
@@ -999,7 +1004,7 @@ def mx_matmul(a, b, b_scale, a_scale=None, a_type: int = FLOAT8E4M3FN, output_dt
     if a_scale is not None:
         a_type = 0
     if out is None:
-        dt = output_dtype or (a.dtype if a_scale is None else torch.bfloat16)
+        dt = output_dtype or (_type_of(a) if a_scale is None else torch.bfloat16)
         out = _empty((*_shape_of(a)[:-1], _shape_of(b)[0]), dt, _device_of(a, b))
     _check(lib().onnxl_amd_mx_matmul(describe(a), describe(a_scale), a_type, describe(b), describe(b_scale),
                                      describe(out), _stream_of(a, b, out)))
@@ -1033,7 +1038,7 @@ def mx_gated_matmul(a, gate, gate_scale, up, up_scale, activation: str = "silu",
         if mx:
             out = (_empty((*shape, N), torch.float8_e4m3fn, dev), _empty((*shape, N // 32), torch.uint8, dev))
         else:
-            out = _empty((*shape, N), output_dtype or (a.dtype if a_scale is None else torch.bfloat16), dev)
+            out = _empty((*shape, N), output_dtype or (_type_of(a) if a_scale is None else torch.bfloat16), dev)
     y, y_scale = out if mx else (out, None)
     _check(lib().onnxl_amd_mx_gated_matmul(describe(a), describe(a_scale), a_type, describe(gate), describe(gate_scale),
                                            describe(up), describe(up_scale), act, describe(y), describe(y_scale),
@@ -1067,7 +1072,7 @@ def rotary_embedding(x, cos, sin, position_ids=None, interleaved: bool = False, 
     first 2 * cos.shape[-1] dimensions of a head turn.  cos, sin [positions, ..]
     with position_ids [batch, seq] or [tokens], else a row for every token."""
     if out is None:
-        out = _torch().empty_like(x)
+        out = _empty(_shape_of(x), _type_of(x), _device_of(x))
     _check(lib().onnxl_amd_rotary_embedding(describe(x), describe(cos), describe(sin), describe(position_ids),
                                             int(interleaved), num_heads, describe(out), _stream_of(x, cos, out)))
     return out
@@ -1109,14 +1114,12 @@ def rotary_kv_cache_append(qkv, cos, sin, cache: KvCache, block_table, query_sta
     keys rotated and values as they are into the cache, as kv_cache_append does;
     returns the rotated queries [tokens, heads, head_dim], on the GPU.  A token's
     position is its place in its sequence, or position_ids [tokens]."""
-    torch = _torch()
     if out is None:
         tokens, rows, D = _shape_of(qkv)
         kv_heads = cache.k_cache.shape[1]
         if rows <= 2 * kv_heads:
             raise InvalidArgument("qkv has no queries beside the cache's keys and values")
-        out = _empty((tokens, rows - 2 * kv_heads, D), torch.from_numpy(qkv).dtype if isinstance(qkv, np.ndarray) else qkv.dtype,
-                     cache.k_cache.device)
+        out = _empty((tokens, rows - 2 * kv_heads, D), _type_of(qkv), cache.k_cache.device)
     _check(lib().onnxl_amd_rotary_kv_cache_append(describe(qkv), describe(cos), describe(sin), describe(position_ids),
                                                   int(interleaved), describe(out), *(describe(t) for t in cache.tensors()),
                                                   describe(block_table), describe(query_start), describe(lengths),
@@ -1129,7 +1132,7 @@ def kv_cache_attention(q, cache: KvCache, block_table, query_start, lengths, sca
     cache, which holds them already; scale defaults to head_dim ** -0.5,
     max_query is the most new tokens of a sequence where known."""
     if out is None:
-        out = _torch().empty_like(q)
+        out = _empty(_shape_of(q), _type_of(q), _device_of(q))
     if scale is None:
         scale = float(_shape_of(q)[-1]) ** -0.5
     _check(lib().onnxl_amd_kv_cache_attention(describe(q), *(describe(t) for t in cache.tensors()),
