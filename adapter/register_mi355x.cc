@@ -1882,7 +1882,7 @@ public:
 };
 
 // ai.rt.amd:RotaryEmbedding(x, cos, sin, position_ids | ""; interleaved = 0,
-// num_heads = 0) = y.
+// num_heads = 0, rotary_embedding_dim = 0: the tables') = y.
 class Mi355xRotaryEmbedding : public Mi355xKernel {
 public:
   static constexpr const char *name = "onnxl_amd:CPU:ai.rt.amd:RotaryEmbedding";
@@ -1893,6 +1893,9 @@ public:
     rt::RequireOutputCount(node, 1);
     const onnxl_amd_tensor x = In(0, ctx), cos = In(1, ctx), sin = In(2, ctx), ids = In(3, ctx);
     if (x.rank < 1) throw std::invalid_argument("RotaryEmbedding: x has no dimensions.");
+    const int64_t dim = rt::GetAttributeIntOrDefault(node, "rotary_embedding_dim", 0);
+    if (dim != 0 && (cos.rank < 1 || dim != 2 * cos.dims[cos.rank - 1]))
+      throw std::invalid_argument("RotaryEmbedding: rotary_embedding_dim is not twice the tables' last dimension.");
     const rt::Shape shape = ShapeOf(x.dims, x.rank);
     rt::Tensor y = ctx.MakeOutputTensor(0, x.data_type, shape, ByteSize(x.data_type, Count(shape)));
     onnxl_amd_tensor dy = DescribeOutput(y);
