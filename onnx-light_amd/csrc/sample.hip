@@ -1092,6 +1092,14 @@ template <int DT> __global__ __launch_bounds__(kThreads) void SampleTakeKernel(c
 //            32 rows    45 | 69       84 | 101      117 | 115
 //   top_k 50  1 row     22 | 26       31 | 27       39 | 27   (fp32)
 //            16 rows    24 | 28       33 | 29       42 | 31
+//  and by 66000, 131072, 200000:
+//   top_k 300 1 row     35 | 41       44 | 47       51 | 54
+//            16 rows    36 | 44       45 | 50       55 | 58
+//   top_k 513 1 row     44 | 39       60 | 46       75 | 53
+//            16 rows    46 | 42       61 | 49       79 | 57
+// (Shared rows have 256 groups, so a top_k of more is counted over the row by its last workgroup, where one
+// workgroup has 1024: from 257 to 512 sharing loses up to 20 %.  top_k is on the device, and the rule cannot
+// look at it.)
 int SlicesOf(const SampleParams &p) { return p.vocab >= 65536 && p.rows <= 16 ? kSlices : 1; }
 
 template <int DT> void LaunchSample(SampleParams p, void *scratch, hipStream_t stream) {
