@@ -50,7 +50,7 @@ inline int64_t WeightRows(const Sizes &p) { return p.output ? 2 * p.N : p.N; }
 //   MXFP4  17 x 2048 x 14336 10.9 | 12.4    20 x 4096 x 11008 21.5 | 17.5
 //          24 x 4096 x 8192 13.5 | 14.8     32 x 8192 x 8192 26.0 | 22.4
 // Of 1600 such sizes, K from 512 to 28672 and N from 1024 to 28672, the side taken is 0.1 to
-// 1.1 % behind the other in the mean of each form, and at most 23 % (gated MXFP8 32 x 2048 x
+// 1.2 % behind the other in the mean of each form, and at most 23 % (gated MXFP8 32 x 2048 x
 // 8192, 10.3 | 12.7).
 inline bool Streams(const Sizes &p) {
   if (p.M <= 16 || p.M > 64) return p.M <= 16;
