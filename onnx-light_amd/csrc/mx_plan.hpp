@@ -127,7 +127,7 @@ inline StreamPlan PlanStream(const Sizes &p) {
 // than CUs, else two, so that two workgroups share a CU.  us, two stages | more: MXFP8 (four
 // waves) 128 x 4096 x 4096 20.5 | 18.2, 1000 x 14336 x 4096 66.9 | 61.7; MXFP4 128 x 4096 x
 // 4096 17.0 | 13.5, 1000 x 14336 x 4096 55.0 | 47.7, but 1000 x 4096 x 6144 27.5 | 28.9,
-// 2000 x 4096 x 4096 31.8 | 32.9; with a tile for each of 256 CUs and K = 2048 up to 9 % worse.
+// 2000 x 4096 x 4096 31.8 | 32.9.
 //
 // Tiles have eight waves, two a SIMD, of which one multiplies while the other waits or
 // stores.  Four read less of LDS, which wins along a long K of E4M3 by large tiles.
