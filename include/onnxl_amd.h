@@ -712,12 +712,13 @@ int onnxl_amd_mx_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_sca
 /* Gated feed-forward: y = act(a gate^T) * (a up^T), both products as
  * onnxl_amd_mx_matmul's (a, a_scale and a_type as there, and what E4M3's sums lose), the
  * activation and the product of the two in fp32: act(g) by the hardware's exponential and
- * reciprocal to 2^-19 (1 + g^2) of itself, 0 where it is below fp32's normal numbers.  gate and up [N, K] of one type with their scales
- * [N, K / 32] of one type.  activation: 0 SiLU, 1 GELU (erf), 2 GELU by tanh, 3 ReLU.
- * y [.., N] FLOAT16 or BFLOAT16, a's type where a has 16 bits, without y_scale; or
- * FLOAT8E4M3FN with y_scale FLOAT8E8M0 or UINT8 [.., N / 32], N a multiple of 32: the
- * MXFP8 that onnxl_amd_mx_quantize makes of the fp32 result, for the product that
- * takes it back.  Codes, y's among them, must be 16-byte aligned. */
+ * reciprocal to 2^-19 (1 + g^2) of itself, 0 where it is below fp32's normal numbers.
+ * gate and up [N, K] of one type with their scales [N, K / 32] of one type.  activation:
+ * 0 SiLU, 1 GELU (erf), 2 GELU by tanh, 3 ReLU.  y [.., N] FLOAT16 or BFLOAT16, a's type
+ * where a has 16 bits, without y_scale; or FLOAT8E4M3FN with y_scale FLOAT8E8M0 or UINT8
+ * [.., N / 32], N a multiple of 32: the MXFP8 that onnxl_amd_mx_quantize makes of the fp32
+ * result, for the product that takes it back.  Codes, y's among them, must be 16-byte
+ * aligned. */
 int onnxl_amd_mx_gated_matmul(const onnxl_amd_tensor *a, const onnxl_amd_tensor *a_scale, int32_t a_type,
                               const onnxl_amd_tensor *gate, const onnxl_amd_tensor *gate_scale,
                               const onnxl_amd_tensor *up, const onnxl_amd_tensor *up_scale, int32_t activation,
@@ -795,13 +796,15 @@ int onnxl_amd_kv_cache_append(const onnxl_amd_tensor *k, const onnxl_amd_tensor 
  * the keys, then the values.  Queries are rotated as onnxl_amd_rotary_embedding does
  * into q [tokens, heads, head_dim] (device memory, as the cache); keys are rotated in
  * fp32 and, unrounded between, appended, values appended as onnxl_amd_kv_cache_append
- * does, the same roundings near the middle between two codes among it.  cos and sin FLOAT or of qkv's type [positions, d / 2], d a multiple of 16.  A
- * token's position is its place in its sequence, length - new tokens + i, or that of
- * position_ids INT32 or INT64 [tokens].  Positions in host memory are checked against
- * the tables; on the device, one outside them makes the token's rotated queries NaN, and
- * its key a value that is not finite, so that its block and head get a NaN scale.  Rows of q of no sequence, or of one whose numbers
- * do not fit, are left alone.  q may not overlap qkv (the call refuses it); the blocks of the new tokens times
- * kv_heads have to stay below 2^31. */
+ * does, the same roundings near the middle between two codes among it.  cos and sin
+ * FLOAT or of qkv's type [positions, d / 2], d a multiple of 16.  A token's position is
+ * its place in its sequence, length - new tokens + i, or that of position_ids INT32 or
+ * INT64 [tokens].  Positions in host memory are checked against the tables; on the
+ * device, one outside them makes the token's rotated queries NaN, and its key a value
+ * that is not finite, so that its block and head get a NaN scale.  Rows of q of no
+ * sequence, or of one whose numbers do not fit, are left alone.  q may not overlap qkv
+ * (the call refuses it); the blocks of the new tokens times kv_heads have to stay below
+ * 2^31. */
 int onnxl_amd_rotary_kv_cache_append(const onnxl_amd_tensor *qkv, const onnxl_amd_tensor *cos,
                                      const onnxl_amd_tensor *sin, const onnxl_amd_tensor *position_ids,
                                      int32_t interleaved, onnxl_amd_tensor *q, onnxl_amd_tensor *k_cache,
